@@ -83,6 +83,17 @@ SIGNATURES = {
                                                   c_int, c_vp, c_vp]),
     "apus_ghip_store_status": (c_int, [c_vp, c_vp, c_int,
                                        ctypes.POINTER(ctypes.c_uint32)]),
+    "apus_ghip_bf16_linear_ep_dev": (c_int, [c_vp] * 5 + [c_size] * 6 + [c_int, c_vp]),
+    "apus_ghip_fp8blk_linear_ep_dev": (c_int, [c_vp] * 6 + [c_size] * 6 + [c_int, c_int, c_vp]),
+    "apus_ghip_bf16_gated_dev": (c_int, [c_vp] * 4 + [c_size] * 5 + [c_int, c_float, c_vp]),
+    "apus_ghip_fp8blk_gated_dev": (c_int, [c_vp] * 6 + [c_size] * 5 + [c_int, c_float, c_int,
+                                                                       c_vp]),
+    "apus_ghip_linear_ep_backward_ws": (c_size, [c_size] * 3),
+    "apus_ghip_bf16_linear_ep_backward_dev": (c_int, [c_vp] * 7 + [c_size] * 6
+                                              + [c_int, c_vp, c_size, c_vp]),
+    "apus_ghip_gated_backward_ws": (c_size, [c_size] * 3),
+    "apus_ghip_bf16_gated_backward_dev": (c_int, [c_vp] * 7 + [c_size] * 6
+                                          + [c_int, c_float, c_vp, c_size, c_vp]),
     "apus_ghip_set_trace_events": (None, [ctypes.POINTER(c_vp), c_int]),
     "apus_ghip_stream_hold": (c_int, [c_vp, ctypes.c_uint32]),
     # include/apus_synth.h

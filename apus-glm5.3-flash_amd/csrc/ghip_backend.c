@@ -20,6 +20,7 @@
 
 #include <hip/hip_runtime_api.h>
 #include <fcntl.h>
+#include <math.h>
 #include <pthread.h>
 #include <semaphore.h>
 #include <stdarg.h>
@@ -579,6 +580,236 @@ int apus_ghip_bf16_gemm_dev(const uint16_t *w, const uint16_t *x,
     if (ghip_init() || check_sizes(M, O, K)) return 1;
     HIPCHK(ghip_launch_bf16_linear(w, x, y, M, O, K, G.trace_n >= 2 ? G.trace_ev : NULL,
                                    (hipStream_t)stream));
+    G.dispatches++;
+    return 0;
+}
+
+/* ------------------------------------------------------------------------ */
+/* dense feed-forward                                                       */
+/* ------------------------------------------------------------------------ */
+
+_Static_assert((int)APUS_GHIP_ACT_NONE == GHIP_ACT_NONE && (int)APUS_GHIP_ACT_RELU == GHIP_ACT_RELU
+                   && (int)APUS_GHIP_ACT_SILU == GHIP_ACT_SILU
+                   && (int)APUS_GHIP_ACT_GELU == GHIP_ACT_GELU
+                   && (int)APUS_GHIP_ACT_GELU_TANH == GHIP_ACT_GELU_TANH,
+               "activation numbers");
+
+/* Launches go to the backend's device, whichever one is current. */
+static void device_scope_end(const int *prev) {
+    if (*prev >= 0) (void)hipSetDevice(*prev);
+}
+#define DEVICE_SCOPE __attribute__((cleanup(device_scope_end))) int prev_device_ = -1
+static int device_scope(int *prev, hipStream_t st) {
+    int cur = -1;
+    HIPCHK(hipGetDevice(&cur));
+    if (cur != G.device) {
+        HIPCHK(hipSetDevice(G.device));
+        *prev = cur;
+    }
+    if (st) {
+        hipDevice_t d = G.device;
+        HIPCHK(hipStreamGetDevice(st, &d));
+        if (d != G.device) {
+            ghip_seterr("the stream is of device %d, the backend of %d", (int)d, G.device);
+            return 1;
+        }
+    }
+    return 0;
+}
+
+/* *ld: 0 -> width; refuses less than the width, or more than 31 bits. */
+static int check_ld(const char *what, size_t *ld, size_t width) {
+    if (*ld == 0) *ld = width;
+    if (*ld < width || *ld > 0x7fffffffu) {
+        ghip_seterr("%s %zu: rows of %zu elements", what, *ld, width);
+        return 1;
+    }
+    return 0;
+}
+
+static int check_ptr(const char *what, const void *p) {
+    if (p) return 0;
+    ghip_seterr("%s is NULL", what);
+    return 1;
+}
+
+static int check_act(int act, float limit) {
+    if (act < GHIP_ACT_NONE || act > GHIP_ACT_GELU_TANH) {
+        ghip_seterr("unknown activation %d", act);
+        return 1;
+    }
+    if (!(limit >= 0.0f)) {
+        ghip_seterr("limit %g", (double)limit);
+        return 1;
+    }
+    return 0;
+}
+
+/* One forward product: scales NULL = BF16 weights; w2 = the up projection. */
+static int ffn_forward(int mode, const void *w, const float *scales, const void *w2,
+                       const float *scales2, const uint16_t *x, const uint16_t *bias,
+                       const uint16_t *residual, uint16_t *y, size_t M, size_t O, size_t K,
+                       size_t ldx, size_t ldr, size_t ldy, int act, float limit, int exact,
+                       hipStream_t st) {
+    if (check_sizes(M, O, K) || check_ptr("weights", w) || check_ptr("x", x)
+        || check_ptr("the output", y)
+        || (mode == GHIP_EP_GATED && check_ptr("up weights", w2)) || check_act(act, limit)
+        || check_ld("ldx", &ldx, K) || check_ld("ldy", &ldy, O) || check_ld("ldr", &ldr, O)
+        || ghip_init())
+        return 1;
+    DEVICE_SCOPE;
+    if (device_scope(&prev_device_, st)) return 1;
+    const GhipProd p = { .a = x, .b = w, .b2 = w2, .s = scales, .s2 = scales2, .ars = ldx,
+                         .aks = 1, .brs = K, .bks = 1, .M = (uint32_t)M, .N = (uint32_t)O,
+                         .K = (uint32_t)K, .exact = exact != 0 };
+    const GhipEp ep = { .bias = bias, .in = residual, .out = y, .ldin = ldr, .ldout = ldy,
+                        .act = act, .limit = limit > 0.0f ? limit : INFINITY };
+    HIPCHK(ghip_launch_ffn(mode, &p, &ep, st));
+    G.dispatches++;
+    return 0;
+}
+
+int apus_ghip_bf16_linear_ep_dev(const uint16_t *w, const uint16_t *x, const uint16_t *bias,
+                                 const uint16_t *residual, uint16_t *y, size_t M, size_t O,
+                                 size_t K, size_t ldx, size_t ldr, size_t ldy, int act,
+                                 void *stream) {
+    return ffn_forward(GHIP_EP_LINEAR, w, NULL, NULL, NULL, x, bias, residual, y, M, O, K, ldx,
+                       ldr, ldy, act, 0.0f, 0, (hipStream_t)stream);
+}
+
+int apus_ghip_fp8blk_linear_ep_dev(const uint8_t *codes, const float *scales, const uint16_t *x,
+                                   const uint16_t *bias, const uint16_t *residual, uint16_t *y,
+                                   size_t M, size_t O, size_t K, size_t ldx, size_t ldr,
+                                   size_t ldy, int act, int exact, void *stream) {
+    if (check_ptr("scales", scales)) return 1;
+    return ffn_forward(GHIP_EP_LINEAR, codes, scales, NULL, NULL, x, bias, residual, y, M, O, K,
+                       ldx, ldr, ldy, act, 0.0f, exact, (hipStream_t)stream);
+}
+
+int apus_ghip_bf16_gated_dev(const uint16_t *wg, const uint16_t *wu, const uint16_t *x,
+                             uint16_t *h, size_t M, size_t I, size_t K, size_t ldx, size_t ldh,
+                             int act, float limit, void *stream) {
+    return ffn_forward(GHIP_EP_GATED, wg, NULL, wu, NULL, x, NULL, NULL, h, M, I, K, ldx, 0, ldh,
+                       act, limit, 0, (hipStream_t)stream);
+}
+
+int apus_ghip_fp8blk_gated_dev(const uint8_t *gate_codes, const float *gate_scales,
+                               const uint8_t *up_codes, const float *up_scales,
+                               const uint16_t *x, uint16_t *h, size_t M, size_t I, size_t K,
+                               size_t ldx, size_t ldh, int act, float limit, int exact,
+                               void *stream) {
+    if (check_ptr("gate scales", gate_scales) || check_ptr("up scales", up_scales)) return 1;
+    return ffn_forward(GHIP_EP_GATED, gate_codes, gate_scales, up_codes, up_scales, x, NULL, NULL,
+                       h, M, I, K, ldx, 0, ldh, act, limit, exact, (hipStream_t)stream);
+}
+
+/* Rows of the workspace's matrices: whole 16-byte vectors. */
+static size_t ffn_ws_ld(size_t N) { return (N + 7) & ~(size_t)7; }
+/* ... and their bytes; 0 for a shape that the entries refuse. */
+static size_t ffn_ws_mat(size_t M, size_t N) {
+    if (M == 0 || N == 0 || M > 0x7fffffffu || N > 0x7fffffffu) return 0;
+    return (M * ffn_ws_ld(N) * 2 + 255) & ~(size_t)255;
+}
+
+size_t apus_ghip_linear_ep_backward_ws(size_t M, size_t O, size_t K) {
+    return K ? ffn_ws_mat(M, O) : 0;
+}
+
+size_t apus_ghip_gated_backward_ws(size_t M, size_t I, size_t K) {
+    return K ? 2 * ffn_ws_mat(M, I) : 0;
+}
+
+static int check_ws(const void *ws, size_t have, size_t need) {
+    if (ws && ((uintptr_t)ws & 15) == 0 && have >= need) return 0;
+    ghip_seterr("workspace of %zu bytes at %p: %zu are needed, 16-byte aligned", have, ws, need);
+    return 1;
+}
+
+/* dx = dz W (+ dz2 W2), dw = dz^T x. */
+static int ffn_dx(const uint16_t *dz, const uint16_t *dz2, size_t lddz, const uint16_t *w,
+                  const uint16_t *w2, uint16_t *dx, size_t M, size_t N, size_t K, size_t lddx,
+                  hipStream_t st) {
+    const GhipProd p = { .a = dz, .a2 = dz2, .b = w, .b2 = w2, .ars = lddz, .aks = 1, .brs = 1,
+                         .bks = K, .M = (uint32_t)M, .N = (uint32_t)K, .K = (uint32_t)N };
+    const GhipEp ep = { .out = dx, .ldout = lddx };
+    HIPCHK(ghip_launch_ffn(GHIP_EP_STORE, &p, &ep, st));
+    return 0;
+}
+
+static int ffn_dw(const uint16_t *dz, size_t lddz, const uint16_t *x, size_t ldx, uint16_t *dw,
+                  size_t M, size_t N, size_t K, hipStream_t st) {
+    const GhipProd p = { .a = dz, .b = x, .ars = 1, .aks = lddz, .brs = 1, .bks = ldx,
+                         .M = (uint32_t)N, .N = (uint32_t)K, .K = (uint32_t)M };
+    const GhipEp ep = { .out = dw, .ldout = K };
+    HIPCHK(ghip_launch_ffn(GHIP_EP_STORE, &p, &ep, st));
+    return 0;
+}
+
+int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
+                                          const uint16_t *bias, const uint16_t *dy, uint16_t *dx,
+                                          uint16_t *dw, uint16_t *dbias, size_t M, size_t O,
+                                          size_t K, size_t ldx, size_t lddy, size_t lddx,
+                                          int act, void *ws, size_t ws_bytes, void *stream) {
+    const int again = act != GHIP_ACT_NONE;              /* z is needed */
+    hipStream_t st = (hipStream_t)stream;
+    if (check_sizes(M, O, K) || check_act(act, 0.0f) || check_ptr("dy", dy)
+        || ((dx || again) && check_ptr("weights", w)) || ((dw || again) && check_ptr("x", x))
+        || check_ld("ldx", &ldx, K) || check_ld("lddy", &lddy, O) || check_ld("lddx", &lddx, K)
+        || (again && check_ws(ws, ws_bytes, ffn_ws_mat(M, O))))
+        return 1;
+    if (!dx && !dw && !dbias) {
+        ghip_seterr("no gradient asked for");
+        return 1;
+    }
+    if (ghip_init()) return 1;
+    DEVICE_SCOPE;
+    if (device_scope(&prev_device_, st)) return 1;
+    const uint16_t *dz = dy;
+    size_t lddz = lddy;
+    if (again) {
+        lddz = ffn_ws_ld(O);
+        dz = (const uint16_t *)ws;
+        const GhipProd p = { .a = x, .b = w, .ars = ldx, .aks = 1, .brs = K, .bks = 1,
+                             .M = (uint32_t)M, .N = (uint32_t)O, .K = (uint32_t)K };
+        const GhipEp ep = { .bias = bias, .in = dy, .out = (uint16_t *)ws, .ldin = lddy,
+                            .ldout = lddz, .act = act, .limit = INFINITY };
+        HIPCHK(ghip_launch_ffn(GHIP_EP_DLINEAR, &p, &ep, st));
+    }
+    if (dx && ffn_dx(dz, NULL, lddz, w, NULL, dx, M, O, K, lddx, st)) return 1;
+    if (dw && ffn_dw(dz, lddz, x, ldx, dw, M, O, K, st)) return 1;
+    if (dbias) HIPCHK(ghip_launch_ffn_colsum(dz, lddz, M, O, dbias, st));
+    G.dispatches++;
+    return 0;
+}
+
+int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, const uint16_t *x,
+                                      const uint16_t *dh, uint16_t *dx, uint16_t *dwg,
+                                      uint16_t *dwu, size_t M, size_t I, size_t K, size_t ldx,
+                                      size_t lddh, size_t lddx, int act, float limit, void *ws,
+                                      size_t ws_bytes, void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    if (check_sizes(M, I, K) || check_act(act, limit) || check_ptr("gate weights", wg)
+        || check_ptr("up weights", wu) || check_ptr("x", x) || check_ptr("dh", dh)
+        || check_ld("ldx", &ldx, K) || check_ld("lddh", &lddh, I) || check_ld("lddx", &lddx, K)
+        || check_ws(ws, ws_bytes, 2 * ffn_ws_mat(M, I)))
+        return 1;
+    if (!dx && !dwg && !dwu) {
+        ghip_seterr("no gradient asked for");
+        return 1;
+    }
+    if (ghip_init()) return 1;
+    DEVICE_SCOPE;
+    if (device_scope(&prev_device_, st)) return 1;
+    const size_t ld = ffn_ws_ld(I);
+    uint16_t *dg = (uint16_t *)ws, *du = (uint16_t *)((uint8_t *)ws + ffn_ws_mat(M, I));
+    const GhipProd p = { .a = x, .b = wg, .b2 = wu, .ars = ldx, .aks = 1, .brs = K, .bks = 1,
+                         .M = (uint32_t)M, .N = (uint32_t)I, .K = (uint32_t)K };
+    const GhipEp ep = { .in = dh, .out = dg, .out2 = du, .ldin = lddh, .ldout = ld, .act = act,
+                        .limit = limit > 0.0f ? limit : INFINITY };
+    HIPCHK(ghip_launch_ffn(GHIP_EP_DGATED, &p, &ep, st));
+    if (dx && ffn_dx(dg, du, ld, wg, wu, dx, M, I, K, lddx, st)) return 1;
+    if (dwg && ffn_dw(dg, ld, x, ldx, dwg, M, I, K, st)) return 1;
+    if (dwu && ffn_dw(du, ld, x, ldx, dwu, M, I, K, st)) return 1;
     G.dispatches++;
     return 0;
 }

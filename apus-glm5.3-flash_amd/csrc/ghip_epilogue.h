@@ -1,0 +1,122 @@
+/*
+ * ghip_epilogue.h — what the dense feed-forward kernels do with a finished
+ * f32 sum before it leaves the registers (k_ffn*.hip):
+ *
+ *   GHIP_EP_STORE   y = z                                     (gradients)
+ *   GHIP_EP_LINEAR  y = act(z + b) + r
+ *   GHIP_EP_GATED   h = act(min(g, limit)) * clamp(u, -limit, limit)
+ *   GHIP_EP_DLINEAR dz = dy * act'(z + b)
+ *   GHIP_EP_DGATED  dg = dh * clamp(u) * act'(min(g, limit)), 0 where g > limit
+ *                   du = dh * act(min(g, limit)), 0 where |u| > limit
+ *
+ * All of it in f32, with one rounding to bf16 (nearest even) at the store: the
+ * sums are f32, so bias, activation, clamp, product and residual cost no
+ * precision. dz, dg and du are rounded because the products that read them
+ * take bf16 operands.
+ *
+ * exp comes from the hardware exp2 and 1/x from the hardware reciprocal (each
+ * about 1 ulp of f32): 2^-22 relative against the output's 2^-9. An argument
+ * whose exp is infinite makes the sigmoid 0.
+ */
+#ifndef GHIP_EPILOGUE_H
+#define GHIP_EPILOGUE_H
+
+#include <type_traits>
+
+#include "ghip_device.h"
+#include "ghip_internal.h"
+
+#define GHIP_GELU_C 0.7978845608028654f          /* sqrt(2 / pi) */
+#define GHIP_GELU_A 0.044715f
+
+__device__ __forceinline__ float ghip_sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
+}
+
+template <int ACT>
+__device__ __forceinline__ float ghip_act(float z) {
+    if constexpr (ACT == GHIP_ACT_RELU) return z < 0.0f ? 0.0f : z;      /* keeps a NaN */
+    else if constexpr (ACT == GHIP_ACT_SILU) return z * ghip_sigmoid(z);
+    else if constexpr (ACT == GHIP_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    else if constexpr (ACT == GHIP_ACT_GELU_TANH)
+        /* (1 + tanh v) / 2 = sigmoid(2 v) */
+        return z * ghip_sigmoid(2.0f * GHIP_GELU_C * (z + GHIP_GELU_A * z * z * z));
+    else return z;
+}
+
+/* The derivative. The smooth ones are 0 or 1 to the last bit well inside +-100
+ * (+-20), and the clamp keeps an infinite z from making 0 * inf of that. */
+template <int ACT>
+__device__ __forceinline__ float ghip_slope(float z) {
+    if constexpr (ACT == GHIP_ACT_RELU) {
+        return z > 0.0f ? 1.0f : 0.0f;
+    } else if constexpr (ACT == GHIP_ACT_SILU) {
+        z = z > 100.0f ? 100.0f : z < -100.0f ? -100.0f : z;
+        const float s = ghip_sigmoid(z);
+        return s * (1.0f + z * (1.0f - s));
+    } else if constexpr (ACT == GHIP_ACT_GELU) {
+        z = z > 20.0f ? 20.0f : z < -20.0f ? -20.0f : z;
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f))
+               + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
+    } else if constexpr (ACT == GHIP_ACT_GELU_TANH) {
+        z = z > 20.0f ? 20.0f : z < -20.0f ? -20.0f : z;
+        const float s = ghip_sigmoid(2.0f * GHIP_GELU_C * (z + GHIP_GELU_A * z * z * z));
+        return s + z * s * (1.0f - s) * 2.0f * GHIP_GELU_C * (1.0f + 3.0f * GHIP_GELU_A * z * z);
+    } else {
+        return 1.0f;
+    }
+}
+
+/* The value(s) that leave the registers: s0 the sum (g), s1 the second one (u),
+ * b the bias, in the residual or the incoming gradient. */
+template <int MODE, int ACT>
+__device__ __forceinline__ void ghip_ep_value(float s0, float s1, float b, float in, float limit,
+                                              float &o0, float &o1) {
+    o1 = 0.0f;
+    if constexpr (MODE == GHIP_EP_STORE) {
+        o0 = s0;
+    } else if constexpr (MODE == GHIP_EP_LINEAR) {
+        o0 = ghip_act<ACT>(s0 + b) + in;
+    } else if constexpr (MODE == GHIP_EP_DLINEAR) {
+        o0 = in * ghip_slope<ACT>(s0 + b);
+    } else {
+        const float g = s0 > limit ? limit : s0;             /* keep a NaN */
+        const float u = s1 > limit ? limit : s1 < -limit ? -limit : s1;
+        if constexpr (MODE == GHIP_EP_GATED) {
+            o0 = ghip_act<ACT>(g) * u;
+        } else {
+            o0 = s0 > limit ? 0.0f : in * u * ghip_slope<ACT>(g);
+            o1 = s1 > limit || s1 < -limit ? 0.0f : in * ghip_act<ACT>(g);
+        }
+    }
+}
+
+/* Run f with the activation as a constant (wave-uniform branch). */
+template <typename F>
+__device__ __forceinline__ void ghip_with_act(int act, F f) {
+    switch (act) {
+    case GHIP_ACT_RELU: f(std::integral_constant<int, GHIP_ACT_RELU>{}); break;
+    case GHIP_ACT_SILU: f(std::integral_constant<int, GHIP_ACT_SILU>{}); break;
+    case GHIP_ACT_GELU: f(std::integral_constant<int, GHIP_ACT_GELU>{}); break;
+    case GHIP_ACT_GELU_TANH: f(std::integral_constant<int, GHIP_ACT_GELU_TANH>{}); break;
+    default: f(std::integral_constant<int, GHIP_ACT_NONE>{}); break;
+    }
+}
+
+/* Modes with two sums a column (the gate's and the up projection's). */
+constexpr bool ghip_ep_dual(int mode) { return mode == GHIP_EP_GATED || mode == GHIP_EP_DGATED; }
+
+/* One output: row m, column n. */
+template <int MODE, int ACT>
+__device__ __forceinline__ void ghip_ep_store1(const GhipEp &ep, uint32_t m, uint32_t n, float s0,
+                                               float s1) {
+    const float b = ep.bias ? ghip_bf16_f32(ep.bias[n]) : 0.0f;
+    const float in = ep.in ? ghip_bf16_f32(ep.in[(size_t)m * ep.ldin + n]) : 0.0f;
+    float o0, o1;
+    ghip_ep_value<MODE, ACT>(s0, s1, b, in, ep.limit, o0, o1);
+    ep.out[(size_t)m * ep.ldout + n] = (uint16_t)ghip_bf16_bits(o0);
+    if constexpr (MODE == GHIP_EP_DGATED)
+        ep.out2[(size_t)m * ep.ldout + n] = (uint16_t)ghip_bf16_bits(o1);
+}
+
+#endif /* GHIP_EPILOGUE_H */

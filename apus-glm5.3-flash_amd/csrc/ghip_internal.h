@@ -260,6 +260,46 @@ float ghip_fp8_gemm_estimate(size_t M, size_t N, size_t K, uint32_t n_cu);
 /* Its tile height << 16 | K splits. */
 uint32_t ghip_fp8_gemm_form(size_t M, size_t N, size_t K, uint32_t n_cu);
 
+/* ---- dense feed-forward (k_ffn*.hip) ------------------------------------ */
+
+/* Activations, as include/backend_hip.h numbers them. */
+enum { GHIP_ACT_NONE, GHIP_ACT_RELU, GHIP_ACT_SILU, GHIP_ACT_GELU, GHIP_ACT_GELU_TANH };
+
+/* What is done with a finished sum (ghip_epilogue.h). */
+enum { GHIP_EP_STORE, GHIP_EP_LINEAR, GHIP_EP_GATED, GHIP_EP_DLINEAR, GHIP_EP_DGATED };
+typedef struct {
+    const uint16_t *bias;        /* bf16 [N] or NULL */
+    const uint16_t *in;          /* bf16 [M, N], rows ldin apart: the residual (may be out) or the
+                                    incoming gradient; NULL = none */
+    uint16_t *out, *out2;        /* bf16 [M, N], rows ldout apart; out2: du of GHIP_EP_DGATED */
+    size_t ldin, ldout;
+    int act;
+    float limit;                 /* clamp of the gated modes, +inf = none */
+} GhipEp;
+
+/* sum_k A(m, k) B(n, k), A(m, k) at a[m * ars + k * aks], B(n, k) at b[n * brs +
+ * k * bks]; aks or ars is 1, and bks or brs. a2, b2: a second product added to
+ * the sum (same steps); b2 alone: the second sum of a dual mode. s, s2: F32
+ * scales [ceil(N/128), ceil(K/128)] make b, b2 FP8 codes (exact: 0 the caller
+ * guarantees no NaN code), NULL bf16. */
+typedef struct {
+    const uint16_t *a, *a2;
+    const void *b, *b2;
+    const float *s, *s2;
+    size_t ars, aks, brs, bks;
+    uint32_t M, N, K;
+    int exact;
+} GhipProd;
+
+/* Any shape, stride and alignment. */
+hipError_t ghip_launch_ffn_any(int mode, const GhipProd *p, const GhipEp *ep, hipStream_t st);
+/* out[n] = bf16(sum over m of dz[m, n]), dz bf16 with rows ld apart. */
+hipError_t ghip_launch_ffn_colsum(const uint16_t *dz, size_t ld, size_t M, size_t N,
+                                  uint16_t *out, hipStream_t st);
+
+/* The product by the kernel that suits its sizes, steps and alignment. */
+hipError_t ghip_launch_ffn(int mode, const GhipProd *p, const GhipEp *ep, hipStream_t st);
+
 /* One expert slab record of a converted v2 container's apus.index.json
  * (c/gcache.h:896-930): the shard file name and the slab's file offset. */
 typedef struct {

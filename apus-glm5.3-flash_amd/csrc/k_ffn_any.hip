@@ -1,0 +1,176 @@
+/*
+ * k_ffn_any.hip — the dense feed-forward products of any shape, stride and
+ * alignment on MFMA (gfx950):
+ *
+ *   out[m, n] = epilogue(sum_p sum_k A_p(m, k) * B_p(n, k))
+ *
+ * with A_p(m, k) at a[m * ars + k * aks] and B_p(n, k) at b[n * brs + k * bks]
+ * (bf16, or FP8 codes with an F32 scale a 128x128 block of (n, k)), one of the
+ * two steps 1. That covers the forward (A = x, B = W: k the fast index of
+ * both), dx = dz W (k the slow index of B; two pairs for the gated block) and
+ * dW = dz^T x (k the slow index of both). In the dual modes the second B gives
+ * a second sum of the same A.
+ *
+ * A workgroup of 4 waves owns 64 x 64 outputs, each wave 32 x 32 as four
+ * v_mfma_f32_16x16x32_bf16 a step of k = 32; tiles reach LDS through registers
+ * by 2-byte (1-byte) loads, the next step's in flight during the products,
+ * elements past M, N or k as zeros. It is bound by those loads' issue: the
+ * route for what the vector kernels cannot take.
+ */
+#include "ghip_epilogue.h"
+
+#define FA_LD 40u                                /* LDS row: 32 values, 80 bytes */
+
+typedef unsigned short fa_u16x8 __attribute__((ext_vector_type(8)));
+
+template <int MODE, bool FP8>
+__global__ __launch_bounds__(256) void k_ffn_any(GhipProd p, GhipEp ep, uint32_t blk0) {
+    constexpr int NB = ghip_ep_dual(MODE) ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) uint16_t as[64 * FA_LD], bs[NB][64 * FA_LD];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6;
+    const uint32_t n16 = lane & 15u, g = lane >> 4;
+    const uint32_t mt = (p.M + 63u) / 64u, t = blk0 + blockIdx.x;
+    const uint32_t row0 = (t % mt) * 64u, col0 = (t / mt) * 64u;
+    const uint32_t rw = (wv >> 1) * 32u, cw = (wv & 1u) * 32u;
+    ghip_f32x4 acc[NB][2][2] = {};
+    const uint32_t nkb = (p.K + 127u) >> 7;
+
+    /* element e of a thread: the operand's fast index runs over the threads */
+    auto at = [&](bool kfast, uint32_t e, uint32_t &r, uint32_t &k) {
+        const uint32_t v = tid + 256u * e;
+        r = kfast ? v >> 5 : v & 63u;
+        k = kfast ? v & 31u : v >> 6;
+    };
+    uint16_t ra[8], rb[NB][8];
+    auto fetch = [&](int pr, uint32_t k0) {
+        const uint16_t *a = pr ? p.a2 : p.a;
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) {
+            uint32_t r, k;
+            at(p.aks == 1, e, r, k);
+            ra[e] = row0 + r < p.M && k0 + k < p.K
+                        ? a[(size_t)(row0 + r) * p.ars + (size_t)(k0 + k) * p.aks] : (uint16_t)0;
+            at(p.bks == 1, e, r, k);
+            const bool in = col0 + r < p.N && k0 + k < p.K;
+            const size_t o = in ? (size_t)(col0 + r) * p.brs + (size_t)(k0 + k) * p.bks : 0;
+#pragma unroll
+            for (int d = 0; d < NB; d++) {
+                const void *b = d || pr ? p.b2 : p.b;
+                uint16_t v = 0;
+                if (in) {
+                    if constexpr (FP8) {
+                        const float s = (d ? p.s2 : p.s)[(size_t)((col0 + r) >> 7) * nkb + ((k0 + k) >> 7)];
+                        v = (uint16_t)ghip_bf16_bits(ghip_e4m3_exact(((const uint8_t *)b)[o]) * s);
+                    } else {
+                        v = ((const uint16_t *)b)[o];
+                    }
+                }
+                rb[d][e] = v;
+            }
+        }
+    };
+    const int pairs = p.a2 ? 2 : 1;
+    const uint32_t steps = (p.K + 31u) / 32u, total = steps * (uint32_t)pairs;
+    fetch(0, 0);
+    for (uint32_t j = 0; j < total; j++) {
+        __syncthreads();
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) {
+            uint32_t r, k;
+            at(p.aks == 1, e, r, k);
+            as[r * FA_LD + k] = ra[e];
+            at(p.bks == 1, e, r, k);
+#pragma unroll
+            for (int d = 0; d < NB; d++) bs[d][r * FA_LD + k] = rb[d][e];
+        }
+        __syncthreads();
+        if (j + 1u < total) fetch((int)((j + 1u) / steps), ((j + 1u) % steps) * 32u);
+        ghip_bf16x8 av[2];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; i++)
+            av[i] = *(const ghip_bf16x8 *)(as + (rw + 16u * i + n16) * FA_LD + 8u * g);
+#pragma unroll
+        for (int d = 0; d < NB; d++)
+#pragma unroll
+            for (uint32_t c = 0; c < 2; c++) {
+                const ghip_bf16x8 bv =
+                    *(const ghip_bf16x8 *)(bs[d] + (cw + 16u * c + n16) * FA_LD + 8u * g);
+#pragma unroll
+                for (uint32_t i = 0; i < 2; i++)
+                    acc[d][i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av[i], bv, acc[d][i][c],
+                                                                          0, 0, 0);
+            }
+    }
+    /* register q of block (i, c): row 16 i + 4 g + q, column 16 c + n16 */
+    ghip_with_act(ep.act, [&](auto act) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2; i++)
+#pragma unroll
+            for (uint32_t c = 0; c < 2; c++)
+#pragma unroll
+                for (uint32_t q = 0; q < 4; q++) {
+                    const uint32_t m = row0 + rw + 16u * i + 4u * g + q, n = col0 + cw + 16u * c + n16;
+                    if (m < p.M && n < p.N)
+                        ghip_ep_store1<MODE, decltype(act)::value>(ep, m, n, acc[0][i][c][q],
+                                                                   acc[NB - 1][i][c][q]);
+                }
+    });
+}
+
+/* dbias[n] = sum_m dz[m, n] in f32, rounded once. A workgroup owns 64 columns,
+ * its 16 groups of rows are added in a fixed order. */
+__global__ __launch_bounds__(1024) void k_ffn_colsum(const uint16_t *__restrict__ dz, size_t ld,
+                                                     uint32_t M, uint32_t N,
+                                                     uint16_t *__restrict__ out) {
+    __shared__ float part[16][64];
+    const uint32_t c = threadIdx.x & 63u, r = threadIdx.x >> 6, n = blockIdx.x * 64u + c;
+    float s = 0.0f;
+    if (n < N)
+        for (uint32_t m = r; m < M; m += 16u) s += ghip_bf16_f32(dz[(size_t)m * ld + n]);
+    part[r][c] = s;
+    __syncthreads();
+    if (r == 0 && n < N) {
+        float v = 0.0f;
+        for (uint32_t i = 0; i < 16; i++) v += part[i][c];
+        out[n] = (uint16_t)ghip_bf16_bits(v);
+    }
+}
+
+template <int MODE, bool FP8>
+static hipError_t fa_run(const GhipProd *p, const GhipEp *ep, hipStream_t st) {
+    const size_t tiles = (((size_t)p->M + 63) / 64) * (((size_t)p->N + 63) / 64);
+    const size_t most = GHIP_MAX_THREADS / 256u;
+    if (tiles > 0xffffffffu) return hipErrorInvalidValue;
+    for (size_t b = 0; b < tiles; b += most) {
+        const size_t n = tiles - b < most ? tiles - b : most;
+        hipLaunchKernelGGL((k_ffn_any<MODE, FP8>), dim3((uint32_t)n), dim3(256), 0, st, *p, *ep,
+                           (uint32_t)b);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+extern "C" hipError_t ghip_launch_ffn_any(int mode, const GhipProd *p, const GhipEp *ep,
+                                          hipStream_t st) {
+    if (p->M == 0 || p->N == 0 || p->K == 0) return hipErrorInvalidValue;
+    const bool fp8 = p->s != nullptr;
+    switch (mode) {
+    case GHIP_EP_STORE: return fp8 ? hipErrorInvalidValue : fa_run<GHIP_EP_STORE, false>(p, ep, st);
+    case GHIP_EP_LINEAR:
+        return fp8 ? fa_run<GHIP_EP_LINEAR, true>(p, ep, st) : fa_run<GHIP_EP_LINEAR, false>(p, ep, st);
+    case GHIP_EP_GATED:
+        return fp8 ? fa_run<GHIP_EP_GATED, true>(p, ep, st) : fa_run<GHIP_EP_GATED, false>(p, ep, st);
+    case GHIP_EP_DLINEAR: return fp8 ? hipErrorInvalidValue : fa_run<GHIP_EP_DLINEAR, false>(p, ep, st);
+    case GHIP_EP_DGATED: return fp8 ? hipErrorInvalidValue : fa_run<GHIP_EP_DGATED, false>(p, ep, st);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+extern "C" hipError_t ghip_launch_ffn_colsum(const uint16_t *dz, size_t ld, size_t M, size_t N,
+                                             uint16_t *out, hipStream_t st) {
+    if (M == 0 || N == 0 || M > 0x7fffffffu || N > 0x7fffffffu) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(k_ffn_colsum, dim3((uint32_t)((N + 63) / 64)), dim3(1024), 0, st, dz, ld,
+                       (uint32_t)M, (uint32_t)N, out);
+    return hipGetLastError();
+}

@@ -349,6 +349,96 @@ int apus_ghip_moe_prefill_dev_noalloc(ApusGhipStore *s, const uint16_t *x, size_
                                       const int32_t *idx, const float *w, int topk,
                                       uint16_t *out, void *stream);
 
+/* --- dense feed-forward operators on device pointers (no counterpart in the
+ * Metal backend; the engine's dense and shared MLPs and its output projections
+ * run them as separate linears, elementwise passes and adds). Extension.
+ *
+ *   linear_ep  y = act(x W^T + bias) + residual
+ *   gated      h = act(min(g, limit)) * clamp(u, -limit, limit),
+ *              g = x Wg^T, u = x Wu^T                (one kernel)
+ *   *_backward their gradients (BF16 weights)
+ *
+ * Common rules.
+ *   - w, wg, wu [O,K] / [I,K] row-major, BF16, or FP8 codes with the F32
+ *     scales of their 128x128 blocks (dequantized bit-exactly, as everywhere);
+ *     x [M,K], bias [O], residual and y [M,O], h and dh [M,I], all BF16.
+ *     bias and residual may be NULL.
+ *   - ldx, ldr, ldy, ldh, lddy, ... are the elements from one row to the next
+ *     of that matrix (0 = its width): rows may lie in a wider buffer, whose
+ *     other columns are neither read into a result nor written. Weights and
+ *     weight gradients are dense.
+ *   - act: APUS_GHIP_ACT_*. GELU is z * Phi(z), GELU_TANH its tanh form. limit
+ *     0 = no clamp (10 for GLM-5.3-Flash's SwiGLU).
+ *   - Sums, bias, activation, product and residual are f32; the result is
+ *     rounded once to BF16 (the MoE entries round g, u, silu(g) and h each, as
+ *     the reference does: their h differs from this one in the last bits).
+ *     Deterministic run to run.
+ *   - residual may be y itself (same ld): each element is read before it is
+ *     written. No other output may overlap an input or another output.
+ *   - exact (FP8): 0 = the caller guarantees no 0x7F/0xFF code, else those two
+ *     decode as +-480. No scan, no state: -1 is taken as 1.
+ *   - Asynchronous on `stream` (a hipStream_t of the backend's device, NULL =
+ *     its null stream), whichever device is current. No allocation, no
+ *     process-wide workspace: calls on different streams may overlap, and all
+ *     of them may be captured into graphs.
+ *   - 0 = queued; 1 = refused or failed (empty or over-large shape, NULL
+ *     operand, a stride below the width, an unknown act, a limit that is
+ *     negative or NaN, a stream of another device, a workspace that is too
+ *     small; apus_ghip_last_error), nothing or only a part launched.
+ *   - Alignment: 16-byte aligned pointers and strides of whole 16 bytes, with
+ *     K % 8 == 0 (K % 16 == 0 for FP8), take the vector kernels; everything
+ *     else a slower general one (same results within the tolerance). */
+enum {
+    APUS_GHIP_ACT_NONE = 0,
+    APUS_GHIP_ACT_RELU = 1,
+    APUS_GHIP_ACT_SILU = 2,
+    APUS_GHIP_ACT_GELU = 3,
+    APUS_GHIP_ACT_GELU_TANH = 4
+};
+int apus_ghip_bf16_linear_ep_dev(const uint16_t *w, const uint16_t *x, const uint16_t *bias,
+                                 const uint16_t *residual, uint16_t *y, size_t M, size_t O,
+                                 size_t K, size_t ldx, size_t ldr, size_t ldy, int act,
+                                 void *stream);
+int apus_ghip_fp8blk_linear_ep_dev(const uint8_t *codes, const float *scales, const uint16_t *x,
+                                   const uint16_t *bias, const uint16_t *residual, uint16_t *y,
+                                   size_t M, size_t O, size_t K, size_t ldx, size_t ldr,
+                                   size_t ldy, int act, int exact, void *stream);
+int apus_ghip_bf16_gated_dev(const uint16_t *wg, const uint16_t *wu, const uint16_t *x,
+                             uint16_t *h, size_t M, size_t I, size_t K, size_t ldx, size_t ldh,
+                             int act, float limit, void *stream);
+int apus_ghip_fp8blk_gated_dev(const uint8_t *gate_codes, const float *gate_scales,
+                               const uint8_t *up_codes, const float *up_scales,
+                               const uint16_t *x, uint16_t *h, size_t M, size_t I, size_t K,
+                               size_t ldx, size_t ldh, int act, float limit, int exact,
+                               void *stream);
+/* The linear's gradients from dy [M,O]: with z = x W^T + bias computed again
+ * (act NONE needs none) and dz = dy * act'(z),
+ *   dx = dz W [M,K], dw = dz^T x [O,K], dbias = sum over the rows of dz [O],
+ * each BF16, each left out where its pointer is NULL (not all). The residual's
+ * gradient is dy. dz is rounded to BF16 once, as the products' operand. ws:
+ * 16-byte aligned device memory of at least
+ * apus_ghip_linear_ep_backward_ws(M, O, K) bytes that no overlapping call uses
+ * (not needed, may be NULL, with act NONE); the call leaves nothing in it that
+ * a later one reads. */
+size_t apus_ghip_linear_ep_backward_ws(size_t M, size_t O, size_t K);
+int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
+                                          const uint16_t *bias, const uint16_t *dy, uint16_t *dx,
+                                          uint16_t *dw, uint16_t *dbias, size_t M, size_t O,
+                                          size_t K, size_t ldx, size_t lddy, size_t lddx,
+                                          int act, void *ws, size_t ws_bytes, void *stream);
+/* The gated projections' gradients from dh [M,I]: g and u computed again,
+ *   dg = dh * clamp(u) * act'(min(g, limit)), 0 where g > limit,
+ *   du = dh * act(min(g, limit)), 0 where |u| > limit,
+ *   dx = dg Wg + du Wu [M,K], dwg = dg^T x, dwu = du^T x [I,K],
+ * each BF16, each left out where its pointer is NULL (not all). dg and du are
+ * rounded to BF16 once. ws as above, apus_ghip_gated_backward_ws(M, I, K). */
+size_t apus_ghip_gated_backward_ws(size_t M, size_t I, size_t K);
+int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, const uint16_t *x,
+                                      const uint16_t *dh, uint16_t *dx, uint16_t *dwg,
+                                      uint16_t *dwu, size_t M, size_t I, size_t K, size_t ldx,
+                                      size_t lddh, size_t lddx, int act, float limit, void *ws,
+                                      size_t ws_bytes, void *stream);
+
 /* --- timing (no reference counterpart; for benchmarks and profilers).
  * events: n caller-created hipEvent_t handles, NULL/0 turns it off. While
  * set, launches carry start/stop events in their dispatch packets
