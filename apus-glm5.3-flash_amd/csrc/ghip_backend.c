@@ -160,6 +160,7 @@ static int ghip_init(void) {
     HIPCHK(ghip_moe_decode_init());
     HIPCHK(ghip_linear_init(G.n_cu));
     HIPCHK(ghip_moe_prefill_init());
+    HIPCHK(ghip_ffn_init(G.n_cu));
     G.pf.n_cu = G.n_cu;
     G.pf_inited = 1;
     /* the allocation-free prefill's scratch: its device address, taken once
@@ -728,19 +729,23 @@ static int check_ws(const void *ws, size_t have, size_t need) {
 /* dx = dz W (+ dz2 W2), dw = dz^T x. */
 static int ffn_dx(const uint16_t *dz, const uint16_t *dz2, size_t lddz, const uint16_t *w,
                   const uint16_t *w2, uint16_t *dx, size_t M, size_t N, size_t K, size_t lddx,
-                  hipStream_t st) {
+                  int apad, hipStream_t st) {
     const GhipProd p = { .a = dz, .a2 = dz2, .b = w, .b2 = w2, .ars = lddz, .aks = 1, .brs = 1,
-                         .bks = K, .M = (uint32_t)M, .N = (uint32_t)K, .K = (uint32_t)N };
+                         .bks = K, .M = (uint32_t)M, .N = (uint32_t)K, .K = (uint32_t)N,
+                         .apad = apad };
     const GhipEp ep = { .out = dx, .ldout = lddx };
     HIPCHK(ghip_launch_ffn(GHIP_EP_STORE, &p, &ep, st));
     return 0;
 }
 
-static int ffn_dw(const uint16_t *dz, size_t lddz, const uint16_t *x, size_t ldx, uint16_t *dw,
-                  size_t M, size_t N, size_t K, hipStream_t st) {
-    const GhipProd p = { .a = dz, .b = x, .ars = 1, .aks = lddz, .brs = 1, .bks = ldx,
-                         .M = (uint32_t)N, .N = (uint32_t)K, .K = (uint32_t)M };
-    const GhipEp ep = { .out = dw, .ldout = K };
+/* dw2, dz2: a second one beside it, in the same launch. */
+static int ffn_dw(const uint16_t *dz, const uint16_t *dz2, size_t lddz, const uint16_t *x,
+                  size_t ldx, uint16_t *dw, uint16_t *dw2, size_t M, size_t N, size_t K, int apad,
+                  hipStream_t st) {
+    const GhipProd p = { .a = dz, .a2 = dz2, .b = x, .b2 = dz2 ? x : NULL, .ars = 1, .aks = lddz,
+                         .brs = 1, .bks = ldx, .M = (uint32_t)N, .N = (uint32_t)K,
+                         .K = (uint32_t)M, .batch = dz2 != NULL, .apad = apad };
+    const GhipEp ep = { .out = dw, .out2 = dw2, .ldout = K };
     HIPCHK(ghip_launch_ffn(GHIP_EP_STORE, &p, &ep, st));
     return 0;
 }
@@ -772,11 +777,11 @@ int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
         const GhipProd p = { .a = x, .b = w, .ars = ldx, .aks = 1, .brs = K, .bks = 1,
                              .M = (uint32_t)M, .N = (uint32_t)O, .K = (uint32_t)K };
         const GhipEp ep = { .bias = bias, .in = dy, .out = (uint16_t *)ws, .ldin = lddy,
-                            .ldout = lddz, .act = act, .limit = INFINITY };
+                            .ldout = lddz, .act = act, .limit = INFINITY, .pad = 1 };
         HIPCHK(ghip_launch_ffn(GHIP_EP_DLINEAR, &p, &ep, st));
     }
-    if (dx && ffn_dx(dz, NULL, lddz, w, NULL, dx, M, O, K, lddx, st)) return 1;
-    if (dw && ffn_dw(dz, lddz, x, ldx, dw, M, O, K, st)) return 1;
+    if (dx && ffn_dx(dz, NULL, lddz, w, NULL, dx, M, O, K, lddx, again, st)) return 1;
+    if (dw && ffn_dw(dz, NULL, lddz, x, ldx, dw, NULL, M, O, K, again, st)) return 1;
     if (dbias) HIPCHK(ghip_launch_ffn_colsum(dz, lddz, M, O, dbias, st));
     G.dispatches++;
     return 0;
@@ -805,11 +810,14 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
     const GhipProd p = { .a = x, .b = wg, .b2 = wu, .ars = ldx, .aks = 1, .brs = K, .bks = 1,
                          .M = (uint32_t)M, .N = (uint32_t)I, .K = (uint32_t)K };
     const GhipEp ep = { .in = dh, .out = dg, .out2 = du, .ldin = lddh, .ldout = ld, .act = act,
-                        .limit = limit > 0.0f ? limit : INFINITY };
+                        .limit = limit > 0.0f ? limit : INFINITY, .pad = 1 };
     HIPCHK(ghip_launch_ffn(GHIP_EP_DGATED, &p, &ep, st));
-    if (dx && ffn_dx(dg, du, ld, wg, wu, dx, M, I, K, lddx, st)) return 1;
-    if (dwg && ffn_dw(dg, ld, x, ldx, dwg, M, I, K, st)) return 1;
-    if (dwu && ffn_dw(du, ld, x, ldx, dwu, M, I, K, st)) return 1;
+    if (dx && ffn_dx(dg, du, ld, wg, wu, dx, M, I, K, lddx, 1, st)) return 1;
+    if (dwg && dwu) {
+        if (ffn_dw(dg, du, ld, x, ldx, dwg, dwu, M, I, K, 1, st)) return 1;
+    } else if (dwg || dwu) {
+        if (ffn_dw(dwg ? dg : du, NULL, ld, x, ldx, dwg ? dwg : dwu, NULL, M, I, K, 1, st)) return 1;
+    }
     G.dispatches++;
     return 0;
 }

@@ -275,11 +275,15 @@ typedef struct {
     size_t ldin, ldout;
     int act;
     float limit;                 /* clamp of the gated modes, +inf = none */
+    int pad;                     /* the columns of out up to the next multiple of 8 are its own
+                                    and get zeros (ldout % 8 == 0, 16-byte aligned) */
 } GhipEp;
 
 /* sum_k A(m, k) B(n, k), A(m, k) at a[m * ars + k * aks], B(n, k) at b[n * brs +
  * k * bks]; aks or ars is 1, and bks or brs. a2, b2: a second product added to
- * the sum (same steps); b2 alone: the second sum of a dual mode. s, s2: F32
+ * the sum (same steps), or with batch a second product of its own, to out2; b2
+ * alone: the second sum of a dual mode. apad: a's rows reach to the next
+ * multiple of 8 elements, with zeros there where they run along k. s, s2: F32
  * scales [ceil(N/128), ceil(K/128)] make b, b2 FP8 codes (exact: 0 the caller
  * guarantees no NaN code), NULL bf16. */
 typedef struct {
@@ -288,7 +292,7 @@ typedef struct {
     const float *s, *s2;
     size_t ars, aks, brs, bks;
     uint32_t M, N, K;
-    int exact;
+    int exact, batch, apad;
 } GhipProd;
 
 /* Any shape, stride and alignment. */
@@ -296,6 +300,26 @@ hipError_t ghip_launch_ffn_any(int mode, const GhipProd *p, const GhipEp *ep, hi
 /* out[n] = bf16(sum over m of dz[m, n]), dz bf16 with rows ld apart. */
 hipError_t ghip_launch_ffn_colsum(const uint16_t *dz, size_t ld, size_t M, size_t N,
                                   uint16_t *out, hipStream_t st);
+
+/* On tiles (k_ffn_gemm.h): fits = the steps and alignments of the vector loads;
+ * pick = the tile shape with the least estimated time (microseconds, in us). */
+int ghip_ffn_gemm_fits(int mode, const GhipProd *p);
+int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us);
+hipError_t ghip_launch_ffn_gemm(int mode, int tile, const GhipProd *p, const GhipEp *ep,
+                                hipStream_t st);
+/* One family of its kernels: the tiles of a mode (k_ffn_nt.hip, k_ffn_bwd.hip). */
+typedef struct {
+    uint32_t bm, bn;             /* output rows and columns */
+    float us;                    /* a stage's time on a full chip, microseconds */
+    uint32_t lds;
+    const void *kern;
+    void (*launch)(const GhipProd *, const GhipEp *, uint32_t, uint32_t, uint32_t, hipStream_t);
+} GhipFfnTile;
+const GhipFfnTile *ghip_ffn_forward_tiles(int mode, int fp8, int *n);
+const GhipFfnTile *ghip_ffn_backward_tiles(int mode, int transposed, int *n);
+
+/* Set-up (dynamic-LDS limits, the CU count of the routes). */
+hipError_t ghip_ffn_init(uint32_t n_cu);
 
 /* The product by the kernel that suits its sizes, steps and alignment. */
 hipError_t ghip_launch_ffn(int mode, const GhipProd *p, const GhipEp *ep, hipStream_t st);

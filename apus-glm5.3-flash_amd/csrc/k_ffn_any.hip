@@ -110,6 +110,10 @@ __global__ __launch_bounds__(256) void k_ffn_any(GhipProd p, GhipEp ep, uint32_t
 #pragma unroll
                 for (uint32_t q = 0; q < 4; q++) {
                     const uint32_t m = row0 + rw + 16u * i + 4u * g + q, n = col0 + cw + 16u * c + n16;
+                    if (ep.pad && m < p.M && n >= p.N && n < ((p.N + 7u) & ~7u)) {
+                        ep.out[(size_t)m * ep.ldout + n] = 0;
+                        if (MODE == GHIP_EP_DGATED) ep.out2[(size_t)m * ep.ldout + n] = 0;
+                    }
                     if (m < p.M && n < p.N)
                         ghip_ep_store1<MODE, decltype(act)::value>(ep, m, n, acc[0][i][c][q],
                                                                    acc[NB - 1][i][c][q]);
@@ -154,6 +158,18 @@ static hipError_t fa_run(const GhipProd *p, const GhipEp *ep, hipStream_t st) {
 extern "C" hipError_t ghip_launch_ffn_any(int mode, const GhipProd *p, const GhipEp *ep,
                                           hipStream_t st) {
     if (p->M == 0 || p->N == 0 || p->K == 0) return hipErrorInvalidValue;
+    if (p->batch) {
+        GhipProd one = *p, two = *p;
+        GhipEp to = *ep;
+        one.batch = two.batch = 0;
+        two.a = p->a2;
+        two.b = p->b2;
+        one.a2 = two.a2 = nullptr;
+        one.b2 = two.b2 = nullptr;
+        to.out = ep->out2;
+        const hipError_t e = ghip_launch_ffn_any(mode, &one, ep, st);
+        return e == hipSuccess ? ghip_launch_ffn_any(mode, &two, &to, st) : e;
+    }
     const bool fp8 = p->s != nullptr;
     switch (mode) {
     case GHIP_EP_STORE: return fp8 ? hipErrorInvalidValue : fa_run<GHIP_EP_STORE, false>(p, ep, st);

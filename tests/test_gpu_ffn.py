@@ -192,7 +192,7 @@ def test_gated_backward(ghip, M, N, K):
 
 
 @pytest.mark.parametrize("weights", ["bf16", "fp8"])
-@pytest.mark.parametrize("M,N,K", [(1, 520, 512), (6, 264, 256), (40, 392, 384), (300, 520, 640)])
+@pytest.mark.parametrize("M,N,K", [(1, 520, 512), (6, 264, 256), (40, 392, 384), (40, 392, 208), (300, 520, 640), (300, 520, 1104)])
 @pytest.mark.parametrize("pad,off", [(8, 8), (64, 0), (3, 1), (1, 0), (8, 3)])
 def test_rows_in_wider_buffers(ghip, M, N, K, weights, pad, off):
     """x, residual and y as slices of wider buffers, 16-byte aligned or not: the
@@ -209,7 +209,7 @@ def test_rows_in_wider_buffers(ghip, M, N, K, weights, pad, off):
     R.check(wide(h.get()), *R.gated(wide(x), w[2], w2[2], R.SILU, 2.0), "gated")
 
 
-@pytest.mark.parametrize("M,N,K", [(6, 264, 256), (300, 520, 640)])
+@pytest.mark.parametrize("M,N,K", [(6, 264, 256), (300, 520, 640), (300, 515, 200)])
 @pytest.mark.parametrize("pad,off", [(8, 8), (3, 1)])
 def test_backward_of_rows_in_wider_buffers(ghip, M, N, K, pad, off):
     rng = seed(6, M, N, K)
