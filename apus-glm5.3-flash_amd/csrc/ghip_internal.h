@@ -318,6 +318,13 @@ typedef struct {
 const GhipFfnTile *ghip_ffn_forward_tiles(int mode, int fp8, int *n);
 const GhipFfnTile *ghip_ffn_backward_tiles(int mode, int transposed, int *n);
 
+/* Streaming the weights past a few rows (k_rows_gemm.h), forward modes. */
+int ghip_ffn_rows_fits(int mode, const GhipProd *p);
+int ghip_ffn_rows_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us);
+hipError_t ghip_launch_ffn_rows(int mode, int form, const GhipProd *p, const GhipEp *ep,
+                                hipStream_t st);
+hipError_t ghip_ffn_rows_init(void);
+
 /* Set-up (dynamic-LDS limits, the CU count of the routes). */
 hipError_t ghip_ffn_init(uint32_t n_cu);
 

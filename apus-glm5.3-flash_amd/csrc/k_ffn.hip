@@ -65,11 +65,11 @@ extern "C" hipError_t ghip_launch_ffn_gemm(int mode, int tile, const GhipProd *p
 
 extern "C" hipError_t ghip_launch_ffn(int mode, const GhipProd *p, const GhipEp *ep,
                                       hipStream_t st) {
-    if (g_ffn_ncu && ghip_ffn_gemm_fits(mode, p)) {
-        float us;
-        const int tile = ghip_ffn_gemm_pick(mode, p, g_ffn_ncu, &us);
-        return ghip_launch_ffn_gemm(mode, tile, p, ep, st);
-    }
+    float us = 1e30f, rows_us = 1e30f;
+    const int tile = g_ffn_ncu && ghip_ffn_gemm_fits(mode, p) ? ghip_ffn_gemm_pick(mode, p, g_ffn_ncu, &us) : -1;
+    const int form = g_ffn_ncu && ghip_ffn_rows_fits(mode, p) ? ghip_ffn_rows_pick(mode, p, g_ffn_ncu, &rows_us) : -1;
+    if (form >= 0 && rows_us <= us) return ghip_launch_ffn_rows(mode, form, p, ep, st);
+    if (tile >= 0) return ghip_launch_ffn_gemm(mode, tile, p, ep, st);
     return ghip_launch_ffn_any(mode, p, ep, st);
 }
 
@@ -85,6 +85,8 @@ extern "C" hipError_t ghip_ffn_init(uint32_t n_cu) {
             if (e != hipSuccess) return e;
         }
     }
+    const hipError_t e = ghip_ffn_rows_init();
+    if (e != hipSuccess) return e;
     g_ffn_ncu = n_cu;
     return hipSuccess;
 }

@@ -1,0 +1,143 @@
+/*
+ * k_ffn_rows.hip — the forward feed-forward products of a few rows: the
+ * weight-streaming kernel (k_rows_gemm.h) with an epilogue, for one weight
+ * matrix (linear) or gate and up together (gated).
+ */
+#include "k_rows_gemm.h"
+
+#define FR_MAX_TILES ((size_t)65535)
+#define FR_MAX_BLOCKS (GHIP_MAX_THREADS / (RW_NW * 64))
+
+/* One launchable form: MR rows of x, NT weight groups of 16 a wave, K over KS
+ * waves. chunk: measured microseconds of a wave's chunk step. */
+struct FrForm {
+    uint32_t mr, nt, ks;
+    float chunk;
+    const void *kern;
+    uint32_t lds;
+    void (*launch)(dim3, uint32_t, hipStream_t, const GhipProd &, const GhipEp &, uint32_t, uint32_t);
+};
+
+template <bool BF, int MR, int NT, int KS, int NA, int SL, int MODE>
+static void fr_run(dim3 grid, uint32_t lds, hipStream_t st, const GhipProd &p, const GhipEp &ep,
+                   uint32_t blk0, uint32_t tile0) {
+    const RwMore more = {(const uint8_t *)p.b2, p.s2, (uint32_t)p.ars, p.exact, ep};
+    hipLaunchKernelGGL((k_rows_gemm<BF, MR, NT, KS, NA, SL, MODE>), grid, dim3(RW_NW * 64), lds, st,
+                       (const uint8_t *)p.b, p.s, p.a, ep.out, p.M, p.N, p.K, nullptr, blk0, tile0,
+                       more);
+}
+
+#define FR_FORM(BF, MR, NT, KS, NA, SL, MODE, T)                                            \
+    {MR, NT, KS, T, (const void *)k_rows_gemm<BF, MR, NT, KS, NA, SL, MODE>,                  \
+     rw_lds<BF, MR, NT, SL>(), fr_run<BF, MR, NT, KS, NA, SL, MODE>}
+
+#define FR_L(BF, MR, NT, KS, NA, SL, T) FR_FORM(BF, MR, NT, KS, NA, SL, GHIP_EP_LINEAR, T)
+static const FrForm fr_linear8[] = {
+    FR_L(false, 4, 1, 8, 2, 2, 0.55f),  FR_L(false, 4, 1, 4, 2, 2, 0.55f),
+    FR_L(false, 4, 1, 2, 2, 2, 0.56f),  FR_L(false, 8, 1, 8, 2, 2, 0.65f),
+    FR_L(false, 8, 1, 4, 2, 2, 0.65f),  FR_L(false, 8, 1, 2, 2, 2, 0.62f),
+    FR_L(false, 16, 1, 8, 1, 1, 0.85f), FR_L(false, 16, 2, 8, 2, 2, 1.30f),
+    FR_L(false, 16, 2, 4, 2, 2, 1.30f), FR_L(false, 32, 1, 8, 1, 1, 1.30f),
+    FR_L(false, 32, 2, 8, 1, 1, 1.70f), FR_L(false, 32, 2, 4, 1, 1, 1.70f),
+    FR_L(false, 64, 2, 4, 1, 1, 2.20f),
+};
+static const FrForm fr_linear16[] = {
+    FR_L(true, 8, 1, 8, 2, 2, 0.50f),  FR_L(true, 8, 1, 4, 2, 2, 0.50f),
+    FR_L(true, 16, 1, 8, 2, 2, 0.58f), FR_L(true, 16, 1, 4, 2, 2, 0.60f),
+    FR_L(true, 16, 2, 4, 2, 2, 0.75f), FR_L(true, 32, 1, 8, 1, 1, 0.85f),
+    FR_L(true, 32, 2, 8, 1, 1, 1.20f), FR_L(true, 32, 2, 4, 1, 1, 1.15f),
+};
+#define FR_G(BF, MR, NT, KS, NA, SL, T) FR_FORM(BF, MR, NT, KS, NA, SL, GHIP_EP_GATED, T)
+static const FrForm fr_gated8[] = {
+    FR_G(false, 4, 2, 8, 2, 2, 0.70f),  FR_G(false, 4, 2, 4, 2, 2, 0.70f),
+    FR_G(false, 4, 2, 2, 2, 2, 0.70f),  FR_G(false, 8, 2, 8, 2, 2, 0.85f),
+    FR_G(false, 8, 2, 4, 2, 2, 0.85f),  FR_G(false, 16, 2, 8, 2, 2, 1.30f),
+    FR_G(false, 16, 2, 4, 2, 2, 1.30f), FR_G(false, 32, 2, 8, 1, 1, 1.70f),
+    FR_G(false, 32, 2, 4, 1, 1, 1.70f), FR_G(false, 64, 2, 4, 1, 1, 2.20f),
+};
+static const FrForm fr_gated16[] = {
+    FR_G(true, 8, 2, 8, 2, 2, 0.65f),  FR_G(true, 8, 2, 4, 2, 2, 0.65f),
+    FR_G(true, 16, 2, 8, 2, 2, 0.75f), FR_G(true, 16, 2, 4, 2, 2, 0.75f),
+    FR_G(true, 32, 2, 8, 1, 1, 1.20f), FR_G(true, 32, 2, 4, 1, 1, 1.15f),
+};
+
+static const FrForm *fr_forms(int mode, bool fp8, int *n) {
+#define FR_TABLE(t) (*n = (int)(sizeof t / sizeof *t), t)
+    if (mode == GHIP_EP_GATED) return fp8 ? FR_TABLE(fr_gated8) : FR_TABLE(fr_gated16);
+    return fp8 ? FR_TABLE(fr_linear8) : FR_TABLE(fr_linear16);
+#undef FR_TABLE
+}
+
+/* Estimated microseconds of a form, as of the plain linear's (k_rows.hip): the
+ * larger of rounds of the chip x a wave's chunks x the chunk time and the
+ * weights at 6.5 TB/s, + a tenth of the other. */
+static float fr_estimate(const FrForm &c, const GhipProd *p, bool dual, uint32_t n_cu) {
+    if (c.mr < 16 && p->M > c.mr) return 1e30f;
+    const double cols = (dual ? 8.0 : 16.0) * c.nt * (RW_NW / c.ks);
+    const double wgs = (double)(size_t)((p->N + cols - 1) / cols) * (double)((p->M + c.mr - 1) / c.mr);
+    const double kb = (double)p->K * (p->s ? 1 : 2), nch = (double)(size_t)((kb + 127) / 128);
+    const double rounds = (double)(size_t)((wgs + n_cu - 1) / n_cu);
+    const double nc = (double)(size_t)((nch + c.ks - 1) / c.ks);
+    const double hbm = (double)p->N * kb * (dual ? 2 : 1) / 6.5e6;
+    const double over = c.mr > 32 ? 3.8 * rounds
+                        : p->s && c.mr * c.nt >= 32 && nc < 8.0 ? 2.0 * (rounds - 1.0) : 0.0;
+    const double t = rounds * nc * c.chunk + over;
+    const double lds = t < hbm ? 0.0015 * hbm * c.mr * c.nt : 0.0;
+    return (float)(2.3 + (t > hbm ? t + 0.1 * hbm : hbm + 0.1 * t) + lds);
+}
+
+/* 16-byte pieces of the weights' rows (FP8 16 codes, BF16 8 values), 32-bit
+ * offsets inside a wave's rows */
+extern "C" int ghip_ffn_rows_fits(int mode, const GhipProd *p) {
+    return (mode == GHIP_EP_LINEAR || mode == GHIP_EP_GATED) && p->aks == 1 && p->bks == 1
+        && p->brs == p->K && p->K % (p->s ? 16 : 8) == 0 && p->K <= (1u << 24) && p->ars % 8 == 0
+        && p->ars <= (1u << 24) && p->M <= 0x7fffffffu && p->N <= 0x7fffffffu
+        && (((uintptr_t)p->a | (uintptr_t)p->b | (uintptr_t)p->b2) & 15) == 0;
+}
+
+extern "C" int ghip_ffn_rows_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us) {
+    int n, best = 0;
+    const FrForm *t = fr_forms(mode, p->s != nullptr, &n);
+    for (int i = 0; i < n; i++) {
+        const float e = fr_estimate(t[i], p, ghip_ep_dual(mode), n_cu);
+        if (i == 0 || e < *us) {
+            best = i;
+            *us = e;
+        }
+    }
+    return best;
+}
+
+extern "C" hipError_t ghip_launch_ffn_rows(int mode, int form, const GhipProd *p,
+                                           const GhipEp *ep, hipStream_t st) {
+    int n;
+    const FrForm *c = fr_forms(mode, p->s != nullptr, &n);
+    if (!ghip_ffn_rows_fits(mode, p) || form < 0 || form >= n || p->M == 0 || p->N == 0 || p->K == 0)
+        return hipErrorInvalidValue;
+    c += form;
+    const size_t cols = (ghip_ep_dual(mode) ? 8u : 16u) * c->nt * (RW_NW / c->ks);
+    const size_t blocks = (p->N + cols - 1) / cols, tiles = ((size_t)p->M + c->mr - 1) / c->mr;
+    for (size_t t0 = 0; t0 < tiles; t0 += FR_MAX_TILES)
+        for (size_t b0 = 0; b0 < blocks; b0 += FR_MAX_BLOCKS) {
+            const size_t nt = tiles - t0 < FR_MAX_TILES ? tiles - t0 : FR_MAX_TILES;
+            const size_t nb = blocks - b0 < FR_MAX_BLOCKS ? blocks - b0 : FR_MAX_BLOCKS;
+            c->launch(dim3((uint32_t)nb, (uint32_t)nt), c->lds, st, *p, *ep, (uint32_t)b0,
+                      (uint32_t)t0);
+            const hipError_t e = hipGetLastError();
+            if (e != hipSuccess) return e;
+        }
+    return hipSuccess;
+}
+
+extern "C" hipError_t ghip_ffn_rows_init(void) {
+    for (int i = 0; i < 4; i++) {
+        int n;
+        const FrForm *t = fr_forms(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i >> 1, &n);
+        for (int k = 0; k < n; k++) {
+            const hipError_t e = hipFuncSetAttribute(
+                t[k].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)t[k].lds);
+            if (e != hipSuccess) return e;
+        }
+    }
+    return hipSuccess;
+}
