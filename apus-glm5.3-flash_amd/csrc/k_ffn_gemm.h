@@ -53,6 +53,17 @@ __device__ __forceinline__ void fg_dma16(const void *base, uint32_t off, void *l
     __builtin_amdgcn_raw_ptr_buffer_load_lds(fg_buf(base), (ghip_lds_t *)lds_wave, 16, off, 0, 0, 0);
 }
 
+/* 4 k x 16 rows of a layout-1 stage, transposed inside 16 lanes: lane i gives
+ * the address of 4 values of k row i / 4 and gets the 4 k of row i. The
+ * restrict keeps the compiler from waiting for every load to LDS in flight
+ * before each of these reads, as it does for a pointer it knows nothing of (dx
+ * of 1024 x 4096 x 4096: 52 -> 38 us); the stages' own waits and barriers order
+ * the two. */
+typedef __attribute__((address_space(3))) fg_s16x4 fg_lds_s16x4;
+__device__ __forceinline__ fg_s16x4 fg_read_tr(fg_lds_s16x4 *__restrict p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+}
+
 /* Layout 1: what the 32-byte slots of k's row of W values are XORed with, so that
  * the 4 k x 32 rows a half wave reads lie in distinct banks. */
 template <uint32_t W>
@@ -274,12 +285,11 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void k_ffn_gemm(GhipProd p, GhipEp 
         if constexpr (decltype(layout_c)::value == 0) {
             return *(const ghip_bf16x8 *)(st + blk * 4096u + off0[s]);
         } else {
-            typedef __attribute__((address_space(3))) fg_s16x4 lds_s16x4;
             const uint32_t k = 32u * h + 8u * (uint32_t)s + (i16 >> 2);
             const uint32_t slot = (2u * blk + c16) ^ fg_swizzle<W>(k);
             const uint8_t *q = st + k * (2u * W) + slot * 32u + (i16 & 3u) * 8u;
-            const fg_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)q);
-            const fg_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(q + 8u * W));
+            const fg_s16x4 lo = fg_read_tr((fg_lds_s16x4 *)q);
+            const fg_s16x4 hi = fg_read_tr((fg_lds_s16x4 *)(q + 8u * W));
             return __builtin_bit_cast(ghip_bf16x8,
                                       __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }

@@ -9,10 +9,11 @@
 #define FR_MAX_BLOCKS (GHIP_MAX_THREADS / (RW_NW * 64))
 
 /* One launchable form: MR rows of x, NT weight groups of 16 a wave, K over KS
- * waves. chunk: measured microseconds of a wave's chunk step. */
+ * waves. chunk, over: microseconds of a wave's chunk step, and of a round's
+ * first loads and reduction. */
 struct FrForm {
     uint32_t mr, nt, ks;
-    float chunk;
+    float chunk, over;
     const void *kern;
     uint32_t lds;
     void (*launch)(dim3, uint32_t, hipStream_t, const GhipProd &, const GhipEp &, uint32_t, uint32_t);
@@ -27,38 +28,60 @@ static void fr_run(dim3 grid, uint32_t lds, hipStream_t st, const GhipProd &p, c
                        more);
 }
 
-#define FR_FORM(BF, MR, NT, KS, NA, SL, MODE, T)                                            \
-    {MR, NT, KS, T, (const void *)k_rows_gemm<BF, MR, NT, KS, NA, SL, MODE>,                  \
+#define FR_FORM(BF, MR, NT, KS, NA, SL, MODE, T, V)                                         \
+    {MR, NT, KS, T, V, (const void *)k_rows_gemm<BF, MR, NT, KS, NA, SL, MODE>,               \
      rw_lds<BF, MR, NT, SL>(), fr_run<BF, MR, NT, KS, NA, SL, MODE>}
 
-#define FR_L(BF, MR, NT, KS, NA, SL, T) FR_FORM(BF, MR, NT, KS, NA, SL, GHIP_EP_LINEAR, T)
+/* The times are fitted to a sweep of every form over M = 1..80, N x K from 1536
+ * x 1536 to 12288 x 4096 and 4096 x 12288 on 256 CUs, operands from HBM; the
+ * form picked by them took 1% longer than the best one on average, 15% at most.
+ * Chunks in flight (NA) and slots (SL) are the plain linear's (k_rows.hip). */
+#define FR_L(BF, MR, NT, KS, NA, SL, T, V) FR_FORM(BF, MR, NT, KS, NA, SL, GHIP_EP_LINEAR, T, V)
 static const FrForm fr_linear8[] = {
-    FR_L(false, 4, 1, 8, 2, 2, 0.55f),  FR_L(false, 4, 1, 4, 2, 2, 0.55f),
-    FR_L(false, 4, 1, 2, 2, 2, 0.56f),  FR_L(false, 8, 1, 8, 2, 2, 0.65f),
-    FR_L(false, 8, 1, 4, 2, 2, 0.65f),  FR_L(false, 8, 1, 2, 2, 2, 0.62f),
-    FR_L(false, 16, 1, 8, 1, 1, 0.85f), FR_L(false, 16, 2, 8, 2, 2, 1.30f),
-    FR_L(false, 16, 2, 4, 2, 2, 1.30f), FR_L(false, 32, 1, 8, 1, 1, 1.30f),
-    FR_L(false, 32, 2, 8, 1, 1, 1.70f), FR_L(false, 32, 2, 4, 1, 1, 1.70f),
-    FR_L(false, 64, 2, 4, 1, 1, 2.20f),
+    FR_L(false, 4, 1, 8, 2, 2, 0.60f, 0.11f),
+    FR_L(false, 4, 1, 4, 2, 2, 0.49f, 0.29f),
+    FR_L(false, 4, 1, 2, 2, 2, 0.44f, 0.37f),
+    FR_L(false, 8, 1, 8, 2, 2, 0.70f, 0.60f),
+    FR_L(false, 8, 1, 4, 2, 2, 0.59f, 0.69f),
+    FR_L(false, 8, 1, 2, 2, 2, 0.51f, 0.72f),
+    FR_L(false, 16, 1, 8, 1, 1, 0.84f, 0.10f),
+    FR_L(false, 16, 2, 8, 2, 2, 1.26f, 0.62f),
+    FR_L(false, 16, 2, 4, 2, 2, 1.06f, 1.36f),
+    FR_L(false, 32, 1, 8, 1, 1, 1.11f, 0.57f),
+    FR_L(false, 32, 2, 8, 1, 1, 1.42f, 0.81f),
+    FR_L(false, 32, 2, 4, 1, 1, 1.30f, 1.35f),
+    FR_L(false, 64, 2, 4, 1, 1, 1.90f, 3.13f),
 };
 static const FrForm fr_linear16[] = {
-    FR_L(true, 8, 1, 8, 2, 2, 0.50f),  FR_L(true, 8, 1, 4, 2, 2, 0.50f),
-    FR_L(true, 16, 1, 8, 2, 2, 0.58f), FR_L(true, 16, 1, 4, 2, 2, 0.60f),
-    FR_L(true, 16, 2, 4, 2, 2, 0.75f), FR_L(true, 32, 1, 8, 1, 1, 0.85f),
-    FR_L(true, 32, 2, 8, 1, 1, 1.20f), FR_L(true, 32, 2, 4, 1, 1, 1.15f),
+    FR_L(true, 8, 1, 8, 2, 2, 0.54f, 0.00f),
+    FR_L(true, 8, 1, 4, 2, 2, 0.45f, 0.00f),
+    FR_L(true, 16, 1, 8, 2, 2, 0.61f, 0.00f),
+    FR_L(true, 16, 1, 4, 2, 2, 0.52f, 0.00f),
+    FR_L(true, 16, 2, 4, 2, 2, 0.82f, 0.03f),
+    FR_L(true, 32, 1, 8, 1, 1, 0.74f, 0.23f),
+    FR_L(true, 32, 2, 8, 1, 1, 1.03f, 0.21f),
+    FR_L(true, 32, 2, 4, 1, 1, 0.94f, 0.36f),
 };
-#define FR_G(BF, MR, NT, KS, NA, SL, T) FR_FORM(BF, MR, NT, KS, NA, SL, GHIP_EP_GATED, T)
+#define FR_G(BF, MR, NT, KS, NA, SL, T, V) FR_FORM(BF, MR, NT, KS, NA, SL, GHIP_EP_GATED, T, V)
 static const FrForm fr_gated8[] = {
-    FR_G(false, 4, 2, 8, 2, 2, 0.70f),  FR_G(false, 4, 2, 4, 2, 2, 0.70f),
-    FR_G(false, 4, 2, 2, 2, 2, 0.70f),  FR_G(false, 8, 2, 8, 2, 2, 0.85f),
-    FR_G(false, 8, 2, 4, 2, 2, 0.85f),  FR_G(false, 16, 2, 8, 2, 2, 1.30f),
-    FR_G(false, 16, 2, 4, 2, 2, 1.30f), FR_G(false, 32, 2, 8, 1, 1, 1.70f),
-    FR_G(false, 32, 2, 4, 1, 1, 1.70f), FR_G(false, 64, 2, 4, 1, 1, 2.20f),
+    FR_G(false, 4, 2, 8, 2, 2, 1.25f, 0.44f),
+    FR_G(false, 4, 2, 4, 2, 2, 0.99f, 0.69f),
+    FR_G(false, 4, 2, 2, 2, 2, 0.86f, 0.72f),
+    FR_G(false, 8, 2, 8, 2, 2, 1.32f, 0.70f),
+    FR_G(false, 8, 2, 4, 2, 2, 1.05f, 0.99f),
+    FR_G(false, 16, 2, 8, 2, 2, 1.46f, 0.39f),
+    FR_G(false, 16, 2, 4, 2, 2, 1.15f, 1.01f),
+    FR_G(false, 32, 2, 8, 1, 1, 1.57f, 0.74f),
+    FR_G(false, 32, 2, 4, 1, 1, 1.35f, 1.12f),
+    FR_G(false, 64, 2, 4, 1, 1, 1.94f, 2.52f),
 };
 static const FrForm fr_gated16[] = {
-    FR_G(true, 8, 2, 8, 2, 2, 0.65f),  FR_G(true, 8, 2, 4, 2, 2, 0.65f),
-    FR_G(true, 16, 2, 8, 2, 2, 0.75f), FR_G(true, 16, 2, 4, 2, 2, 0.75f),
-    FR_G(true, 32, 2, 8, 1, 1, 1.20f), FR_G(true, 32, 2, 4, 1, 1, 1.15f),
+    FR_G(true, 8, 2, 8, 2, 2, 0.97f, 0.00f),
+    FR_G(true, 8, 2, 4, 2, 2, 0.81f, 0.00f),
+    FR_G(true, 16, 2, 8, 2, 2, 1.08f, 0.00f),
+    FR_G(true, 16, 2, 4, 2, 2, 0.87f, 0.00f),
+    FR_G(true, 32, 2, 8, 1, 1, 1.12f, 0.00f),
+    FR_G(true, 32, 2, 4, 1, 1, 0.99f, 0.00f),
 };
 
 static const FrForm *fr_forms(int mode, bool fp8, int *n) {
@@ -68,9 +91,10 @@ static const FrForm *fr_forms(int mode, bool fp8, int *n) {
 #undef FR_TABLE
 }
 
-/* Estimated microseconds of a form, as of the plain linear's (k_rows.hip): the
- * larger of rounds of the chip x a wave's chunks x the chunk time and the
- * weights at 6.5 TB/s, + a tenth of the other. */
+/* Estimated microseconds of a form: 2.3 + the larger of its rounds of the chip
+ * and the weights at 6.5 TB/s + a tenth of the other (within 10-15% rms of the
+ * sweep). Forms of 4 and 8 rows only take as many: more row tiles would re-read
+ * the weights. */
 static float fr_estimate(const FrForm &c, const GhipProd *p, bool dual, uint32_t n_cu) {
     if (c.mr < 16 && p->M > c.mr) return 1e30f;
     const double cols = (dual ? 8.0 : 16.0) * c.nt * (RW_NW / c.ks);
@@ -79,11 +103,8 @@ static float fr_estimate(const FrForm &c, const GhipProd *p, bool dual, uint32_t
     const double rounds = (double)(size_t)((wgs + n_cu - 1) / n_cu);
     const double nc = (double)(size_t)((nch + c.ks - 1) / c.ks);
     const double hbm = (double)p->N * kb * (dual ? 2 : 1) / 6.5e6;
-    const double over = c.mr > 32 ? 3.8 * rounds
-                        : p->s && c.mr * c.nt >= 32 && nc < 8.0 ? 2.0 * (rounds - 1.0) : 0.0;
-    const double t = rounds * nc * c.chunk + over;
-    const double lds = t < hbm ? 0.0015 * hbm * c.mr * c.nt : 0.0;
-    return (float)(2.3 + (t > hbm ? t + 0.1 * hbm : hbm + 0.1 * t) + lds);
+    const double t = rounds * (nc * c.chunk + c.over);
+    return (float)(2.3 + (t > hbm ? t + 0.1 * hbm : hbm + 0.1 * t));
 }
 
 /* 16-byte pieces of the weights' rows (FP8 16 codes, BF16 8 values), 32-bit
