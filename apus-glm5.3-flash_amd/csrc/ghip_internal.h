@@ -315,7 +315,8 @@ typedef struct {
     const void *kern;
     void (*launch)(const GhipProd *, const GhipEp *, uint32_t, uint32_t, uint32_t, hipStream_t);
 } GhipFfnTile;
-const GhipFfnTile *ghip_ffn_forward_tiles(int mode, int fp8, int *n);
+/* w8: 0 bf16 weights, 1 FP8, 2 FP8 with NaN codes */
+const GhipFfnTile *ghip_ffn_forward_tiles(int mode, int w8, int *n);
 const GhipFfnTile *ghip_ffn_backward_tiles(int mode, int transposed, int *n);
 
 /* Streaming the weights past a few rows (k_rows_gemm.h), forward modes. */

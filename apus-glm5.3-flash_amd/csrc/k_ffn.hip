@@ -7,7 +7,7 @@ static uint32_t g_ffn_ncu;                       /* CUs: the routes' rounds */
 
 static const GhipFfnTile *tiles_of(int mode, const GhipProd *p, int *n) {
     return mode == GHIP_EP_LINEAR || mode == GHIP_EP_GATED
-               ? ghip_ffn_forward_tiles(mode, p->s != nullptr, n)
+               ? ghip_ffn_forward_tiles(mode, p->s ? p->exact ? 2 : 1 : 0, n)
                : ghip_ffn_backward_tiles(mode, p->aks != 1, n);
 }
 
@@ -74,11 +74,11 @@ extern "C" hipError_t ghip_launch_ffn(int mode, const GhipProd *p, const GhipEp 
 }
 
 extern "C" hipError_t ghip_ffn_init(uint32_t n_cu) {
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < 10; i++) {
         static const int bwd[4][2] = {{GHIP_EP_DLINEAR, 0}, {GHIP_EP_DGATED, 0}, {GHIP_EP_STORE, 0}, {GHIP_EP_STORE, 1}};
         int n;
-        const GhipFfnTile *t = i < 4 ? ghip_ffn_forward_tiles(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i >> 1, &n)
-                                     : ghip_ffn_backward_tiles(bwd[i - 4][0], bwd[i - 4][1], &n);
+        const GhipFfnTile *t = i < 6 ? ghip_ffn_forward_tiles(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i >> 1, &n)
+                                     : ghip_ffn_backward_tiles(bwd[i - 6][0], bwd[i - 6][1], &n);
         for (int k = 0; k < n; k++) {
             const hipError_t e = hipFuncSetAttribute(
                 t[k].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)t[k].lds);

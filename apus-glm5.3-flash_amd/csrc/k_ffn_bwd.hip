@@ -8,8 +8,9 @@
 template <int MODE>
 static const GhipFfnTile *dz_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<MODE, false, 0, 0, 2, 4, 4, 2>(1.60f), fg_tile<MODE, false, 0, 0, 2, 2, 2, 4>(0.55f),
-        fg_tile<MODE, false, 0, 0, 2, 2, 1, 5>(0.40f),
+        fg_tile<MODE, 0, 0, 0, 8, 8, 2>(1.50f), fg_tile<MODE, 0, 0, 0, 8, 4, 2>(0.90f),
+        fg_tile<MODE, 0, 0, 0, 4, 4, 4>(0.55f), fg_tile<MODE, 0, 0, 0, 2, 4, 5>(0.40f),
+        fg_tile<MODE, 0, 0, 0, 2, 2, 6>(0.30f),
     };
     *n = sizeof t / sizeof *t;
     return t;
@@ -18,9 +19,9 @@ static const GhipFfnTile *dz_tiles(int *n) {
 template <int AL>
 static const GhipFfnTile *grad_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_STORE, false, AL, 1, 2, 4, 4, 2>(1.80f),
-        fg_tile<GHIP_EP_STORE, false, AL, 1, 2, 2, 2, 4>(0.62f),
-        fg_tile<GHIP_EP_STORE, false, AL, 1, 2, 2, 1, 5>(0.45f),
+        fg_tile<GHIP_EP_STORE, 0, AL, 1, 8, 8, 2>(1.50f), fg_tile<GHIP_EP_STORE, 0, AL, 1, 8, 4, 2>(0.90f),
+        fg_tile<GHIP_EP_STORE, 0, AL, 1, 4, 4, 4>(0.55f), fg_tile<GHIP_EP_STORE, 0, AL, 1, 2, 4, 5>(0.40f),
+        fg_tile<GHIP_EP_STORE, 0, AL, 1, 2, 2, 6>(0.30f),
     };
     *n = sizeof t / sizeof *t;
     return t;

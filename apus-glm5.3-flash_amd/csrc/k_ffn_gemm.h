@@ -1,56 +1,93 @@
 /*
  * k_ffn_gemm.h — the tiled MFMA product of the dense feed-forward operators
  * (gfx950): out[m, n] = epilogue(sum_k A(m, k) B(n, k)); instantiated by
- * k_ffn_nt.hip (forward), k_ffn_nn.hip (dx) and k_ffn_tn.hip (dW).
+ * k_ffn_nt.hip (forward) and k_ffn_bwd.hip (backward).
  *
- * A workgroup of WM x WN waves owns 32 RB WM rows (of A) x 64 WN rows of B;
- * wave (wr, wc) computes 32 RB x 64 outputs with v_mfma_f32_32x32x16_bf16, B
- * as the A operand of the instruction, so a lane ends with four consecutive
- * columns of one output row. k is walked in stages of 64 through a ring of NS
- * stages in LDS.
+ * A workgroup of 4 waves owns 32 RB rows of A x 32 CB rows of B; wave (wr, wc)
+ * computes 16 RB x 16 CB outputs with v_mfma_f32_16x16x32_bf16, B as the A
+ * operand of the instruction, so a lane ends with four consecutive columns of
+ * one output row. k is walked in stages of 64, two MFMA steps each.
+ *
+ * What bounds it, and what follows. A full chip of these products is at its
+ * power limit (4096 x 4096 x 4096 of zeros runs at 1800 TFLOP/s, of normal
+ * values at 1430), so what costs energy or idles counts:
+ *   - 16x16x32 MFMAs, which move half the accumulators of 32x32x16 a product
+ *     (1180 -> 1290), walked in a snake so that one operand stays (+2%);
+ *   - accumulators of the largest tile fill all 256 AGPRs; the MFMAs are inline
+ *     asm that updates them in place, which the compiler's register allocation
+ *     does not keep (it moved half of them every stage: 1116);
+ *   - 128 x 128 outputs a wave, the least LDS reads a product; one wave a SIMD,
+ *     whose order of MFMAs, operand reads and loads is written out (evenly
+ *     spread loads: +4%; in a burst after the barrier they block the issue);
+ *   - loads go straight to LDS and are issued L stages ahead: A's in the first
+ *     step (a ring of L + 1 slots), B's after the stage's one barrier, which
+ *     frees their slot (a ring of L). L = 2 with the largest tile fills the
+ *     160 KB (one stage ahead: 1380 against 1505 at 4096 x 4096 x 12288, from
+ *     HBM).
  *
  * Operand layouts. 0: k is the fast index in memory (x, W in the forward). The
  * stage is [row][64 k], whole 128-byte lines, 16-byte piece p of row r at p ^
  * ((r >> 1) & 7); an operand of 8 k values is one ds_read_b128. 1: the row is
- * (W in dx, dz and x in dW). The stage is [64 k][rows], 32-byte slot s of k at
- * s ^ 2 (k & 3), and an operand is two ds_read_b64_tr_b16: each transposes 4 k
- * x 16 rows inside 16 lanes, so no transposed copy of a matrix is made. In
- * both, lane half h of MFMA step s takes k = 32 h + 8 s + [0, 8), so either
- * layout may meet the other. (Rows of 64 values: slot s at s ^ 2 ((k >> 1) & 1).)
+ * (W in dx, dz and x in dW). The stage is [64 k][rows], 32-byte slots XORed
+ * with k (fg_swizzle), and an operand is two ds_read_b64_tr_b16: each
+ * transposes 4 k x 16 rows inside 16 lanes, so no transposed copy of a matrix
+ * is made. In both, lane group g of MFMA step s takes k = 16 g + 8 s + [0, 8),
+ * so either layout may meet the other. No read has bank conflicts.
  *
- * Loads go straight to LDS (buffer loads, 16 bytes a lane). Rows past the
- * matrix and k past its end are given an offset outside the buffer, which
- * loads zeros: no other row is read in their place and a ragged K needs no
- * separate kernel. FP8 weights go through registers instead: 16 codes a load,
- * dequantized bit-exactly while the products of the stage before run, and
- * written in the same layout.
+ * Rows past the matrix and k past its end are given an offset outside the
+ * buffer, which loads zeros: no other row is read in their place and a ragged
+ * K needs no separate kernel.
  *
- * Dual modes (gate and up): the tile's B rows alternate in blocks of 32 between
- * the two matrices, so a wave holds g and u of the same 32 columns and the
- * product of the two needs no exchange.
+ * FP8 weights lie in LDS as codes, [row][64 codes], 16-byte piece p of row r at
+ * p ^ ((r >> 2) & 3): one read gives the 16 codes of both steps, which are
+ * dequantized bit-exactly in registers between the MFMAs of the step before
+ * (both waves of a column do so; against dequantizing once and writing bf16
+ * back to LDS it takes half the loads and writes).
  *
- * The epilogue passes the sums through a wave-private piece of the ring 32 rows
+ * Dual modes (gate and up): the tile's B rows alternate in blocks of 16 between
+ * the two matrices, so a lane holds g and u of the same columns and the product
+ * of the two needs no exchange.
+ *
+ * The epilogue passes the sums through a wave-private piece of the ring 16 rows
  * at a time, so that bias, residual and output are 16-byte accesses along a
  * row.
  */
 #ifndef K_FFN_GEMM_H
 #define K_FFN_GEMM_H
 
+#include <utility>
+
 #include "ghip_epilogue.h"
 
-typedef float fg_f32x16 __attribute__((ext_vector_type(16)));
 typedef short fg_s16x4 __attribute__((ext_vector_type(4)));
-typedef short fg_s16x8 __attribute__((ext_vector_type(8)));
 
 #define FG_LDS_MAX (160u * 1024u)
 #define FG_OOB 0xFFFFFFF0u                       /* past every buffer: loads zeros */
 #define FG_SPAN 0x80000000u                      /* valid offsets are below */
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t fg_buf(const void *p) {
-    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, FG_SPAN, 0x20000);
+__device__ __forceinline__ void fg_dma16(const void *base, uint32_t span, uint32_t off,
+                                         void *lds_wave) {
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, span, 0x20000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (ghip_lds_t *)lds_wave, 16, off, 0, 0, 0);
 }
-__device__ __forceinline__ void fg_dma16(const void *base, uint32_t off, void *lds_wave) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(fg_buf(base), (ghip_lds_t *)lds_wave, 16, off, 0, 0, 0);
+
+/* acc += b . a, in place. The compiler knows no MFMA in it: operands are
+ * written (by LDS reads or VALU) at least two instructions ahead, which
+ * tests/test_ffn_asm.py checks in the built code, and sums are read after
+ * fg_settle. */
+__device__ __forceinline__ void fg_mfma(ghip_f32x4 &acc, const ghip_bf16x8 &b,
+                                        const ghip_bf16x8 &a) {
+    asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(b), "v"(a));
+}
+/* The last MFMAs have written their sums (32 wait states; they need 4 passes). */
+template <int R, int C>
+__device__ __forceinline__ void fg_settle(ghip_f32x4 (&acc)[R][C]) {
+    asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[R - 1][C - 1]));
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int c = 0; c < C; c++) asm volatile("" : "+a"(acc[r][c]));
 }
 
 /* 4 k x 16 rows of a layout-1 stage, transposed inside 16 lanes: lane i gives
@@ -64,12 +101,26 @@ __device__ __forceinline__ fg_s16x4 fg_read_tr(fg_lds_s16x4 *__restrict p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
 }
 
-/* Layout 1: what the 32-byte slots of k's row of W values are XORed with, so that
- * the 4 k x 32 rows a half wave reads lie in distinct banks. */
+/* Layout 1: what the 32-byte slots of k's row of W values are XORed with, so
+ * that the 8 k rows two lane groups read from one slot lie in distinct banks. */
 template <uint32_t W>
 __device__ __forceinline__ uint32_t fg_swizzle(uint32_t k) {
-    static_assert(W == 64 || W == 128 || W == 256, "whole rounds of the banks");
-    return W == 64 ? k & 2u : (k & 3u) << 1;
+    static_assert(W % 64u == 0, "half rounds of the banks");
+    return W % 128u ? ((k >> 1) & 1u) | ((k >> 3) & 2u) : ((k & 3u) << 1) | ((k >> 4) & 1u);
+}
+
+/* f(0), f(1), ... f(N - 1), the argument a constant */
+template <typename F, int... I>
+__device__ __forceinline__ void fg_each_of(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void fg_each(F f) {
+    fg_each_of(f, std::make_integer_sequence<int, N>{});
+}
+/* Of n things spread over slots [from, to): how many come in slots before i. */
+constexpr int fg_spread(int n, int i, int from, int to) {
+    return i <= from ? 0 : i >= to ? n : (n * (i - from) + (to - from) - 1) / (to - from);
 }
 
 /* 8 outputs of row m from column n0 on: s0 (and s1) their sums. */
@@ -120,28 +171,31 @@ __device__ __forceinline__ void fg_store8(const GhipEp &ep, uint16_t *out, uint3
     if constexpr (MODE == GHIP_EP_DGATED) store(ep.out2 + (size_t)m * ep.ldout + n0, o1);
 }
 
-template <int MODE, bool FP8, int AL, int BL, int WM, int WN, int RB, int NS>
-__global__ __launch_bounds__(WM *WN * 64, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint32_t mt,
-                                                              uint32_t nt) {
-    constexpr bool DUAL = ghip_ep_dual(MODE);
-    constexpr uint32_t CB = 2, NW = WM * WN, BM = 32u * RB * WM, BN = 64u * WN;
+/* W8: 0 bf16 weights, 1 FP8 codes, 2 FP8 codes with NaN codes among them */
+template <int MODE, int W8, int AL, int BL, int RB, int CB, int L>
+__global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint32_t mt,
+                                                     uint32_t nt) {
+    constexpr bool DUAL = ghip_ep_dual(MODE), FP8 = W8 != 0;
+    constexpr uint32_t BM = 32u * RB, BN = 32u * CB;
     constexpr uint32_t OUTN = DUAL ? BN / 2 : BN;        /* output columns of a tile */
-    constexpr uint32_t ASTG = BM * 128u, STG = (BM + BN) * 128u;
-    constexpr uint32_t NAL = BM / 8u / NW, NBL = FP8 ? 0 : BN / 8u / NW, LPS = NAL + NBL;
-    constexpr uint32_t NC = FP8 ? BN / 16u / NW : 1u;    /* code loads of a lane a stage */
-    static_assert(NAL * NW * 8u == BM && BN / 8u % NW == 0 && BN / 16u % NW == 0, "loads");
-    static_assert(NS * STG <= FG_LDS_MAX && NS >= 2 && LPS * (NS - 1) <= 63, "ring");
-    static_assert(NS * STG / NW >= 8192u, "epilogue staging");
-    static_assert(!FP8 || (NS == 2 && BL == 0), "codes are staged through two slots");
+    constexpr uint32_t AST = BM * 128u, BST = BN * (FP8 ? 64u : 128u);  /* slot bytes */
+    constexpr uint32_t NAL = RB, NBL = FP8 ? CB / 2 : CB, LPS = NAL + NBL;
+    constexpr uint32_t RING = (L + 1u) * AST + L * BST;
+    constexpr int NM = RB * CB;                          /* MFMAs of a step */
+    static_assert(RING <= FG_LDS_MAX && RING >= 4u * 1024u * CB, "ring, epilogue staging");
+    static_assert(L >= 2 && (L - 1) * NAL + (L - 2) * NBL <= 63 && (L - 1) * LPS <= 63, "waits");
+    static_assert(CB % 2 == 0 && (!FP8 || (BL == 0 && 128 % (16 * CB) == 0)), "columns");
     extern __shared__ __attribute__((aligned(1024))) uint8_t fg_lds[];
+    uint8_t *bring = fg_lds + (L + 1u) * AST;
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t wr = wv / WN, wc = wv % WN, n = lane & 31u, h = lane >> 5;
+    const uint32_t wr = wv >> 1, wc = wv & 1u, n = lane & 15u, g = lane >> 4;
 
     /* tile t: the workgroups of one XCD (b % 8) take a run of consecutive
-     * tiles, which go down 8 row tiles before the next column, so that an XCD's
-     * L2 holds few rows of A and of B at a time. A batch of two: the second
-     * half of the tiles is the second product. */
+     * tiles, which go down 4 row tiles before the next column, so that an XCD's
+     * L2 holds few rows of A and of B at a time (8192 x 24576 x 4096: 4 1.148
+     * ms, 8 1.157, 16 1.18). A batch of two: the second half of the tiles is the
+     * second product. */
     uint32_t t;
     {
         const uint32_t T = gridDim.x, x = blockIdx.x & 7u, i = blockIdx.x >> 3;
@@ -153,14 +207,19 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void k_ffn_gemm(GhipProd p, GhipEp 
         second = p.batch && t >= mt * nt;
         if (second) t -= mt * nt;
     }
-    const uint32_t strip = t / (8u * nt), in_strip = t - strip * (8u * nt);
-    const uint32_t sr = min(8u, mt - strip * 8u);
-    const uint32_t row0 = (strip * 8u + in_strip % sr) * BM, col0 = in_strip / sr * OUTN;
+    const uint32_t strip = t / (4u * nt), in_strip = t - strip * (4u * nt);
+    const uint32_t sr = min(4u, mt - strip * 4u);
+    const uint32_t row0 = (strip * 4u + in_strip % sr) * BM, col0 = in_strip / sr * OUTN;
     const uint32_t rows = min(p.M - row0, BM), cols = min(p.N - col0, OUTN);
     const uint32_t nst1 = (p.K + 63u) >> 6;              /* stages of one product */
     const uint32_t nst = MODE == GHIP_EP_STORE && p.a2 && !p.batch ? 2u * nst1 : nst1;
     const size_t astep = AL == 0 ? 128u : (size_t)p.aks * 128u;
     const size_t bstep = BL == 0 ? (FP8 ? 64u : 128u) : (size_t)p.bks * 128u;
+    const uint32_t lda = (uint32_t)(AL == 0 ? p.ars : p.aks);
+    const uint32_t ldb = (uint32_t)(BL == 0 ? p.brs : p.bks);
+    /* dual modes: this wave's loads are all of one matrix (16-row blocks of B
+     * rows alternate, and a wave's lie an even number of blocks apart) */
+    const bool up = DUAL && (FP8 ? wv & 1u : wv >> 1);
     auto base_a = [&](const uint16_t *a) {
         return (const uint8_t *)(a + (AL == 0 ? (size_t)row0 * p.ars : row0));
     };
@@ -168,24 +227,24 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void k_ffn_gemm(GhipProd p, GhipEp 
         return (const uint8_t *)b
                + (BL == 0 ? (size_t)col0 * p.brs : col0) * (FP8 ? (size_t)1 : (size_t)2);
     };
-    const uint8_t *a0 = base_a(second ? p.a2 : p.a), *b0 = base_b(second ? p.b2 : p.b);
-    const uint8_t *a1 = nst > nst1 ? base_a(p.a2) : a0;
-    const uint8_t *b1 = DUAL || nst > nst1 ? base_b(p.b2) : b0;
+    /* the next stage to load: its address, number and slots */
+    const uint8_t *pa = base_a(second ? p.a2 : p.a), *pb = base_b(second || up ? p.b2 : p.b);
+    uint32_t ja = 0, jb = 0, sa = 0, sb = 0;
 
-    /* Byte offset of this lane's 16 bytes of 1 KB load c in a stage of W rows,
-     * `live` of them inside the matrix; kq: the k (layout 0: of the piece) it
-     * holds. The load's lane l goes to byte 16 l of the KB. */
+    /* Byte offset of this lane's 16 bytes of 1 KB load c in a stage, the load's
+     * lane l going to byte 16 l of the KB; past the matrix: FG_OOB. kq: the
+     * stage's k that the piece starts at (layout 0) */
+    uint32_t ao[NAL], bo[NBL], akq = 0, bkq = 0;
     auto place = [&](auto layout_c, auto w_c, uint32_t c, uint32_t live, uint32_t ld,
                      uint32_t &kq) -> uint32_t {
         constexpr uint32_t W = decltype(w_c)::value;
         if constexpr (decltype(layout_c)::value == 0) {
             const uint32_t r = 8u * c + (lane >> 3), q = (lane & 7u) ^ ((r >> 1) & 7u);
-            kq = 8u * q;
+            kq = 8u * q;                                 /* the same for every c of a wave */
             return r < live ? r * ld * 2u + 16u * q : FG_OOB;
         } else {
-            const uint32_t e = c * 64u + lane, k = e / (W / 8u);
-            const uint32_t q = e % (W / 8u) ^ 2u * fg_swizzle<W>(k);
-            kq = k;
+            const uint32_t e = c * 64u + lane, k = e / (W / 8u), s = e % (W / 8u);
+            const uint32_t q = s ^ 2u * fg_swizzle<W>(k);
             return 8u * q < live ? k * ld * 2u + 16u * q : FG_OOB;
         }
     };
@@ -193,250 +252,242 @@ __global__ __launch_bounds__(WM *WN * 64, 1) void k_ffn_gemm(GhipProd p, GhipEp 
     using LB = std::integral_constant<int, BL>;
     using WA = std::integral_constant<uint32_t, BM>;
     using WB = std::integral_constant<uint32_t, BN>;
-    const uint32_t lda = (uint32_t)(AL == 0 ? p.ars : p.aks);
-    const uint32_t ldb = (uint32_t)(BL == 0 ? p.brs : p.bks);
-    /* B row r of the tile: in the dual modes row 32 (r / 64) + r % 32 of the
-     * gate (even blocks of 32) or up matrix */
-    uint32_t ao[NAL], ak[NAL], bo[NBL ? NBL : 1], bk[NBL ? NBL : 1];
 #pragma unroll
-    for (uint32_t i = 0; i < NAL; i++) ao[i] = place(LA{}, WA{}, wv + NW * i, rows, lda, ak[i]);
-    if constexpr (!FP8) {
+    for (uint32_t i = 0; i < NAL; i++) ao[i] = place(LA{}, WA{}, wv + 4u * i, rows, lda, akq);
 #pragma unroll
-        for (uint32_t i = 0; i < NBL; i++) {
-            const uint32_t c = wv + NW * i;
-            bo[i] = place(LB{}, WB{}, c, DUAL ? BN : cols, ldb, bk[i]);
+    for (uint32_t i = 0; i < NBL; i++) {
+        if constexpr (FP8) {                             /* 16 rows of 64 codes */
+            const uint32_t b = wv + 4u * i, r = lane >> 2, q = (lane & 3u) ^ ((r >> 2) & 3u);
+            const uint32_t mr = 16u * (DUAL ? b >> 1 : b) + r;
+            bkq = 16u * q;
+            bo[i] = mr < cols ? mr * ldb + 16u * q : FG_OOB;
+        } else {
+            const uint32_t c = wv + 4u * i;
             if constexpr (DUAL) {
-                const uint32_t r = 8u * c + (lane >> 3), mr = 32u * (r >> 6) + (r & 31u);
-                bo[i] = mr < cols ? bo[i] - (r - mr) * ldb * 2u : FG_OOB;
+                const uint32_t r = 8u * c + (lane >> 3), q = (lane & 7u) ^ ((r >> 1) & 7u);
+                const uint32_t mr = 16u * (r >> 5) + (r & 15u);
+                bkq = 8u * q;
+                bo[i] = mr < cols ? mr * ldb * 2u + 16u * q : FG_OOB;
+            } else {
+                bo[i] = place(LB{}, WB{}, c, cols, ldb, bkq);
             }
         }
     }
-    /* FP8: load i of wave wv covers 16 rows (wv + NW i), 4 lanes a row */
-    uint32_t co[NC], cw[NC][2], ck = 0;
-    if constexpr (FP8) {
-        ck = 16u * (lane & 3u);
-#pragma unroll
-        for (uint32_t i = 0; i < NC; i++) {
-            const uint32_t r = 16u * (wv + NW * i) + (lane >> 2);
-            const uint32_t mr = DUAL ? 32u * (r >> 6) + (r & 31u) : r;
-            co[i] = mr < cols ? mr * ldb + ck : FG_OOB;
-#pragma unroll
-            for (uint32_t d = 0; d < 2; d++)
-                cw[i][d] = ASTG + r * 128u + 16u * ((2u * (lane & 3u) + d) ^ ((r >> 1) & 7u));
-        }
-    }
-    /* whether 1 KB load c (FP8: of 16 rows) is of the up matrix: wave-uniform */
-    auto up = [&](uint32_t c) { return DUAL && (((FP8 ? 2u * c : c) >> 2) & 1u); };
-
-    auto issue = [&](uint32_t j) {
-        uint8_t *st = fg_lds + (j % NS) * STG;
-        const bool nd = j >= nst1;
-        const uint32_t jj = nd ? j - nst1 : j, k0 = jj * 64u, left = p.K - k0;
-        const uint8_t *aj = (nd ? a1 : a0) + jj * astep;
-        const uint8_t *bj = (nd && !DUAL ? b1 : b0) + jj * bstep, *uj = b1 + jj * bstep;
-        if (left >= 64u) {
-#pragma unroll
-            for (uint32_t i = 0; i < NAL; i++) fg_dma16(aj, ao[i], st + (wv + NW * i) * 1024u);
-#pragma unroll
-            for (uint32_t i = 0; i < NBL; i++)
-                fg_dma16(up(wv + NW * i) ? uj : bj, bo[i], st + ASTG + (wv + NW * i) * 1024u);
-        } else {                                         /* the stage that ends at K */
-#pragma unroll
-            for (uint32_t i = 0; i < NAL; i++)
-                fg_dma16(aj, ak[i] < left ? ao[i] : FG_OOB, st + (wv + NW * i) * 1024u);
-#pragma unroll
-            for (uint32_t i = 0; i < NBL; i++)
-                fg_dma16(up(wv + NW * i) ? uj : bj, bk[i] < left ? bo[i] : FG_OOB,
-                         st + ASTG + (wv + NW * i) * 1024u);
-        }
+    /* load i of the next stage of A (of B). A stage that K cuts: layout 0 drops
+     * the pieces past it, layout 1 the k rows, by the buffer's end */
+    auto left = [&](uint32_t j) { return p.K - (j >= nst1 ? j - nst1 : j) * 64u; };
+    auto load_a = [&](uint32_t i) {
+        const uint32_t lf = left(ja);
+        const uint32_t span = AL == 1 && lf < 64u ? lf * lda * 2u : FG_SPAN;
+        fg_dma16(pa, span, AL == 0 && akq >= lf ? FG_OOB : ao[i], fg_lds + sa + (wv + 4u * i) * 1024u);
     };
-    /* FP8: stage j's codes into registers, and from there dequantized into its
-     * slot. A load's rows share a scale (whole blocks of 128, or half of one) */
-    ghip_u32x4 codes[NC];
-    float sc[NC];
-    auto fetch_codes = [&](uint32_t j) {
-        const uint32_t left = p.K - j * 64u, nkb = (p.K + 127u) >> 7;
-#pragma unroll
-        for (uint32_t i = 0; i < NC; i++) {
-            const uint32_t c = wv + NW * i, r = 16u * c, mr = DUAL ? 32u * (r >> 6) + (r & 31u) : r;
-            const bool u = up(c);
-            codes[i] = __builtin_bit_cast(
-                ghip_u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                fg_buf((u ? b1 : b0) + j * bstep), ck < left ? co[i] : FG_OOB, 0, 0));
-            const uint32_t last = (p.N - 1u) >> 7, sb = min((col0 + mr) >> 7, last);
-            sc[i] = ghip_sload(u ? p.s2 : p.s, sb * nkb + (j >> 1));
-        }
+    auto load_b = [&](uint32_t i) {
+        const uint32_t lf = left(jb);
+        const uint32_t span = BL == 1 && lf < 64u ? lf * ldb * 2u : FG_SPAN;
+        fg_dma16(pb, span, BL == 0 && bkq >= lf ? FG_OOB : bo[i], bring + sb + (wv + 4u * i) * 1024u);
     };
-    auto put_codes = [&](uint32_t j, uint32_t i) {
-        uint8_t *st = fg_lds + (j % NS) * STG;
-        ghip_u32x4 lo, hi;
-        if (p.exact) ghip_deq16_u32<true>(codes[i], sc[i], lo, hi);
-        else ghip_deq16_u32<false>(codes[i], sc[i], lo, hi);
-        *(ghip_u32x4 *)(st + cw[i][0]) = lo;
-        *(ghip_u32x4 *)(st + cw[i][1]) = hi;
+    auto next_a = [&]() {
+        ja++;
+        pa += astep;
+        if (MODE == GHIP_EP_STORE && ja == nst1 && nst > nst1) pa = base_a(p.a2);
+        sa = sa == L * AST ? 0u : sa + AST;
+    };
+    auto next_b = [&]() {
+        jb++;
+        pb += bstep;
+        if (MODE == GHIP_EP_STORE && jb == nst1 && nst > nst1) pb = base_b(p.b2);
+        sb = sb == (L - 1u) * BST ? 0u : sb + BST;
     };
 
-    uint32_t off0[4];                                    /* layout 0 operand reads */
+    /* operand reads: block blk of 16 rows, step s */
+    uint32_t off0[2];
 #pragma unroll
-    for (uint32_t s = 0; s < 4; s++) off0[s] = n * 128u + 16u * ((4u * h + s) ^ ((n >> 1) & 7u));
-    const uint32_t i16 = lane & 15u, c16 = (lane >> 4) & 1u;
+    for (uint32_t s = 0; s < 2; s++) off0[s] = n * 128u + 16u * ((2u * g + s) ^ ((n >> 1) & 7u));
     auto frag = [&](auto layout_c, auto w_c, const uint8_t *st, uint32_t blk, int s) -> ghip_bf16x8 {
         constexpr uint32_t W = decltype(w_c)::value;
         if constexpr (decltype(layout_c)::value == 0) {
-            return *(const ghip_bf16x8 *)(st + blk * 4096u + off0[s]);
+            return *(const ghip_bf16x8 *)(st + blk * 2048u + off0[s]);
         } else {
-            const uint32_t k = 32u * h + 8u * (uint32_t)s + (i16 >> 2);
-            const uint32_t slot = (2u * blk + c16) ^ fg_swizzle<W>(k);
-            const uint8_t *q = st + k * (2u * W) + slot * 32u + (i16 & 3u) * 8u;
+            const uint32_t k = 16u * g + 8u * (uint32_t)s + (n >> 2);
+            const uint8_t *q =
+                st + k * (2u * W) + (blk ^ fg_swizzle<W>(k)) * 32u + (n & 3u) * 8u;
+            /* k + 4 has the same swizzle */
             const fg_s16x4 lo = fg_read_tr((fg_lds_s16x4 *)q);
             const fg_s16x4 hi = fg_read_tr((fg_lds_s16x4 *)(q + 8u * W));
             return __builtin_bit_cast(ghip_bf16x8,
                                       __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         }
     };
-    fg_f32x16 acc[RB][CB];
+    ghip_f32x4 acc[RB][CB];
 #pragma unroll
     for (int r = 0; r < RB; r++)
 #pragma unroll
-        for (uint32_t c = 0; c < CB; c++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) acc[r][c][i] = 0.0f;
+        for (int c = 0; c < CB; c++) acc[r][c] = (ghip_f32x4){0.f, 0.f, 0.f, 0.f};
     ghip_bf16x8 xa[2][RB], wa[2][CB];
-    auto fetch = [&](int set, uint32_t j, int s) {
-        const uint8_t *st = fg_lds + (j % NS) * STG;
-#pragma unroll
-        for (uint32_t r = 0; r < RB; r++) xa[set][r] = frag(LA{}, WA{}, st, wr * RB + r, s);
-#pragma unroll
-        for (uint32_t c = 0; c < CB; c++) wa[set][c] = frag(LB{}, WB{}, st + ASTG, wc * CB + c, s);
+    ghip_u32x4 codes[FP8 ? CB : 1];
+    auto read_a = [&](int set, int r, const uint8_t *st, int s) {
+        xa[set][r] = frag(LA{}, WA{}, st, wr * RB + r, s);
     };
-    /* all NS stages in flight, then the first step's operands */
+    auto read_b = [&](int set, int c, const uint8_t *st, int s) {
+        if constexpr (FP8)
+            codes[c] = *(const ghip_u32x4 *)(st + (wc * CB + c) * 1024u + n * 64u
+                                             + 16u * (g ^ (n >> 2)));
+        else
+            wa[set][c] = frag(LB{}, WB{}, st, wc * CB + c, s);
+    };
+    /* FP8: quarter q of column block c's operand of step s (4 codes) */
+    float sc0 = 0.0f, sc1 = 0.0f;
+    uint32_t srow0 = 0, srow1 = 0;
     if constexpr (FP8) {
-        issue(0);
-        fetch_codes(0);
-#pragma unroll
-        for (uint32_t i = 0; i < NC; i++) put_codes(0, i);
-        GHIP_VMCNT(0);
-        __builtin_amdgcn_s_waitcnt(0xc07f);
-        if (nst > 1u) {
-            issue(1);
-            fetch_codes(1);
-        }
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < NS; i++)
-            if (i < nst) issue(i);
-        ghip_wait_stages<LPS, NS - 1>(nst - 1u);
+        /* the wave's rows of a matrix lie in one block of 128 (tiles start at
+         * multiples of their width, which divides it or is 256) */
+        const uint32_t nkb = (p.K + 127u) >> 7, last = (p.N - 1u) >> 7;
+        const uint32_t w0 = col0 + wc * (DUAL ? 8u * CB : 16u * CB);
+        srow0 = srow1 = min(w0 >> 7, last) * nkb;
     }
+    auto scales = [&](uint32_t j) {                      /* of stage j */
+        sc0 = ghip_sload(p.s, srow0 + (j >> 1));
+        if constexpr (DUAL) sc1 = ghip_sload(p.s2, srow1 + (j >> 1));
+    };
+    auto dequant = [&](int set, int c, int s, int h) {
+        const float sc = DUAL && (c & 1) ? sc1 : sc0;
+        const ghip_u32x2 d = ghip_deq4<W8 == 2>(codes[c][2 * s + h], sc);
+        ghip_u32x4 v = __builtin_bit_cast(ghip_u32x4, wa[set][c]);
+        v[2 * h] = d[0];
+        v[2 * h + 1] = d[1];
+        wa[set][c] = __builtin_bit_cast(ghip_bf16x8, v);
+    };
+
+    /* L stages in flight, then the first step's operands */
+#pragma unroll
+    for (uint32_t j = 0; j < (uint32_t)L; j++)
+        if (j < nst) {
+#pragma unroll
+            for (uint32_t i = 0; i < NAL; i++) load_a(i);
+            next_a();
+#pragma unroll
+            for (uint32_t i = 0; i < NBL; i++) load_b(i);
+            next_b();
+        }
+    if constexpr (FP8) scales(0);
+    ghip_wait_stages<LPS, L - 1>(nst - 1u);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    fetch(0, 0u, 0);
-    constexpr int READS = (AL ? 2 : 1) * RB + (BL ? 2 : 1) * (int)CB;
-    constexpr int PER = (READS + RB * (int)CB - 1) / (RB * (int)CB);
-
-    /* MAIN: stage j + NS exists and is loaded during this one. Operands are
-     * read one MFMA step ahead; the stage's one barrier sits before its last
-     * step, when its last operands are in registers, and frees its slot. FP8:
-     * the codes of stage j + 1 are written during the first two steps (its slot
-     * is free since the barrier of stage j - 1), those of stage j + 2 loaded in
-     * the third. */
+#pragma unroll
+    for (int c = 0; c < CB; c++) read_b(0, c, bring, 0);
+#pragma unroll
+    for (int r = 0; r < RB; r++) read_a(0, r, fg_lds, 0);
+    if constexpr (FP8) {
+#pragma unroll
+        for (int c = 0; c < CB; c++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) dequant(0, c, 0, h);
+    }
+    uint32_t ra = 0, rb = 0;                             /* slots of stage j */
+    /* MAIN: stage j + L exists and is loaded during this one. Operands are read
+     * one step ahead; the barrier sits between the steps, when the stage's last
+     * operands are in registers, and frees its B slot (its A slot is written
+     * again from the next stage's first step on). */
     auto stage = [&](uint32_t j, auto main_c) {
         constexpr bool MAIN = decltype(main_c)::value;
-        const uint32_t jn = MAIN ? j + 1u : min(j + 1u, nst - 1u);
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-            if (s == 3) {
+        const bool more = MAIN || j + 1u < nst;          /* else re-read this stage, unused */
+        const uint32_t na = !more ? ra : ra == L * AST ? 0u : ra + AST;
+        const uint32_t nb = !more ? rb : rb == (L - 1u) * BST ? 0u : rb + BST;
+        fg_each<2>([&](auto step) {
+            constexpr int S = decltype(step)::value;
+            if constexpr (S == 1) {
                 /* own loads of stage j + 1 done, own reads of stage j done;
                  * after the barrier that holds for every wave */
-                if constexpr (FP8) {
-                    /* the x loads of stage j + 1 are older than the codes of
-                     * stage j + 2 */
-                    if (MAIN) GHIP_VMCNT(NC);
-                    else GHIP_VMCNT(0);
-                } else if (MAIN) {
-                    GHIP_VMCNT(LPS * (NS - 2));
-                } else {
-                    ghip_wait_stages<LPS, NS - 2>(nst - 1u - jn);
-                }
+                if (MAIN) GHIP_VMCNT((L - 1) * NAL + (L - 2) * NBL);
+                else ghip_wait_stages<LPS, L - 2>(more ? nst - 2u - j : 0u);
                 __builtin_amdgcn_s_waitcnt(0xc07f);
                 __builtin_amdgcn_s_barrier();
                 __builtin_amdgcn_sched_barrier(0);
-                if (MAIN) issue(j + NS);
+                if constexpr (FP8) scales(more ? j + 1u : j);
             }
-            const int cur = s & 1, nxt = cur ^ 1;
-            if constexpr (FP8) {
-                if (s < 2 && (MAIN || j + 1u < nst)) {
-#pragma unroll
-                    for (uint32_t i = (uint32_t)s; i < NC; i += 2) put_codes(j + 1u, i);
-                }
-                if (s == 2 && MAIN) {
-                    fetch_codes(j + 2u);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-            if (s < 3) fetch(nxt, j, s + 1);
-            else fetch(nxt, jn, 0);
-#pragma unroll
-            for (int r = 0; r < RB; r++)
-#pragma unroll
-                for (uint32_t c = 0; c < CB; c++)
-                    acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wa[cur][c], xa[cur][r],
-                                                                       acc[r][c], 0, 0, 0);
-            if constexpr (!FP8) {
-#pragma unroll
-                for (int i = 0; i < RB * (int)CB; i++) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                    if (i * PER < READS) __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
-                }
+            const uint8_t *as = fg_lds + (S == 0 ? ra : na), *bs = bring + (S == 0 ? rb : nb);
+            /* between the MFMAs: the next step's reads (FP8: in the first half,
+             * codes only in step 1, which serve both steps), its dequantization
+             * (in step 1 in the second half), and the loads */
+            constexpr int B0 = FP8 && S == 0 ? (int)CB : 0, NR = RB + (int)CB - B0;
+            constexpr int RE = FP8 ? NM / 2 : NM, DF = S == 1 ? NM / 2 : 0, NQ = FP8 ? 2 * CB : 0;
+            constexpr int NL = !MAIN ? 0 : S == 0 ? (int)NAL : (int)NBL;
+            fg_each<NM>([&](auto slot) {
+                constexpr int I = decltype(slot)::value, R = I / CB;
+                constexpr int C = R & 1 ? CB - 1 - I % CB : I % CB;
+                fg_mfma(acc[R][C], wa[S][C], xa[S][R]);
+                constexpr int R0 = fg_spread(NR, I, 0, RE), R1 = fg_spread(NR, I + 1, 0, RE);
+                constexpr int Q0 = fg_spread(NQ, I, DF, NM), Q1 = fg_spread(NQ, I + 1, DF, NM);
+                constexpr int L0 = fg_spread(NL, I, 0, NM), L1 = fg_spread(NL, I + 1, 0, NM);
+                fg_each<R1 - R0>([&](auto k) {
+                    constexpr int O = R0 + decltype(k)::value + B0;
+                    if constexpr (O < (int)CB) read_b(S ^ 1, O, bs, S ^ 1);
+                    else read_a(S ^ 1, O - CB, as, S ^ 1);
+                });
+                fg_each<Q1 - Q0>([&](auto k) {
+                    constexpr int Q = Q0 + decltype(k)::value;
+                    dequant(S ^ 1, Q >> 1, S ^ 1, Q & 1);
+                });
+                fg_each<L1 - L0>([&](auto k) {
+                    constexpr uint32_t O = L0 + decltype(k)::value;
+                    if constexpr (S == 0) load_a(O);
+                    else load_b(O);
+                });
+                if constexpr (R1 > R0 || Q1 > Q0 || L1 > L0) __builtin_amdgcn_sched_barrier(0);
+            });
+            if constexpr (MAIN) {
+                if constexpr (S == 0) next_a();
+                else next_b();
             }
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
+        ra = na;
+        rb = nb;
     };
     uint32_t j = 0;
-    for (; j + NS < nst; j++) stage(j, std::true_type{});
+    for (; j + L < nst; j++) stage(j, std::true_type{});
     for (; j < nst; j++) stage(j, std::false_type{});
+    fg_settle(acc);
 
-    /* register 4q + i of block (r, c) is row 32 r + n, column 32 c + 8 q + 4 h +
-     * i: 32 rows x 64 columns of f32 at a time, 16-byte piece p of row n at p ^
-     * (n & 15) */
+    /* register i of block (r, c): row 16 r + n, column 16 c + 4 g + i. 16 rows of
+     * f32 at a time, 16-byte piece q of row n at q XOR a function of n */
     __builtin_amdgcn_s_waitcnt(0xc07f);
     __builtin_amdgcn_s_barrier();
-    uint8_t *sw = fg_lds + wv * 8192u;
+    constexpr uint32_t RBY = 64u * CB;                   /* bytes of a staged row */
+    auto spot = [&](uint32_t row, uint32_t q) {
+        return row * RBY + 16u * (q ^ (CB >= 4 ? row : (row >> 1) & 7u));
+    };
+    uint8_t *sw = fg_lds + wv * (16u * RBY);
     uint16_t *out = second ? ep.out2 : ep.out;
     const bool vin = ((uintptr_t)ep.in & 15u) == 0u && (ep.ldin & 7u) == 0u;
     const bool vout = (((uintptr_t)out | (uintptr_t)ep.out2) & 15u) == 0u && (ep.ldout & 7u) == 0u;
     const bool vbias = ((uintptr_t)ep.bias & 15u) == 0u;
-    constexpr uint32_t LPR = DUAL ? 4u : 8u;             /* lanes of a row */
+    constexpr uint32_t LPR = DUAL ? CB : 2u * CB;        /* groups of 8 columns of a row */
     ghip_with_act(MODE == GHIP_EP_STORE ? GHIP_ACT_NONE : ep.act, [&](auto act) {
 #pragma unroll
         for (int r = 0; r < RB; r++) {
 #pragma unroll
-            for (uint32_t c = 0; c < CB; c++)
-#pragma unroll
-                for (uint32_t q = 0; q < 4; q++) {
-                    ghip_f32x4 v;
-#pragma unroll
-                    for (int i = 0; i < 4; i++) v[i] = acc[r][c][4 * q + i];
-                    *(ghip_f32x4 *)(sw + n * 256u + 16u * ((8u * c + 2u * q + h) ^ (n & 15u))) = v;
-                }
+            for (uint32_t c = 0; c < CB; c++) *(ghip_f32x4 *)(sw + spot(n, 4u * c + g)) = acc[r][c];
             __builtin_amdgcn_s_waitcnt(0xc07f);
             __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
-            for (uint32_t i = 0; i < LPR / 2u; i++) {
-                const uint32_t lr = lane / LPR + 64u / LPR * i, pc = lane % LPR;
+            for (uint32_t v = lane; v < 16u * LPR; v += 64u) {
+                const uint32_t lr = v / LPR, pc = v % LPR;
                 auto read8 = [&](uint32_t first, float (&s)[8]) {
 #pragma unroll
                     for (uint32_t d = 0; d < 2; d++) {
-                        const ghip_f32x4 v =
-                            *(const ghip_f32x4 *)(sw + lr * 256u + 16u * ((first + d) ^ (lr & 15u)));
+                        const ghip_f32x4 x = *(const ghip_f32x4 *)(sw + spot(lr, first + d));
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[4 * d + e] = v[e];
+                        for (int e = 0; e < 4; e++) s[4 * d + e] = x[e];
                     }
                 };
+                /* dual: column block c of 16 is staged as gate block 2c, up block 2c + 1 */
                 float s0[8], s1[8] = {};
-                read8(2u * pc, s0);
-                if constexpr (DUAL) read8(8u + 2u * pc, s1);
-                const uint32_t m = row0 + 32u * (wr * RB + r) + lr;
-                const uint32_t c0 = (DUAL ? 32u : 64u) * wc + 8u * pc;
+                const uint32_t q0 = DUAL ? 8u * (pc >> 1) + 2u * (pc & 1u) : 2u * pc;
+                read8(q0, s0);
+                if constexpr (DUAL) read8(q0 + 4u, s1);
+                const uint32_t m = row0 + 16u * (wr * RB + r) + lr;
+                const uint32_t c0 = (DUAL ? 8u : 16u) * CB * wc + 8u * pc;
                 if (m < p.M && c0 < cols)
                     fg_store8<MODE, decltype(act)::value>(ep, out, m, col0 + c0, p.N, s0, s1, vin,
                                                           vout, vbias);
