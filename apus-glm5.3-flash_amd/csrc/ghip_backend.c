@@ -780,8 +780,18 @@ int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
                             .ldout = lddz, .act = act, .limit = INFINITY, .pad = 1 };
         HIPCHK(ghip_launch_ffn(GHIP_EP_DLINEAR, &p, &ep, st));
     }
-    if (dx && ffn_dx(dz, NULL, lddz, w, NULL, dx, M, O, K, lddx, again, st)) return 1;
-    if (dw && ffn_dw(dz, NULL, lddz, x, ldx, dw, NULL, M, O, K, again, st)) return 1;
+    /* without an activation dz is dy; rows that the products cannot load as
+     * vectors are laid out again where there is room */
+    int pad = again;
+    if (!again && (dx || dw) && ws && check_ws(ws, ws_bytes, ffn_ws_mat(M, O)) == 0 && K % 8 == 0
+        && (((uintptr_t)dy & 15) || lddy % 8 || O % 8)) {
+        HIPCHK(ghip_launch_ffn_pack(dy, lddy, M, O, (uint16_t *)ws, st));
+        dz = (const uint16_t *)ws;
+        lddz = ffn_ws_ld(O);
+        pad = 1;
+    }
+    if (dx && ffn_dx(dz, NULL, lddz, w, NULL, dx, M, O, K, lddx, pad, st)) return 1;
+    if (dw && ffn_dw(dz, NULL, lddz, x, ldx, dw, NULL, M, O, K, pad, st)) return 1;
     if (dbias) HIPCHK(ghip_launch_ffn_colsum(dz, lddz, M, O, dbias, st));
     G.dispatches++;
     return 0;

@@ -108,21 +108,21 @@ constexpr bool ghip_ep_dual(int mode) { return mode == GHIP_EP_GATED || mode == 
 
 /* One output, row m, column n, from its sums, bias and incoming value. */
 template <int MODE, int ACT>
-__device__ __forceinline__ void ghip_ep_put(const GhipEp &ep, uint32_t m, uint32_t n, float s0,
-                                            float s1, float b, float in) {
+__device__ __forceinline__ void ghip_ep_put(const GhipEp &ep, uint16_t *out, uint32_t m, uint32_t n,
+                                            float s0, float s1, float b, float in) {
     float o0, o1;
     ghip_ep_value<MODE, ACT>(s0, s1, b, in, ep.limit, o0, o1);
-    ep.out[(size_t)m * ep.ldout + n] = (uint16_t)ghip_bf16_bits(o0);
+    out[(size_t)m * ep.ldout + n] = (uint16_t)ghip_bf16_bits(o0);
     if constexpr (MODE == GHIP_EP_DGATED)
         ep.out2[(size_t)m * ep.ldout + n] = (uint16_t)ghip_bf16_bits(o1);
 }
 
 template <int MODE, int ACT>
-__device__ __forceinline__ void ghip_ep_store1(const GhipEp &ep, uint32_t m, uint32_t n, float s0,
-                                               float s1) {
+__device__ __forceinline__ void ghip_ep_store(const GhipEp &ep, uint16_t *out, uint32_t m,
+                                              uint32_t n, float s0, float s1) {
     const float b = ep.bias ? ghip_bf16_f32(ep.bias[n]) : 0.0f;
     const float in = ep.in ? ghip_bf16_f32(ep.in[(size_t)m * ep.ldin + n]) : 0.0f;
-    ghip_ep_put<MODE, ACT>(ep, m, n, s0, s1, b, in);
+    ghip_ep_put<MODE, ACT>(ep, out, m, n, s0, s1, b, in);
 }
 
 #endif /* GHIP_EPILOGUE_H */

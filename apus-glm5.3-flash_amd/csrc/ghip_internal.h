@@ -301,22 +301,30 @@ hipError_t ghip_launch_ffn_any(int mode, const GhipProd *p, const GhipEp *ep, hi
 hipError_t ghip_launch_ffn_colsum(const uint16_t *dz, size_t ld, size_t M, size_t N,
                                   uint16_t *out, hipStream_t st);
 
+/* dst [M, N up to a multiple of 8] = src's rows (ld apart, any alignment), zeros
+ * behind; dst 16-byte aligned. */
+hipError_t ghip_launch_ffn_pack(const uint16_t *src, size_t ld, size_t M, size_t N,
+                                uint16_t *dst, hipStream_t st);
+
 /* On tiles (k_ffn_gemm.h): fits = the steps and alignments of the vector loads;
  * pick = the tile shape with the least estimated time (microseconds, in us). */
 int ghip_ffn_gemm_fits(int mode, const GhipProd *p);
 int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us);
 hipError_t ghip_launch_ffn_gemm(int mode, int tile, const GhipProd *p, const GhipEp *ep,
                                 hipStream_t st);
-/* One family of its kernels: the tiles of a mode (k_ffn_nt.hip, k_ffn_bwd.hip). */
+/* One family of its kernels: the tiles of a mode (k_ffn_nt.hip, k_ffn_nt8.hip, k_ffn_bwd.hip). */
 typedef struct {
     uint32_t bm, bn;             /* output rows and columns */
-    float us;                    /* a stage's time on a full chip, microseconds */
+    uint32_t occ;                /* workgroups a CU holds */
+    float low, full, over;       /* microseconds: a stage on a nearly empty and on a full chip,
+                                    and a round's first loads and epilogue */
     uint32_t lds;
     const void *kern;
     void (*launch)(const GhipProd *, const GhipEp *, uint32_t, uint32_t, uint32_t, hipStream_t);
 } GhipFfnTile;
 /* w8: 0 bf16 weights, 1 FP8, 2 FP8 with NaN codes */
 const GhipFfnTile *ghip_ffn_forward_tiles(int mode, int w8, int *n);
+const GhipFfnTile *ghip_ffn_fp8_tiles(int mode, int w8, int *n);
 const GhipFfnTile *ghip_ffn_backward_tiles(int mode, int transposed, int *n);
 
 /* Streaming the weights past a few rows (k_rows_gemm.h), forward modes. */

@@ -43,8 +43,11 @@ extern "C" int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, fl
     for (int i = 0; i < n; i++) {
         const double wgs = (double)((p->M + t[i].bm - 1) / t[i].bm)
                            * (double)((p->N + t[i].bn - 1) / t[i].bn) * (p->batch ? 2 : 1);
-        const double rounds = (double)(size_t)((wgs + n_cu - 1) / n_cu);
-        const float e = (float)(4.0 + rounds * (stages * t[i].us * (0.75 + 0.25 * wgs / (rounds * n_cu)) + 1.5));
+        const double cap = (double)n_cu * t[i].occ, whole = (double)(size_t)(wgs / cap);
+        const double part = wgs / cap - whole;           /* of the last round */
+        const double e64 = 3.0 + whole * (stages * t[i].full + t[i].over)
+                           + (part > 0.0 ? stages * (t[i].low + (t[i].full - t[i].low) * part) + t[i].over : 0.0);
+        const float e = (float)e64;
         if (i == 0 || e < *us) {
             best = i;
             *us = e;

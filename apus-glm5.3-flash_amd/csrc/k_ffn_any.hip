@@ -13,9 +13,10 @@
  *
  * A workgroup of 4 waves owns 64 x 64 outputs, each wave 32 x 32 as four
  * v_mfma_f32_16x16x32_bf16 a step of k = 32; tiles reach LDS through registers
- * by 2-byte (1-byte) loads, the next step's in flight during the products,
- * elements past M, N or k as zeros. It is bound by those loads' issue: the
- * route for what the vector kernels cannot take.
+ * by loads of 8 elements at any alignment (8 of one element at the matrix's
+ * edges), the next step's in flight during the products, elements past M, N or
+ * k as zeros. It is bound by the two barriers of a step and its load's latency:
+ * the route for what the kernels with direct loads cannot take.
  */
 #include "ghip_epilogue.h"
 
@@ -35,38 +36,69 @@ __global__ __launch_bounds__(256) void k_ffn_any(GhipProd p, GhipEp ep, uint32_t
     ghip_f32x4 acc[NB][2][2] = {};
     const uint32_t nkb = (p.K + 127u) >> 7;
 
-    /* element e of a thread: the operand's fast index runs over the threads */
-    auto at = [&](bool kfast, uint32_t e, uint32_t &r, uint32_t &k) {
-        const uint32_t v = tid + 256u * e;
-        r = kfast ? v >> 5 : v & 63u;
-        k = kfast ? v & 31u : v >> 6;
+    /* A thread loads 8 elements along the operand's fast index: k 8 (tid % 4) ..
+     * of row tid / 4, or rows 8 (tid % 8) .. of k tid / 8. Where all 8 exist that
+     * is one load at whatever alignment the row has, else one each */
+    auto spot = [&](bool kfast, uint32_t &r, uint32_t &k) {
+        r = kfast ? tid >> 2 : 8u * (tid & 7u);
+        k = kfast ? 8u * (tid & 3u) : tid >> 3;
     };
-    uint16_t ra[8], rb[NB][8];
+    auto load8 = [&](const uint16_t *q, bool whole, uint32_t live, fa_u16x8 &v) {
+        if (whole) {
+            __builtin_memcpy(&v, q, 16);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) v[e] = e < live ? q[e] : (uint16_t)0;
+        }
+    };
+    fa_u16x8 ra, rb[NB];
     auto fetch = [&](int pr, uint32_t k0) {
-        const uint16_t *a = pr ? p.a2 : p.a;
+        uint32_t r, k;
+        spot(p.aks == 1, r, k);
+        {
+            const uint32_t m = row0 + r, kk = k0 + k;
+            const uint32_t left = p.aks == 1 ? (kk < p.K ? p.K - kk : 0u) : (m < p.M ? p.M - m : 0u);
+            const bool in = m < p.M && kk < p.K;
+            const uint16_t *q = (pr ? p.a2 : p.a) + (in ? (size_t)m * p.ars + (size_t)kk * p.aks : 0);
+            load8(q, in && left >= 8u, in ? left : 0u, ra);
+        }
+        spot(p.bks == 1, r, k);
+        const uint32_t n = col0 + r, kk = k0 + k;
+        const uint32_t left = p.bks == 1 ? (kk < p.K ? p.K - kk : 0u) : (n < p.N ? p.N - n : 0u);
+        const bool in = n < p.N && kk < p.K;
+        const size_t o = in ? (size_t)n * p.brs + (size_t)kk * p.bks : 0;
 #pragma unroll
-        for (uint32_t e = 0; e < 8; e++) {
-            uint32_t r, k;
-            at(p.aks == 1, e, r, k);
-            ra[e] = row0 + r < p.M && k0 + k < p.K
-                        ? a[(size_t)(row0 + r) * p.ars + (size_t)(k0 + k) * p.aks] : (uint16_t)0;
-            at(p.bks == 1, e, r, k);
-            const bool in = col0 + r < p.N && k0 + k < p.K;
-            const size_t o = in ? (size_t)(col0 + r) * p.brs + (size_t)(k0 + k) * p.bks : 0;
-#pragma unroll
-            for (int d = 0; d < NB; d++) {
-                const void *b = d || pr ? p.b2 : p.b;
-                uint16_t v = 0;
-                if (in) {
-                    if constexpr (FP8) {
-                        const float s = (d ? p.s2 : p.s)[(size_t)((col0 + r) >> 7) * nkb + ((k0 + k) >> 7)];
-                        v = (uint16_t)ghip_bf16_bits(ghip_e4m3_exact(((const uint8_t *)b)[o]) * s);
-                    } else {
-                        v = ((const uint16_t *)b)[o];
-                    }
+        for (int d = 0; d < NB; d++) {
+            const void *b = d || pr ? p.b2 : p.b;
+            if constexpr (FP8) {
+                uint64_t c = 0;
+                const uint8_t *q = (const uint8_t *)b + o;
+                if (in && left >= 8u) {
+                    __builtin_memcpy(&c, q, 8);
+                } else if (in) {
+                    for (uint32_t e = 0; e < left; e++) c |= (uint64_t)q[e] << (8u * e);
                 }
-                rb[d][e] = v;
+                const float sc = in ? (d ? p.s2 : p.s)[(size_t)(n >> 7) * nkb + (kk >> 7)] : 0.0f;
+                const ghip_u32x2 lo = ghip_deq4<true>((uint32_t)c, sc), hi = ghip_deq4<true>((uint32_t)(c >> 32), sc);
+                const ghip_u32x4 v = {lo[0], lo[1], hi[0], hi[1]};
+                rb[d] = __builtin_bit_cast(fa_u16x8, v);
+                if (in && left < 8u) {                   /* codes past K: 0, not 0 * scale */
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; e++) rb[d][e] = e < left ? rb[d][e] : (uint16_t)0;
+                }
+            } else {
+                load8((const uint16_t *)b + o, in && left >= 8u, in ? left : 0u, rb[d]);
             }
+        }
+    };
+    auto put = [&](uint16_t *to, bool kfast, const fa_u16x8 &v) {
+        uint32_t r, k;
+        spot(kfast, r, k);
+        if (kfast) {
+            *(fa_u16x8 *)(to + r * FA_LD + k) = v;
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) to[(r + e) * FA_LD + k] = v[e];
         }
     };
     const int pairs = p.a2 ? 2 : 1;
@@ -74,15 +106,9 @@ __global__ __launch_bounds__(256) void k_ffn_any(GhipProd p, GhipEp ep, uint32_t
     fetch(0, 0);
     for (uint32_t j = 0; j < total; j++) {
         __syncthreads();
+        put(as, p.aks == 1, ra);
 #pragma unroll
-        for (uint32_t e = 0; e < 8; e++) {
-            uint32_t r, k;
-            at(p.aks == 1, e, r, k);
-            as[r * FA_LD + k] = ra[e];
-            at(p.bks == 1, e, r, k);
-#pragma unroll
-            for (int d = 0; d < NB; d++) bs[d][r * FA_LD + k] = rb[d][e];
-        }
+        for (int d = 0; d < NB; d++) put(bs[d], p.bks == 1, rb[d]);
         __syncthreads();
         if (j + 1u < total) fetch((int)((j + 1u) / steps), ((j + 1u) % steps) * 32u);
         ghip_bf16x8 av[2];
@@ -115,8 +141,8 @@ __global__ __launch_bounds__(256) void k_ffn_any(GhipProd p, GhipEp ep, uint32_t
                         if (MODE == GHIP_EP_DGATED) ep.out2[(size_t)m * ep.ldout + n] = 0;
                     }
                     if (m < p.M && n < p.N)
-                        ghip_ep_store1<MODE, decltype(act)::value>(ep, m, n, acc[0][i][c][q],
-                                                                   acc[NB - 1][i][c][q]);
+                        ghip_ep_store<MODE, decltype(act)::value>(ep, ep.out, m, n, acc[0][i][c][q],
+                                                                  acc[NB - 1][i][c][q]);
                 }
     });
 }
@@ -137,6 +163,27 @@ __global__ __launch_bounds__(1024) void k_ffn_colsum(const uint16_t *__restrict_
         float v = 0.0f;
         for (uint32_t i = 0; i < 16; i++) v += part[i][c];
         out[n] = (uint16_t)ghip_bf16_bits(v);
+    }
+}
+
+/* dst[m, 0 .. N up to a multiple of 8) = src[m, 0 .. N), zeros behind: rows of any
+ * alignment as whole vectors. */
+__global__ __launch_bounds__(256) void k_ffn_pack(const uint16_t *__restrict__ src, size_t ld,
+                                                  uint32_t M, uint32_t N, uint32_t per,
+                                                  uint16_t *__restrict__ dst) {
+    for (size_t v = (size_t)blockIdx.x * 256u + threadIdx.x; v < (size_t)M * per;
+         v += (size_t)gridDim.x * 256u) {
+        const size_t m = v / per;
+        const uint32_t n = (uint32_t)(v % per) * 8u;
+        const uint16_t *q = src + m * ld + n;
+        fa_u16x8 d;
+        if (n + 8u <= N) {
+            __builtin_memcpy(&d, q, 16);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) d[e] = n + e < N ? q[e] : (uint16_t)0;
+        }
+        *(fa_u16x8 *)(dst + v * 8u) = d;
     }
 }
 
@@ -188,5 +235,15 @@ extern "C" hipError_t ghip_launch_ffn_colsum(const uint16_t *dz, size_t ld, size
     if (M == 0 || N == 0 || M > 0x7fffffffu || N > 0x7fffffffu) return hipErrorInvalidValue;
     hipLaunchKernelGGL(k_ffn_colsum, dim3((uint32_t)((N + 63) / 64)), dim3(1024), 0, st, dz, ld,
                        (uint32_t)M, (uint32_t)N, out);
+    return hipGetLastError();
+}
+
+extern "C" hipError_t ghip_launch_ffn_pack(const uint16_t *src, size_t ld, size_t M, size_t N,
+                                           uint16_t *dst, hipStream_t st) {
+    if (M == 0 || N == 0 || M > 0x7fffffffu || N > 0x7fffffffu || ((uintptr_t)dst & 15u))
+        return hipErrorInvalidValue;
+    const size_t per = (N + 7) / 8, blocks = (M * per + 255) / 256;
+    hipLaunchKernelGGL(k_ffn_pack, dim3((uint32_t)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, st,
+                       src, ld, (uint32_t)M, (uint32_t)N, (uint32_t)per, dst);
     return hipGetLastError();
 }

@@ -3,10 +3,10 @@
  * (gfx950): out[m, n] = epilogue(sum_k A(m, k) B(n, k)); instantiated by
  * k_ffn_nt.hip (forward) and k_ffn_bwd.hip (backward).
  *
- * A workgroup of 4 waves owns 32 RB rows of A x 32 CB rows of B; wave (wr, wc)
- * computes 16 RB x 16 CB outputs with v_mfma_f32_16x16x32_bf16, B as the A
- * operand of the instruction, so a lane ends with four consecutive columns of
- * one output row. k is walked in stages of 64, two MFMA steps each.
+ * A workgroup of WM x WN = 4 waves owns 16 RB WM rows of A x 16 CB WN rows of B;
+ * wave (wr, wc) computes 16 RB x 16 CB outputs with v_mfma_f32_16x16x32_bf16, B
+ * as the A operand of the instruction, so a lane ends with four consecutive
+ * columns of one output row. k is walked in stages of 64, two MFMA steps each.
  *
  * What bounds it, and what follows. A full chip of these products is at its
  * power limit (4096 x 4096 x 4096 of zeros runs at 1800 TFLOP/s, of normal
@@ -41,8 +41,8 @@
  * FP8 weights lie in LDS as codes, [row][64 codes], 16-byte piece p of row r at
  * p ^ ((r >> 2) & 3): one read gives the 16 codes of both steps, which are
  * dequantized bit-exactly in registers between the MFMAs of the step before
- * (both waves of a column do so; against dequantizing once and writing bf16
- * back to LDS it takes half the loads and writes).
+ * (against writing bf16 back to LDS it takes half the loads and writes). Its
+ * waves lie side by side (WM = 1), so that no two dequantize the same codes.
  *
  * Dual modes (gate and up): the tile's B rows alternate in blocks of 16 between
  * the two matrices, so a lane holds g and u of the same columns and the product
@@ -123,73 +123,44 @@ constexpr int fg_spread(int n, int i, int from, int to) {
     return i <= from ? 0 : i >= to ? n : (n * (i - from) + (to - from) - 1) / (to - from);
 }
 
-/* 8 outputs of row m from column n0 on: s0 (and s1) their sums. */
-template <int MODE, int ACT>
-__device__ __forceinline__ void fg_store8(const GhipEp &ep, uint16_t *out, uint32_t m, uint32_t n0,
-                                          uint32_t N, const float (&s0)[8], const float (&s1)[8],
-                                          bool vin, bool vout, bool vbias) {
-    float b[8] = {}, in[8] = {}, o0[8], o1[8];
-    const bool whole = n0 + 8u <= N;
-    auto load = [&](const uint16_t *p, bool vec, float (&v)[8]) {
-        if (whole && vec) {
-            const ghip_u32x4 d = *(const ghip_u32x4 *)p;
+/* 8 bf16 values as f32, and back with one rounding */
+__device__ __forceinline__ void fg_unpack(const ghip_u32x4 &d, float (&v)[8]) {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                v[e] = ghip_bf16_f32(e & 1 ? d[e >> 1] >> 16 : d[e >> 1] & 0xffffu);
-        } else {
+    for (int e = 0; e < 8; e++) v[e] = ghip_bf16_f32(e & 1 ? d[e >> 1] >> 16 : d[e >> 1] & 0xffffu);
+}
+__device__ __forceinline__ ghip_u32x4 fg_pack(const float (&v)[8]) {
+    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+    ghip_u32x4 d;
 #pragma unroll
-            for (uint32_t e = 0; e < 8; e++) v[e] = n0 + e < N ? ghip_bf16_f32(p[e]) : 0.0f;
-        }
-    };
-    if constexpr (MODE == GHIP_EP_LINEAR || MODE == GHIP_EP_DLINEAR)
-        if (ep.bias) load(ep.bias + n0, vbias, b);
-    if constexpr (MODE != GHIP_EP_STORE && MODE != GHIP_EP_GATED)
-        if (ep.in) load(ep.in + (size_t)m * ep.ldin + n0, vin, in);
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-        ghip_ep_value<MODE, ACT>(s0[e], s1[e], b[e], in[e], ep.limit, o0[e], o1[e]);
-    auto store = [&](uint16_t *p, const float (&v)[8]) {
-        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-        ghip_u32x4 d;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const bool pad = n0 + 2u * e >= N, half = n0 + 2u * e + 1u >= N;
-            bf2 t;
-            t[0] = (__bf16)(!whole && pad ? 0.0f : v[2 * e]);
-            t[1] = (__bf16)(!whole && half ? 0.0f : v[2 * e + 1]);
-            d[e] = __builtin_bit_cast(uint32_t, t);
-        }
-        if (vout && (whole || ep.pad)) {
-            *(ghip_u32x4 *)p = d;
-        } else {
-#pragma unroll
-            for (uint32_t e = 0; e < 8; e++)
-                if (n0 + e < N) p[e] = (uint16_t)(d[e >> 1] >> (16u * (e & 1u)));
-        }
-    };
-    store(out + (size_t)m * ep.ldout + n0, o0);
-    if constexpr (MODE == GHIP_EP_DGATED) store(ep.out2 + (size_t)m * ep.ldout + n0, o1);
+    for (int e = 0; e < 4; e++) {
+        bf2 t;
+        t[0] = (__bf16)v[2 * e];
+        t[1] = (__bf16)v[2 * e + 1];
+        d[e] = __builtin_bit_cast(uint32_t, t);
+    }
+    return d;
 }
 
 /* W8: 0 bf16 weights, 1 FP8 codes, 2 FP8 codes with NaN codes among them */
-template <int MODE, int W8, int AL, int BL, int RB, int CB, int L>
+template <int MODE, int W8, int AL, int BL, int WM, int RB, int CB, int L>
 __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint32_t mt,
                                                      uint32_t nt) {
     constexpr bool DUAL = ghip_ep_dual(MODE), FP8 = W8 != 0;
-    constexpr uint32_t BM = 32u * RB, BN = 32u * CB;
+    constexpr uint32_t WN = 4 / WM, BM = 16u * RB * WM, BN = 16u * CB * WN;
     constexpr uint32_t OUTN = DUAL ? BN / 2 : BN;        /* output columns of a tile */
     constexpr uint32_t AST = BM * 128u, BST = BN * (FP8 ? 64u : 128u);  /* slot bytes */
-    constexpr uint32_t NAL = RB, NBL = FP8 ? CB / 2 : CB, LPS = NAL + NBL;
+    constexpr uint32_t NAL = BM / 32u, NBL = FP8 ? BN / 64u : BN / 32u, LPS = NAL + NBL;
     constexpr uint32_t RING = (L + 1u) * AST + L * BST;
     constexpr int NM = RB * CB;                          /* MFMAs of a step */
-    static_assert(RING <= FG_LDS_MAX && RING >= 4u * 1024u * CB, "ring, epilogue staging");
+    static_assert(RING <= FG_LDS_MAX, "ring");
+    static_assert(WM * WN == 4 && BM % 32 == 0 && BN % (FP8 ? 64 : 32) == 0, "waves, whole loads");
     static_assert(L >= 2 && (L - 1) * NAL + (L - 2) * NBL <= 63 && (L - 1) * LPS <= 63, "waits");
-    static_assert(CB % 2 == 0 && (!FP8 || (BL == 0 && 128 % (16 * CB) == 0)), "columns");
+    static_assert((!DUAL || CB % 2 == 0) && (!FP8 || (BL == 0 && 128 % (16 * CB) == 0)), "columns");
     extern __shared__ __attribute__((aligned(1024))) uint8_t fg_lds[];
     uint8_t *bring = fg_lds + (L + 1u) * AST;
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
     const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t wr = wv >> 1, wc = wv & 1u, n = lane & 15u, g = lane >> 4;
+    const uint32_t wr = wv / WN, wc = wv % WN, n = lane & 15u, g = lane >> 4;
 
     /* tile t: the workgroups of one XCD (b % 8) take a run of consecutive
      * tiles, which go down 4 row tiles before the next column, so that an XCD's
@@ -449,48 +420,112 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
     for (; j < nst; j++) stage(j, std::false_type{});
     fg_settle(acc);
 
-    /* register i of block (r, c): row 16 r + n, column 16 c + 4 g + i. 16 rows of
-     * f32 at a time, 16-byte piece q of row n at q XOR a function of n */
+    /* register i of block (r, c): row 16 r + n, column 16 c + 4 g + i. G blocks of
+     * 16 rows of f32 at a time, 16-byte piece q of a row at q XOR a function of
+     * the row; then 8 columns of a row a lane, the same columns every time */
     __builtin_amdgcn_s_waitcnt(0xc07f);
     __builtin_amdgcn_s_barrier();
+    constexpr int G = RING / 4u >= 1024u * CB * RB ? RB : RING / 4u >= 512u * CB * RB ? RB / 2 : RB / 4;
+    static_assert(RING / 4u >= 1024u * CB * G && RB % G == 0, "epilogue staging");
     constexpr uint32_t RBY = 64u * CB;                   /* bytes of a staged row */
-    auto spot = [&](uint32_t row, uint32_t q) {
-        return row * RBY + 16u * (q ^ (CB >= 4 ? row : (row >> 1) & 7u));
-    };
-    uint8_t *sw = fg_lds + wv * (16u * RBY);
-    uint16_t *out = second ? ep.out2 : ep.out;
-    const bool vin = ((uintptr_t)ep.in & 15u) == 0u && (ep.ldin & 7u) == 0u;
-    const bool vout = (((uintptr_t)out | (uintptr_t)ep.out2) & 15u) == 0u && (ep.ldout & 7u) == 0u;
-    const bool vbias = ((uintptr_t)ep.bias & 15u) == 0u;
     constexpr uint32_t LPR = DUAL ? CB : 2u * CB;        /* groups of 8 columns of a row */
+    constexpr int IT = G * (int)LPR / 4, U = IT % 4 == 0 ? 4 : IT % 2 == 0 ? 2 : 1;
+    uint8_t *sw = fg_lds + wv * (1024u * CB * G);
+    auto spot = [&](uint32_t row, uint32_t q) {
+        return row * RBY + 16u * (q ^ (CB >= 4 ? row & 15u : CB == 2 ? (row >> 1) & 7u : (row >> 2) & 3u));
+    };
+    const uint32_t pc = lane % LPR, c0 = (DUAL ? 8u : 16u) * CB * wc + 8u * pc, n0 = col0 + c0;
+    const uint32_t m0 = row0 + 16u * wr * RB + lane / LPR;
+    /* dual: block c of 16 output columns is staged as gate block 2c, up block 2c + 1 */
+    const uint32_t q0 = DUAL ? 8u * (pc >> 1) + 2u * (pc & 1u) : 2u * pc;
+    constexpr bool BIAS = MODE == GHIP_EP_LINEAR || MODE == GHIP_EP_DLINEAR;
+    constexpr bool IN = BIAS || MODE == GHIP_EP_DGATED;
+    uint16_t *out = second ? ep.out2 : ep.out;
+    /* 16-byte accesses: whole pieces of 8 columns (the last one's padding is the
+     * output's own where ep.pad says so) */
+    const bool vec = (((uintptr_t)out | (uintptr_t)ep.out2) & 15u) == 0u && (ep.ldout & 7u) == 0u
+                     && (p.N & 7u) == 0u
+                     && (!IN || (((uintptr_t)ep.in & 15u) == 0u && (ep.ldin & 7u) == 0u))
+                     && (!BIAS || ((uintptr_t)ep.bias & 15u) == 0u);
+    float bias[8] = {};
+    if constexpr (BIAS)
+        if (ep.bias && vec && c0 < cols) fg_unpack(*(const ghip_u32x4 *)(ep.bias + n0), bias);
     ghip_with_act(MODE == GHIP_EP_STORE ? GHIP_ACT_NONE : ep.act, [&](auto act) {
+        auto values = [&](uint32_t lr, const float (&in)[8], float (&o0)[8], float (&o1)[8]) {
+            float s0[8], s1[8] = {};
+            auto read8 = [&](uint32_t q, float (&v)[8]) {
 #pragma unroll
-        for (int r = 0; r < RB; r++) {
+                for (uint32_t d = 0; d < 2; d++) {
+                    const ghip_f32x4 x = *(const ghip_f32x4 *)(sw + spot(lr, q + d));
 #pragma unroll
-            for (uint32_t c = 0; c < CB; c++) *(ghip_f32x4 *)(sw + spot(n, 4u * c + g)) = acc[r][c];
+                    for (int e = 0; e < 4; e++) v[4 * d + e] = x[e];
+                }
+            };
+            read8(q0, s0);
+            if constexpr (DUAL) read8(q0 + 4u, s1);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                ghip_ep_value<MODE, decltype(act)::value>(s0[e], s1[e], bias[e], in[e], ep.limit,
+                                                          o0[e], o1[e]);
+        };
+#pragma unroll
+        for (int rg = 0; rg < RB; rg += G) {
+#pragma unroll
+            for (int r = 0; r < G; r++)
+#pragma unroll
+                for (uint32_t c = 0; c < CB; c++)
+                    *(ghip_f32x4 *)(sw + spot(16u * r + n, 4u * c + g)) = acc[rg + r][c];
             __builtin_amdgcn_s_waitcnt(0xc07f);
             __builtin_amdgcn_wave_barrier();
+            const uint32_t mg = m0 + 16u * rg;           /* this lane's first row */
+            if (vec) {
 #pragma unroll 1
-            for (uint32_t v = lane; v < 16u * LPR; v += 64u) {
-                const uint32_t lr = v / LPR, pc = v % LPR;
-                auto read8 = [&](uint32_t first, float (&s)[8]) {
+                for (int it = 0; it < IT; it += U) {
+                    ghip_u32x4 d[U];
+                    if constexpr (IN)
+                        if (ep.in) {
 #pragma unroll
-                    for (uint32_t d = 0; d < 2; d++) {
-                        const ghip_f32x4 x = *(const ghip_f32x4 *)(sw + spot(lr, first + d));
+                            for (int u = 0; u < U; u++) {
+                                const uint32_t m = min(mg + (it + u) * (64u / LPR), p.M - 1u);
+                                d[u] = *(const ghip_u32x4 *)(ep.in + (size_t)m * ep.ldin
+                                                             + min(n0, p.N - 8u));
+                            }
+                        }
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[4 * d + e] = x[e];
+                    for (int u = 0; u < U; u++) {
+                        const uint32_t dr = (it + u) * (64u / LPR), m = mg + dr;
+                        float in[8] = {}, o0[8], o1[8];
+                        if constexpr (IN)
+                            if (ep.in) fg_unpack(d[u], in);
+                        values(lane / LPR + dr, in, o0, o1);
+                        if (m < p.M && c0 < cols) {
+                            *(ghip_u32x4 *)(out + (size_t)m * ep.ldout + n0) = fg_pack(o0);
+                            if constexpr (MODE == GHIP_EP_DGATED)
+                                *(ghip_u32x4 *)(ep.out2 + (size_t)m * ep.ldout + n0) = fg_pack(o1);
+                        }
                     }
-                };
-                /* dual: column block c of 16 is staged as gate block 2c, up block 2c + 1 */
-                float s0[8], s1[8] = {};
-                const uint32_t q0 = DUAL ? 8u * (pc >> 1) + 2u * (pc & 1u) : 2u * pc;
-                read8(q0, s0);
-                if constexpr (DUAL) read8(q0 + 4u, s1);
-                const uint32_t m = row0 + 16u * (wr * RB + r) + lr;
-                const uint32_t c0 = (DUAL ? 8u : 16u) * CB * wc + 8u * pc;
-                if (m < p.M && c0 < cols)
-                    fg_store8<MODE, decltype(act)::value>(ep, out, m, col0 + c0, p.N, s0, s1, vin,
-                                                          vout, vbias);
+                }
+            } else {
+                /* any width and alignment: a column a lane, so that accesses of
+                 * 2 bytes still run along a row; columns up to the next multiple
+                 * of 8 get zeros where they are the output's own */
+                constexpr uint32_t WD = DUAL ? 8u * CB : 16u * CB;
+                const uint32_t end = ep.pad ? (p.N + 7u) & ~7u : p.N;
+#pragma unroll 4
+                for (uint32_t it = 0; it < 16u * G * WD / 64u; it++) {
+                    const uint32_t v = lane + 64u * it, lr = v / WD, cc = v % WD;
+                    const uint32_t m = row0 + 16u * (wr * RB + rg) + lr, nn = col0 + WD * wc + cc;
+                    const uint32_t q = DUAL ? 8u * (cc >> 4) + ((cc >> 2) & 3u) : cc >> 2;
+                    const float s0 = *(const float *)(sw + spot(lr, q) + 4u * (cc & 3u));
+                    const float s1 = DUAL ? *(const float *)(sw + spot(lr, q + 4u) + 4u * (cc & 3u)) : 0.0f;
+                    if (m >= p.M || nn >= end) continue;
+                    if (nn < p.N) {
+                        ghip_ep_store<MODE, decltype(act)::value>(ep, out, m, nn, s0, s1);
+                    } else {
+                        out[(size_t)m * ep.ldout + nn] = 0;
+                        if constexpr (MODE == GHIP_EP_DGATED) ep.out2[(size_t)m * ep.ldout + nn] = 0;
+                    }
+                }
             }
             __builtin_amdgcn_s_waitcnt(0xc07f);
             __builtin_amdgcn_wave_barrier();

@@ -1,36 +1,43 @@
 /*
  * k_ffn_nt.hip — the forward products (x and W both with k as the fast index)
- * on tiles: y = act(x W^T + b) + r and h = act(x Wg^T) * (x Wu^T), BF16 or
- * FP8-block weights. The kernel is k_ffn_gemm.h's.
+ * on tiles: y = act(x W^T + b) + r and h = act(x Wg^T) * (x Wu^T), BF16 weights.
+ * The kernel is k_ffn_gemm.h's.
  */
 #include "k_ffn_tile.h"
 
-template <int MODE>
-static const GhipFfnTile *bf16_tiles(int *n) {
+static const GhipFfnTile *linear_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<MODE, 0, 0, 0, 8, 8, 2>(1.50f), fg_tile<MODE, 0, 0, 0, 8, 4, 2>(0.90f),
-        fg_tile<MODE, 0, 0, 0, 4, 4, 4>(0.55f), fg_tile<MODE, 0, 0, 0, 2, 4, 5>(0.40f),
-        fg_tile<MODE, 0, 0, 0, 2, 2, 6>(0.30f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 8, 8, 2>(0.99f, 1.39f, 9.6f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 6, 8, 2>(0.87f, 1.12f, 4.2f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 6, 4, 2>(0.59f, 0.76f, 0.0f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 4, 4, 4>(0.38f, 0.54f, 1.1f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 4, 4, 2>(0.47f, 0.98f, 0.0f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 4, 5>(0.32f, 0.38f, 0.0f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 2, 6>(0.22f, 0.25f, 0.8f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 2, 3>(0.20f, 0.42f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;
 }
 
-template <int MODE, int W8>
-static const GhipFfnTile *fp8_tiles(int *n) {
+static const GhipFfnTile *gated_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<MODE, W8, 0, 0, 8, 8, 2>(1.60f), fg_tile<MODE, W8, 0, 0, 8, 4, 3>(1.00f),
-        fg_tile<MODE, W8, 0, 0, 4, 4, 4>(0.60f), fg_tile<MODE, W8, 0, 0, 2, 4, 5>(0.45f),
-        fg_tile<MODE, W8, 0, 0, 2, 2, 6>(0.32f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 8, 8, 2>(1.02f, 1.35f, 6.1f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 6, 8, 2>(1.01f, 1.13f, 0.9f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 8, 4, 2>(0.73f, 0.87f, 0.5f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 6, 4, 2>(0.69f, 0.76f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 5, 4, 2>(0.68f, 0.74f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 4, 4, 4>(0.39f, 0.53f, 0.8f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 4, 4, 2>(0.58f, 0.94f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 4, 5>(0.39f, 0.39f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 2, 6>(0.26f, 0.25f, 0.4f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 2, 3>(0.25f, 0.44f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;
 }
 
 extern "C" const GhipFfnTile *ghip_ffn_forward_tiles(int mode, int w8, int *n) {
-    if (mode == GHIP_EP_GATED)
-        return w8 == 2 ? fp8_tiles<GHIP_EP_GATED, 2>(n)
-               : w8    ? fp8_tiles<GHIP_EP_GATED, 1>(n) : bf16_tiles<GHIP_EP_GATED>(n);
-    return w8 == 2 ? fp8_tiles<GHIP_EP_LINEAR, 2>(n)
-           : w8    ? fp8_tiles<GHIP_EP_LINEAR, 1>(n) : bf16_tiles<GHIP_EP_LINEAR>(n);
+    if (w8) return ghip_ffn_fp8_tiles(mode, w8, n);
+    return mode == GHIP_EP_GATED ? gated_tiles(n) : linear_tiles(n);
 }

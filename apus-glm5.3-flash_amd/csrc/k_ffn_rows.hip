@@ -107,11 +107,11 @@ static float fr_estimate(const FrForm &c, const GhipProd *p, bool dual, uint32_t
     return (float)(2.3 + (t > hbm ? t + 0.1 * hbm : hbm + 0.1 * t));
 }
 
-/* 16-byte pieces of the weights' rows (FP8 16 codes, BF16 8 values), 32-bit
- * offsets inside a wave's rows */
+/* Whole 16-byte pieces of x's rows (FP8 weight rows then start at 8 bytes, and
+ * have 16 codes to read a half piece from), 32-bit offsets inside a wave's rows */
 extern "C" int ghip_ffn_rows_fits(int mode, const GhipProd *p) {
     return (mode == GHIP_EP_LINEAR || mode == GHIP_EP_GATED) && p->aks == 1 && p->bks == 1
-        && p->brs == p->K && p->K % (p->s ? 16 : 8) == 0 && p->K <= (1u << 24) && p->ars % 8 == 0
+        && p->brs == p->K && p->K % 8 == 0 && (!p->s || p->K >= 16) && p->K <= (1u << 24) && p->ars % 8 == 0
         && p->ars <= (1u << 24) && p->M <= 0x7fffffffu && p->N <= 0x7fffffffu
         && (((uintptr_t)p->a | (uintptr_t)p->b | (uintptr_t)p->b2) & 15) == 0;
 }

@@ -3,8 +3,8 @@
  * (gfx950), as k_rows.hip (plain: MODE GHIP_EP_STORE) and k_ffn_rows.hip (with
  * an epilogue, one or two weight matrices) instantiate it. k_rows.hip's header
  * describes it. With an epilogue:
- *   - x's rows may be apart, and K need only be whole 16-byte pieces of the
- *     weights: the chunk that K cuts is completed with zeros in LDS;
+ *   - x's rows may be apart, and K need only be a multiple of 8: the chunk that
+ *     K cuts is completed with zeros in LDS;
  *   - dual modes: a wave's weight groups alternate between gate and up, so that
  *     one pass of x serves both and the reduction finds g and u of a column
  *     side by side;
@@ -30,6 +30,9 @@ constexpr uint32_t rw_lds() {
     const uint32_t red = RW_NW * MR * 16u * NT * 4u;
     return ring > red ? ring : red;
 }
+
+/* Weight rows of FP8 may start at any 8 bytes (the forms with an epilogue). */
+typedef ghip_u32x4 rw_u32x4 __attribute__((aligned(8)));
 
 /* What the forms with an epilogue take besides: the up projection of the dual
  * modes, x's row stride, and the epilogue. */
@@ -65,7 +68,10 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
     const uint32_t KB = BF ? 2u * K : K;                 /* weight row stride, bytes */
     const uint32_t nch = EPI ? (KB + 127u) >> 7 : KB >> 7, nkb = EPI ? (K + 127u) >> 7 : K >> 7;
     const uint32_t ldx = EPI ? more.ldx : K;
-    const uint32_t end = EPI ? (KB & 127u) >> 4 : 0u;    /* pieces of a last chunk that K cuts */
+    /* pieces of a last chunk that K cuts; FP8 with K % 16 == 8: the last one is
+     * half */
+    const uint32_t end = EPI ? ((KB & 127u) + 15u) >> 4 : 0u;
+    const bool half = EPI && !BF && (K & 8u);
     const uint32_t part = wv % KS, slot = wv / KS;
     const uint32_t c0 = part * nch / KS, c1 = (part + 1u) * nch / KS, nc = c1 - c0;
     const uint32_t blk = blk0 + blockIdx.x, grp = blk * GPP + slot, row0 = grp * (16u * OG);
@@ -132,8 +138,16 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
         /* the chunk that K cuts: pieces past it are read at the chunk's start and
          * put into LDS as zeros, on both sides */
         const uint32_t q0 = (lane & 7u) ^ ((lane >> 4) & 7u), q1 = (lane & 7u) ^ ((4u + (lane >> 4)) & 7u);
-        const uint32_t xend = BF ? end : 2u * end;
+        const uint32_t xend = BF ? end : 2u * end - (half ? 1u : 0u);
         auto cut = [&](uint32_t c) { return EPI && end && c == nch - 1u; };
+        /* the half piece is read 8 bytes early, where its row has them (in the
+         * chunk before where it is the chunk's first); pieces past K as the
+         * chunk's first one */
+        auto from = [&](uint32_t c, const uint8_t *wb, uint32_t off, uint32_t q) {
+            const bool past = cut(c) && q >= end;
+            const bool early = cut(c) && half && (past ? 0u : q) == end - 1u;
+            return (const rw_u32x4 *)(wb + (past ? off - 16u * q : off) - (early ? 8 : 0));
+        };
         ghip_u32x4 xr[NA][XI], wr[NA][2 * NT];
         auto load = [&](auto set_c, uint32_t c) {
             constexpr int A = decltype(set_c)::value;
@@ -144,10 +158,8 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
 #pragma unroll
             for (int b = 0; b < NT; b++) {
                 const uint8_t *wb = DUAL && (b & 1) ? rows2 + (size_t)c * 128u : wc;
-                const uint32_t f0 = cut(c) && q0 >= end ? d[b].off0 - 16u * q0 : d[b].off0;
-                const uint32_t f1 = cut(c) && q1 >= end ? d[b].off1 - 16u * q1 : d[b].off1;
-                wr[A][2 * b] = __builtin_nontemporal_load((const ghip_u32x4 *)(wb + f0));
-                wr[A][2 * b + 1] = __builtin_nontemporal_load((const ghip_u32x4 *)(wb + f1));
+                wr[A][2 * b] = __builtin_nontemporal_load(from(c, wb, d[b].off0, q0));
+                wr[A][2 * b + 1] = __builtin_nontemporal_load(from(c, wb, d[b].off1, q1));
             }
             __builtin_amdgcn_sched_barrier(0);
         };
@@ -164,8 +176,12 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
                     if (xq[u] >= xend) xr[A][u] = zero;
 #pragma unroll
                 for (int b = 0; b < NT; b++) {
-                    if (q0 >= end) wr[A][2 * b] = zero;
-                    if (q1 >= end) wr[A][2 * b + 1] = zero;
+                    auto tail = [&](uint32_t q, ghip_u32x4 &v) {
+                        if (q >= end) v = zero;
+                        else if (half && q == end - 1u) v = (ghip_u32x4){v[2], v[3], 0u, 0u};
+                    };
+                    tail(q0, wr[A][2 * b]);
+                    tail(q1, wr[A][2 * b + 1]);
                 }
             }
 #pragma unroll
@@ -297,11 +313,11 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
                     if (DUAL) s1 += p[16];
                 }
                 if constexpr (EARLY)
-                    ghip_ep_put<MODE, decltype(act)::value>(more.ep, m0 + m, o, s0, s1,
+                    ghip_ep_put<MODE, decltype(act)::value>(more.ep, more.ep.out, m0 + m, o, s0, s1,
                                                             ghip_bf16_f32(ebias[i]),
                                                             ghip_bf16_f32(ein[i]));
                 else
-                    ghip_ep_store1<MODE, decltype(act)::value>(more.ep, m0 + m, o, s0, s1);
+                    ghip_ep_store<MODE, decltype(act)::value>(more.ep, more.ep.out, m0 + m, o, s0, s1);
             }
         });
     }

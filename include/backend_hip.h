@@ -386,8 +386,10 @@ int apus_ghip_moe_prefill_dev_noalloc(ApusGhipStore *s, const uint16_t *x, size_
  *     negative or NaN, a stream of another device, a workspace that is too
  *     small; apus_ghip_last_error), nothing or only a part launched.
  *   - Alignment: 16-byte aligned pointers and strides of whole 16 bytes, with
- *     K % 8 == 0 (K % 16 == 0 for FP8), take the vector kernels; everything
- *     else a slower general one (same results within the tolerance). */
+ *     K % 8 == 0 (from a few dozen rows on K % 16 == 0 for FP8), take the
+ *     kernels with direct loads; everything else a slower general one (same
+ *     results within the tolerance). Outputs, bias and residual may have any
+ *     alignment. */
 enum {
     APUS_GHIP_ACT_NONE = 0,
     APUS_GHIP_ACT_RELU = 1,
@@ -417,9 +419,10 @@ int apus_ghip_fp8blk_gated_dev(const uint8_t *gate_codes, const float *gate_scal
  * each BF16, each left out where its pointer is NULL (not all). The residual's
  * gradient is dy. dz is rounded to BF16 once, as the products' operand. ws:
  * 16-byte aligned device memory of at least
- * apus_ghip_linear_ep_backward_ws(M, O, K) bytes that no overlapping call uses
- * (not needed, may be NULL, with act NONE); the call leaves nothing in it that
- * a later one reads. */
+ * apus_ghip_linear_ep_backward_ws(M, O, K) bytes that no overlapping call uses;
+ * the call leaves nothing in it that a later one reads. With act NONE it may
+ * be NULL; given, rows of dy that are not whole aligned vectors are laid out in
+ * it for the faster kernels. */
 size_t apus_ghip_linear_ep_backward_ws(size_t M, size_t O, size_t K);
 int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
                                           const uint16_t *bias, const uint16_t *dy, uint16_t *dx,

@@ -73,7 +73,7 @@ def seed(*a):
 
 
 # M, N, K: one row, a few, tiles and their edges, K of one step and of ragged ends
-SHAPES = [(1, 1, 1), (1, 5, 8), (1, 300, 2048), (2, 4096, 128), (3, 257, 100), (4, 1000, 4096), (5, 96, 264), (7, 2050, 640),
+SHAPES = [(1, 1, 1), (1, 5, 8), (1, 300, 2048), (2, 4096, 128), (3, 257, 100), (4, 1000, 4096), (5, 96, 264), (2, 200, 1080), (9, 77, 24), (1, 40, 8), (7, 2050, 640),
           (8, 129, 1536), (13, 64, 64), (16, 768, 192), (17, 33, 31), (31, 520, 1000), (33, 1025, 576), (64, 512, 1024),
           (65, 255, 72), (100, 2048, 512), (129, 130, 131), (200, 1537, 320), (255, 257, 256), (256, 256, 64), (300, 520, 1088),
           (513, 1032, 136), (700, 2049, 192), (1111, 640, 448), (2049, 1030, 256)]
