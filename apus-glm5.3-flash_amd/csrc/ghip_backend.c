@@ -712,12 +712,20 @@ static size_t ffn_ws_mat(size_t M, size_t N) {
     return (M * ffn_ws_ld(N) * 2 + 255) & ~(size_t)255;
 }
 
+/* The products' partial sums come behind them: as much as dx or dW may use. */
+static size_t ffn_ws_part(size_t M, size_t N, size_t K, size_t n) {
+    const size_t dx = ghip_ffn_part_bytes(M, K, n * N), dw = ghip_ffn_part_bytes(n * N, K, M);
+    return dx > dw ? dx : dw;
+}
+
 size_t apus_ghip_linear_ep_backward_ws(size_t M, size_t O, size_t K) {
-    return K ? ffn_ws_mat(M, O) : 0;
+    const size_t mat = K && K <= 0x7fffffffu ? ffn_ws_mat(M, O) : 0;
+    return mat ? mat + ffn_ws_part(M, O, K, 1) : 0;
 }
 
 size_t apus_ghip_gated_backward_ws(size_t M, size_t I, size_t K) {
-    return K ? 2 * ffn_ws_mat(M, I) : 0;
+    const size_t mat = K && K <= 0x7fffffffu ? 2 * ffn_ws_mat(M, I) : 0;
+    return mat ? mat + ffn_ws_part(M, I, K, 2) : 0;
 }
 
 static int check_ws(const void *ws, size_t have, size_t need) {
@@ -729,10 +737,10 @@ static int check_ws(const void *ws, size_t have, size_t need) {
 /* dx = dz W (+ dz2 W2), dw = dz^T x. */
 static int ffn_dx(const uint16_t *dz, const uint16_t *dz2, size_t lddz, const uint16_t *w,
                   const uint16_t *w2, uint16_t *dx, size_t M, size_t N, size_t K, size_t lddx,
-                  int apad, hipStream_t st) {
+                  int apad, void *part, size_t part_bytes, hipStream_t st) {
     const GhipProd p = { .a = dz, .a2 = dz2, .b = w, .b2 = w2, .ars = lddz, .aks = 1, .brs = 1,
                          .bks = K, .M = (uint32_t)M, .N = (uint32_t)K, .K = (uint32_t)N,
-                         .apad = apad };
+                         .apad = apad, .part = (float *)part, .part_bytes = part_bytes };
     const GhipEp ep = { .out = dx, .ldout = lddx };
     HIPCHK(ghip_launch_ffn(GHIP_EP_STORE, &p, &ep, st));
     return 0;
@@ -741,10 +749,11 @@ static int ffn_dx(const uint16_t *dz, const uint16_t *dz2, size_t lddz, const ui
 /* dw2, dz2: a second one beside it, in the same launch. */
 static int ffn_dw(const uint16_t *dz, const uint16_t *dz2, size_t lddz, const uint16_t *x,
                   size_t ldx, uint16_t *dw, uint16_t *dw2, size_t M, size_t N, size_t K, int apad,
-                  hipStream_t st) {
+                  void *part, size_t part_bytes, hipStream_t st) {
     const GhipProd p = { .a = dz, .a2 = dz2, .b = x, .b2 = dz2 ? x : NULL, .ars = 1, .aks = lddz,
                          .brs = 1, .bks = ldx, .M = (uint32_t)N, .N = (uint32_t)K,
-                         .K = (uint32_t)M, .batch = dz2 != NULL, .apad = apad };
+                         .K = (uint32_t)M, .batch = dz2 != NULL, .apad = apad,
+                         .part = (float *)part, .part_bytes = part_bytes };
     const GhipEp ep = { .out = dw, .out2 = dw2, .ldout = K };
     HIPCHK(ghip_launch_ffn(GHIP_EP_STORE, &p, &ep, st));
     return 0;
@@ -760,7 +769,7 @@ int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
     if (check_sizes(M, O, K) || check_act(act, 0.0f) || check_ptr("dy", dy)
         || ((dx || again) && check_ptr("weights", w)) || ((dw || again) && check_ptr("x", x))
         || check_ld("ldx", &ldx, K) || check_ld("lddy", &lddy, O) || check_ld("lddx", &lddx, K)
-        || (again && check_ws(ws, ws_bytes, ffn_ws_mat(M, O))))
+        || ((again || ws) && check_ws(ws, ws_bytes, apus_ghip_linear_ep_backward_ws(M, O, K))))
         return 1;
     if (!dx && !dw && !dbias) {
         ghip_seterr("no gradient asked for");
@@ -783,15 +792,17 @@ int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
     /* without an activation dz is dy; rows that the products cannot load as
      * vectors are laid out again where there is room */
     int pad = again;
-    if (!again && (dx || dw) && ws && check_ws(ws, ws_bytes, ffn_ws_mat(M, O)) == 0 && K % 8 == 0
+    if (!again && (dx || dw) && ws && K % 8 == 0
         && (((uintptr_t)dy & 15) || lddy % 8 || O % 8)) {
         HIPCHK(ghip_launch_ffn_pack(dy, lddy, M, O, (uint16_t *)ws, st));
         dz = (const uint16_t *)ws;
         lddz = ffn_ws_ld(O);
         pad = 1;
     }
-    if (dx && ffn_dx(dz, NULL, lddz, w, NULL, dx, M, O, K, lddx, pad, st)) return 1;
-    if (dw && ffn_dw(dz, NULL, lddz, x, ldx, dw, NULL, M, O, K, pad, st)) return 1;
+    const size_t mat = ffn_ws_mat(M, O), part_bytes = ws ? ffn_ws_part(M, O, K, 1) : 0;
+    void *part = part_bytes ? (uint8_t *)ws + mat : NULL;
+    if (dx && ffn_dx(dz, NULL, lddz, w, NULL, dx, M, O, K, lddx, pad, part, part_bytes, st)) return 1;
+    if (dw && ffn_dw(dz, NULL, lddz, x, ldx, dw, NULL, M, O, K, pad, part, part_bytes, st)) return 1;
     if (dbias) HIPCHK(ghip_launch_ffn_colsum(dz, lddz, M, O, dbias, st));
     G.dispatches++;
     return 0;
@@ -806,7 +817,7 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
     if (check_sizes(M, I, K) || check_act(act, limit) || check_ptr("gate weights", wg)
         || check_ptr("up weights", wu) || check_ptr("x", x) || check_ptr("dh", dh)
         || check_ld("ldx", &ldx, K) || check_ld("lddh", &lddh, I) || check_ld("lddx", &lddx, K)
-        || check_ws(ws, ws_bytes, 2 * ffn_ws_mat(M, I)))
+        || check_ws(ws, ws_bytes, apus_ghip_gated_backward_ws(M, I, K)))
         return 1;
     if (!dx && !dwg && !dwu) {
         ghip_seterr("no gradient asked for");
@@ -822,11 +833,14 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
     const GhipEp ep = { .in = dh, .out = dg, .out2 = du, .ldin = lddh, .ldout = ld, .act = act,
                         .limit = limit > 0.0f ? limit : INFINITY, .pad = 1 };
     HIPCHK(ghip_launch_ffn(GHIP_EP_DGATED, &p, &ep, st));
-    if (dx && ffn_dx(dg, du, ld, wg, wu, dx, M, I, K, lddx, 1, st)) return 1;
-    if (dwg && dwu) {
-        if (ffn_dw(dg, du, ld, x, ldx, dwg, dwu, M, I, K, 1, st)) return 1;
-    } else if (dwg || dwu) {
-        if (ffn_dw(dwg ? dg : du, NULL, ld, x, ldx, dwg ? dwg : dwu, NULL, M, I, K, 1, st)) return 1;
+    const size_t part_bytes = ffn_ws_part(M, I, K, 2);
+    void *part = part_bytes ? (uint8_t *)ws + 2 * ffn_ws_mat(M, I) : NULL;
+    if (dx && ffn_dx(dg, du, ld, wg, wu, dx, M, I, K, lddx, 1, part, part_bytes, st)) return 1;
+    if (dwg || dwu) {
+        const int both = dwg && dwu;
+        if (ffn_dw(dwg ? dg : du, both ? du : NULL, ld, x, ldx, dwg ? dwg : dwu, both ? dwu : NULL,
+                   M, I, K, 1, part, part_bytes, st))
+            return 1;
     }
     G.dispatches++;
     return 0;

@@ -293,6 +293,11 @@ typedef struct {
     size_t ars, aks, brs, bks;
     uint32_t M, N, K;
     int exact, batch, apad;
+    /* GHIP_EP_STORE on tiles: part, 16-byte aligned f32 memory of part_bytes (or NULL) in which
+     * the k range may be split; splits is the launcher's */
+    float *part;
+    size_t part_bytes;
+    uint32_t splits;
 } GhipProd;
 
 /* Any shape, stride and alignment. */
@@ -309,15 +314,18 @@ hipError_t ghip_launch_ffn_pack(const uint16_t *src, size_t ld, size_t M, size_t
 /* On tiles (k_ffn_gemm.h): fits = the steps and alignments of the vector loads;
  * pick = the tile shape with the least estimated time (microseconds, in us). */
 int ghip_ffn_gemm_fits(int mode, const GhipProd *p);
-int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us);
-hipError_t ghip_launch_ffn_gemm(int mode, int tile, const GhipProd *p, const GhipEp *ep,
-                                hipStream_t st);
+int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us, uint32_t *splits);
+hipError_t ghip_launch_ffn_gemm(int mode, int tile, uint32_t splits, const GhipProd *p,
+                                const GhipEp *ep, hipStream_t st);
+/* Bytes of part that a product of M x N outputs over K may use. */
+size_t ghip_ffn_part_bytes(size_t M, size_t N, size_t K);
 /* One family of its kernels: the tiles of a mode (k_ffn_nt.hip, k_ffn_nt8.hip, k_ffn_bwd.hip). */
 typedef struct {
     uint32_t bm, bn;             /* output rows and columns */
     uint32_t occ;                /* workgroups a CU holds */
-    float low, full, over;       /* microseconds: a stage on a nearly empty and on a full chip,
-                                    and a round's first loads and epilogue */
+    float low, mid, full, over;  /* microseconds: a stage on a nearly empty chip, with one
+                                    workgroup a CU where it holds two, and on a full chip; and a
+                                    round's first loads and epilogue */
     uint32_t lds;
     const void *kern;
     void (*launch)(const GhipProd *, const GhipEp *, uint32_t, uint32_t, uint32_t, hipStream_t);

@@ -1,6 +1,8 @@
 /*
  * k_ffn.hip — which kernel a dense feed-forward product takes (gfx950).
  */
+#include <math.h>
+
 #include "ghip_epilogue.h"
 
 static uint32_t g_ffn_ncu;                       /* CUs: the routes' rounds */
@@ -32,47 +34,135 @@ extern "C" int ghip_ffn_gemm_fits(int mode, const GhipProd *p) {
         || !vectors(p->b, p->brs, p->bks, p->N, p->K, per, false))
         return 0;
     if ((p->a2 && ((uintptr_t)p->a2 & 15)) || (p->b2 && ((uintptr_t)p->b2 & 15))) return 0;
-    /* the smallest tile's grid: under 2^32 threads */
-    return ((size_t)(p->M + 63) / 64) * ((size_t)(p->N + 63) / 64) * 2 * 256 <= GHIP_MAX_THREADS;
+    /* the smallest tile's grid, two products of 16 splits: under 2^32 threads */
+    return ((size_t)(p->M + 63) / 64) * ((size_t)(p->N + 63) / 64) * 2 * 256 * 16 <= GHIP_MAX_THREADS;
 }
 
-extern "C" int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us) {
+/* Splits of k are for products of few tiles over a long k (dx of a wide block,
+ * dW of many rows): each split's f32 sums go to memory and are added in order
+ * by k_ffn_join. At most 16, of at least 8 stages, and 32 MiB of sums. */
+#define FFN_MAX_SPLITS 16u
+#define FFN_PART_BYTES ((size_t)32 << 20)
+
+extern "C" size_t ghip_ffn_part_bytes(size_t M, size_t N, size_t K) {
+    const size_t row = (N + 7) & ~(size_t)7, most = K / 512;
+    if (M == 0 || N == 0 || row > FFN_PART_BYTES / 4 / M) return 0;
+    const size_t one = M * row * 4;
+    size_t n = FFN_PART_BYTES / one;
+    if (n > most) n = most;
+    if (n > FFN_MAX_SPLITS) n = FFN_MAX_SPLITS;
+    return n < 2 ? 0 : (n * one + 255) & ~(size_t)255;
+}
+
+/* Estimated microseconds of a tile on n_cu CUs: 3 for the launch, and for each
+ * round of the chip the stages and what a round costs besides. A round that
+ * does not fill the chip runs at a time between the empty chip's and the full
+ * one's; where a CU holds two workgroups, the few that share a CU set the
+ * round's time long before all do. */
+static double tile_us(const GhipFfnTile *t, const GhipProd *p, double stages, uint32_t splits,
+                      uint32_t n_cu) {
+    const double wgs = (double)((p->M + t->bm - 1) / t->bm) * (double)((p->N + t->bn - 1) / t->bn)
+                       * (p->batch ? 2 : 1) * splits;
+    const double cap = (double)n_cu * t->occ, whole = (double)(size_t)(wgs / cap);
+    const double part = wgs / cap - whole;               /* of the last round */
+    double us = t->low + (t->full - t->low) * part;
+    if (t->occ == 2)
+        us = part <= 0.5 ? t->low + (t->mid - t->low) * 2.0 * part
+                         : t->mid + (t->full - t->mid) * sqrt(2.0 * part - 1.0);
+    return 3.0 + whole * (stages * t->full + t->over) + (part > 0.0 ? stages * us + t->over : 0.0);
+}
+
+extern "C" int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us,
+                                  uint32_t *splits) {
     int n, best = 0;
     const GhipFfnTile *t = tiles_of(mode, p, &n);
     const double stages = (double)((p->K + 63) / 64) * (p->a2 && !p->batch ? 2 : 1);
-    for (int i = 0; i < n; i++) {
-        const double wgs = (double)((p->M + t[i].bm - 1) / t[i].bm)
-                           * (double)((p->N + t[i].bn - 1) / t[i].bn) * (p->batch ? 2 : 1);
-        const double cap = (double)n_cu * t[i].occ, whole = (double)(size_t)(wgs / cap);
-        const double part = wgs / cap - whole;           /* of the last round */
-        const double e64 = 3.0 + whole * (stages * t[i].full + t[i].over)
-                           + (part > 0.0 ? stages * (t[i].low + (t[i].full - t[i].low) * part) + t[i].over : 0.0);
-        const float e = (float)e64;
-        if (i == 0 || e < *us) {
-            best = i;
-            *us = e;
-        }
+    const size_t cells = (size_t)p->M * (((size_t)p->N + 7) & ~(size_t)7) * (p->batch ? 2 : 1);
+    uint32_t most = 1;
+    if (mode == GHIP_EP_STORE && p->part) {
+        const size_t fit = p->part_bytes / 4 / cells, len = (size_t)(stages / 8);
+        most = (uint32_t)(fit < len ? fit : len);
+        if (most > FFN_MAX_SPLITS) most = FFN_MAX_SPLITS;
+        if (most < 1) most = 1;
     }
+    *us = 1e30f;
+    for (int i = 0; i < n; i++)
+        for (uint32_t s = 1; s <= most; s++) {
+            /* the sums' way out and back at 3 TB/s, and one more launch */
+            const double join = s > 1 ? 4.0 + (double)cells * 4.0 * s * 2.0 / 3e6 : 0.0;
+            const float e = (float)(tile_us(t + i, p, (double)(size_t)((stages + s - 1) / s), s, n_cu) + join);
+            if (e < *us) {
+                best = i;
+                *us = e;
+                *splits = s;
+            }
+        }
     return best;
 }
 
-extern "C" hipError_t ghip_launch_ffn_gemm(int mode, int tile, const GhipProd *p, const GhipEp *ep,
-                                           hipStream_t st) {
+/* out[m, n] = bf16(sum over the splits of part[s, m, n]), in order. */
+__global__ __launch_bounds__(256) void k_ffn_join(const float *__restrict__ part, uint32_t splits,
+                                                  uint32_t M, uint32_t N, size_t ldout,
+                                                  uint16_t *out, uint16_t *out2) {
+    const uint32_t per = (N + 7u) / 8u;
+    const size_t one = (size_t)M * per * 8u, all = (size_t)M * per * (out2 ? 2u : 1u);
+    for (size_t v = (size_t)blockIdx.x * 256u + threadIdx.x; v < all; v += (size_t)gridDim.x * 256u) {
+        const bool second = v >= (size_t)M * per;
+        const size_t w = second ? v - (size_t)M * per : v, m = w / per;
+        const uint32_t n = (uint32_t)(w % per) * 8u;
+        const float *q = part + (second ? splits * one : 0) + w * 8u;
+        ghip_f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
+#pragma unroll 4
+        for (uint32_t s = 0; s < splits; s++) {
+            a += *(const ghip_f32x4 *)(q + s * one);
+            b += *(const ghip_f32x4 *)(q + s * one + 4);
+        }
+        uint16_t *o = (second ? out2 : out) + m * ldout + n, r[8];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; e++) r[e] = (uint16_t)ghip_bf16_bits(e < 4 ? a[e & 3u] : b[e & 3u]);
+        if (n + 8u <= N) {
+            __builtin_memcpy(o, r, 16);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++)
+                if (n + e < N) o[e] = r[e];
+        }
+    }
+}
+
+extern "C" hipError_t ghip_launch_ffn_gemm(int mode, int tile, uint32_t splits, const GhipProd *p,
+                                           const GhipEp *ep, hipStream_t st) {
     int n;
     const GhipFfnTile *t = tiles_of(mode, p, &n);
-    if (!ghip_ffn_gemm_fits(mode, p) || tile < 0 || tile >= n) return hipErrorInvalidValue;
+    if (!ghip_ffn_gemm_fits(mode, p) || tile < 0 || tile >= n || splits < 1) return hipErrorInvalidValue;
+    const size_t cells = (size_t)p->M * (((size_t)p->N + 7) & ~(size_t)7) * (p->batch ? 2 : 1);
+    const size_t stages = (size_t)((p->K + 63) / 64) * (p->a2 && !p->batch ? 2 : 1);
+    if (splits > 1
+        && (mode != GHIP_EP_STORE || !p->part || splits > stages || splits > p->part_bytes / 4 / cells
+            || ((uintptr_t)p->part & 15)))
+        return hipErrorInvalidValue;
+    GhipProd q = *p;
+    q.splits = splits;
+    if (splits == 1) q.part = nullptr;
     t += tile;
-    t->launch(p, ep, (p->M + t->bm - 1) / t->bm, (p->N + t->bn - 1) / t->bn, t->lds, st);
+    t->launch(&q, ep, (p->M + t->bm - 1) / t->bm, (p->N + t->bn - 1) / t->bn, t->lds, st);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || splits == 1) return e;
+    const size_t blocks = (cells / 8 + 255) / 256;
+    hipLaunchKernelGGL(k_ffn_join, dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st,
+                       q.part, splits, p->M, p->N, ep->ldout, ep->out, p->batch ? ep->out2 : nullptr);
     return hipGetLastError();
 }
 
 extern "C" hipError_t ghip_launch_ffn(int mode, const GhipProd *p, const GhipEp *ep,
                                       hipStream_t st) {
     float us = 1e30f, rows_us = 1e30f;
-    const int tile = g_ffn_ncu && ghip_ffn_gemm_fits(mode, p) ? ghip_ffn_gemm_pick(mode, p, g_ffn_ncu, &us) : -1;
+    uint32_t splits = 1;
+    const int tile = g_ffn_ncu && ghip_ffn_gemm_fits(mode, p)
+                         ? ghip_ffn_gemm_pick(mode, p, g_ffn_ncu, &us, &splits) : -1;
     const int form = g_ffn_ncu && ghip_ffn_rows_fits(mode, p) ? ghip_ffn_rows_pick(mode, p, g_ffn_ncu, &rows_us) : -1;
     if (form >= 0 && rows_us <= us) return ghip_launch_ffn_rows(mode, form, p, ep, st);
-    if (tile >= 0) return ghip_launch_ffn_gemm(mode, tile, p, ep, st);
+    if (tile >= 0) return ghip_launch_ffn_gemm(mode, tile, splits, p, ep, st);
     return ghip_launch_ffn_any(mode, p, ep, st);
 }
 

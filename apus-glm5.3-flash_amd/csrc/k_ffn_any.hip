@@ -148,21 +148,43 @@ __global__ __launch_bounds__(256) void k_ffn_any(GhipProd p, GhipEp ep, uint32_t
 }
 
 /* dbias[n] = sum_m dz[m, n] in f32, rounded once. A workgroup owns 64 columns,
- * its 16 groups of rows are added in a fixed order. */
+ * a thread 8 of them in every 128th row (one load at any alignment); the 128
+ * rows' sums are added in a fixed order. Bound by latency: 300 x 2048 2.5 us
+ * (one column and 16 rows a thread at a time: 7.2). */
 __global__ __launch_bounds__(1024) void k_ffn_colsum(const uint16_t *__restrict__ dz, size_t ld,
                                                      uint32_t M, uint32_t N,
                                                      uint16_t *__restrict__ out) {
-    __shared__ float part[16][64];
-    const uint32_t c = threadIdx.x & 63u, r = threadIdx.x >> 6, n = blockIdx.x * 64u + c;
-    float s = 0.0f;
-    if (n < N)
-        for (uint32_t m = r; m < M; m += 16u) s += ghip_bf16_f32(dz[(size_t)m * ld + n]);
-    part[r][c] = s;
+    __shared__ float sum[128][65];
+    const uint32_t c = 8u * (threadIdx.x & 7u), r = threadIdx.x >> 3, n = blockIdx.x * 64u + c;
+    float s[8] = {};
+    if (n + 8u <= N) {
+#pragma unroll 4
+        for (uint32_t m = r; m < M; m += 128u) {
+            fa_u16x8 d;
+            __builtin_memcpy(&d, dz + (size_t)m * ld + n, 16);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) s[e] += ghip_bf16_f32(d[e]);
+        }
+    } else {
+        for (uint32_t m = r; m < M; m += 128u)
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++)
+                if (n + e < N) s[e] += ghip_bf16_f32(dz[(size_t)m * ld + n + e]);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8; e++) sum[r][c + e] = s[e];
+    /* 16 threads a column, then the first of them */
     __syncthreads();
-    if (r == 0 && n < N) {
-        float v = 0.0f;
-        for (uint32_t i = 0; i < 16; i++) v += part[i][c];
-        out[n] = (uint16_t)ghip_bf16_bits(v);
+    const uint32_t q = threadIdx.x & 63u, g = threadIdx.x >> 6;
+    float v = 0.0f;
+    for (uint32_t i = 0; i < 8; i++) v += sum[8u * g + i][q];
+    __syncthreads();
+    sum[g][q] = v;
+    __syncthreads();
+    if (g == 0 && blockIdx.x * 64u + q < N) {
+        v = 0.0f;
+        for (uint32_t i = 0; i < 16; i++) v += sum[i][q];
+        out[blockIdx.x * 64u + q] = (uint16_t)ghip_bf16_bits(v);
     }
 }
 

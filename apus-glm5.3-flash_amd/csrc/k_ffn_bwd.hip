@@ -7,15 +7,15 @@
 
 static const GhipFfnTile *dlinear_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 8, 8, 2>(0.99f, 1.39f, 9.6f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 6, 8, 2>(0.87f, 1.12f, 4.2f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 8, 4, 2>(0.65f, 0.88f, 1.9f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 6, 4, 2>(0.59f, 0.76f, 0.0f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 4, 4, 4>(0.38f, 0.54f, 1.1f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 4, 4, 2>(0.47f, 0.98f, 0.0f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 4, 5>(0.32f, 0.38f, 0.0f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 2, 6>(0.22f, 0.25f, 0.8f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 2, 3>(0.20f, 0.42f, 0.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 8, 8, 2>(1.01f, 0.00f, 1.39f, 8.5f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 6, 8, 2>(0.88f, 0.00f, 1.12f, 3.5f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 8, 4, 2>(0.65f, 0.00f, 0.88f, 2.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 6, 4, 2>(0.58f, 0.00f, 0.74f, 0.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 4, 4, 4>(0.40f, 0.00f, 0.54f, 0.9f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 4, 4, 2>(0.49f, 0.66f, 0.97f, 0.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 4, 5>(0.32f, 0.00f, 0.38f, 0.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 2, 6>(0.22f, 0.00f, 0.26f, 0.6f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 2, 3>(0.22f, 0.28f, 0.42f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;
@@ -23,14 +23,14 @@ static const GhipFfnTile *dlinear_tiles(int *n) {
 
 static const GhipFfnTile *dgated_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 8, 8, 2>(1.01f, 1.37f, 15.3f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 6, 8, 2>(1.00f, 1.15f, 8.7f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 6, 4, 2>(0.72f, 0.82f, 2.0f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 4, 4, 4>(0.41f, 0.55f, 3.2f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 4, 4, 2>(0.66f, 1.02f, 0.0f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 4, 5>(0.44f, 0.43f, 0.4f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 2, 6>(0.28f, 0.27f, 1.0f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 2, 3>(0.28f, 0.46f, 0.0f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 8, 8, 2>(1.02f, 0.00f, 1.39f, 15.3f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 6, 8, 2>(1.02f, 0.00f, 1.14f, 8.1f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 6, 4, 2>(0.74f, 0.00f, 0.81f, 1.3f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 4, 4, 4>(0.43f, 0.00f, 0.54f, 2.8f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 4, 4, 2>(0.69f, 0.80f, 1.01f, 0.0f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 4, 5>(0.45f, 0.00f, 0.42f, 0.1f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 2, 6>(0.28f, 0.00f, 0.28f, 1.2f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 2, 3>(0.27f, 0.39f, 0.46f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;
@@ -38,13 +38,12 @@ static const GhipFfnTile *dgated_tiles(int *n) {
 
 static const GhipFfnTile *dx_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 8, 8, 2>(1.01f, 1.42f, 7.0f),
-        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 8, 4, 2>(0.56f, 0.82f, 4.0f),
-        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 4, 4, 4>(0.37f, 0.52f, 2.8f),
-        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 4, 4, 2>(0.33f, 0.92f, 2.8f),
-        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 2, 4, 5>(0.26f, 0.36f, 2.0f),
-        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 2, 2, 6>(0.19f, 0.25f, 1.6f),
-        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 2, 2, 3>(0.16f, 0.42f, 1.2f),
+        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 8, 8, 2>(1.02f, 0.00f, 1.41f, 7.1f),
+        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 8, 4, 2>(0.58f, 0.00f, 0.81f, 4.4f),
+        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 4, 4, 2>(0.38f, 0.49f, 0.93f, 2.9f),
+        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 2, 4, 5>(0.27f, 0.00f, 0.35f, 2.2f),
+        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 2, 2, 6>(0.19f, 0.00f, 0.25f, 1.8f),
+        fg_tile<GHIP_EP_STORE, 0, 0, 1, 2, 2, 2, 3>(0.17f, 0.28f, 0.42f, 1.4f),
     };
     *n = sizeof t / sizeof *t;
     return t;
@@ -52,12 +51,11 @@ static const GhipFfnTile *dx_tiles(int *n) {
 
 static const GhipFfnTile *dw_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 8, 8, 2>(1.09f, 1.51f, 7.1f),
-        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 4, 4, 4>(0.43f, 0.54f, 2.9f),
-        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 4, 4, 2>(0.34f, 0.93f, 2.9f),
-        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 4, 5>(0.28f, 0.36f, 2.1f),
-        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 2, 6>(0.22f, 0.27f, 1.6f),
-        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 2, 3>(0.18f, 0.43f, 1.2f),
+        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 8, 8, 2>(1.11f, 0.00f, 1.49f, 7.4f),
+        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 4, 4, 2>(0.40f, 0.49f, 0.93f, 3.1f),
+        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 4, 5>(0.29f, 0.00f, 0.36f, 2.4f),
+        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 2, 6>(0.23f, 0.00f, 0.28f, 1.9f),
+        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 2, 3>(0.24f, 0.23f, 0.44f, 1.5f),
     };
     *n = sizeof t / sizeof *t;
     return t;

@@ -166,7 +166,7 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
      * tiles, which go down 4 row tiles before the next column, so that an XCD's
      * L2 holds few rows of A and of B at a time (8192 x 24576 x 4096: 4 1.148
      * ms, 8 1.157, 16 1.18). A batch of two: the second half of the tiles is the
-     * second product. */
+     * second product. Splits of k: each walks its share of the stages. */
     uint32_t t;
     {
         const uint32_t T = gridDim.x, x = blockIdx.x & 7u, i = blockIdx.x >> 3;
@@ -174,16 +174,22 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
         t = x * q + (x < r ? x : r) + i;
     }
     bool second = false;
+    uint32_t split = 0;
     if constexpr (MODE == GHIP_EP_STORE) {
-        second = p.batch && t >= mt * nt;
-        if (second) t -= mt * nt;
+        split = t / (mt * nt);
+        t -= split * (mt * nt);
+        second = p.batch && split >= p.splits;
+        if (second) split -= p.splits;
     }
     const uint32_t strip = t / (4u * nt), in_strip = t - strip * (4u * nt);
     const uint32_t sr = min(4u, mt - strip * 4u);
     const uint32_t row0 = (strip * 4u + in_strip % sr) * BM, col0 = in_strip / sr * OUTN;
     const uint32_t rows = min(p.M - row0, BM), cols = min(p.N - col0, OUTN);
     const uint32_t nst1 = (p.K + 63u) >> 6;              /* stages of one product */
-    const uint32_t nst = MODE == GHIP_EP_STORE && p.a2 && !p.batch ? 2u * nst1 : nst1;
+    const uint32_t all = MODE == GHIP_EP_STORE && p.a2 && !p.batch ? 2u * nst1 : nst1;
+    const uint32_t j0 = MODE == GHIP_EP_STORE ? (uint32_t)((uint64_t)all * split / p.splits) : 0u;
+    const uint32_t nst =                                 /* of this split */
+        MODE == GHIP_EP_STORE ? (uint32_t)((uint64_t)all * (split + 1u) / p.splits) - j0 : all;
     const size_t astep = AL == 0 ? 128u : (size_t)p.aks * 128u;
     const size_t bstep = BL == 0 ? (FP8 ? 64u : 128u) : (size_t)p.bks * 128u;
     const uint32_t lda = (uint32_t)(AL == 0 ? p.ars : p.aks);
@@ -199,8 +205,14 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
                + (BL == 0 ? (size_t)col0 * p.brs : col0) * (FP8 ? (size_t)1 : (size_t)2);
     };
     /* the next stage to load: its address, number and slots */
-    const uint8_t *pa = base_a(second ? p.a2 : p.a), *pb = base_b(second || up ? p.b2 : p.b);
-    uint32_t ja = 0, jb = 0, sa = 0, sb = 0;
+    const bool late = second || j0 >= nst1;              /* starts in the second product */
+    const uint8_t *pa = base_a(late ? p.a2 : p.a), *pb = base_b(late || up ? p.b2 : p.b);
+    uint32_t ja = j0, jb = j0, sa = 0, sb = 0;
+    if constexpr (MODE == GHIP_EP_STORE) {
+        const size_t from = j0 >= nst1 ? j0 - nst1 : j0;
+        pa += from * astep;
+        pb += from * bstep;
+    }
 
     /* Byte offset of this lane's 16 bytes of 1 KB load c in a stage, the load's
      * lane l going to byte 16 l of the KB; past the matrix: FG_OOB. kq: the
@@ -260,13 +272,13 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
     auto next_a = [&]() {
         ja++;
         pa += astep;
-        if (MODE == GHIP_EP_STORE && ja == nst1 && nst > nst1) pa = base_a(p.a2);
+        if (MODE == GHIP_EP_STORE && ja == nst1 && all > nst1) pa = base_a(p.a2);
         sa = sa == L * AST ? 0u : sa + AST;
     };
     auto next_b = [&]() {
         jb++;
         pb += bstep;
-        if (MODE == GHIP_EP_STORE && jb == nst1 && nst > nst1) pb = base_b(p.b2);
+        if (MODE == GHIP_EP_STORE && jb == nst1 && all > nst1) pb = base_b(p.b2);
         sb = sb == (L - 1u) * BST ? 0u : sb + BST;
     };
 
@@ -441,15 +453,41 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
     constexpr bool BIAS = MODE == GHIP_EP_LINEAR || MODE == GHIP_EP_DLINEAR;
     constexpr bool IN = BIAS || MODE == GHIP_EP_DGATED;
     uint16_t *out = second ? ep.out2 : ep.out;
-    /* 16-byte accesses: whole pieces of 8 columns (the last one's padding is the
-     * output's own where ep.pad says so) */
-    const bool vec = (((uintptr_t)out | (uintptr_t)ep.out2) & 15u) == 0u && (ep.ldout & 7u) == 0u
-                     && (p.N & 7u) == 0u
-                     && (!IN || (((uintptr_t)ep.in & 15u) == 0u && (ep.ldin & 7u) == 0u))
-                     && (!BIAS || ((uintptr_t)ep.bias & 15u) == 0u);
+    /* 8 values at any alignment: the device takes 16-byte accesses at 2 bytes. A
+     * tile that holds a row's last piece where that is a part (!fast) goes by
+     * elements there; columns behind it up to the next multiple of 8 get zeros
+     * where they are the output's own */
+    const bool live = c0 < cols, whole = n0 + 8u <= p.N;
+    const bool fast = (p.N & 7u) == 0u || cols == OUTN;
+    const uint32_t nc = live ? n0 : col0;                /* loads of dead lanes stay inside */
+    auto load8 = [&](auto fast_c, const uint16_t *row, float (&v)[8]) {
+        if (decltype(fast_c)::value) {
+            ghip_u32x4 d;
+            __builtin_memcpy(&d, row + nc, 16);
+            fg_unpack(d, v);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) v[e] = n0 + e < p.N ? ghip_bf16_f32(row[n0 + e]) : 0.0f;
+        }
+    };
+    auto store8 = [&](auto fast_c, uint16_t *row, const float (&v)[8]) {
+        const ghip_u32x4 d = fg_pack(v);
+        if (decltype(fast_c)::value || whole) {
+            __builtin_memcpy(row + n0, &d, 16);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) {
+                if (n0 + e < p.N) row[n0 + e] = (uint16_t)(d[e >> 1] >> (16u * (e & 1u)));
+                else if (ep.pad) row[n0 + e] = 0;
+            }
+        }
+    };
     float bias[8] = {};
     if constexpr (BIAS)
-        if (ep.bias && vec && c0 < cols) fg_unpack(*(const ghip_u32x4 *)(ep.bias + n0), bias);
+        if (ep.bias) {
+            if (fast) load8(std::true_type{}, ep.bias, bias);
+            else load8(std::false_type{}, ep.bias, bias);
+        }
     ghip_with_act(MODE == GHIP_EP_STORE ? GHIP_ACT_NONE : ep.act, [&](auto act) {
         auto values = [&](uint32_t lr, const float (&in)[8], float (&o0)[8], float (&o1)[8]) {
             float s0[8], s1[8] = {};
@@ -478,55 +516,43 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
             __builtin_amdgcn_s_waitcnt(0xc07f);
             __builtin_amdgcn_wave_barrier();
             const uint32_t mg = m0 + 16u * rg;           /* this lane's first row */
-            if (vec) {
+            auto rows_out = [&](auto fast_c, auto u_c) {
+                constexpr int UU = decltype(u_c)::value;
 #pragma unroll 1
-                for (int it = 0; it < IT; it += U) {
-                    ghip_u32x4 d[U];
+                for (int it = 0; it < IT; it += UU) {
+                    float in[UU][8] = {};
                     if constexpr (IN)
                         if (ep.in) {
 #pragma unroll
-                            for (int u = 0; u < U; u++) {
+                            for (int u = 0; u < UU; u++) {
                                 const uint32_t m = min(mg + (it + u) * (64u / LPR), p.M - 1u);
-                                d[u] = *(const ghip_u32x4 *)(ep.in + (size_t)m * ep.ldin
-                                                             + min(n0, p.N - 8u));
+                                load8(fast_c, ep.in + (size_t)m * ep.ldin, in[u]);
                             }
                         }
 #pragma unroll
-                    for (int u = 0; u < U; u++) {
+                    for (int u = 0; u < UU; u++) {
                         const uint32_t dr = (it + u) * (64u / LPR), m = mg + dr;
-                        float in[8] = {}, o0[8], o1[8];
-                        if constexpr (IN)
-                            if (ep.in) fg_unpack(d[u], in);
-                        values(lane / LPR + dr, in, o0, o1);
-                        if (m < p.M && c0 < cols) {
-                            *(ghip_u32x4 *)(out + (size_t)m * ep.ldout + n0) = fg_pack(o0);
-                            if constexpr (MODE == GHIP_EP_DGATED)
-                                *(ghip_u32x4 *)(ep.out2 + (size_t)m * ep.ldout + n0) = fg_pack(o1);
+                        float o0[8], o1[8];
+                        values(lane / LPR + dr, in[u], o0, o1);
+                        if (m < p.M && live) {
+                            if (MODE == GHIP_EP_STORE && p.part) {
+                                /* f32 partial sums, rows of whole pieces */
+                                const size_t ld = (p.N + 7u) & ~7u;
+                                float *q = p.part
+                                           + (((second ? p.splits : 0u) + split) * (size_t)p.M + m) * ld + n0;
+                                *(ghip_f32x4 *)q = (ghip_f32x4){o0[0], o0[1], o0[2], o0[3]};
+                                *(ghip_f32x4 *)(q + 4) = (ghip_f32x4){o0[4], o0[5], o0[6], o0[7]};
+                            } else {
+                                store8(fast_c, out + (size_t)m * ep.ldout, o0);
+                                if constexpr (MODE == GHIP_EP_DGATED)
+                                    store8(fast_c, ep.out2 + (size_t)m * ep.ldout, o1);
+                            }
                         }
                     }
                 }
-            } else {
-                /* any width and alignment: a column a lane, so that accesses of
-                 * 2 bytes still run along a row; columns up to the next multiple
-                 * of 8 get zeros where they are the output's own */
-                constexpr uint32_t WD = DUAL ? 8u * CB : 16u * CB;
-                const uint32_t end = ep.pad ? (p.N + 7u) & ~7u : p.N;
-#pragma unroll 4
-                for (uint32_t it = 0; it < 16u * G * WD / 64u; it++) {
-                    const uint32_t v = lane + 64u * it, lr = v / WD, cc = v % WD;
-                    const uint32_t m = row0 + 16u * (wr * RB + rg) + lr, nn = col0 + WD * wc + cc;
-                    const uint32_t q = DUAL ? 8u * (cc >> 4) + ((cc >> 2) & 3u) : cc >> 2;
-                    const float s0 = *(const float *)(sw + spot(lr, q) + 4u * (cc & 3u));
-                    const float s1 = DUAL ? *(const float *)(sw + spot(lr, q + 4u) + 4u * (cc & 3u)) : 0.0f;
-                    if (m >= p.M || nn >= end) continue;
-                    if (nn < p.N) {
-                        ghip_ep_store<MODE, decltype(act)::value>(ep, out, m, nn, s0, s1);
-                    } else {
-                        out[(size_t)m * ep.ldout + nn] = 0;
-                        if constexpr (MODE == GHIP_EP_DGATED) ep.out2[(size_t)m * ep.ldout + nn] = 0;
-                    }
-                }
-            }
+            };
+            if (fast) rows_out(std::true_type{}, std::integral_constant<int, U>{});
+            else rows_out(std::false_type{}, std::integral_constant<int, 1>{});
             __builtin_amdgcn_s_waitcnt(0xc07f);
             __builtin_amdgcn_wave_barrier();
         }

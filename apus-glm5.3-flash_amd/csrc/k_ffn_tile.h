@@ -1,7 +1,7 @@
 /*
  * k_ffn_tile.h — an entry of a tile table (GhipFfnTile) over k_ffn_gemm.
  *
- * Its three times are fitted, family by family, to a sweep of every tile over M
+ * Its times are fitted, family by family, to a sweep of every tile over M
  * = 64..4096 and N x K from 1536 x 1536 to 12288 x 4096 and 4096 x 12288
  * (backward products: 19 shapes each) on 256 CUs; the tile picked by them took
  * 1.5-3% longer than the best one on average, 25% at most. Tiles of at most 80
@@ -18,14 +18,15 @@ template <int MODE, int W8, int AL, int BL, int WM, int RB, int CB, int L>
 static void fg_run(const GhipProd *p, const GhipEp *ep, uint32_t mt, uint32_t nt, uint32_t lds,
                    hipStream_t st) {
     hipLaunchKernelGGL((k_ffn_gemm<MODE, W8, AL, BL, WM, RB, CB, L>),
-                       dim3(mt * nt * (p->batch ? 2u : 1u)), dim3(256), lds, st, *p, *ep, mt, nt);
+                       dim3(mt * nt * p->splits * (p->batch ? 2u : 1u)), dim3(256), lds, st, *p,
+                       *ep, mt, nt);
 }
 
 template <int MODE, int W8, int AL, int BL, int WM, int RB, int CB, int L>
-static constexpr GhipFfnTile fg_tile(float low, float full, float over) {
+static constexpr GhipFfnTile fg_tile(float low, float mid, float full, float over) {
     constexpr uint32_t bm = 16u * RB * WM, bn = 16u * CB * (4 / WM);
     constexpr uint32_t lds = (L + 1u) * bm * 128u + L * bn * (W8 ? 64u : 128u);
-    return {bm, ghip_ep_dual(MODE) ? bn / 2 : bn, lds <= FG_LDS_MAX / 2 ? 2u : 1u, low, full, over, lds,
+    return {bm, ghip_ep_dual(MODE) ? bn / 2 : bn, lds <= FG_LDS_MAX / 2 ? 2u : 1u, low, mid, full, over, lds,
             (const void *)k_ffn_gemm<MODE, W8, AL, BL, WM, RB, CB, L>,
             fg_run<MODE, W8, AL, BL, WM, RB, CB, L>};
 }

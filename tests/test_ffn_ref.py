@@ -113,9 +113,15 @@ def test_refusals_come_before_the_device(pkg, call, args):
 
 
 def test_workspace_sizes(pkg):
+    """dz's matrix (two of them), in whole 256 bytes, and the partial sums of the
+    products that may be split: at most 16 times the outputs and 32 MiB."""
     lib = pkg.load()
     one, two = lib.apus_ghip_linear_ep_backward_ws, lib.apus_ghip_gated_backward_ws
-    assert one(4, 16, 32) == 256 and two(4, 16, 32) == 512          # 4 rows of 32 bytes, in whole 256 bytes
+    assert one(4, 16, 32) == 256 and two(4, 16, 32) == 512          # 4 rows of 32 bytes
     assert one(3, 9, 5) == 256 and one(100, 9, 5) == 3328            # rows of 9 take 16 elements
-    assert one(1 << 20, 1 << 14, 8) == 1 << 35 and two(1 << 20, 1 << 14, 8) == 1 << 36
-    assert [f(*s) for f in (one, two) for s in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (BIG, 1, 1))] == [0] * 8
+    # outputs of 2^20 x 8 (dx) over 2^14, of 2^14 x 8 (dW) over 2^20
+    assert one(1 << 20, 1 << 14, 8) == (1 << 35) + 16 * (1 << 17) * 4
+    # dx: 16 x 64 outputs over 8192 split 16 times; over 2 x 8192 the same
+    assert one(16, 8192, 64) == 16 * 8192 * 2 + 16 * 16 * 64 * 4
+    assert two(16, 8192, 64) == 2 * 16 * 8192 * 2 + 16 * 16 * 64 * 4
+    assert [f(*s) for f in (one, two) for s in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (BIG, 1, 1), (1, 1, BIG))] == [0] * 10
