@@ -312,7 +312,8 @@ hipError_t ghip_launch_ffn_pack(const uint16_t *src, size_t ld, size_t M, size_t
                                 uint16_t *dst, hipStream_t st);
 
 /* On tiles (k_ffn_gemm.h): fits = the steps and alignments of the vector loads;
- * pick = the tile shape with the least estimated time (microseconds, in us). */
+ * pick = the tile shape and splits of k with the least estimated time (microseconds,
+ * in us); -1: no tile's grid is small enough for a launch. */
 int ghip_ffn_gemm_fits(int mode, const GhipProd *p);
 int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us, uint32_t *splits);
 hipError_t ghip_launch_ffn_gemm(int mode, int tile, uint32_t splits, const GhipProd *p,
@@ -335,7 +336,8 @@ const GhipFfnTile *ghip_ffn_forward_tiles(int mode, int w8, int *n);
 const GhipFfnTile *ghip_ffn_fp8_tiles(int mode, int w8, int *n);
 const GhipFfnTile *ghip_ffn_backward_tiles(int mode, int transposed, int *n);
 
-/* Streaming the weights past a few rows (k_rows_gemm.h), forward modes. */
+/* Streaming the weights past a few rows (k_rows_gemm.h), every mode but
+ * GHIP_EP_STORE; FP8 in the forward ones. */
 int ghip_ffn_rows_fits(int mode, const GhipProd *p);
 int ghip_ffn_rows_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us);
 hipError_t ghip_launch_ffn_rows(int mode, int form, const GhipProd *p, const GhipEp *ep,

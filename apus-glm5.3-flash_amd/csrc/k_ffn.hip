@@ -34,8 +34,13 @@ extern "C" int ghip_ffn_gemm_fits(int mode, const GhipProd *p) {
         || !vectors(p->b, p->brs, p->bks, p->N, p->K, per, false))
         return 0;
     if ((p->a2 && ((uintptr_t)p->a2 & 15)) || (p->b2 && ((uintptr_t)p->b2 & 15))) return 0;
-    /* the smallest tile's grid, two products of 16 splits: under 2^32 threads */
-    return ((size_t)(p->M + 63) / 64) * ((size_t)(p->N + 63) / 64) * 2 * 256 * 16 <= GHIP_MAX_THREADS;
+    return 1;
+}
+
+/* Workgroups of a tile; 0 where they are more than a launch takes. */
+static size_t tile_grid(const GhipFfnTile *t, const GhipProd *p, uint32_t splits) {
+    const size_t n = (((size_t)p->M + t->bm - 1) / t->bm) * (((size_t)p->N + t->bn - 1) / t->bn);
+    return n > GHIP_MAX_THREADS / 256 / 2 / splits ? 0 : n * (p->batch ? 2 : 1) * splits;
 }
 
 /* Splits of k are for products of few tiles over a long k (dx of a wide block,
@@ -61,8 +66,7 @@ extern "C" size_t ghip_ffn_part_bytes(size_t M, size_t N, size_t K) {
  * round's time long before all do. */
 static double tile_us(const GhipFfnTile *t, const GhipProd *p, double stages, uint32_t splits,
                       uint32_t n_cu) {
-    const double wgs = (double)((p->M + t->bm - 1) / t->bm) * (double)((p->N + t->bn - 1) / t->bn)
-                       * (p->batch ? 2 : 1) * splits;
+    const double wgs = (double)tile_grid(t, p, splits);
     const double cap = (double)n_cu * t->occ, whole = (double)(size_t)(wgs / cap);
     const double part = wgs / cap - whole;               /* of the last round */
     double us = t->low + (t->full - t->low) * part;
@@ -74,7 +78,7 @@ static double tile_us(const GhipFfnTile *t, const GhipProd *p, double stages, ui
 
 extern "C" int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us,
                                   uint32_t *splits) {
-    int n, best = 0;
+    int n, best = -1;
     const GhipFfnTile *t = tiles_of(mode, p, &n);
     const double stages = (double)((p->K + 63) / 64) * (p->a2 && !p->batch ? 2 : 1);
     const size_t cells = (size_t)p->M * (((size_t)p->N + 7) & ~(size_t)7) * (p->batch ? 2 : 1);
@@ -88,6 +92,7 @@ extern "C" int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, fl
     *us = 1e30f;
     for (int i = 0; i < n; i++)
         for (uint32_t s = 1; s <= most; s++) {
+            if (!tile_grid(t + i, p, s)) continue;
             /* the sums' way out and back at 3 TB/s, and one more launch */
             const double join = s > 1 ? 4.0 + (double)cells * 4.0 * s * 2.0 / 3e6 : 0.0;
             const float e = (float)(tile_us(t + i, p, (double)(size_t)((stages + s - 1) / s), s, n_cu) + join);
@@ -145,6 +150,7 @@ extern "C" hipError_t ghip_launch_ffn_gemm(int mode, int tile, uint32_t splits, 
     q.splits = splits;
     if (splits == 1) q.part = nullptr;
     t += tile;
+    if (!tile_grid(t, p, splits)) return hipErrorInvalidValue;
     t->launch(&q, ep, (p->M + t->bm - 1) / t->bm, (p->N + t->bn - 1) / t->bn, t->lds, st);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;

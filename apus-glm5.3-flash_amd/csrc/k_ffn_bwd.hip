@@ -54,7 +54,6 @@ static const GhipFfnTile *dw_tiles(int *n) {
         fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 8, 8, 2>(1.11f, 0.00f, 1.49f, 7.4f),
         fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 4, 4, 2>(0.40f, 0.49f, 0.93f, 3.1f),
         fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 4, 5>(0.29f, 0.00f, 0.36f, 2.4f),
-        fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 2, 6>(0.23f, 0.00f, 0.28f, 1.9f),
         fg_tile<GHIP_EP_STORE, 0, 1, 1, 2, 2, 2, 3>(0.24f, 0.23f, 0.44f, 1.5f),
     };
     *n = sizeof t / sizeof *t;

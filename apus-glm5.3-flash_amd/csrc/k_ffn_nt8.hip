@@ -26,7 +26,6 @@ static const GhipFfnTile *gated_tiles(int *n) {
         fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 12, 2, 2>(0.71f, 0.00f, 0.78f, 2.4f),
         fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 8, 2, 4>(0.56f, 0.00f, 0.62f, 2.4f),
         fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 8, 2, 2>(0.60f, 0.67f, 1.00f, 1.0f),
-        fg_tile<GHIP_EP_GATED, W8, 0, 0, 2, 2, 2, 6>(0.32f, 0.40f, 0.48f, 1.7f),
         fg_tile<GHIP_EP_GATED, W8, 0, 0, 2, 2, 2, 3>(0.31f, 0.43f, 0.44f, 0.6f),
     };
     *n = sizeof t / sizeof *t;

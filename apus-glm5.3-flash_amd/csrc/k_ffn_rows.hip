@@ -1,7 +1,8 @@
 /*
- * k_ffn_rows.hip — the forward feed-forward products of a few rows: the
- * weight-streaming kernel (k_rows_gemm.h) with an epilogue, for one weight
- * matrix (linear) or gate and up together (gated).
+ * k_ffn_rows.hip — the feed-forward products x W^T of a few rows (the forward,
+ * and the sums that a backward pass computes again): the weight-streaming
+ * kernel (k_rows_gemm.h) with an epilogue, for one weight matrix (linear) or
+ * gate and up together (gated).
  */
 #include "k_rows_gemm.h"
 
@@ -84,8 +85,32 @@ static const FrForm fr_gated16[] = {
     FR_G(true, 32, 2, 4, 1, 1, 0.99f, 0.00f),
 };
 
+/* dz, dg and du: the forward's sums again, at its times */
+#define FR_DL(BF, MR, NT, KS, NA, SL, T, V) FR_FORM(BF, MR, NT, KS, NA, SL, GHIP_EP_DLINEAR, T, V)
+static const FrForm fr_dlinear[] = {
+    FR_DL(true, 8, 1, 8, 2, 2, 0.54f, 0.00f),
+    FR_DL(true, 8, 1, 4, 2, 2, 0.45f, 0.00f),
+    FR_DL(true, 16, 1, 8, 2, 2, 0.61f, 0.00f),
+    FR_DL(true, 16, 1, 4, 2, 2, 0.52f, 0.00f),
+    FR_DL(true, 16, 2, 4, 2, 2, 0.82f, 0.03f),
+    FR_DL(true, 32, 1, 8, 1, 1, 0.74f, 0.23f),
+    FR_DL(true, 32, 2, 8, 1, 1, 1.03f, 0.21f),
+    FR_DL(true, 32, 2, 4, 1, 1, 0.94f, 0.36f),
+};
+#define FR_DG(BF, MR, NT, KS, NA, SL, T, V) FR_FORM(BF, MR, NT, KS, NA, SL, GHIP_EP_DGATED, T, V)
+static const FrForm fr_dgated[] = {
+    FR_DG(true, 8, 2, 8, 2, 2, 0.97f, 0.00f),
+    FR_DG(true, 8, 2, 4, 2, 2, 0.81f, 0.00f),
+    FR_DG(true, 16, 2, 8, 2, 2, 1.08f, 0.00f),
+    FR_DG(true, 16, 2, 4, 2, 2, 0.87f, 0.00f),
+    FR_DG(true, 32, 2, 8, 1, 1, 1.12f, 0.00f),
+    FR_DG(true, 32, 2, 4, 1, 1, 0.99f, 0.00f),
+};
+
 static const FrForm *fr_forms(int mode, bool fp8, int *n) {
 #define FR_TABLE(t) (*n = (int)(sizeof t / sizeof *t), t)
+    if (mode == GHIP_EP_DLINEAR) return FR_TABLE(fr_dlinear);
+    if (mode == GHIP_EP_DGATED) return FR_TABLE(fr_dgated);
     if (mode == GHIP_EP_GATED) return fp8 ? FR_TABLE(fr_gated8) : FR_TABLE(fr_gated16);
     return fp8 ? FR_TABLE(fr_linear8) : FR_TABLE(fr_linear16);
 #undef FR_TABLE
@@ -110,7 +135,7 @@ static float fr_estimate(const FrForm &c, const GhipProd *p, bool dual, uint32_t
 /* Whole 16-byte pieces of x's rows (FP8 weight rows then start at 8 bytes, and
  * have 16 codes to read a half piece from), 32-bit offsets inside a wave's rows */
 extern "C" int ghip_ffn_rows_fits(int mode, const GhipProd *p) {
-    return (mode == GHIP_EP_LINEAR || mode == GHIP_EP_GATED) && p->aks == 1 && p->bks == 1
+    return mode != GHIP_EP_STORE && (!p->s || mode == GHIP_EP_LINEAR || mode == GHIP_EP_GATED) && p->aks == 1 && p->bks == 1
         && p->brs == p->K && p->K % 8 == 0 && (!p->s || p->K >= 16) && p->K <= (1u << 24) && p->ars % 8 == 0
         && p->ars <= (1u << 24) && p->M <= 0x7fffffffu && p->N <= 0x7fffffffu
         && (((uintptr_t)p->a | (uintptr_t)p->b | (uintptr_t)p->b2) & 15) == 0;
@@ -151,9 +176,11 @@ extern "C" hipError_t ghip_launch_ffn_rows(int mode, int form, const GhipProd *p
 }
 
 extern "C" hipError_t ghip_ffn_rows_init(void) {
-    for (int i = 0; i < 4; i++) {
+    static const int modes[6][2] = {{GHIP_EP_LINEAR, 0}, {GHIP_EP_LINEAR, 1}, {GHIP_EP_GATED, 0},
+                                    {GHIP_EP_GATED, 1}, {GHIP_EP_DLINEAR, 0}, {GHIP_EP_DGATED, 0}};
+    for (int i = 0; i < 6; i++) {
         int n;
-        const FrForm *t = fr_forms(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i >> 1, &n);
+        const FrForm *t = fr_forms(modes[i][0], modes[i][1], &n);
         for (int k = 0; k < n; k++) {
             const hipError_t e = hipFuncSetAttribute(
                 t[k].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)t[k].lds);

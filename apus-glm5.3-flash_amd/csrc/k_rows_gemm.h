@@ -50,6 +50,8 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
     uint16_t *__restrict__ Y, uint32_t M, uint32_t O, uint32_t K,
     const uint32_t *__restrict__ exact_flag, uint32_t blk0, uint32_t tile0, RwMore more) {
     constexpr bool EPI = MODE != GHIP_EP_STORE, DUAL = ghip_ep_dual(MODE);
+    /* the backward's dx reads the same weights next: they stay in the caches */
+    constexpr bool AGAIN = MODE == GHIP_EP_DLINEAR || MODE == GHIP_EP_DGATED;
     constexpr uint32_t GPP = RW_NW / KS;                 /* row groups per workgroup */
     constexpr uint32_t OG = DUAL ? NT / 2 : NT;          /* output groups of 16 a wave */
     static_assert(!DUAL || NT % 2 == 0, "gate and up groups alternate");
@@ -158,8 +160,13 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
 #pragma unroll
             for (int b = 0; b < NT; b++) {
                 const uint8_t *wb = DUAL && (b & 1) ? rows2 + (size_t)c * 128u : wc;
-                wr[A][2 * b] = __builtin_nontemporal_load(from(c, wb, d[b].off0, q0));
-                wr[A][2 * b + 1] = __builtin_nontemporal_load(from(c, wb, d[b].off1, q1));
+                if constexpr (AGAIN) {
+                    wr[A][2 * b] = *from(c, wb, d[b].off0, q0);
+                    wr[A][2 * b + 1] = *from(c, wb, d[b].off1, q1);
+                } else {
+                    wr[A][2 * b] = __builtin_nontemporal_load(from(c, wb, d[b].off0, q0));
+                    wr[A][2 * b + 1] = __builtin_nontemporal_load(from(c, wb, d[b].off1, q1));
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         };
@@ -301,7 +308,15 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
             for (uint32_t i = 0; i < NV; i++) {
                 uint32_t m, o;
                 const uint32_t v = tid + i * (RW_NW * 64u);
-                if (!place(v, m, o)) continue;
+                if (!place(v, m, o)) {
+                    /* the output's own columns behind its width */
+                    if (AGAIN && more.ep.pad && v < NOUT
+                        && m < mrows && o < ((O + 7u) & ~7u)) {
+                        more.ep.out[(size_t)(m0 + m) * more.ep.ldout + o] = 0;
+                        if (DUAL) more.ep.out2[(size_t)(m0 + m) * more.ep.ldout + o] = 0;
+                    }
+                    continue;
+                }
                 const uint32_t sl = v / (MR * 16u * OG), c = v % (16u * OG);
                 /* dual: gate group, up group, ... of 16 columns */
                 const uint32_t e = m * (16u * NT) + (DUAL ? 32u * (c >> 4) + (c & 15u) : c);

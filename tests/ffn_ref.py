@@ -92,20 +92,24 @@ def gated(x, wg, wu, a, limit):
     return h, tol + HALF * np.abs(h) + 1e-38
 
 
+def dz_linear(x, w, bias, dy, a):
+    """[(dz, bound)], dz rounded to bf16."""
+    z, e = product(x, w)
+    if bias is not None:
+        z, e = z + bias, e + 2.0 ** -23 * (np.abs(z) + np.abs(bias))
+    dz = dy * slope(a, z)
+    ez = np.abs(dy) * ((np.abs(z) <= e) if a == RELU else 1.1 * e + _eval(z)) + HALF * np.abs(dz)
+    return [(dz, ez)]
+
+
 def linear_backward(x, w, bias, dy, a):
     """{dx, dw, db}: (value, bound)."""
-    if a == NONE:
-        dz, ez = dy, np.zeros_like(dy)
-    else:
-        z, e = product(x, w)
-        if bias is not None:
-            z, e = z + bias, e + 2.0 ** -23 * (np.abs(z) + np.abs(bias))
-        dz = dy * slope(a, z)
-        ez = np.abs(dy) * ((np.abs(z) <= e) if a == RELU else 1.1 * e + _eval(z)) + HALF * np.abs(dz)
+    [(dz, ez)] = [(dy, np.zeros_like(dy))] if a == NONE else dz_linear(x, w, bias, dy, a)
     return _grads(x, [(w, dz, ez)])
 
 
-def gated_backward(x, wg, wu, dh, a, limit):
+def dz_gated(x, wg, wu, dh, a, limit):
+    """[(dg, bound), (du, bound)], both rounded to bf16."""
     lim = limit or math.inf
     g, eg = product(x, wg)
     u, eu = product(x, wu)
@@ -118,6 +122,11 @@ def gated_backward(x, wg, wu, dh, a, limit):
     tg = np.abs(dh) * ((np.abs(s) + es) * eu + np.abs(uc) * es) + near * np.abs(dh * uc * s) + HALF * np.abs(dg)
     near = np.abs(np.abs(u) - lim) <= eu
     tu = np.abs(dh) * (1.13 * eg + _eval(gc)) + near * np.abs(dh * v) + HALF * np.abs(du)
+    return [(dg, tg), (du, tu)]
+
+
+def gated_backward(x, wg, wu, dh, a, limit):
+    (dg, tg), (du, tu) = dz_gated(x, wg, wu, dh, a, limit)
     return _grads(x, [(wg, dg, tg), (wu, du, tu)])
 
 
