@@ -109,6 +109,10 @@ __device__ __forceinline__ uint32_t fg_swizzle(uint32_t k) {
     return W % 128u ? ((k >> 1) & 1u) | ((k >> 3) & 2u) : ((k & 3u) << 1) | ((k >> 4) & 1u);
 }
 
+/* Layout 0 (FP8 codes): what the 16-byte pieces of row r are XORed with. */
+__device__ __forceinline__ uint32_t fg_rot8(uint32_t r) { return ((r >> 1) + 2u) & 7u; }
+__device__ __forceinline__ uint32_t fg_rot4(uint32_t r) { return ((r >> 2) + 1u) & 3u; }
+
 /* f(0), f(1), ... f(N - 1), the argument a constant */
 template <typename F, int... I>
 __device__ __forceinline__ void fg_each_of(F f, std::integer_sequence<int, I...>) {
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
                      uint32_t &kq) -> uint32_t {
         constexpr uint32_t W = decltype(w_c)::value;
         if constexpr (decltype(layout_c)::value == 0) {
-            const uint32_t r = 8u * c + (lane >> 3), q = (lane & 7u) ^ ((r >> 1) & 7u);
+            const uint32_t r = 8u * c + (lane >> 3), q = (lane & 7u) ^ fg_rot8(r);
             kq = 8u * q;                                 /* the same for every c of a wave */
             return r < live ? r * ld * 2u + 16u * q : FG_OOB;
         } else {
@@ -240,14 +244,14 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
 #pragma unroll
     for (uint32_t i = 0; i < NBL; i++) {
         if constexpr (FP8) {                             /* 16 rows of 64 codes */
-            const uint32_t b = wv + 4u * i, r = lane >> 2, q = (lane & 3u) ^ ((r >> 2) & 3u);
+            const uint32_t b = wv + 4u * i, r = lane >> 2, q = (lane & 3u) ^ fg_rot4(r);
             const uint32_t mr = 16u * (DUAL ? b >> 1 : b) + r;
             bkq = 16u * q;
             bo[i] = mr < cols ? mr * ldb + 16u * q : FG_OOB;
         } else {
             const uint32_t c = wv + 4u * i;
             if constexpr (DUAL) {
-                const uint32_t r = 8u * c + (lane >> 3), q = (lane & 7u) ^ ((r >> 1) & 7u);
+                const uint32_t r = 8u * c + (lane >> 3), q = (lane & 7u) ^ fg_rot8(r);
                 const uint32_t mr = 16u * (r >> 5) + (r & 15u);
                 bkq = 8u * q;
                 bo[i] = mr < cols ? mr * ldb * 2u + 16u * q : FG_OOB;
@@ -285,7 +289,7 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
     /* operand reads: block blk of 16 rows, step s */
     uint32_t off0[2];
 #pragma unroll
-    for (uint32_t s = 0; s < 2; s++) off0[s] = n * 128u + 16u * ((2u * g + s) ^ ((n >> 1) & 7u));
+    for (uint32_t s = 0; s < 2; s++) off0[s] = n * 128u + 16u * ((2u * g + s) ^ fg_rot8(n));
     auto frag = [&](auto layout_c, auto w_c, const uint8_t *st, uint32_t blk, int s) -> ghip_bf16x8 {
         constexpr uint32_t W = decltype(w_c)::value;
         if constexpr (decltype(layout_c)::value == 0) {
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
     auto read_b = [&](int set, int c, const uint8_t *st, int s) {
         if constexpr (FP8)
             codes[c] = *(const ghip_u32x4 *)(st + (wc * CB + c) * 1024u + n * 64u
-                                             + 16u * (g ^ (n >> 2)));
+                                             + 16u * (g ^ fg_rot4(n)));
         else
             wa[set][c] = frag(LB{}, WB{}, st, wc * CB + c, s);
     };
