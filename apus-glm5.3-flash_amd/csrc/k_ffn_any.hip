@@ -15,8 +15,11 @@
  * v_mfma_f32_16x16x32_bf16 a step of k = 32; tiles reach LDS through registers
  * by loads of 8 elements at any alignment (8 of one element at the matrix's
  * edges), the next step's in flight during the products, elements past M, N or
- * k as zeros. It is bound by the two barriers of a step and its load's latency:
- * the route for what the kernels with direct loads cannot take.
+ * k as zeros. It is bound by the two barriers of a step and its load's latency,
+ * 0.8 us a step: the route for what the kernels with direct loads cannot take
+ * (linear with SiLU, BF16, odd K: 1 x 4096 x 4095 106 us, 64 x 2000 x 2001 40, 1111
+ * x 2048 x 4095 116, 4096 x 4096 x 4095 453, 300 TFLOP/s; FP8 97 to 130% of
+ * that).
  */
 #include "ghip_epilogue.h"
 
@@ -149,8 +152,8 @@ __global__ __launch_bounds__(256) void k_ffn_any(GhipProd p, GhipEp ep, uint32_t
 
 /* dbias[n] = sum_m dz[m, n] in f32, rounded once. A workgroup owns 64 columns,
  * a thread 8 of them in every 128th row (one load at any alignment); the 128
- * rows' sums are added in a fixed order. Bound by latency: 300 x 2048 2.5 us
- * (one column and 16 rows a thread at a time: 7.2). */
+ * rows' sums are added in a fixed order. Bound by latency: 300 x 2048 3.3 us
+ * under the profiler (one column and 16 rows a thread at a time: 7.2). */
 __global__ __launch_bounds__(1024) void k_ffn_colsum(const uint16_t *__restrict__ dz, size_t ld,
                                                      uint32_t M, uint32_t N,
                                                      uint16_t *__restrict__ out) {

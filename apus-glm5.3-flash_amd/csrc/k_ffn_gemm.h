@@ -27,19 +27,20 @@
  *
  * Operand layouts. 0: k is the fast index in memory (x, W in the forward). The
  * stage is [row][64 k], whole 128-byte lines, 16-byte piece p of row r at p ^
- * ((r >> 1) & 7); an operand of 8 k values is one ds_read_b128. 1: the row is
+ * fg_rot8(r); an operand of 8 k values is one ds_read_b128. 1: the row is
  * (W in dx, dz and x in dW). The stage is [64 k][rows], 32-byte slots XORed
  * with k (fg_swizzle), and an operand is two ds_read_b64_tr_b16: each
  * transposes 4 k x 16 rows inside 16 lanes, so no transposed copy of a matrix
  * is made. In both, lane group g of MFMA step s takes k = 16 g + 8 s + [0, 8),
- * so either layout may meet the other. No read has bank conflicts.
+ * so either layout may meet the other. SQ_LDS_BANK_CONFLICT is 0 to 3% of the
+ * LDS cycles.
  *
  * Rows past the matrix and k past its end are given an offset outside the
  * buffer, which loads zeros: no other row is read in their place and a ragged
  * K needs no separate kernel.
  *
  * FP8 weights lie in LDS as codes, [row][64 codes], 16-byte piece p of row r at
- * p ^ ((r >> 2) & 3): one read gives the 16 codes of both steps, which are
+ * p ^ fg_rot4(r): one read gives the 16 codes of both steps, which are
  * dequantized bit-exactly in registers between the MFMAs of the step before
  * (against writing bf16 back to LDS it takes half the loads and writes). Its
  * waves lie side by side (WM = 1), so that no two dequantize the same codes.
@@ -109,7 +110,12 @@ __device__ __forceinline__ uint32_t fg_swizzle(uint32_t k) {
     return W % 128u ? ((k >> 1) & 1u) | ((k >> 3) & 2u) : ((k & 3u) << 1) | ((k >> 4) & 1u);
 }
 
-/* Layout 0 (FP8 codes): what the 16-byte pieces of row r are XORed with. */
+/* Layout 0 (FP8 codes): what the 16-byte pieces of row r are XORed with. A
+ * ds_read_b128 is served 16 lanes at a time, rows 0-3 and 12-15 of one lane
+ * group together with rows 4-11 of the next: the rotation gives the middle rows
+ * a set of values that the other group's XOR with 2 (1) maps to itself, so the
+ * 16 pieces fill the 64 banks. With r >> 1 alone 49% of the LDS cycles were
+ * conflicts (gated FP8 1111 x 2048 x 4096: 52 us, now 49). */
 __device__ __forceinline__ uint32_t fg_rot8(uint32_t r) { return ((r >> 1) + 2u) & 7u; }
 __device__ __forceinline__ uint32_t fg_rot4(uint32_t r) { return ((r >> 2) + 1u) & 3u; }
 

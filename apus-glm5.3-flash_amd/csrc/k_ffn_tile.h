@@ -7,7 +7,7 @@
  * 1.5-3% longer than the best one on average, 25% at most. Tiles of at most 80
  * KB of LDS run two to a CU: deeper rings against a second workgroup to hide
  * the first's waits is why some shapes are there twice. Every tile listed is
- * the pick of at least 1% of shapes drawn log-uniformly over that range.
+ * the pick of at least 0.8% of shapes drawn log-uniformly from 1 to 16384.
  */
 #ifndef K_FFN_TILE_H
 #define K_FFN_TILE_H

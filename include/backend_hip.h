@@ -420,9 +420,12 @@ int apus_ghip_fp8blk_gated_dev(const uint8_t *gate_codes, const float *gate_scal
  * gradient is dy. dz is rounded to BF16 once, as the products' operand. ws:
  * 16-byte aligned device memory of at least
  * apus_ghip_linear_ep_backward_ws(M, O, K) bytes that no overlapping call uses;
- * the call leaves nothing in it that a later one reads. With act NONE it may
- * be NULL; given, rows of dy that are not whole aligned vectors are laid out in
- * it for the faster kernels. */
+ * the call leaves nothing in it that a later one reads. It holds dz and, for
+ * products of few outputs over a long k, the f32 sums of up to 16 pieces of k
+ * (32 MiB at most), added in order. With act NONE it may be NULL, ws_bytes is
+ * then not read and k is not split; given, it has the full size too, and rows of
+ * dy that are not whole aligned vectors are laid out in it for the faster
+ * kernels. */
 size_t apus_ghip_linear_ep_backward_ws(size_t M, size_t O, size_t K);
 int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
                                           const uint16_t *bias, const uint16_t *dy, uint16_t *dx,
