@@ -21,7 +21,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 C_SRCS = ["ghip_backend.c", "ghip_synth.c", "ghip_container.c"]
 HIP_SRCS = ["k_dequant.hip", "k_linear.hip", "k_gemm_bf16.hip", "k_rows.hip",
             "k_moe.hip", "k_moe_rows.hip", "k_moe_prefill.hip", "k_ffn.hip", "k_ffn_any.hip",
-            "k_ffn_nt.hip", "k_ffn_nt8.hip", "k_ffn_bwd.hip", "k_ffn_rows.hip", "k_synth.hip"]
+            "k_ffn_nt.hip", "k_ffn_nt8.hip", "k_ffn_bwd.hip", "k_ffn_grads.hip", "k_ffn_rows.hip", "k_synth.hip"]
 
 INC = ["-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
 CFLAGS = ["-std=c11", "-O2", "-Wall", "-Wextra", "-fPIC", "-ffp-contract=off",
@@ -77,7 +77,7 @@ def resource_usage(out):
 # resource-usage remarks, or words them differently, the gate would see
 # nothing and pass, so their absence fails the build instead
 REQUIRED_KERNELS = ("k_moe_decode", "k_pf_gemm", "k_fp8_gemv_stream", "k_fp8_gemm", "k_bf16_gemm",
-                    "k_rows_gemm", "k_ffn_gemm", "k_ffn_any")
+                    "k_rows_gemm", "k_ffn_gemm", "k_ffn_any", "k_ffn_grads")
 
 # kernels whose inner loop an SGPR spill lands in (a lane read per use): the
 # most they may spill. k_fp8_gemm with 4 ran 1-4% longer than with none.

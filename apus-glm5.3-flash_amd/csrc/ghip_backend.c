@@ -734,28 +734,33 @@ static int check_ws(const void *ws, size_t have, size_t need) {
     return 1;
 }
 
-/* dx = dz W (+ dz2 W2), dw = dz^T x. */
-static int ffn_dx(const uint16_t *dz, const uint16_t *dz2, size_t lddz, const uint16_t *w,
-                  const uint16_t *w2, uint16_t *dx, size_t M, size_t N, size_t K, size_t lddx,
-                  int apad, void *part, size_t part_bytes, hipStream_t st) {
-    const GhipProd p = { .a = dz, .a2 = dz2, .b = w, .b2 = w2, .ars = lddz, .aks = 1, .brs = 1,
-                         .bks = K, .M = (uint32_t)M, .N = (uint32_t)K, .K = (uint32_t)N,
-                         .apad = apad, .part = (float *)part, .part_bytes = part_bytes };
-    const GhipEp ep = { .out = dx, .ldout = lddx };
-    HIPCHK(ghip_launch_ffn(GHIP_EP_STORE, &p, &ep, st));
-    return 0;
-}
-
-/* dw2, dz2: a second one beside it, in the same launch. */
-static int ffn_dw(const uint16_t *dz, const uint16_t *dz2, size_t lddz, const uint16_t *x,
-                  size_t ldx, uint16_t *dw, uint16_t *dw2, size_t M, size_t N, size_t K, int apad,
-                  void *part, size_t part_bytes, hipStream_t st) {
-    const GhipProd p = { .a = dz, .a2 = dz2, .b = x, .b2 = dz2 ? x : NULL, .ars = 1, .aks = lddz,
-                         .brs = 1, .bks = ldx, .M = (uint32_t)N, .N = (uint32_t)K,
-                         .K = (uint32_t)M, .batch = dz2 != NULL, .apad = apad,
-                         .part = (float *)part, .part_bytes = part_bytes };
-    const GhipEp ep = { .out = dw, .out2 = dw2, .ldout = K };
-    HIPCHK(ghip_launch_ffn(GHIP_EP_STORE, &p, &ep, st));
+/* dx = dz W (+ dz2 W2), dw = dz^T x (dw2 = dz2^T x), dbias from dz; each left out
+ * where NULL. */
+typedef struct {
+    const uint16_t *dz, *dz2, *w, *w2, *x;
+    uint16_t *dx, *dw, *dw2, *dbias;
+    size_t M, N, K, lddz, ldx, lddx;
+    int pad;                             /* dz's rows reach to the next multiple of 8 */
+    void *part;
+    size_t part_bytes;
+} FfnGrads;
+static int ffn_grads(const FfnGrads *g, hipStream_t st) {
+    const GhipProd dx = { .a = g->dz, .a2 = g->dz2, .b = g->w, .b2 = g->w2, .ars = g->lddz,
+                          .aks = 1, .brs = 1, .bks = g->K, .M = (uint32_t)g->M,
+                          .N = (uint32_t)g->K, .K = (uint32_t)g->N, .apad = g->pad,
+                          .part = (float *)g->part, .part_bytes = g->part_bytes };
+    const GhipEp edx = { .out = g->dx, .ldout = g->lddx };
+    /* two of them in the same launch, or the one that is wanted */
+    const int both = g->dw && g->dw2;
+    const GhipProd dw = { .a = g->dw ? g->dz : g->dz2, .a2 = both ? g->dz2 : NULL, .b = g->x,
+                          .b2 = both ? g->x : NULL, .ars = 1, .aks = g->lddz, .brs = 1,
+                          .bks = g->ldx, .M = (uint32_t)g->N, .N = (uint32_t)g->K,
+                          .K = (uint32_t)g->M, .batch = both, .apad = g->pad,
+                          .part = (float *)g->part, .part_bytes = g->part_bytes };
+    const GhipEp edw = { .out = g->dw ? g->dw : g->dw2, .out2 = both ? g->dw2 : NULL, .ldout = g->K };
+    const GhipFfnSum sum = { .dz = g->dz, .ld = g->lddz, .M = g->M, .N = g->N, .out = g->dbias };
+    HIPCHK(ghip_launch_ffn_grads(g->dx ? &dx : NULL, &edx, g->dw || g->dw2 ? &dw : NULL, &edw,
+                                 g->dbias ? &sum : NULL, st));
     return 0;
 }
 
@@ -799,11 +804,12 @@ int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
         lddz = ffn_ws_ld(O);
         pad = 1;
     }
-    const size_t mat = ffn_ws_mat(M, O), part_bytes = ws ? ffn_ws_part(M, O, K, 1) : 0;
-    void *part = part_bytes ? (uint8_t *)ws + mat : NULL;
-    if (dx && ffn_dx(dz, NULL, lddz, w, NULL, dx, M, O, K, lddx, pad, part, part_bytes, st)) return 1;
-    if (dw && ffn_dw(dz, NULL, lddz, x, ldx, dw, NULL, M, O, K, pad, part, part_bytes, st)) return 1;
-    if (dbias) HIPCHK(ghip_launch_ffn_colsum(dz, lddz, M, O, dbias, st));
+    const size_t part_bytes = ws ? ffn_ws_part(M, O, K, 1) : 0;
+    const FfnGrads g = { .dz = dz, .w = w, .x = x, .dx = dx, .dw = dw, .dbias = dbias, .M = M,
+                         .N = O, .K = K, .lddz = lddz, .ldx = ldx, .lddx = lddx, .pad = pad,
+                         .part = part_bytes ? (uint8_t *)ws + ffn_ws_mat(M, O) : NULL,
+                         .part_bytes = part_bytes };
+    if (ffn_grads(&g, st)) return 1;
     G.dispatches++;
     return 0;
 }
@@ -834,14 +840,12 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
                         .limit = limit > 0.0f ? limit : INFINITY, .pad = 1 };
     HIPCHK(ghip_launch_ffn(GHIP_EP_DGATED, &p, &ep, st));
     const size_t part_bytes = ffn_ws_part(M, I, K, 2);
-    void *part = part_bytes ? (uint8_t *)ws + 2 * ffn_ws_mat(M, I) : NULL;
-    if (dx && ffn_dx(dg, du, ld, wg, wu, dx, M, I, K, lddx, 1, part, part_bytes, st)) return 1;
-    if (dwg || dwu) {
-        const int both = dwg && dwu;
-        if (ffn_dw(dwg ? dg : du, both ? du : NULL, ld, x, ldx, dwg ? dwg : dwu, both ? dwu : NULL,
-                   M, I, K, 1, part, part_bytes, st))
-            return 1;
-    }
+    const FfnGrads grads = { .dz = dg, .dz2 = du, .w = wg, .w2 = wu, .x = x, .dx = dx, .dw = dwg,
+                             .dw2 = dwu, .M = M, .N = I, .K = K, .lddz = ld, .ldx = ldx,
+                             .lddx = lddx, .pad = 1,
+                             .part = part_bytes ? (uint8_t *)ws + 2 * ffn_ws_mat(M, I) : NULL,
+                             .part_bytes = part_bytes };
+    if (ffn_grads(&grads, st)) return 1;
     G.dispatches++;
     return 0;
 }

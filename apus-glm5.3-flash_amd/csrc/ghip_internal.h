@@ -303,8 +303,12 @@ typedef struct {
 /* Any shape, stride and alignment. */
 hipError_t ghip_launch_ffn_any(int mode, const GhipProd *p, const GhipEp *ep, hipStream_t st);
 /* out[n] = bf16(sum over m of dz[m, n]), dz bf16 with rows ld apart. */
-hipError_t ghip_launch_ffn_colsum(const uint16_t *dz, size_t ld, size_t M, size_t N,
-                                  uint16_t *out, hipStream_t st);
+typedef struct {
+    const uint16_t *dz;
+    size_t ld, M, N;
+    uint16_t *out;
+} GhipFfnSum;
+hipError_t ghip_launch_ffn_colsum(const GhipFfnSum *p, hipStream_t st);
 
 /* dst [M, N up to a multiple of 8] = src's rows (ld apart, any alignment), zeros
  * behind; dst 16-byte aligned. */
@@ -336,6 +340,20 @@ const GhipFfnTile *ghip_ffn_forward_tiles(int mode, int w8, int *n);
 const GhipFfnTile *ghip_ffn_fp8_tiles(int mode, int w8, int *n);
 const GhipFfnTile *ghip_ffn_backward_tiles(int mode, int transposed, int *n);
 
+/* Two of them in one launch (k_ffn_grads.hip): the tiles (height, width, LDS) of dx
+ * and dW, the kernel, and its launch with the dbias sum (or NULL). */
+typedef struct {
+    uint32_t dx[3], dw[3];
+    const void *kern;
+    void (*launch)(const GhipProd *dx, const GhipEp *edx, const GhipProd *dw, const GhipEp *edw,
+                   const GhipFfnSum *sum, const GhipFfnTile *tx, const GhipFfnTile *tw,
+                   hipStream_t st);
+} GhipFfnPair;
+const GhipFfnPair *ghip_ffn_pairs(int *n);
+/* The pair that dx and dW make, with their tiles and splits; -1: none. */
+int ghip_ffn_pair_pick(const GhipProd *dx, const GhipProd *dw, uint32_t n_cu, int tile[2],
+                       uint32_t splits[2]);
+
 /* Streaming the weights past a few rows (k_rows_gemm.h), every mode but
  * GHIP_EP_STORE; FP8 in the forward ones. */
 int ghip_ffn_rows_fits(int mode, const GhipProd *p);
@@ -349,6 +367,10 @@ hipError_t ghip_ffn_init(uint32_t n_cu);
 
 /* The product by the kernel that suits its sizes, steps and alignment. */
 hipError_t ghip_launch_ffn(int mode, const GhipProd *p, const GhipEp *ep, hipStream_t st);
+/* dx, dW and dbias of one dz, each left out where NULL; the parts of dx and dw are
+ * the same memory. */
+hipError_t ghip_launch_ffn_grads(const GhipProd *dx, const GhipEp *edx, const GhipProd *dw,
+                                 const GhipEp *edw, const GhipFfnSum *sum, hipStream_t st);
 
 /* One expert slab record of a converted v2 container's apus.index.json
  * (c/gcache.h:896-930): the shard file name and the slab's file offset. */

@@ -76,19 +76,28 @@ static double tile_us(const GhipFfnTile *t, const GhipProd *p, double stages, ui
     return 3.0 + whole * (stages * t->full + t->over) + (part > 0.0 ? stages * us + t->over : 0.0);
 }
 
+static double stages_of(const GhipProd *p) {
+    return (double)((p->K + 63) / 64) * (p->a2 && !p->batch ? 2 : 1);
+}
+
+/* Cells of one split's sums, and how many splits there may be. */
+static size_t cells_of(const GhipProd *p) {
+    return (size_t)p->M * (((size_t)p->N + 7) & ~(size_t)7) * (p->batch ? 2 : 1);
+}
+static uint32_t most_splits(const GhipProd *p) {
+    if (!p->part) return 1;
+    const size_t fit = p->part_bytes / 4 / cells_of(p), len = (size_t)(stages_of(p) / 8);
+    const size_t n = fit < len ? fit : len;
+    return n < 1 ? 1u : n > FFN_MAX_SPLITS ? FFN_MAX_SPLITS : (uint32_t)n;
+}
+
 extern "C" int ghip_ffn_gemm_pick(int mode, const GhipProd *p, uint32_t n_cu, float *us,
                                   uint32_t *splits) {
     int n, best = -1;
     const GhipFfnTile *t = tiles_of(mode, p, &n);
-    const double stages = (double)((p->K + 63) / 64) * (p->a2 && !p->batch ? 2 : 1);
-    const size_t cells = (size_t)p->M * (((size_t)p->N + 7) & ~(size_t)7) * (p->batch ? 2 : 1);
-    uint32_t most = 1;
-    if (mode == GHIP_EP_STORE && p->part) {
-        const size_t fit = p->part_bytes / 4 / cells, len = (size_t)(stages / 8);
-        most = (uint32_t)(fit < len ? fit : len);
-        if (most > FFN_MAX_SPLITS) most = FFN_MAX_SPLITS;
-        if (most < 1) most = 1;
-    }
+    const double stages = stages_of(p);
+    const size_t cells = cells_of(p);
+    const uint32_t most = mode == GHIP_EP_STORE ? most_splits(p) : 1;
     *us = 1e30f;
     for (int i = 0; i < n; i++)
         for (uint32_t s = 1; s <= most; s++) {
@@ -135,29 +144,132 @@ __global__ __launch_bounds__(256) void k_ffn_join(const float *__restrict__ part
     }
 }
 
+/* p as tile t takes it in `splits` pieces of k; false where it cannot. */
+static bool split_up(int mode, const GhipFfnTile *t, uint32_t splits, const GhipProd *p, GhipProd *q) {
+    if (splits < 1 || !tile_grid(t, p, splits)) return false;
+    if (splits > 1
+        && (mode != GHIP_EP_STORE || !p->part || splits > stages_of(p) || splits > p->part_bytes / 4 / cells_of(p)
+            || ((uintptr_t)p->part & 15)))
+        return false;
+    *q = *p;
+    q->splits = splits;
+    if (splits == 1) q->part = nullptr;
+    return true;
+}
+
+static hipError_t join(const GhipProd *p, const GhipEp *ep, hipStream_t st) {
+    const size_t blocks = (cells_of(p) / 8 + 255) / 256;
+    hipLaunchKernelGGL(k_ffn_join, dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st,
+                       p->part, p->splits, p->M, p->N, ep->ldout, ep->out, p->batch ? ep->out2 : nullptr);
+    return hipGetLastError();
+}
+
 extern "C" hipError_t ghip_launch_ffn_gemm(int mode, int tile, uint32_t splits, const GhipProd *p,
                                            const GhipEp *ep, hipStream_t st) {
     int n;
     const GhipFfnTile *t = tiles_of(mode, p, &n);
-    if (!ghip_ffn_gemm_fits(mode, p) || tile < 0 || tile >= n || splits < 1) return hipErrorInvalidValue;
-    const size_t cells = (size_t)p->M * (((size_t)p->N + 7) & ~(size_t)7) * (p->batch ? 2 : 1);
-    const size_t stages = (size_t)((p->K + 63) / 64) * (p->a2 && !p->batch ? 2 : 1);
-    if (splits > 1
-        && (mode != GHIP_EP_STORE || !p->part || splits > stages || splits > p->part_bytes / 4 / cells
-            || ((uintptr_t)p->part & 15)))
+    GhipProd q;
+    if (!ghip_ffn_gemm_fits(mode, p) || tile < 0 || tile >= n || !split_up(mode, t + tile, splits, p, &q))
         return hipErrorInvalidValue;
-    GhipProd q = *p;
-    q.splits = splits;
-    if (splits == 1) q.part = nullptr;
     t += tile;
-    if (!tile_grid(t, p, splits)) return hipErrorInvalidValue;
     t->launch(&q, ep, (p->M + t->bm - 1) / t->bm, (p->N + t->bn - 1) / t->bn, t->lds, st);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || splits == 1) return e;
-    const size_t blocks = (cells / 8 + 255) / 256;
-    hipLaunchKernelGGL(k_ffn_join, dim3((uint32_t)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st,
-                       q.part, splits, p->M, p->N, ep->ldout, ep->out, p->batch ? ep->out2 : nullptr);
-    return hipGetLastError();
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess || splits == 1 ? e : join(&q, ep, st);
+}
+
+/* dx and dW in one launch take about 3 us, the larger of the longest workgroup's
+ * time and the whole's share of the full chip, and 0.7 of the other (within 18%
+ * rms of 150 shapes; the choice by it 2% slower than the best one on average, 24%
+ * faster than two launches). At most one of the two is split, as they would share
+ * the partial sums' memory. */
+extern "C" int ghip_ffn_pair_pick(const GhipProd *dx, const GhipProd *dw, uint32_t n_cu, int tile[2],
+                                  uint32_t splits[2]) {
+    const GhipProd *const p[2] = {dx, dw};
+    const GhipFfnTile *t[2];
+    int nt[2], n, best = -1;
+    double stages[2], join[2], us = 0.0;
+    uint32_t most[2];
+    for (int i = 0; i < 2; i++) {
+        float one;
+        uint32_t s;
+        if (!n_cu || !ghip_ffn_gemm_fits(GHIP_EP_STORE, p[i])
+            || ghip_ffn_gemm_pick(GHIP_EP_STORE, p[i], n_cu, &one, &s) < 0)
+            return -1;
+        us += one;
+        t[i] = tiles_of(GHIP_EP_STORE, p[i], &nt[i]);
+        stages[i] = stages_of(p[i]);
+        most[i] = most_splits(p[i]);
+        join[i] = (double)cells_of(p[i]) * 4.0 * 2.0 / 3e6;
+    }
+    const GhipFfnPair *const pairs = ghip_ffn_pairs(&n);
+    for (int i = 0; i < n; i++) {
+        int at[2];
+        for (int k = 0; k < 2; k++) {
+            const uint32_t *want = k ? pairs[i].dw : pairs[i].dx;
+            for (at[k] = 0; at[k] < nt[k]; at[k]++) {
+                const GhipFfnTile *c = t[k] + at[k];
+                if (c->bm == want[0] && c->bn == want[1] && c->lds == want[2]) break;
+            }
+            if (at[k] == nt[k]) return -1;
+        }
+        for (uint32_t v = 1; v < most[0] + most[1]; v++) {
+            const uint32_t s[2] = {v <= most[0] ? v : 1u, v <= most[0] ? 1u : v - most[0] + 1u};
+            double longest = 0.0, whole = 0.0, extra = 0.0;
+            bool fits = true;
+            for (int k = 0; k < 2; k++) {
+                const GhipFfnTile *c = t[k] + at[k];
+                const size_t grid = tile_grid(c, p[k], s[k]);
+                const double len = (double)(size_t)((stages[k] + s[k] - 1) / s[k]);
+                const double chain = len * c->low + c->over;
+                fits = fits && grid;
+                whole += (double)grid / ((double)n_cu * c->occ) * (len * c->full + c->over);
+                if (chain > longest) longest = chain;
+                if (s[k] > 1) extra = 4.0 + join[k] * s[k];
+            }
+            const double e = 3.0 + (whole > longest ? whole + 0.7 * longest : longest + 0.7 * whole) + extra;
+            if (fits && e < us) {
+                us = e;
+                best = i;
+                for (int k = 0; k < 2; k++) {
+                    tile[k] = at[k];
+                    splits[k] = s[k];
+                }
+            }
+        }
+    }
+    return best;
+}
+
+/* dbias goes with the products up to this many rows: its 256 threads a workgroup
+ * take 32 of them at a time, a launch of its own 256. A pair of 12.4 us takes 12.5
+ * with the sum of 1024 x 2048 (16.8 with a launch more) and 26.6 with that of 2048
+ * x 2048 (19.2). */
+#define FFN_SUM_ROWS 1024u
+#define FFN_PAIR_LDS (80u * 1024u)                 /* two workgroups a CU */
+
+extern "C" hipError_t ghip_launch_ffn_grads(const GhipProd *dx, const GhipEp *edx, const GhipProd *dw,
+                                            const GhipEp *edw, const GhipFfnSum *sum, hipStream_t st) {
+    int tile[2], n;
+    uint32_t splits[2];
+    hipError_t e = hipSuccess;
+    const int pair = dx && dw ? ghip_ffn_pair_pick(dx, dw, g_ffn_ncu, tile, splits) : -1;
+    GhipProd x, w;
+    if (pair >= 0) {
+        const GhipFfnTile *tx = tiles_of(GHIP_EP_STORE, dx, &n) + tile[0];
+        const GhipFfnTile *tw = tiles_of(GHIP_EP_STORE, dw, &n) + tile[1];
+        const bool with = sum && sum->M <= FFN_SUM_ROWS;
+        if (split_up(GHIP_EP_STORE, tx, splits[0], dx, &x) && split_up(GHIP_EP_STORE, tw, splits[1], dw, &w)
+            && tile_grid(tx, dx, splits[0]) + tile_grid(tw, dw, splits[1]) <= GHIP_MAX_THREADS / 256 / 2) {
+            ghip_ffn_pairs(&n)[pair].launch(&x, edx, &w, edw, with ? sum : nullptr, tx, tw, st);
+            e = hipGetLastError();
+            if (e == hipSuccess && splits[0] > 1) e = join(&x, edx, st);
+            if (e == hipSuccess && splits[1] > 1) e = join(&w, edw, st);
+            return e == hipSuccess && sum && !with ? ghip_launch_ffn_colsum(sum, st) : e;
+        }
+    }
+    if (dx) e = ghip_launch_ffn(GHIP_EP_STORE, dx, edx, st);
+    if (e == hipSuccess && dw) e = ghip_launch_ffn(GHIP_EP_STORE, dw, edw, st);
+    return e == hipSuccess && sum ? ghip_launch_ffn_colsum(sum, st) : e;
 }
 
 extern "C" hipError_t ghip_launch_ffn(int mode, const GhipProd *p, const GhipEp *ep,
@@ -183,6 +295,13 @@ extern "C" hipError_t ghip_ffn_init(uint32_t n_cu) {
                 t[k].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)t[k].lds);
             if (e != hipSuccess) return e;
         }
+    }
+    int n;
+    const GhipFfnPair *pairs = ghip_ffn_pairs(&n);
+    for (int i = 0; i < n; i++) {
+        const hipError_t e = hipFuncSetAttribute(
+            pairs[i].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(FFN_PAIR_LDS));
+        if (e != hipSuccess) return e;
     }
     const hipError_t e = ghip_ffn_rows_init();
     if (e != hipSuccess) return e;

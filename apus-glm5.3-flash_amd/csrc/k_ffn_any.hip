@@ -22,6 +22,7 @@
  * that).
  */
 #include "ghip_epilogue.h"
+#include "k_ffn_colsum.h"
 
 #define FA_LD 40u                                /* LDS row: 32 values, 80 bytes */
 
@@ -150,45 +151,12 @@ __global__ __launch_bounds__(256) void k_ffn_any(GhipProd p, GhipEp ep, uint32_t
     });
 }
 
-/* dbias[n] = sum_m dz[m, n] in f32, rounded once. A workgroup owns 64 columns,
- * a thread 8 of them in every 128th row (one load at any alignment); the 128
- * rows' sums are added in a fixed order. Bound by latency: 300 x 2048 3.3 us
- * under the profiler (one column and 16 rows a thread at a time: 7.2). */
-__global__ __launch_bounds__(1024) void k_ffn_colsum(const uint16_t *__restrict__ dz, size_t ld,
-                                                     uint32_t M, uint32_t N,
-                                                     uint16_t *__restrict__ out) {
-    __shared__ float sum[128][65];
-    const uint32_t c = 8u * (threadIdx.x & 7u), r = threadIdx.x >> 3, n = blockIdx.x * 64u + c;
-    float s[8] = {};
-    if (n + 8u <= N) {
-#pragma unroll 4
-        for (uint32_t m = r; m < M; m += 128u) {
-            fa_u16x8 d;
-            __builtin_memcpy(&d, dz + (size_t)m * ld + n, 16);
-#pragma unroll
-            for (uint32_t e = 0; e < 8; e++) s[e] += ghip_bf16_f32(d[e]);
-        }
-    } else {
-        for (uint32_t m = r; m < M; m += 128u)
-#pragma unroll
-            for (uint32_t e = 0; e < 8; e++)
-                if (n + e < N) s[e] += ghip_bf16_f32(dz[(size_t)m * ld + n + e]);
-    }
-#pragma unroll
-    for (uint32_t e = 0; e < 8; e++) sum[r][c + e] = s[e];
-    /* 16 threads a column, then the first of them */
-    __syncthreads();
-    const uint32_t q = threadIdx.x & 63u, g = threadIdx.x >> 6;
-    float v = 0.0f;
-    for (uint32_t i = 0; i < 8; i++) v += sum[8u * g + i][q];
-    __syncthreads();
-    sum[g][q] = v;
-    __syncthreads();
-    if (g == 0 && blockIdx.x * 64u + q < N) {
-        v = 0.0f;
-        for (uint32_t i = 0; i < 16; i++) v += sum[i][q];
-        out[blockIdx.x * 64u + q] = (uint16_t)ghip_bf16_bits(v);
-    }
+/* dbias. Bound by latency: with the launch, 300 x 2048 2.8 us, 4096 x 2048 10.9 (64
+ * columns a workgroup: 14; 16: 13.8). */
+#define FA_SUM 32u                               /* columns of a workgroup */
+__global__ __launch_bounds__(1024) void k_ffn_colsum(GhipFfnSum p) {
+    __shared__ float sum[8 * 1024 / FA_SUM][FA_SUM + 1];
+    fc_colsum<1024, FA_SUM>(p, blockIdx.x, sum);
 }
 
 /* dst[m, 0 .. N up to a multiple of 8) = src[m, 0 .. N), zeros behind: rows of any
@@ -255,11 +223,9 @@ extern "C" hipError_t ghip_launch_ffn_any(int mode, const GhipProd *p, const Ghi
     }
 }
 
-extern "C" hipError_t ghip_launch_ffn_colsum(const uint16_t *dz, size_t ld, size_t M, size_t N,
-                                             uint16_t *out, hipStream_t st) {
-    if (M == 0 || N == 0 || M > 0x7fffffffu || N > 0x7fffffffu) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_ffn_colsum, dim3((uint32_t)((N + 63) / 64)), dim3(1024), 0, st, dz, ld,
-                       (uint32_t)M, (uint32_t)N, out);
+extern "C" hipError_t ghip_launch_ffn_colsum(const GhipFfnSum *p, hipStream_t st) {
+    if (p->M == 0 || p->N == 0 || p->M > 0x7fffffffu || p->N > 0x7fffffffu) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(k_ffn_colsum, dim3((uint32_t)((p->N + FA_SUM - 1) / FA_SUM)), dim3(1024), 0, st, *p);
     return hipGetLastError();
 }
 

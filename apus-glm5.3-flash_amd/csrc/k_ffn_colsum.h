@@ -1,0 +1,54 @@
+/*
+ * k_ffn_colsum.h — dbias[n] = sum_m dz[m, n] in f32, rounded once (gfx950): the
+ * body of a workgroup of T threads (k_ffn_any.hip, k_ffn_grads.hip).
+ *
+ * It owns C columns, a thread 8 of them in every 8T/C-th row (one load at any
+ * alignment); the 8T/C threads' sums are added in a fixed order.
+ */
+#ifndef K_FFN_COLSUM_H
+#define K_FFN_COLSUM_H
+
+#include "ghip_device.h"
+#include "ghip_internal.h"
+
+typedef unsigned short fc_u16x8 __attribute__((ext_vector_type(8)));
+
+/* sum: 8T/C rows in LDS */
+template <uint32_t T, uint32_t C>
+__device__ __forceinline__ void fc_colsum(const GhipFfnSum &p, uint32_t block,
+                                          float (*sum)[C + 1]) {
+    constexpr uint32_t R = 8u * T / C;
+    const uint32_t c = 8u * (threadIdx.x % (C / 8u)), r = threadIdx.x / (C / 8u), n = block * C + c;
+    float s[8] = {};
+    if (n + 8u <= p.N) {
+#pragma unroll 8
+        for (uint32_t m = r; m < p.M; m += R) {
+            fc_u16x8 d;
+            __builtin_memcpy(&d, p.dz + (size_t)m * p.ld + n, 16);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) s[e] += ghip_bf16_f32(d[e]);
+        }
+    } else {
+        for (uint32_t m = r; m < p.M; m += R)
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++)
+                if (n + e < p.N) s[e] += ghip_bf16_f32(p.dz[(size_t)m * p.ld + n + e]);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8; e++) sum[r][c + e] = s[e];
+    /* C threads add 8 rows' sums, then the first of them the T/C sums */
+    __syncthreads();
+    const uint32_t q = threadIdx.x % C, g = threadIdx.x / C;
+    float v = 0.0f;
+    for (uint32_t i = 0; i < 8; i++) v += sum[8u * g + i][q];
+    __syncthreads();
+    sum[g][q] = v;
+    __syncthreads();
+    if (g == 0 && block * C + q < p.N) {
+        v = 0.0f;
+        for (uint32_t i = 0; i < T / C; i++) v += sum[i][q];
+        p.out[block * C + q] = (uint16_t)ghip_bf16_bits(v);
+    }
+}
+
+#endif /* K_FFN_COLSUM_H */

@@ -153,8 +153,8 @@ __device__ __forceinline__ ghip_u32x4 fg_pack(const float (&v)[8]) {
 
 /* W8: 0 bf16 weights, 1 FP8 codes, 2 FP8 codes with NaN codes among them */
 template <int MODE, int W8, int AL, int BL, int WM, int RB, int CB, int L>
-__global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint32_t mt,
-                                                     uint32_t nt) {
+__device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, uint32_t mt,
+                                           uint32_t nt, uint32_t block, uint32_t blocks) {
     constexpr bool DUAL = ghip_ep_dual(MODE), FP8 = W8 != 0;
     constexpr uint32_t WN = 4 / WM, BM = 16u * RB * WM, BN = 16u * CB * WN;
     constexpr uint32_t OUTN = DUAL ? BN / 2 : BN;        /* output columns of a tile */
@@ -172,15 +172,14 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
     const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t wr = wv / WN, wc = wv % WN, n = lane & 15u, g = lane >> 4;
 
-    /* tile t: the workgroups of one XCD (b % 8) take a run of consecutive
+    /* tile t of block b: the workgroups of one XCD (b % 8) take a run of consecutive
      * tiles, which go down 4 row tiles before the next column, so that an XCD's
      * L2 holds few rows of A and of B at a time (8192 x 24576 x 4096: 4 1.148
      * ms, 8 1.157, 16 1.18). A batch of two: the second half of the tiles is the
      * second product. Splits of k: each walks its share of the stages. */
     uint32_t t;
     {
-        const uint32_t T = gridDim.x, x = blockIdx.x & 7u, i = blockIdx.x >> 3;
-        const uint32_t q = T >> 3, r = T & 7u;
+        const uint32_t x = block & 7u, i = block >> 3, q = blocks >> 3, r = blocks & 7u;
         t = x * q + (x < r ? x : r) + i;
     }
     bool second = false;
@@ -567,6 +566,12 @@ __global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint
             __builtin_amdgcn_wave_barrier();
         }
     });
+}
+
+template <int MODE, int W8, int AL, int BL, int WM, int RB, int CB, int L>
+__global__ __launch_bounds__(256, 1) void k_ffn_gemm(GhipProd p, GhipEp ep, uint32_t mt,
+                                                     uint32_t nt) {
+    fg_product<MODE, W8, AL, BL, WM, RB, CB, L>(p, ep, mt, nt, blockIdx.x, gridDim.x);
 }
 
 #endif /* K_FFN_GEMM_H */

@@ -14,6 +14,11 @@
 
 #include "k_ffn_gemm.h"
 
+/* LDS of bm rows of A and bst bytes a stage of B, L stages ahead */
+static constexpr uint32_t fg_ring(uint32_t bm, uint32_t bst, uint32_t L) {
+    return (L + 1u) * bm * 128u + L * bst;
+}
+
 template <int MODE, int W8, int AL, int BL, int WM, int RB, int CB, int L>
 static void fg_run(const GhipProd *p, const GhipEp *ep, uint32_t mt, uint32_t nt, uint32_t lds,
                    hipStream_t st) {
@@ -25,7 +30,7 @@ static void fg_run(const GhipProd *p, const GhipEp *ep, uint32_t mt, uint32_t nt
 template <int MODE, int W8, int AL, int BL, int WM, int RB, int CB, int L>
 static constexpr GhipFfnTile fg_tile(float low, float mid, float full, float over) {
     constexpr uint32_t bm = 16u * RB * WM, bn = 16u * CB * (4 / WM);
-    constexpr uint32_t lds = (L + 1u) * bm * 128u + L * bn * (W8 ? 64u : 128u);
+    constexpr uint32_t lds = fg_ring(bm, bn * (W8 ? 64u : 128u), L);
     return {bm, ghip_ep_dual(MODE) ? bn / 2 : bn, lds <= FG_LDS_MAX / 2 ? 2u : 1u, low, mid, full, over, lds,
             (const void *)k_ffn_gemm<MODE, W8, AL, BL, WM, RB, CB, L>,
             fg_run<MODE, W8, AL, BL, WM, RB, CB, L>};

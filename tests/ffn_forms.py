@@ -95,3 +95,29 @@ def route(lib, family, p):
 def part_bytes(lib, M, N, K):
     lib.ghip_ffn_part_bytes.restype = ctypes.c_size_t
     return lib.ghip_ffn_part_bytes(*(ctypes.c_size_t(v) for v in (M, N, K)))
+
+
+class Sum(ctypes.Structure):
+    _fields_ = [("dz", ctypes.c_void_p)] + [(n, ctypes.c_size_t) for n in ("ld", "M", "N")] + [("out", ctypes.c_void_p)]
+
+
+class Pair(ctypes.Structure):
+    _fields_ = [("dx", ctypes.c_uint32 * 3), ("dw", ctypes.c_uint32 * 3), ("kern", ctypes.c_void_p),
+                ("launch", ctypes.CFUNCTYPE(None, *[ctypes.c_void_p] * 8))]
+
+
+PAIRS = 4
+
+
+def pairs(lib):
+    n = ctypes.c_int()
+    lib.ghip_ffn_pairs.restype = ctypes.POINTER(Pair)
+    t = lib.ghip_ffn_pairs(ctypes.byref(n))
+    return [t[i] for i in range(n.value)]
+
+
+def pair_pick(lib, dx, dw):
+    """(pair, tiles, splits) of dx and dW in one launch; pair -1: two launches."""
+    tile, splits = (ctypes.c_int * 2)(), (ctypes.c_uint32 * 2)()
+    i = lib.ghip_ffn_pair_pick(ctypes.byref(dx), ctypes.byref(dw), ctypes.c_uint32(NCU), tile, splits)
+    return i, list(tile), list(splits)

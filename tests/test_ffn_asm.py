@@ -17,7 +17,7 @@ from conftest import ROOT
 
 OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
 BUILD = os.path.join(ROOT, "apus-glm5.3-flash_amd", "_build")
-OBJECTS = ["k_ffn_nt.hip.o", "k_ffn_nt8.hip.o", "k_ffn_bwd.hip.o"]
+OBJECTS = ["k_ffn_nt.hip.o", "k_ffn_nt8.hip.o", "k_ffn_bwd.hip.o", "k_ffn_grads.hip.o"]
 
 
 def registers(text):
@@ -56,7 +56,7 @@ def kernels(path, tmp_path):
     text = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", os.path.join(tmp_path, code[0])], check=True,
                           capture_output=True, text=True).stdout
     out = {}
-    for name, body in re.findall(r"^[0-9a-f]+ <(\S*k_ffn_gemm\S*)>:\n((?:[ \t].*\n)+)", text, re.M):
+    for name, body in re.findall(r"^[0-9a-f]+ <(\S*k_ffn_g(?:emm|rads)\S*)>:\n((?:[ \t].*\n)+)", text, re.M):
         start, ins, at, branches = None, [], {}, []
         for line in body.splitlines():
             s, _, addr = line.partition("//")

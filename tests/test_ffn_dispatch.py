@@ -135,3 +135,42 @@ def test_launchers_refuse_before_the_device(lib):
     for form in (-1, 99):
         assert lib.ghip_launch_ffn_rows(F.LINEAR, form, ctypes.byref(r), ctypes.byref(e), None)
     assert lib.ghip_launch_ffn_rows(F.STORE, 0, ctypes.byref(p), ctypes.byref(e), None)
+
+
+def block(lib, M, N, K, two):
+    """The dx and dW products of a backward pass, in one workspace."""
+    n, ld = 2 if two else 1, -(-N // 8) * 8
+    more = dict(a2=F.AT, b2=F.AT) if two else {}
+    dx, dw = F.prod("dx", M, K, N, lda=ld, apad=1, **more), F.prod("dw", N, K, M, lda=ld, apad=1, batch=int(two), **more)
+    room = max(F.part_bytes(lib, M, K, n * N), F.part_bytes(lib, n * N, K, M))
+    for p in (dx, dw):
+        p.part, p.part_bytes = F.AT if room else None, room
+    return dx, dw
+
+
+def test_pairs(lib):
+    """Every pair is some backward pass's choice, alone and with either product
+    split, never with both; its tiles are in the tables."""
+    pairs = F.pairs(lib)
+    assert len(pairs) == F.PAIRS
+    taken, apart = set(), 0
+    for i, (M, N, K) in enumerate(shapes(12000, 8)):
+        dx, dw = block(lib, M, N, K, i % 2)
+        pair, tile, splits = F.pair_pick(lib, dx, dw)
+        if pair < 0:
+            apart += 1
+            continue
+        for k, (family, want, p) in enumerate((("dx", pairs[pair].dx, dx), ("dw", pairs[pair].dw, dw))):
+            t = F.tiles(lib, family)[tile[k]]
+            assert (t.bm, t.bn, t.lds) == tuple(want) and t.occ == 2
+            stages = (p.K + 63) // 64 * (2 if family == "dx" and p.a2 else 1)
+            assert splits[k] == 1 or (splits[k] <= 16 and stages // splits[k] >= 8
+                                      and splits[k] * p.M * p.N * 4 * (2 if p.batch else 1) <= p.part_bytes)
+        assert min(splits) == 1
+        taken.add((pair, splits[0] > 1, splits[1] > 1))
+    assert {t[0] for t in taken} == set(range(F.PAIRS)) and apart > 500
+    assert {t[1:] for t in taken} == {(False, False), (True, False), (False, True)}
+    dx, dw = block(lib, 300, 512, 256, 0)
+    assert F.pair_pick(lib, dx, dw)[0] >= 0
+    dw.b = F.AT + 2                                                 # x that direct loads cannot take
+    assert F.pair_pick(lib, dx, dw)[0] == -1

@@ -9,6 +9,7 @@ import ffn_forms as F
 import ffn_ref as R
 import gpu_util as G
 import oracle as O
+import test_gpu_ffn as T
 from test_gpu_ffn import Mat, bf, fp8, seed, wide
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +142,70 @@ def test_gradient_tile(ghip, family, two, tile, splits):
             want, tol = sums([(wide(a), wide(b)) for a, b in of])
             R.check(wide(out.get()), want, tol, (family, tile, M, N, K, splits, two))
         assert np.isnan(G.host(part, np.float32, size // 4 + 64)[size // 4:]).all()
+
+
+@pytest.mark.parametrize("pair", range(F.PAIRS))
+@pytest.mark.parametrize("sx,sw", [(1, 1), (3, 1), (1, 2)])
+@pytest.mark.parametrize("two", [0, 1])
+@pytest.mark.parametrize("M,N,K", [(200, 264, 192), (395, 129, 328), (130, 8, 1032)])
+def test_pair(ghip, pair, sx, sw, two, M, N, K):
+    """dx, dW and dbias in one launch: any of them in pieces of k."""
+    pr = F.pairs(ghip)[pair]
+    tiles = [[t for t in F.tiles(ghip, f) if (t.bm, t.bn, t.lds) == tuple(w)][0] for f, w in (("dx", pr.dx), ("dw", pr.dw))]
+    rng = seed(M, N, K, two, pair)
+    dz, w = [bf(rng.standard_normal((M, N))) for _ in range(1 + two)], [bf(rng.standard_normal((N, K)) / np.sqrt(K)) for _ in range(1 + two)]
+    x = bf(rng.standard_normal((M, K)))
+    dzd, wd, xd = [laid(z, 0) for z in dz], [G.dev(v) for v in w], G.dev(x)
+    ld = dzd[0][1]
+    stages = -(-N // 64) * (1 + two), -(-M // 64)
+    sx, sw = min(sx, stages[0]), min(sw, stages[1])
+    cells = sx * M * K if sx > 1 else sw * N * K * (1 + two)
+    part = G.dev(np.full(cells + 64, np.nan, np.float32))
+    more = lambda a, b: dict(a2=addr(a[0]), b2=addr(b)) if two else {}  # noqa: E731
+    px = F.prod("dx", M, K, N, a=addr(dzd[0][0]), b=addr(wd[0]), lda=ld, apad=1, splits=sx, part=addr(part) if sx > 1 else None,
+                **more(dzd[-1], wd[-1]))
+    pw = F.prod("dw", N, K, M, a=addr(dzd[0][0]), b=addr(xd), lda=ld, apad=1, batch=two, splits=sw, part=addr(part) if sw > 1 else None,
+                **more(dzd[-1], xd))
+    dx, dw, db = Mat.out(M, K, 3, 1), [Mat.out(N, K) for _ in range(1 + two)], Mat.out(1, N)
+    ex, ew = F.Ep(out=dx.p.value, ldout=dx.ld), F.Ep(out=dw[0].p.value, out2=dw[-1].p.value, ldout=K)
+    sm = F.Sum(dz=addr(dzd[0][0]), ld=ld, M=M, N=N, out=db.p.value)
+    at = lambda s: ctypes.cast(ctypes.byref(s), ctypes.c_void_p)    # noqa: E731
+    pr.launch(at(px), at(ex), at(pw), at(ew), at(sm), at(tiles[0]), at(tiles[1]), None)
+    f = G.host(part, np.float32, cells + 64)
+    assert np.isnan(f[cells:]).all()
+    grads = R._grads(wide(x), [(wide(v), wide(z), np.zeros((M, N))) for v, z in zip(w, dz)])
+    if sx > 1:                                                      # the sums that would be joined
+        got = f[:cells].reshape(sx, M, K).astype(np.float64).sum(0)
+        assert np.all(np.abs(got - grads["dx"][0]) <= grads["dx"][1]) and (dx.get() == 0x7E57).all()
+    else:
+        R.check(wide(dx.get()), *grads["dx"], "dx")
+    for i, m in enumerate(dw):
+        if sw > 1:
+            got = f[:cells].reshape(1 + two, sw, N, K)[i].astype(np.float64).sum(0)
+            assert np.all(np.abs(got - grads["dw%d" % i][0]) <= grads["dw%d" % i][1]) and (m.get() == 0x7E57).all()
+        else:
+            R.check(wide(m.get()), *grads["dw%d" % i], "dw%d" % i)
+    R.check(wide(db.get())[0], *grads["db"], "db")
+
+
+# M, N, K, two: a pair alone, with dx split, with dW split, with the sum in a launch of its own; two launches; rows of odd widths
+BACKWARDS = [(300, 512, 256, 0), (57, 3400, 1472, 1), (2165, 72, 288, 1), (1200, 96, 264, 0), (600, 2048, 2048, 1), (333, 129, 72, 0),
+             (90, 257, 136, 1)]
+
+
+@pytest.mark.parametrize("M,N,K,two", BACKWARDS)
+def test_gradients_of_the_entries(ghip, M, N, K, two):
+    rng = seed(M, N, K, two, 77)
+    x, w = bf(rng.standard_normal((M, K))), [bf(rng.standard_normal((N, K)) / np.sqrt(K)) for _ in range(1 + two)]
+    dy = bf(rng.standard_normal((M, N)))
+    if two:
+        got = T.run_gated_bwd(ghip, G.dev(w[0]), G.dev(w[1]), Mat(x), Mat(dy), M, N, K, R.SILU, 0.0)
+        want = R.gated_backward(wide(x), wide(w[0]), wide(w[1]), wide(dy), R.SILU, 0.0)
+        names = {"dx": "dx", "dwg": "dw0", "dwu": "dw1"}
+    else:
+        got = T.run_linear_bwd(ghip, G.dev(w[0]), Mat(x), None, Mat(dy), M, N, K, R.GELU)
+        want = R.linear_backward(wide(x), wide(w[0]), None, wide(dy), R.GELU)
+        names = {"dx": "dx", "dw": "dw0", "db": "db"}
+    for a, b in names.items():
+        v, tol = want[b]
+        R.check(wide(got[a]).reshape(v.shape), v, tol, (M, N, K, a))
