@@ -13,7 +13,8 @@ static const GhipFfnTile *tiles_of(int mode, const GhipProd *p, int *n) {
                : ghip_ffn_backward_tiles(mode, p->aks != 1, n);
 }
 
-/* 16-byte loads along the fast index, from whole vectors, with offsets of 31
+/* 16-byte loads along the fast index, from whole vectors (FP8: from whole 8
+ * bytes), with offsets of 31
  * bits inside a tile (256 rows, or 64 k). */
 static bool vectors(const void *q, size_t rs, size_t ks, size_t rows, size_t k, size_t per,
                     bool pad) {
@@ -24,15 +25,15 @@ static bool vectors(const void *q, size_t rs, size_t ks, size_t rows, size_t k, 
 
 extern "C" int ghip_ffn_gemm_fits(int mode, const GhipProd *p) {
     const bool fp8 = p->s != nullptr;
-    const size_t per = fp8 ? 16 : 8;
     if (fp8 && mode != GHIP_EP_LINEAR && mode != GHIP_EP_GATED) return 0;
     /* the layouts that are built: k fast in both, in A alone, in neither */
     if (p->aks != 1 && p->bks == 1) return 0;
     if (mode != GHIP_EP_STORE && (p->aks != 1 || p->bks != 1)) return 0;
     if (mode == GHIP_EP_STORE && p->bks == 1) return 0;
     if (!vectors(p->a, p->ars, p->aks, p->M, p->K, 8, p->apad)
-        || !vectors(p->b, p->brs, p->bks, p->N, p->K, per, false))
+        || !vectors(p->b, p->brs, p->bks, p->N, p->K, 8, false))
         return 0;
+    if (fp8 && p->K < 16) return 0;                      /* a row's half piece needs a whole one */
     if ((p->a2 && ((uintptr_t)p->a2 & 15)) || (p->b2 && ((uintptr_t)p->b2 & 15))) return 0;
     return 1;
 }

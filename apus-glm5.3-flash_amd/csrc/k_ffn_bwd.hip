@@ -7,15 +7,15 @@
 
 static const GhipFfnTile *dlinear_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 8, 8, 2>(1.01f, 0.00f, 1.39f, 8.5f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 6, 8, 2>(0.88f, 0.00f, 1.12f, 3.5f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 8, 4, 2>(0.65f, 0.00f, 0.88f, 2.0f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 6, 4, 2>(0.58f, 0.00f, 0.74f, 0.0f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 4, 4, 4>(0.40f, 0.00f, 0.54f, 0.9f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 4, 4, 2>(0.49f, 0.66f, 0.97f, 0.0f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 4, 5>(0.32f, 0.00f, 0.38f, 0.0f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 2, 6>(0.22f, 0.00f, 0.26f, 0.6f),
-        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 2, 3>(0.22f, 0.28f, 0.42f, 0.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 8, 8, 2>(1.03f, 0.00f, 1.42f, 9.7f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 6, 8, 2>(0.94f, 0.00f, 1.20f, 4.7f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 8, 4, 2>(0.72f, 0.00f, 0.97f, 3.2f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 6, 4, 2>(0.66f, 0.00f, 0.84f, 1.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 4, 4, 4>(0.45f, 0.00f, 0.60f, 2.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 4, 4, 2>(0.57f, 0.76f, 1.11f, 1.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 4, 5>(0.35f, 0.00f, 0.42f, 1.0f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 2, 6>(0.23f, 0.00f, 0.27f, 1.6f),
+        fg_tile<GHIP_EP_DLINEAR, 0, 0, 0, 2, 2, 2, 3>(0.24f, 0.31f, 0.46f, 1.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;
@@ -23,14 +23,14 @@ static const GhipFfnTile *dlinear_tiles(int *n) {
 
 static const GhipFfnTile *dgated_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 8, 8, 2>(1.02f, 0.00f, 1.39f, 15.3f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 6, 8, 2>(1.02f, 0.00f, 1.14f, 8.1f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 6, 4, 2>(0.74f, 0.00f, 0.81f, 1.3f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 4, 4, 4>(0.43f, 0.00f, 0.54f, 2.8f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 4, 4, 2>(0.69f, 0.80f, 1.01f, 0.0f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 4, 5>(0.45f, 0.00f, 0.42f, 0.1f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 2, 6>(0.28f, 0.00f, 0.28f, 1.2f),
-        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 2, 3>(0.27f, 0.39f, 0.46f, 0.0f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 8, 8, 2>(1.03f, 0.00f, 1.40f, 16.5f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 6, 8, 2>(1.02f, 0.00f, 1.13f, 9.0f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 6, 4, 2>(0.72f, 0.00f, 0.78f, 2.2f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 4, 4, 4>(0.48f, 0.00f, 0.59f, 4.1f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 4, 4, 2>(0.66f, 0.77f, 0.97f, 1.0f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 4, 5>(0.43f, 0.00f, 0.41f, 1.1f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 2, 6>(0.26f, 0.00f, 0.26f, 2.2f),
+        fg_tile<GHIP_EP_DGATED, 0, 0, 0, 2, 2, 2, 3>(0.26f, 0.38f, 0.45f, 1.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;

@@ -273,6 +273,16 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
         const uint32_t span = AL == 1 && lf < 64u ? lf * lda * 2u : FG_SPAN;
         fg_dma16(pa, span, AL == 0 && akq >= lf ? FG_OOB : ao[i], fg_lds + sa + (wv + 4u * i) * 1024u);
     };
+    /* FP8 rows of K % 16 == 8 codes end in half a piece: the last stage's is read 8
+     * bytes early, and its codes move down when they are read from LDS */
+    const bool half = FP8 && (p.K & 8u);
+    auto half_loads = [&]() {
+        if (half && jb + 1u == nst1) {
+            pb -= 8;
+#pragma unroll
+            for (uint32_t i = 0; i < NBL; i++) bo[i] += left(jb) - bkq == 8u ? 0u : 8u;
+        }
+    };
     auto load_b = [&](uint32_t i) {
         const uint32_t lf = left(jb);
         const uint32_t span = BL == 1 && lf < 64u ? lf * ldb * 2u : FG_SPAN;
@@ -289,7 +299,9 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
         pb += bstep;
         if (MODE == GHIP_EP_STORE && jb == nst1 && all > nst1) pb = base_b(p.b2);
         sb = sb == (L - 1u) * BST ? 0u : sb + BST;
+        if constexpr (FP8) half_loads();
     };
+    if constexpr (FP8) half_loads();                     /* one stage */
 
     /* operand reads: block blk of 16 rows, step s */
     uint32_t off0[2];
@@ -326,6 +338,12 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
                                              + 16u * (g ^ fg_rot4(n)));
         else
             wa[set][c] = frag(LB{}, WB{}, st, wc * CB + c, s);
+    };
+    auto half_codes = [&]() {                            /* of the last stage */
+        if (half && left(nst1 - 1u) - 16u * g == 8u) {
+#pragma unroll
+            for (int c = 0; c < CB; c++) codes[FP8 ? c : 0] = (ghip_u32x4){codes[FP8 ? c : 0][2], codes[FP8 ? c : 0][3], 0u, 0u};
+        }
     };
     /* FP8: quarter q of column block c's operand of step s (4 codes) */
     float sc0 = 0.0f, sc1 = 0.0f;
@@ -370,6 +388,7 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
 #pragma unroll
     for (int r = 0; r < RB; r++) read_a(0, r, fg_lds, 0);
     if constexpr (FP8) {
+        if (nst == 1u) half_codes();
 #pragma unroll
         for (int c = 0; c < CB; c++)
 #pragma unroll
@@ -416,6 +435,8 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
                     if constexpr (O < (int)CB) read_b(S ^ 1, O, bs, S ^ 1);
                     else read_a(S ^ 1, O - CB, as, S ^ 1);
                 });
+                if constexpr (FP8 && S == 1 && !MAIN && I == DF)
+                    if (more && j + 2u == nst) half_codes();
                 fg_each<Q1 - Q0>([&](auto k) {
                     constexpr int Q = Q0 + decltype(k)::value;
                     dequant(S ^ 1, Q >> 1, S ^ 1, Q & 1);

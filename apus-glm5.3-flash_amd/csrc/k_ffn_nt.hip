@@ -7,14 +7,14 @@
 
 static const GhipFfnTile *linear_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 8, 8, 2>(1.01f, 0.00f, 1.39f, 8.5f),
-        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 6, 8, 2>(0.88f, 0.00f, 1.12f, 3.5f),
-        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 6, 4, 2>(0.58f, 0.00f, 0.74f, 0.0f),
-        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 4, 4, 4>(0.40f, 0.00f, 0.54f, 0.9f),
-        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 4, 4, 2>(0.49f, 0.66f, 0.97f, 0.0f),
-        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 4, 5>(0.32f, 0.00f, 0.38f, 0.0f),
-        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 2, 6>(0.22f, 0.00f, 0.26f, 0.6f),
-        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 2, 3>(0.22f, 0.28f, 0.42f, 0.0f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 8, 8, 2>(1.03f, 0.00f, 1.42f, 8.7f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 6, 8, 2>(0.94f, 0.00f, 1.20f, 3.7f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 6, 4, 2>(0.66f, 0.00f, 0.84f, 0.0f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 4, 4, 4>(0.45f, 0.00f, 0.60f, 1.0f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 4, 4, 2>(0.57f, 0.76f, 1.11f, 0.0f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 4, 5>(0.35f, 0.00f, 0.42f, 0.0f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 2, 6>(0.23f, 0.00f, 0.27f, 0.6f),
+        fg_tile<GHIP_EP_LINEAR, 0, 0, 0, 2, 2, 2, 3>(0.24f, 0.31f, 0.46f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;
@@ -22,16 +22,15 @@ static const GhipFfnTile *linear_tiles(int *n) {
 
 static const GhipFfnTile *gated_tiles(int *n) {
     static const GhipFfnTile t[] = {
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 8, 8, 2>(1.03f, 0.00f, 1.33f, 5.9f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 6, 8, 2>(1.03f, 0.00f, 1.11f, 0.4f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 8, 4, 2>(0.75f, 0.00f, 0.86f, 0.0f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 6, 4, 2>(0.69f, 0.00f, 0.74f, 0.0f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 5, 4, 2>(0.68f, 0.00f, 0.73f, 0.0f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 4, 4, 4>(0.41f, 0.00f, 0.53f, 0.2f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 4, 4, 2>(0.60f, 0.72f, 0.92f, 0.0f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 4, 5>(0.40f, 0.00f, 0.39f, 0.0f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 2, 6>(0.26f, 0.00f, 0.26f, 0.4f),
-        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 2, 3>(0.24f, 0.34f, 0.43f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 8, 8, 2>(1.04f, 0.00f, 1.34f, 6.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 6, 8, 2>(1.03f, 0.00f, 1.10f, 0.4f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 6, 4, 2>(0.67f, 0.00f, 0.72f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 5, 4, 2>(0.65f, 0.00f, 0.70f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 4, 4, 4>(0.46f, 0.00f, 0.58f, 0.2f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 4, 4, 2>(0.58f, 0.70f, 0.88f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 4, 5>(0.39f, 0.00f, 0.38f, 0.0f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 2, 6>(0.25f, 0.00f, 0.25f, 0.4f),
+        fg_tile<GHIP_EP_GATED, 0, 0, 0, 2, 2, 2, 3>(0.23f, 0.33f, 0.43f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;

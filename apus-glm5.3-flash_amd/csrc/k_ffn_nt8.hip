@@ -9,10 +9,10 @@ static const GhipFfnTile *linear_tiles(int *n) {
     static const GhipFfnTile t[] = {
         fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 16, 4, 2>(1.25f, 0.00f, 1.54f, 8.0f),
         fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 12, 4, 2>(1.04f, 0.00f, 1.20f, 6.2f),
-        fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 12, 2, 2>(0.72f, 0.00f, 0.80f, 3.6f),
-        fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 8, 2, 4>(0.57f, 0.00f, 0.63f, 2.7f),
-        fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 8, 2, 2>(0.61f, 0.70f, 1.03f, 0.7f),
-        fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 4, 1, 3>(0.29f, 0.36f, 0.38f, 0.8f),
+        fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 12, 2, 2>(0.66f, 0.00f, 0.74f, 3.3f),
+        fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 8, 2, 4>(0.54f, 0.00f, 0.60f, 2.6f),
+        fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 8, 2, 2>(0.59f, 0.68f, 1.00f, 0.7f),
+        fg_tile<GHIP_EP_LINEAR, W8, 0, 0, 1, 4, 1, 3>(0.28f, 0.35f, 0.37f, 0.8f),
     };
     *n = sizeof t / sizeof *t;
     return t;
@@ -23,10 +23,10 @@ static const GhipFfnTile *gated_tiles(int *n) {
     static const GhipFfnTile t[] = {
         fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 16, 4, 2>(1.22f, 0.00f, 1.49f, 6.7f),
         fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 12, 4, 2>(1.02f, 0.00f, 1.18f, 5.2f),
-        fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 12, 2, 2>(0.71f, 0.00f, 0.78f, 2.4f),
-        fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 8, 2, 4>(0.56f, 0.00f, 0.62f, 2.4f),
-        fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 8, 2, 2>(0.60f, 0.67f, 1.00f, 1.0f),
-        fg_tile<GHIP_EP_GATED, W8, 0, 0, 2, 2, 2, 3>(0.31f, 0.43f, 0.44f, 0.6f),
+        fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 12, 2, 2>(0.67f, 0.00f, 0.74f, 2.3f),
+        fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 8, 2, 4>(0.54f, 0.00f, 0.60f, 2.3f),
+        fg_tile<GHIP_EP_GATED, W8, 0, 0, 1, 8, 2, 2>(0.58f, 0.64f, 0.96f, 1.0f),
+        fg_tile<GHIP_EP_GATED, W8, 0, 0, 2, 2, 2, 3>(0.32f, 0.45f, 0.46f, 0.6f),
     };
     *n = sizeof t / sizeof *t;
     return t;

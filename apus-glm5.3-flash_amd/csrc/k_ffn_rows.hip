@@ -122,8 +122,8 @@ static const FrForm *fr_forms(int mode, bool fp8, int *n) {
 
 /* Estimated microseconds of a form: 2.3 + the larger of its rounds of the chip
  * and the weights at 6.5 TB/s + a tenth of the other (within 10-15% rms of the
- * sweep). Forms of 4 and 8 rows only take as many: more row tiles would re-read
- * the weights. */
+ * sweep); several row tiles of FP8 take 15% more on average for M = 64 to 300.
+ * Forms of 4 and 8 rows only take as many. */
 static float fr_estimate(const FrForm &c, const GhipProd *p, bool dual, uint32_t n_cu) {
     if (c.mr < 16 && p->M > c.mr) return 1e30f;
     const double cols = (dual ? 8.0 : 16.0) * c.nt * (RW_NW / c.ks);
@@ -133,7 +133,8 @@ static float fr_estimate(const FrForm &c, const GhipProd *p, bool dual, uint32_t
     const double nc = (double)(size_t)((nch + c.ks - 1) / c.ks);
     const double hbm = (double)p->N * kb * (dual ? 2 : 1) / 6.5e6;
     const double t = rounds * (nc * c.chunk + c.over);
-    return (float)(2.3 + (t > hbm ? t + 0.1 * hbm : hbm + 0.1 * t));
+    const double again = p->s && p->M > c.mr ? 1.15 : 1.0;
+    return (float)(2.3 + again * (t > hbm ? t + 0.1 * hbm : hbm + 0.1 * t));
 }
 
 /* Whole 16-byte pieces of x's rows (FP8 weight rows then start at 8 bytes, and

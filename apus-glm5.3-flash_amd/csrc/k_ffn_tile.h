@@ -1,13 +1,15 @@
 /*
  * k_ffn_tile.h — an entry of a tile table (GhipFfnTile) over k_ffn_gemm.
  *
- * Its times are fitted, family by family, to a sweep of every tile over M
+ * Its times lie between those of operands from HBM and of operands that other
+ * calls left in the chip's cache (BF16 tiles below 256 x 256 are 1.1 to 1.4 times
+ * apart). They were fitted, family by family, to a sweep of every tile over M
  * = 64..4096 and N x K from 1536 x 1536 to 12288 x 4096 and 4096 x 12288
  * (backward products: 19 shapes each) on 256 CUs; the tile picked by them took
  * 1.5-3% longer than the best one on average, 25% at most. Tiles of at most 80
  * KB of LDS run two to a CU: deeper rings against a second workgroup to hide
  * the first's waits is why some shapes are there twice. Every tile listed is
- * the pick of at least 0.8% of shapes drawn log-uniformly from 1 to 16384.
+ * the pick of some shapes among 12000 drawn log-uniformly from 1 to 16384.
  */
 #ifndef K_FFN_TILE_H
 #define K_FFN_TILE_H

@@ -92,8 +92,10 @@ def test_what_direct_loads_cannot_take(lib, args):
         assert F.gemm_fits(lib, family, F.prod(family, **ok))
         assert not F.gemm_fits(lib, family, F.prod(family, **{**ok, **args}))
     for w8 in ("linear fp8", "gated fp8 exact"):
-        assert F.gemm_fits(lib, w8, F.prod(w8, 256, 512, 1040))
-        assert not F.gemm_fits(lib, w8, F.prod(w8, 256, 512, 1032))  # 8-byte code rows
+        assert F.gemm_fits(lib, w8, F.prod(w8, 256, 512, 1032)) and F.gemm_fits(lib, w8, F.prod(w8, 256, 512, 24))
+        assert not F.gemm_fits(lib, w8, F.prod(w8, 256, 512, 1028))
+        assert not F.gemm_fits(lib, w8, F.prod(w8, 256, 512, 8))    # a half piece alone
+        assert not F.gemm_fits(lib, w8, F.prod(w8, 256, 512, 1032, b=F.AT + 8))
 
 
 def test_what_rows_can_take(lib):

@@ -14,7 +14,7 @@ from test_gpu_ffn import Mat, bf, fp8, seed, wide
 
 pytestmark = pytest.mark.gpu
 
-TILES = {"linear": 8, "linear fp8": 6, "linear fp8 exact": 6, "gated": 10, "gated fp8": 6, "gated fp8 exact": 6, "dlinear": 9,
+TILES = {"linear": 8, "linear fp8": 6, "linear fp8 exact": 6, "gated": 9, "gated fp8": 6, "gated fp8 exact": 6, "dlinear": 9,
          "dgated": 8, "dx": 6, "dw": 4}
 
 
@@ -79,7 +79,8 @@ def test_tile(ghip, family, tile):
     assert len(F.tiles(ghip, family)) == TILES[family]
     t = F.tiles(ghip, family)[tile]
     mode, w8, _, _ = F.FAMILIES[family]
-    for M, N, K in [(t.bm + 19, t.bn + 13, 400), (t.bm, 2 * t.bn, 64), (3, 8, 16), (2 * t.bm - 1, t.bn + 8, 1040)]:
+    for M, N, K in [(t.bm + 19, t.bn + 13, 400), (t.bm, 2 * t.bn, 64), (3, 8, 16), (2 * t.bm - 1, t.bn + 8, 1040),
+                    (t.bm + 5, t.bn + 33, 72), (5, 40, 24), (t.bm, 2 * t.bn, 1096), (33, 130, 56), (70, 129, 168)]:
         c = Case(family, M, N, K, *forward(family, tile + M), pad=16 if w8 else 8)
         assert F.gemm_fits(ghip, family, c.p)
         assert ghip.ghip_launch_ffn_gemm(mode, tile, ctypes.c_uint32(1), ctypes.byref(c.p), ctypes.byref(c.ep), None) == 0
