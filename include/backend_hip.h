@@ -386,8 +386,7 @@ int apus_ghip_moe_prefill_dev_noalloc(ApusGhipStore *s, const uint16_t *x, size_
  *     negative or NaN, a stream of another device, a workspace that is too
  *     small; apus_ghip_last_error), nothing or only a part launched.
  *   - Alignment: 16-byte aligned pointers and strides of whole 16 bytes, with
- *     K % 8 == 0 (from a few dozen rows on K % 16 == 0 for FP8), take the
- *     kernels with direct loads; everything else a slower general one (same
+ *     K % 8 == 0 (FP8: and K >= 16), take the kernels with direct loads; everything else a slower general one (same
  *     results within the tolerance). Outputs, bias and residual may have any
  *     alignment. */
 enum {
