@@ -225,8 +225,17 @@ extern "C" hipError_t ghip_launch_ffn_any(int mode, const GhipProd *p, const Ghi
 
 extern "C" hipError_t ghip_launch_ffn_colsum(const GhipFfnSum *p, hipStream_t st) {
     if (p->M == 0 || p->N == 0 || p->M > 0x7fffffffu || p->N > 0x7fffffffu) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_ffn_colsum, dim3((uint32_t)((p->N + FA_SUM - 1) / FA_SUM)), dim3(1024), 0, st, *p);
-    return hipGetLastError();
+    const size_t most = GHIP_MAX_THREADS / 1024u * FA_SUM;   /* columns of a launch */
+    for (size_t n0 = 0; n0 < p->N; n0 += most) {
+        GhipFfnSum q = *p;
+        q.dz += n0;
+        q.out += n0;
+        q.N = p->N - n0 < most ? p->N - n0 : most;
+        hipLaunchKernelGGL(k_ffn_colsum, dim3((uint32_t)((q.N + FA_SUM - 1) / FA_SUM)), dim3(1024), 0, st, q);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 extern "C" hipError_t ghip_launch_ffn_pack(const uint16_t *src, size_t ld, size_t M, size_t N,
