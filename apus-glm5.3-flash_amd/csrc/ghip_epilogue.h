@@ -14,9 +14,12 @@
  * precision. dz, dg and du are rounded because the products that read them
  * take bf16 operands.
  *
- * exp comes from the hardware exp2 and 1/x from the hardware reciprocal (each
- * about 1 ulp of f32): 2^-22 relative against the output's 2^-9. An argument
- * whose exp is infinite makes the sigmoid 0.
+ * exp comes from the hardware exp2 and 1/x from the hardware reciprocal, each
+ * about 1 ulp of f32; an argument v of exp is itself rounded a few times, which
+ * adds up to 8 |v| 2^-24 relative (|v| is under 88 where the result is not 0):
+ * at most 2^-14 against the output's half step of 2^-8, for values far left of 0
+ * as for all others. An argument whose exp is above 2^126 makes the sigmoid 0,
+ * so values of 1 + |z| times 2^-126 and less are lost.
  */
 #ifndef GHIP_EPILOGUE_H
 #define GHIP_EPILOGUE_H
@@ -33,11 +36,34 @@ __device__ __forceinline__ float ghip_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __expf(-z));
 }
 
+/* Phi(z) = (1 + erf(z / sqrt 2)) / 2, and e = exp(-z^2 / 2). The sum cancels left
+ * of 0 (4% off at z = -5, 0 below -5.6); so Phi(-|z|) = e R(|z|), where R (the
+ * Mills ratio over sqrt(2 pi)) falls like 1 / |z| and is t times a polynomial of
+ * t = 1 / (1 + 0.326 |z|): the minimax one of degree 7, 2^-20 relative for every
+ * z. Its exp serves the slope too, and it takes no branch: 4096 x 4096 x 1024
+ * with GELU 42 us, 56 with the library's erfc (53 with its erf). */
+__device__ __forceinline__ float ghip_phi(float z, float &e) {
+    const float u = __builtin_fabsf(z);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.326f, u, 1.0f));
+    float q = 0.0337685977f;
+    q = __builtin_fmaf(q, t, -0.112105614f);
+    q = __builtin_fmaf(q, t, 0.0818245333f);
+    q = __builtin_fmaf(q, t, 0.0275429578f);
+    q = __builtin_fmaf(q, t, 0.0929912787f);
+    q = __builtin_fmaf(q, t, 0.115857593f);
+    q = __builtin_fmaf(q, t, 0.130065828f);
+    q = __builtin_fmaf(q, t, 0.130055185f);
+    e = __expf(-0.5f * z * z);
+    const float low = e * t * q;
+    return z < 0.0f ? low : 1.0f - low;
+}
+
 template <int ACT>
 __device__ __forceinline__ float ghip_act(float z) {
+    [[maybe_unused]] float e;
     if constexpr (ACT == GHIP_ACT_RELU) return z < 0.0f ? 0.0f : z;      /* keeps a NaN */
     else if constexpr (ACT == GHIP_ACT_SILU) return z * ghip_sigmoid(z);
-    else if constexpr (ACT == GHIP_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    else if constexpr (ACT == GHIP_ACT_GELU) return z * ghip_phi(z, e);
     else if constexpr (ACT == GHIP_ACT_GELU_TANH)
         /* (1 + tanh v) / 2 = sigmoid(2 v) */
         return z * ghip_sigmoid(2.0f * GHIP_GELU_C * (z + GHIP_GELU_A * z * z * z));
@@ -56,8 +82,9 @@ __device__ __forceinline__ float ghip_slope(float z) {
         return s * (1.0f + z * (1.0f - s));
     } else if constexpr (ACT == GHIP_ACT_GELU) {
         z = z > 20.0f ? 20.0f : z < -20.0f ? -20.0f : z;
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f))
-               + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
+        float e;
+        const float phi = ghip_phi(z, e);
+        return phi + z * e * 0.3989422804014327f;
     } else if constexpr (ACT == GHIP_ACT_GELU_TANH) {
         z = z > 20.0f ? 20.0f : z < -20.0f ? -20.0f : z;
         const float s = ghip_sigmoid(2.0f * GHIP_GELU_C * (z + GHIP_GELU_A * z * z * z));
