@@ -70,13 +70,12 @@ __device__ __forceinline__ float ghip_act(float z) {
     else return z;
 }
 
-/* The derivative. The smooth ones are 0 or 1 to the last bit well inside +-100
- * (+-20), and the clamp keeps an infinite z from making 0 * inf of that. */
+/* The derivative (ReLU's: ghip_pull). The smooth ones are 0 or 1 to the last bit
+ * well inside +-100 (+-20), and the clamp keeps an infinite z from making 0 * inf
+ * of that. */
 template <int ACT>
 __device__ __forceinline__ float ghip_slope(float z) {
-    if constexpr (ACT == GHIP_ACT_RELU) {
-        return z > 0.0f ? 1.0f : 0.0f;
-    } else if constexpr (ACT == GHIP_ACT_SILU) {
+    if constexpr (ACT == GHIP_ACT_SILU) {
         z = z > 100.0f ? 100.0f : z < -100.0f ? -100.0f : z;
         const float s = ghip_sigmoid(z);
         return s * (1.0f + z * (1.0f - s));
@@ -94,6 +93,14 @@ __device__ __forceinline__ float ghip_slope(float z) {
     }
 }
 
+/* d * act'(z). ReLU selects, as the clamps do: nothing passes where z <= 0, not
+ * 0 * inf either, and a NaN z stays one. */
+template <int ACT>
+__device__ __forceinline__ float ghip_pull(float z, float d) {
+    if constexpr (ACT == GHIP_ACT_RELU) return z > 0.0f ? d : z <= 0.0f ? 0.0f : z;
+    else return d * ghip_slope<ACT>(z);
+}
+
 /* The value(s) that leave the registers: s0 the sum (g), s1 the second one (u),
  * b the bias, in the residual or the incoming gradient. */
 template <int MODE, int ACT>
@@ -105,14 +112,14 @@ __device__ __forceinline__ void ghip_ep_value(float s0, float s1, float b, float
     } else if constexpr (MODE == GHIP_EP_LINEAR) {
         o0 = ghip_act<ACT>(s0 + b) + in;
     } else if constexpr (MODE == GHIP_EP_DLINEAR) {
-        o0 = in * ghip_slope<ACT>(s0 + b);
+        o0 = ghip_pull<ACT>(s0 + b, in);
     } else {
         const float g = s0 > limit ? limit : s0;             /* keep a NaN */
         const float u = s1 > limit ? limit : s1 < -limit ? -limit : s1;
         if constexpr (MODE == GHIP_EP_GATED) {
             o0 = ghip_act<ACT>(g) * u;
         } else {
-            o0 = s0 > limit ? 0.0f : in * u * ghip_slope<ACT>(g);
+            o0 = s0 > limit ? 0.0f : ghip_pull<ACT>(g, in * u);
             o1 = s1 > limit || s1 < -limit ? 0.0f : in * ghip_act<ACT>(g);
         }
     }

@@ -368,7 +368,9 @@ int apus_ghip_moe_prefill_dev_noalloc(ApusGhipStore *s, const uint16_t *x, size_
  *     other columns are neither read into a result nor written. Weights and
  *     weight gradients are dense.
  *   - act: APUS_GHIP_ACT_*. GELU is z * Phi(z), GELU_TANH its tanh form. limit
- *     0 = no clamp (10 for GLM-5.3-Flash's SwiGLU).
+ *     0 = no clamp (10 for GLM-5.3-Flash's SwiGLU). No gradient passes a
+ *     clamp past its limit, or RELU at z <= 0, whatever comes in, infinities
+ *     included; RELU keeps a NaN z in both directions.
  *   - Sums, bias, activation, product and residual are f32; the result is
  *     rounded once to BF16 (the MoE entries round g, u, silu(g) and h each, as
  *     the reference does: their h differs from this one in the last bits).
