@@ -59,12 +59,11 @@
 #include <utility>
 
 #include "ghip_epilogue.h"
+#include "k_ffn_addr.h"
 
 typedef short fg_s16x4 __attribute__((ext_vector_type(4)));
 
 #define FG_LDS_MAX (160u * 1024u)
-#define FG_OOB 0xFFFFFFF0u                       /* past every buffer: loads zeros */
-#define FG_SPAN 0x80000000u                      /* valid offsets are below */
 
 __device__ __forceinline__ void fg_dma16(const void *base, uint32_t span, uint32_t off,
                                          void *lds_wave) {
@@ -101,23 +100,6 @@ typedef __attribute__((address_space(3))) fg_s16x4 fg_lds_s16x4;
 __device__ __forceinline__ fg_s16x4 fg_read_tr(fg_lds_s16x4 *__restrict p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
 }
-
-/* Layout 1: what the 32-byte slots of k's row of W values are XORed with, so
- * that the 8 k rows two lane groups read from one slot lie in distinct banks. */
-template <uint32_t W>
-__device__ __forceinline__ uint32_t fg_swizzle(uint32_t k) {
-    static_assert(W % 64u == 0, "half rounds of the banks");
-    return W % 128u ? ((k >> 1) & 1u) | ((k >> 3) & 2u) : ((k & 3u) << 1) | ((k >> 4) & 1u);
-}
-
-/* Layout 0 (FP8 codes): what the 16-byte pieces of row r are XORed with. A
- * ds_read_b128 is served 16 lanes at a time, rows 0-3 and 12-15 of one lane
- * group together with rows 4-11 of the next: the rotation gives the middle rows
- * a set of values that the other group's XOR with 2 (1) maps to itself, so the
- * 16 pieces fill the 64 banks. With r >> 1 alone 49% of the LDS cycles were
- * conflicts (gated FP8 1111 x 2048 x 4096: 52 us, now 49). */
-__device__ __forceinline__ uint32_t fg_rot8(uint32_t r) { return ((r >> 1) + 2u) & 7u; }
-__device__ __forceinline__ uint32_t fg_rot4(uint32_t r) { return ((r >> 2) + 1u) & 3u; }
 
 /* f(0), f(1), ... f(N - 1), the argument a constant */
 template <typename F, int... I>
@@ -223,55 +205,25 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
         pb += from * bstep;
     }
 
-    /* Byte offset of this lane's 16 bytes of 1 KB load c in a stage, the load's
-     * lane l going to byte 16 l of the KB; past the matrix: FG_OOB. kq: the
-     * stage's k that the piece starts at (layout 0) */
+    /* this lane's offsets in a stage's loads (k_ffn_addr.h) */
     uint32_t ao[NAL], bo[NBL], akq = 0, bkq = 0;
-    auto place = [&](auto layout_c, auto w_c, uint32_t c, uint32_t live, uint32_t ld,
-                     uint32_t &kq) -> uint32_t {
-        constexpr uint32_t W = decltype(w_c)::value;
-        if constexpr (decltype(layout_c)::value == 0) {
-            const uint32_t r = 8u * c + (lane >> 3), q = (lane & 7u) ^ fg_rot8(r);
-            kq = 8u * q;                                 /* the same for every c of a wave */
-            return r < live ? r * ld * 2u + 16u * q : FG_OOB;
-        } else {
-            const uint32_t e = c * 64u + lane, k = e / (W / 8u), s = e % (W / 8u);
-            const uint32_t q = s ^ 2u * fg_swizzle<W>(k);
-            return 8u * q < live ? k * ld * 2u + 16u * q : FG_OOB;
-        }
-    };
     using LA = std::integral_constant<int, AL>;
     using LB = std::integral_constant<int, BL>;
     using WA = std::integral_constant<uint32_t, BM>;
     using WB = std::integral_constant<uint32_t, BN>;
 #pragma unroll
-    for (uint32_t i = 0; i < NAL; i++) ao[i] = place(LA{}, WA{}, wv + 4u * i, rows, lda, akq);
+    for (uint32_t i = 0; i < NAL; i++) ao[i] = fg_place<AL, BM>(wv + 4u * i, lane, rows, lda, akq);
 #pragma unroll
     for (uint32_t i = 0; i < NBL; i++) {
-        if constexpr (FP8) {                             /* 16 rows of 64 codes */
-            const uint32_t b = wv + 4u * i, r = lane >> 2, q = (lane & 3u) ^ fg_rot4(r);
-            const uint32_t mr = 16u * (DUAL ? b >> 1 : b) + r;
-            bkq = 16u * q;
-            bo[i] = mr < cols ? mr * ldb + 16u * q : FG_OOB;
-        } else {
-            const uint32_t c = wv + 4u * i;
-            if constexpr (DUAL) {
-                const uint32_t r = 8u * c + (lane >> 3), q = (lane & 7u) ^ fg_rot8(r);
-                const uint32_t mr = 16u * (r >> 5) + (r & 15u);
-                bkq = 8u * q;
-                bo[i] = mr < cols ? mr * ldb * 2u + 16u * q : FG_OOB;
-            } else {
-                bo[i] = place(LB{}, WB{}, c, cols, ldb, bkq);
-            }
-        }
+        if constexpr (FP8) bo[i] = fg_place_codes(DUAL, wv + 4u * i, lane, cols, ldb, bkq);
+        else if constexpr (DUAL) bo[i] = fg_place_dual(wv + 4u * i, lane, cols, ldb, bkq);
+        else bo[i] = fg_place<BL, BN>(wv + 4u * i, lane, cols, ldb, bkq);
     }
-    /* load i of the next stage of A (of B). A stage that K cuts: layout 0 drops
-     * the pieces past it, layout 1 the k rows, by the buffer's end */
+    /* load i of the next stage of A (of B) */
     auto left = [&](uint32_t j) { return p.K - (j >= nst1 ? j - nst1 : j) * 64u; };
     auto load_a = [&](uint32_t i) {
         const uint32_t lf = left(ja);
-        const uint32_t span = AL == 1 && lf < 64u ? lf * lda * 2u : FG_SPAN;
-        fg_dma16(pa, span, AL == 0 && akq >= lf ? FG_OOB : ao[i], fg_lds + sa + (wv + 4u * i) * 1024u);
+        fg_dma16(pa, fg_span<AL>(lf, lda), AL == 0 ? fg_cut(ao[i], lf, akq) : ao[i], fg_lds + sa + (wv + 4u * i) * 1024u);
     };
     /* FP8 rows of K % 16 == 8 codes end in half a piece: the last stage's is read 8
      * bytes early, and its codes move down when they are read from LDS */
@@ -280,13 +232,12 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
         if (half && jb + 1u == nst1) {
             pb -= 8;
 #pragma unroll
-            for (uint32_t i = 0; i < NBL; i++) bo[i] += left(jb) - bkq == 8u ? 0u : 8u;
+            for (uint32_t i = 0; i < NBL; i++) bo[i] = fg_half(bo[i], left(jb), bkq);
         }
     };
     auto load_b = [&](uint32_t i) {
         const uint32_t lf = left(jb);
-        const uint32_t span = BL == 1 && lf < 64u ? lf * ldb * 2u : FG_SPAN;
-        fg_dma16(pb, span, BL == 0 && bkq >= lf ? FG_OOB : bo[i], bring + sb + (wv + 4u * i) * 1024u);
+        fg_dma16(pb, fg_span<BL>(lf, ldb), BL == 0 ? fg_cut(bo[i], lf, bkq) : bo[i], bring + sb + (wv + 4u * i) * 1024u);
     };
     auto next_a = [&]() {
         ja++;
@@ -306,15 +257,14 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
     /* operand reads: block blk of 16 rows, step s */
     uint32_t off0[2];
 #pragma unroll
-    for (uint32_t s = 0; s < 2; s++) off0[s] = n * 128u + 16u * ((2u * g + s) ^ fg_rot8(n));
+    for (uint32_t s = 0; s < 2; s++) off0[s] = fg_at0(n, 2u * g + s);
     auto frag = [&](auto layout_c, auto w_c, const uint8_t *st, uint32_t blk, int s) -> ghip_bf16x8 {
         constexpr uint32_t W = decltype(w_c)::value;
         if constexpr (decltype(layout_c)::value == 0) {
             return *(const ghip_bf16x8 *)(st + blk * 2048u + off0[s]);
         } else {
             const uint32_t k = 16u * g + 8u * (uint32_t)s + (n >> 2);
-            const uint8_t *q =
-                st + k * (2u * W) + (blk ^ fg_swizzle<W>(k)) * 32u + (n & 3u) * 8u;
+            const uint8_t *q = fg_at1<W>(st, k, blk) + (n & 3u) * 8u;
             /* k + 4 has the same swizzle */
             const fg_s16x4 lo = fg_read_tr((fg_lds_s16x4 *)q);
             const fg_s16x4 hi = fg_read_tr((fg_lds_s16x4 *)(q + 8u * W));
@@ -334,8 +284,7 @@ __device__ __forceinline__ void fg_product(const GhipProd &p, const GhipEp &ep, 
     };
     auto read_b = [&](int set, int c, const uint8_t *st, int s) {
         if constexpr (FP8)
-            codes[c] = *(const ghip_u32x4 *)(st + (wc * CB + c) * 1024u + n * 64u
-                                             + 16u * (g ^ fg_rot4(n)));
+            codes[c] = *(const ghip_u32x4 *)(st + (wc * CB + c) * 1024u + fg_at_codes(n, g));
         else
             wa[set][c] = frag(LB{}, WB{}, st, wc * CB + c, s);
     };
