@@ -15,6 +15,7 @@
 #define K_ROWS_GEMM_H
 
 #include "ghip_epilogue.h"
+#include "k_rows_addr.h"
 
 #define RW_NW 8                  /* waves per workgroup */
 #define RW_LDS_MAX (160u * 1024u)
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
     const uint32_t ldx = EPI ? more.ldx : K;
     /* pieces of a last chunk that K cuts; FP8 with K % 16 == 8: the last one is
      * half */
-    const uint32_t end = EPI ? ((KB & 127u) + 15u) >> 4 : 0u;
+    const uint32_t end = EPI ? rw_end(KB) : 0u;
     const bool half = EPI && !BF && (K & 8u);
     const uint32_t part = wv % KS, slot = wv / KS;
     const uint32_t c0 = part * nch / KS, c1 = (part + 1u) * nch / KS, nc = c1 - c0;
@@ -140,18 +141,11 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
             xq[u] = (lane & (LPR - 1u)) ^ sw;
             xo[u] = min(r, mrows - 1u) * ldx * 2u + 16u * xq[u];
         }
-        /* the chunk that K cuts: pieces past it are read at the chunk's start and
-         * put into LDS as zeros, on both sides */
-        const uint32_t q0 = (lane & 7u) ^ ((lane >> 4) & 7u), q1 = (lane & 7u) ^ ((4u + (lane >> 4)) & 7u);
-        const uint32_t xend = BF ? end : 2u * end - (half ? 1u : 0u);
+        /* the chunk that K cuts (k_rows_addr.h) */
+        const uint32_t q0 = rw_piece(lane, 0), q1 = rw_piece(lane, 1), xend = rw_xend(BF, end, half);
         auto cut = [&](uint32_t c) { return EPI && end && c == nch - 1u; };
-        /* the half piece is read 8 bytes early, where its row has them (in the
-         * chunk before where it is the chunk's first); pieces past K as the
-         * chunk's first one */
         auto from = [&](uint32_t c, const uint8_t *wb, uint32_t off, uint32_t q) {
-            const bool past = cut(c) && q >= end;
-            const bool early = cut(c) && half && (past ? 0u : q) == end - 1u;
-            return (const rw_u32x4 *)(wb + (past ? off - 16u * q : off) - (early ? 8 : 0));
+            return (const rw_u32x4 *)rw_from(wb, off, q, cut(c), half, end);
         };
         ghip_u32x4 xr[NA][XI], wr[NA][2 * NT];
         auto load = [&](auto set_c, uint32_t c) {
@@ -159,7 +153,7 @@ __global__ __launch_bounds__(RW_NW * 64, 1) void k_rows_gemm(
             const uint8_t *xc = xb + (size_t)c * XROW, *wc = rows + (size_t)c * 128u;
 #pragma unroll
             for (uint32_t u = 0; u < XI; u++)
-                xr[A][u] = *(const ghip_u32x4 *)(xc + (cut(c) && xq[u] >= xend ? xo[u] - 16u * xq[u] : xo[u]));
+                xr[A][u] = *(const ghip_u32x4 *)(xc + rw_x(xo[u], xq[u], cut(c), xend));
 #pragma unroll
             for (int b = 0; b < NT; b++) {
                 const uint8_t *wb = DUAL && (b & 1) ? rows2 + (size_t)c * 128u : wc;

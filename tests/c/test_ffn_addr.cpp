@@ -1,6 +1,7 @@
 /*
- * The dense feed-forward tiles' loads on the CPU (k_ffn_addr.h): every lane of
- * every load of every stage, over ragged rows and k. Each access lies inside its
+ * The dense feed-forward tiles' loads on the CPU (k_ffn_addr.h), and those of the
+ * weight-streaming kernel (k_rows_addr.h): every lane of every load of every
+ * stage or chunk, over ragged rows and k. Each access lies inside its
  * own row of the matrix or is marked as past the buffer, with its whole 16 bytes
  * below 2^32; and what the operand reads then find in LDS is the matrix's value,
  * or zero past its end.
@@ -10,6 +11,7 @@
 #include <vector>
 
 #include "k_ffn_addr.h"
+#include "k_rows_addr.h"
 
 static long g_loads, g_marked;
 
@@ -168,7 +170,61 @@ static void tiles(uint32_t R, uint32_t K) {
     k_slow<T>(R, K + 3, ((R + 7u) & ~7u) + 16);
 }
 
+/* the weight rows [O, K] of wave groups of NT blocks of 16, chunk by chunk: FP8
+ * codes, or bf16 where bf */
+static void weights(uint32_t O, uint32_t K, uint32_t NT, bool bf) {
+    const uint32_t KB = bf ? 2 * K : K, nch = (KB + 127u) / 128u, end = rw_end(KB);
+    const bool half = !bf && (K & 8u);
+    const long bytes = (long)O * KB;
+    for (uint32_t row0 = 0; row0 < O; row0 += 16 * NT)
+        for (uint32_t b = 0; b < NT; b++)
+            for (uint32_t c = 0; c < nch; c++)
+                for (uint32_t i = 0; i < 128; i++) {
+                    const uint32_t lane = i % 64, h = i / 64, q = rw_piece(lane, h), r = 16 * b + 8 * h + lane / 8;
+                    const uint32_t last = O - 1 - row0, row = row0 + (r < last ? r : last);
+                    const bool cut = end && c == nch - 1;
+                    const uint8_t *zero = nullptr;
+                    const long at = rw_from(zero, (row - row0) * KB + 16 * q, q, cut, half, end) - zero + (long)row0 * KB + 128l * c;
+                    g_loads++;
+                    REQUIRE(at >= 0 && at + 16 <= bytes, "weights O %u K %u bf %d: byte %ld of %ld", O, K, bf, at, bytes);
+                    REQUIRE(at >= (long)row * KB && at + 16 <= (long)(row + 1) * KB, "weights O %u K %u bf %d: past a row", O, K, bf);
+                    if (cut && q >= end) {               /* becomes zeros */
+                        g_marked++;
+                        continue;
+                    }
+                    /* where LDS row r has the piece, it is the row's, or its last 8
+                     * bytes are in the upper half */
+                    const long want = (long)row * KB + 128l * c + 16l * q;
+                    const bool down = cut && half && q == end - 1;
+                    REQUIRE(at == want - (down ? 8 : 0), "weights O %u K %u bf %d row %u chunk %u piece %u", O, K, bf, row, c, q);
+                    REQUIRE(want + (down ? 8 : 16) <= (long)(row + 1) * KB, "weights O %u K %u bf %d: a piece past K", O, K, bf);
+                }
+}
+
+/* x's pieces of a chunk: those of K are kept and lie in the row, the others are
+ * read inside the row */
+static void inputs(uint32_t K, bool bf) {
+    const uint32_t KB = bf ? 2 * K : K, nch = (KB + 127u) / 128u, end = rw_end(KB), pieces = bf ? 8 : 16;
+    const uint32_t xend = rw_xend(bf, end, !bf && (K & 8u));
+    for (uint32_t c = 0; c < nch; c++)
+        for (uint32_t q = 0; q < pieces; q++) {
+            const bool cut = end && c == nch - 1;
+            const long at = (long)c * pieces * 16 + rw_x(16 * q, q, cut, xend), own = 16l * (c * pieces + q);
+            g_loads++;
+            REQUIRE(at >= 0 && at + 16 <= 2l * K, "x K %u bf %d: byte %ld", K, bf, at);
+            REQUIRE((own + 16 <= 2l * K) == !(cut && q >= xend), "x K %u bf %d chunk %u piece %u", K, bf, c, q);
+            REQUIRE((cut && q >= xend) || at == own, "x K %u bf %d chunk %u piece %u", K, bf, c, q);
+        }
+}
+
 int main() {
+    for (uint32_t K = 8; K <= 1032; K += 8)
+        for (int bf = 0; bf < 2; bf++) {
+            if (!bf && K < 16) continue;                 /* a half piece needs a whole one */
+            inputs(K, bf);
+            for (uint32_t O : {1u, 5u, 16u, 17u, 40u, 96u, 129u})
+                for (uint32_t NT : {1u, 2u}) weights(O, K, NT, bf);
+        }
     static const uint32_t rows[] = {1, 5, 33, 64, 130, 265};
     for (uint32_t R : rows) {
         for (uint32_t K : {16u, 24u, 40u, 56u, 64u, 72u, 88u, 120u, 128u, 136u, 200u, 1032u})
