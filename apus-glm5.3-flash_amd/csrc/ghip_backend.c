@@ -595,18 +595,20 @@ _Static_assert((int)APUS_GHIP_ACT_NONE == GHIP_ACT_NONE && (int)APUS_GHIP_ACT_RE
                    && (int)APUS_GHIP_ACT_GELU_TANH == GHIP_ACT_GELU_TANH,
                "activation numbers");
 
-/* Launches go to the backend's device, whichever one is current. */
+/* Initialise; launches then go to the backend's device, and the one that was
+ * current is so again at the end of the scope, also where initialising made the
+ * backend's current. */
 static void device_scope_end(const int *prev) {
     if (*prev >= 0) (void)hipSetDevice(*prev);
 }
 #define DEVICE_SCOPE __attribute__((cleanup(device_scope_end))) int prev_device_ = -1
 static int device_scope(int *prev, hipStream_t st) {
     int cur = -1;
-    HIPCHK(hipGetDevice(&cur));
-    if (cur != G.device) {
-        HIPCHK(hipSetDevice(G.device));
-        *prev = cur;
-    }
+    if (hipGetDevice(&cur) != hipSuccess) cur = -1;      /* no device: ghip_init says so */
+    if (!G.inited) *prev = cur;
+    if (ghip_init()) return 1;
+    *prev = cur == G.device ? -1 : cur;
+    if (cur != G.device) HIPCHK(hipSetDevice(G.device));
     if (st) {
         hipDevice_t d = G.device;
         HIPCHK(hipStreamGetDevice(st, &d));
@@ -655,8 +657,7 @@ static int ffn_forward(int mode, const void *w, const float *scales, const void 
     if (check_sizes(M, O, K) || check_ptr("weights", w) || check_ptr("x", x)
         || check_ptr("the output", y)
         || (mode == GHIP_EP_GATED && check_ptr("up weights", w2)) || check_act(act, limit)
-        || check_ld("ldx", &ldx, K) || check_ld("ldy", &ldy, O) || check_ld("ldr", &ldr, O)
-        || ghip_init())
+        || check_ld("ldx", &ldx, K) || check_ld("ldy", &ldy, O) || check_ld("ldr", &ldr, O))
         return 1;
     DEVICE_SCOPE;
     if (device_scope(&prev_device_, st)) return 1;
@@ -780,7 +781,6 @@ int apus_ghip_bf16_linear_ep_backward_dev(const uint16_t *w, const uint16_t *x,
         ghip_seterr("no gradient asked for");
         return 1;
     }
-    if (ghip_init()) return 1;
     DEVICE_SCOPE;
     if (device_scope(&prev_device_, st)) return 1;
     const uint16_t *dz = dy;
@@ -829,7 +829,6 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
         ghip_seterr("no gradient asked for");
         return 1;
     }
-    if (ghip_init()) return 1;
     DEVICE_SCOPE;
     if (device_scope(&prev_device_, st)) return 1;
     const size_t ld = ffn_ws_ld(I);
