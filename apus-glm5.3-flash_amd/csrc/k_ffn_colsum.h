@@ -2,6 +2,12 @@
  * k_ffn_colsum.h — dbias[n] = sum_m dz[m, n] in f32, rounded once (gfx950): the
  * body of a workgroup of T threads (k_ffn_any.hip, k_ffn_grads.hip).
  *
+ * dz is the bf16 matrix that the products read. The f32 values exist in the
+ * registers of the kernel that makes it, tile by tile: their sums would need 4
+ * bytes a column for every row tile until all are there, and the workspace holds dz
+ * alone. The rounding costs dbias 0.0023 of its 2-norm instead of 0.0017 (300 x
+ * 2048 with GELU).
+ *
  * It owns C columns, a thread 8 of them in every 8T/C-th row (one load at any
  * alignment); the 8T/C threads' sums are added in a fixed order.
  */

@@ -3,10 +3,10 @@
  * and the sums that a backward pass computes again): the weight-streaming
  * kernel (k_rows_gemm.h) with an epilogue, for one weight matrix (linear) or
  * gate and up together (gated). Bound by HBM where the weights fill the chip
- * (operands from HBM: gated FP8 12288 x 4096, M = 1, 18.9 us, 5.3 TB/s; FP8 4096 x
- * 16384, M = 4, 12.5 us, 5.4 TB/s), by the launch, the first loads and the
- * reduction below that (under the profiler BF16 4096 x 2048, M = 1, 5.0 us; 1537 x
- * 4096, M = 37, 9.9).
+ * (operands from HBM: gated FP8 12288 x 4096, M = 1, 18.8 us, 5.4 TB/s; FP8 4096 x
+ * 16384, M = 4, 12.8 us, 5.3 TB/s), by the launch, the first loads and the
+ * reduction below that (under the profiler BF16 4096 x 2048, M = 1, 5.1 us; 1537 x
+ * 4096, M = 37, 7.7).
  */
 #include "k_rows_gemm.h"
 
