@@ -94,6 +94,24 @@ SIGNATURES = {
     "apus_ghip_gated_backward_ws": (c_size, [c_size] * 3),
     "apus_ghip_bf16_gated_backward_dev": (c_int, [c_vp] * 7 + [c_size] * 6
                                           + [c_int, c_float, c_vp, c_size, c_vp]),
+    # norm, microscaled values, projections with MXFP4 weights
+    "apus_ghip_mx_scale_ld": (c_size, [c_size]),
+    "apus_ghip_mx_quantize_dev": (c_int, [c_int] + [c_vp] * 3 + [c_size] * 3 + [c_vp]),
+    "apus_ghip_mx_dequant_dev": (c_int, [c_int] + [c_vp] * 3 + [c_size] * 3 + [c_vp]),
+    "apus_ghip_rmsnorm_dev": (c_int, [c_vp] * 8 + [c_size] * 6 + [c_float, c_vp]),
+    "apus_ghip_rmsnorm_backward_ws": (c_size, [c_size] * 2),
+    "apus_ghip_rmsnorm_backward_dev": (c_int, [c_vp] * 7 + [c_size] * 6
+                                       + [c_float, c_vp, c_size, c_vp]),
+    "apus_ghip_mxfp4_linear_dev": (c_int, [c_vp] * 2 + [c_int] + [c_vp] * 5 + [c_size] * 6
+                                   + [c_int, c_vp]),
+    "apus_ghip_mxfp4_gated_dev": (c_int, [c_vp] * 4 + [c_int] + [c_vp] * 3 + [c_size] * 5
+                                  + [c_int, c_float, c_vp]),
+    "apus_ghip_mxfp4_linear_backward_ws": (c_size, [c_size] * 3),
+    "apus_ghip_mxfp4_linear_backward_dev": (c_int, [c_vp] * 7 + [c_size] * 6
+                                            + [c_int, c_vp, c_size, c_vp]),
+    "apus_ghip_mxfp4_gated_backward_ws": (c_size, [c_size] * 3),
+    "apus_ghip_mxfp4_gated_backward_dev": (c_int, [c_vp] * 7 + [c_size] * 6
+                                           + [c_int, c_float, c_vp, c_size, c_vp]),
     "apus_ghip_set_trace_events": (None, [ctypes.POINTER(c_vp), c_int]),
     "apus_ghip_stream_hold": (c_int, [c_vp, ctypes.c_uint32]),
     # include/apus_synth.h

@@ -850,6 +850,242 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
 }
 
 /* ------------------------------------------------------------------------ */
+/* norm, microscaled values and the products with them                      */
+/* ------------------------------------------------------------------------ */
+
+_Static_assert((int)APUS_GHIP_BF16 == GHIP_BF16 && (int)APUS_GHIP_MXFP8 == GHIP_MXFP8
+                   && (int)APUS_GHIP_MXFP4 == GHIP_MXFP4,
+               "type numbers");
+
+static int check_aligned(const char *what, const void *p, size_t to) {
+    if (check_ptr(what, p)) return 1;
+    if (((uintptr_t)p & (to - 1)) == 0) return 0;
+    ghip_seterr("%s at %p: %zu-byte alignment is needed", what, p, to);
+    return 1;
+}
+
+/* Whole blocks of 32. */
+static int check_blocks(const char *what, size_t K) {
+    if (K % 32 == 0) return 0;
+    ghip_seterr("%s %zu is no multiple of 32", what, K);
+    return 1;
+}
+
+static int check_mx(int type, const uint8_t *codes, const uint8_t *scales, size_t R, size_t K) {
+    if (type != GHIP_MXFP8 && type != GHIP_MXFP4) {
+        ghip_seterr("type %d is not microscaled", type);
+        return 1;
+    }
+    return check_sizes(1, R, K) || check_blocks("K", K) || check_aligned("codes", codes, 16)
+        || check_aligned("scales", scales, 4);
+}
+
+size_t apus_ghip_mx_scale_ld(size_t K) { return K && K <= 0x7fffffffu ? ghip_mx_scale_ld(K) : 0; }
+
+int apus_ghip_mx_quantize_dev(int type, const uint16_t *x, uint8_t *codes, uint8_t *scales,
+                              size_t R, size_t K, size_t ldx, void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    if (check_mx(type, codes, scales, R, K) || check_ptr("x", x) || check_ld("ldx", &ldx, K)) return 1;
+    DEVICE_SCOPE;
+    if (device_scope(&prev_device_, st)) return 1;
+    HIPCHK(ghip_launch_mx_quantize(type, x, codes, scales, R, K, ldx, st));
+    G.dispatches++;
+    return 0;
+}
+
+int apus_ghip_mx_dequant_dev(int type, const uint8_t *codes, const uint8_t *scales, uint16_t *out,
+                             size_t R, size_t K, size_t ldo, void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    if (check_mx(type, codes, scales, R, K) || check_ptr("the output", out) || check_ld("ldo", &ldo, K))
+        return 1;
+    DEVICE_SCOPE;
+    if (device_scope(&prev_device_, st)) return 1;
+    HIPCHK(ghip_launch_mx_dequant(type, codes, scales, out, R, K, ldo, st));
+    G.dispatches++;
+    return 0;
+}
+
+static int check_eps(float eps) {
+    if (eps >= 0.0f && eps <= 3.4028234663852886e38f) return 0;
+    ghip_seterr("eps %g", (double)eps);
+    return 1;
+}
+
+int apus_ghip_rmsnorm_dev(const uint16_t *x, const uint16_t *residual, const uint16_t *gamma,
+                          uint16_t *sum, uint16_t *y, uint8_t *codes, uint8_t *scales, float *rstd,
+                          size_t M, size_t D, size_t ldx, size_t ldr, size_t lds, size_t ldy,
+                          float eps, void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    if (check_sizes(M, 1, D) || check_ptr("x", x) || check_eps(eps) || check_ld("ldx", &ldx, D)
+        || check_ld("ldr", &ldr, D) || check_ld("lds", &lds, D) || check_ld("ldy", &ldy, D)
+        || (codes && (check_blocks("D", D) || check_aligned("codes", codes, 16)
+                      || check_aligned("scales", scales, 4))))
+        return 1;
+    if (!y && !codes) {
+        ghip_seterr("no output asked for");
+        return 1;
+    }
+    if (sum && !residual) {
+        ghip_seterr("a sum without a residual");
+        return 1;
+    }
+    if (sum && sum == y) {
+        ghip_seterr("the sum and y are the same buffer");
+        return 1;
+    }
+    DEVICE_SCOPE;
+    if (device_scope(&prev_device_, st)) return 1;
+    const GhipNorm p = { .x = x, .r = residual, .gamma = gamma, .sum = sum, .y = y, .codes = codes,
+                         .scales = scales, .rstd = rstd, .M = M, .ldx = ldx, .ldr = ldr, .lds = lds,
+                         .ldy = ldy, .D = (uint32_t)D, .eps = eps };
+    HIPCHK(ghip_launch_rmsnorm(&p, st));
+    G.dispatches++;
+    return 0;
+}
+
+size_t apus_ghip_rmsnorm_backward_ws(size_t M, size_t D) {
+    return M && D && M <= 0x7fffffffu && D <= 0x7fffffffu ? ghip_rmsnorm_part_bytes(M, D) : 0;
+}
+
+int apus_ghip_rmsnorm_backward_dev(const uint16_t *s, const uint16_t *gamma, const float *rstd,
+                                   const uint16_t *dy, const uint16_t *ds, uint16_t *dx,
+                                   uint16_t *dgamma, size_t M, size_t D, size_t lds, size_t lddy,
+                                   size_t ldds, size_t lddx, float eps, void *ws, size_t ws_bytes,
+                                   void *stream) {
+    hipStream_t st = (hipStream_t)stream;
+    if (check_sizes(M, 1, D) || check_ptr("s", s) || check_ptr("dy", dy) || check_eps(eps)
+        || check_ld("lds", &lds, D) || check_ld("lddy", &lddy, D) || check_ld("ldds", &ldds, D)
+        || check_ld("lddx", &lddx, D)
+        || (dgamma && check_ws(ws, ws_bytes, apus_ghip_rmsnorm_backward_ws(M, D))))
+        return 1;
+    if (!dx && !dgamma) {
+        ghip_seterr("no gradient asked for");
+        return 1;
+    }
+    DEVICE_SCOPE;
+    if (device_scope(&prev_device_, st)) return 1;
+    const GhipNormGrad p = { .s = s, .gamma = gamma, .dy = dy, .ds = ds, .rstd = rstd, .dx = dx,
+                             .dgamma = dgamma, .part = dgamma ? (float *)ws : NULL, .M = M, .lds = lds,
+                             .lddy = lddy, .ldds = ldds, .lddx = lddx, .D = (uint32_t)D, .eps = eps };
+    HIPCHK(ghip_launch_rmsnorm_grad(&p, st));
+    G.dispatches++;
+    return 0;
+}
+
+/* One forward product with MXFP4 weights (w2: the up projection). */
+static int mx_forward(int mode, const uint8_t *w, const uint8_t *ws, const uint8_t *w2,
+                      const uint8_t *ws2, int x_type, const void *x, const uint8_t *x_scales,
+                      const uint16_t *bias, const uint16_t *residual, uint16_t *y, size_t M,
+                      size_t O, size_t K, size_t ldx, size_t ldr, size_t ldy, int act, float limit,
+                      hipStream_t st) {
+    const int wide = x_type == GHIP_BF16;
+    if (check_sizes(M, O, K) || check_blocks("K", K) || check_aligned("codes", w, 16)
+        || check_aligned("scales", ws, 4)
+        || (mode == GHIP_EP_GATED && (check_aligned("up codes", w2, 16) || check_aligned("up scales", ws2, 4)))
+        || check_aligned("x", x, 16) || check_ptr("the output", y) || check_act(act, limit)
+        || check_ld("ldx", &ldx, K) || check_ld("ldy", &ldy, O) || check_ld("ldr", &ldr, O))
+        return 1;
+    if (x_type < GHIP_BF16 || x_type > GHIP_MXFP4) {
+        ghip_seterr("unknown type %d of x", x_type);
+        return 1;
+    }
+    if (!wide && (check_aligned("x's scales", x_scales, 4))) return 1;
+    if (wide ? ldx % 8 != 0 : ldx != K) {
+        ghip_seterr(wide ? "ldx %zu is no multiple of 8" : "ldx %zu: microscaled rows are dense", ldx);
+        return 1;
+    }
+    DEVICE_SCOPE;
+    if (device_scope(&prev_device_, st)) return 1;
+    const GhipMxProd p = { .w = w, .w2 = w2, .ws = ws, .ws2 = ws2, .x = (const uint8_t *)x,
+                           .xs = x_scales, .xld = wide ? 2 * ldx : x_type == GHIP_MXFP8 ? K : K / 2,
+                           .M = (uint32_t)M, .N = (uint32_t)O, .K = (uint32_t)K, .xt = x_type };
+    const GhipEp ep = { .bias = bias, .in = residual, .out = y, .ldin = ldr, .ldout = ldy,
+                        .act = act, .limit = limit > 0.0f ? limit : INFINITY };
+    HIPCHK(ghip_launch_mx(mode, &p, &ep, st));
+    G.dispatches++;
+    return 0;
+}
+
+int apus_ghip_mxfp4_linear_dev(const uint8_t *codes, const uint8_t *scales, int x_type,
+                               const void *x, const uint8_t *x_scales, const uint16_t *bias,
+                               const uint16_t *residual, uint16_t *y, size_t M, size_t O, size_t K,
+                               size_t ldx, size_t ldr, size_t ldy, int act, void *stream) {
+    return mx_forward(GHIP_EP_LINEAR, codes, scales, NULL, NULL, x_type, x, x_scales, bias,
+                      residual, y, M, O, K, ldx, ldr, ldy, act, 0.0f, (hipStream_t)stream);
+}
+
+int apus_ghip_mxfp4_gated_dev(const uint8_t *gate_codes, const uint8_t *gate_scales,
+                              const uint8_t *up_codes, const uint8_t *up_scales, int x_type,
+                              const void *x, const uint8_t *x_scales, uint16_t *h, size_t M,
+                              size_t I, size_t K, size_t ldx, size_t ldh, int act, float limit,
+                              void *stream) {
+    return mx_forward(GHIP_EP_GATED, gate_codes, gate_scales, up_codes, up_scales, x_type, x,
+                      x_scales, NULL, NULL, h, M, I, K, ldx, 0, ldh, act, limit,
+                      (hipStream_t)stream);
+}
+
+/* The backward passes read the weights as BF16, which holds MXFP4 values exactly
+ * (between 2^-126 and 2^127): n matrices of them stand in the workspace in front of
+ * that of the BF16 operator. */
+static size_t mx_wide(size_t O, size_t K) { return (O * K * 2 + 255) & ~(size_t)255; }
+
+size_t apus_ghip_mxfp4_linear_backward_ws(size_t M, size_t O, size_t K) {
+    const size_t n = apus_ghip_linear_ep_backward_ws(M, O, K);
+    return n && K % 32 == 0 ? mx_wide(O, K) + n : 0;
+}
+
+size_t apus_ghip_mxfp4_gated_backward_ws(size_t M, size_t I, size_t K) {
+    const size_t n = apus_ghip_gated_backward_ws(M, I, K);
+    return n && K % 32 == 0 ? 2 * mx_wide(I, K) + n : 0;
+}
+
+int apus_ghip_mxfp4_linear_backward_dev(const uint8_t *codes, const uint8_t *scales,
+                                        const uint16_t *x, const uint16_t *bias,
+                                        const uint16_t *dy, uint16_t *dx, uint16_t *dbias, size_t M,
+                                        size_t O, size_t K, size_t ldx, size_t lddy, size_t lddx,
+                                        int act, void *ws, size_t ws_bytes, void *stream) {
+    const size_t need = apus_ghip_mxfp4_linear_backward_ws(M, O, K), wide = mx_wide(O, K);
+    size_t ldx_ = ldx, lddy_ = lddy, lddx_ = lddx;
+    if (check_sizes(M, O, K) || check_mx(GHIP_MXFP4, codes, scales, O, K) || check_act(act, 0.0f)
+        || check_ptr("dy", dy) || (act != GHIP_ACT_NONE && check_ptr("x", x))
+        || check_ld("ldx", &ldx_, K) || check_ld("lddy", &lddy_, O) || check_ld("lddx", &lddx_, K)
+        || check_ws(ws, ws_bytes, need))
+        return 1;
+    if (!dx && !dbias) {
+        ghip_seterr("no gradient asked for");
+        return 1;
+    }
+    if ((dx || act != GHIP_ACT_NONE)
+        && apus_ghip_mx_dequant_dev(GHIP_MXFP4, codes, scales, (uint16_t *)ws, O, K, 0, stream))
+        return 1;
+    return apus_ghip_bf16_linear_ep_backward_dev((const uint16_t *)ws, x, bias, dy, dx, NULL, dbias,
+                                                 M, O, K, ldx, lddy, lddx, act,
+                                                 (uint8_t *)ws + wide, need - wide, stream);
+}
+
+int apus_ghip_mxfp4_gated_backward_dev(const uint8_t *gate_codes, const uint8_t *gate_scales,
+                                       const uint8_t *up_codes, const uint8_t *up_scales,
+                                       const uint16_t *x, const uint16_t *dh, uint16_t *dx,
+                                       size_t M, size_t I, size_t K, size_t ldx, size_t lddh,
+                                       size_t lddx, int act, float limit, void *ws,
+                                       size_t ws_bytes, void *stream) {
+    const size_t need = apus_ghip_mxfp4_gated_backward_ws(M, I, K), wide = mx_wide(I, K);
+    size_t ldx_ = ldx, lddh_ = lddh, lddx_ = lddx;
+    uint8_t *const up = (uint8_t *)ws + wide;
+    if (check_sizes(M, I, K) || check_mx(GHIP_MXFP4, gate_codes, gate_scales, I, K)
+        || check_mx(GHIP_MXFP4, up_codes, up_scales, I, K) || check_act(act, limit)
+        || check_ptr("x", x) || check_ptr("dh", dh) || check_ptr("dx", dx)
+        || check_ld("ldx", &ldx_, K) || check_ld("lddh", &lddh_, I) || check_ld("lddx", &lddx_, K)
+        || check_ws(ws, ws_bytes, need)
+        || apus_ghip_mx_dequant_dev(GHIP_MXFP4, gate_codes, gate_scales, (uint16_t *)ws, I, K, 0, stream)
+        || apus_ghip_mx_dequant_dev(GHIP_MXFP4, up_codes, up_scales, (uint16_t *)up, I, K, 0, stream))
+        return 1;
+    return apus_ghip_bf16_gated_backward_dev((const uint16_t *)ws, (const uint16_t *)up, x, dh, dx,
+                                             NULL, NULL, M, I, K, ldx, lddh, lddx, act, limit,
+                                             up + wide, need - 2 * wide, stream);
+}
+
+/* ------------------------------------------------------------------------ */
 /* HBM expert slab store                                                    */
 /* ------------------------------------------------------------------------ */
 

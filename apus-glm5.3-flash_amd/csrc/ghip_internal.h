@@ -372,6 +372,60 @@ hipError_t ghip_launch_ffn(int mode, const GhipProd *p, const GhipEp *ep, hipStr
 hipError_t ghip_launch_ffn_grads(const GhipProd *dx, const GhipEp *edx, const GhipProd *dw,
                                  const GhipEp *edw, const GhipFfnSum *sum, hipStream_t st);
 
+/* ---- norm, microscaled values and the products with them (k_norm.hip, k_mx*.hip) */
+
+/* Types of an operand, as include/backend_hip.h numbers them. */
+enum { GHIP_BF16, GHIP_MXFP8, GHIP_MXFP4 };
+
+/* Bytes of a row of scales of K values: whole words. */
+size_t ghip_mx_scale_ld(size_t K);
+/* K % 32 == 0; codes 8-byte (MXFP4: 4-byte) aligned. */
+hipError_t ghip_launch_mx_quantize(int type, const uint16_t *x, uint8_t *codes, uint8_t *scales,
+                                   size_t R, size_t K, size_t ldx, hipStream_t st);
+hipError_t ghip_launch_mx_dequant(int type, const uint8_t *codes, const uint8_t *scales,
+                                  uint16_t *out, size_t R, size_t K, size_t ldo, hipStream_t st);
+
+/* The norm: r (residual), gamma, sum, y, codes with scales, rstd may be NULL. codes:
+ * D % 32 == 0, 8-byte aligned. sum or y may be x or r. */
+typedef struct {
+    const uint16_t *x, *r, *gamma;
+    uint16_t *sum, *y;
+    uint8_t *codes, *scales;
+    float *rstd;
+    size_t M, ldx, ldr, lds, ldy;
+    uint32_t D;
+    float eps;
+} GhipNorm;
+hipError_t ghip_launch_rmsnorm(const GhipNorm *p, hipStream_t st);
+
+/* Its gradient: gamma, rstd, ds, dx, dgamma may be NULL. part: 16-byte aligned, of
+ * ghip_rmsnorm_part_bytes, where dgamma is wanted. */
+typedef struct {
+    const uint16_t *s, *gamma, *dy, *ds;
+    const float *rstd;
+    uint16_t *dx, *dgamma;
+    float *part;
+    size_t M, lds, lddy, ldds, lddx;
+    uint32_t D;
+    float eps;
+} GhipNormGrad;
+size_t ghip_rmsnorm_part_bytes(size_t M, size_t D);
+hipError_t ghip_launch_rmsnorm_grad(const GhipNormGrad *p, hipStream_t st);
+
+/* x W^T with MXFP4 weights w (w2: the up projection of GHIP_EP_GATED), codes [N,
+ * K/2], scales [N, ghip_mx_scale_ld(K)]; x of type xt, rows xld bytes apart, scales
+ * xs where it is microscaled. K % 32 == 0, codes and x 16-byte aligned with xld %
+ * 16 == 0, scales 4-byte aligned. */
+typedef struct {
+    const uint8_t *w, *w2, *ws, *ws2, *x, *xs;
+    size_t xld;
+    uint32_t M, N, K;
+    int xt;
+} GhipMxProd;
+hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp *ep, hipStream_t st);
+/* Set-up, by ghip_ffn_init. */
+hipError_t ghip_mx_init(uint32_t n_cu);
+
 /* One expert slab record of a converted v2 container's apus.index.json
  * (c/gcache.h:896-930): the shard file name and the slab's file offset. */
 typedef struct {

@@ -304,8 +304,8 @@ extern "C" hipError_t ghip_ffn_init(uint32_t n_cu) {
             pairs[i].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(FFN_PAIR_LDS));
         if (e != hipSuccess) return e;
     }
-    const hipError_t e = ghip_ffn_rows_init();
-    if (e != hipSuccess) return e;
+    hipError_t e = ghip_ffn_rows_init();
+    if (e != hipSuccess || (e = ghip_mx_init(n_cu)) != hipSuccess) return e;
     g_ffn_ncu = n_cu;
     return hipSuccess;
 }
