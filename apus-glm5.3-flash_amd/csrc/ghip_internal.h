@@ -426,6 +426,24 @@ hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp *ep, hipSt
 /* Set-up, by ghip_ffn_init. */
 hipError_t ghip_mx_init(uint32_t n_cu);
 
+/* The weight-streaming kernel's forms (k_mx_rows.hip). */
+hipError_t ghip_launch_mx_rows(int mode, int form, const GhipMxProd *p, const GhipEp *ep, hipStream_t st);
+hipError_t ghip_mx_rows_init(void);
+/* The tiles of a mode and type (k_mx_gemm.h): the launch's rows and output columns,
+ * workgroups a CU holds, LDS, and microseconds of a step on a nearly empty and a full
+ * chip and of a round besides. */
+typedef struct {
+    uint32_t bm, bn, occ, lds;
+    float low, full, over;
+    const void *kern;
+    void (*launch)(const GhipMxProd *, const GhipEp *, uint32_t, uint32_t, hipStream_t);
+} GhipMxTile;
+const GhipMxTile *ghip_mx_fp8_tiles(int mode, int *n);
+const GhipMxTile *ghip_mx_fp4_tiles(int mode, int *n);
+int ghip_mx_gemm_tiles(int mode, int xt);
+int ghip_mx_gemm_fits(const GhipMxProd *p);
+hipError_t ghip_launch_mx_gemm(int mode, int tile, const GhipMxProd *p, const GhipEp *ep, hipStream_t st);
+
 /* One expert slab record of a converted v2 container's apus.index.json
  * (c/gcache.h:896-930): the shard file name and the slab's file offset. */
 typedef struct {

@@ -1,0 +1,59 @@
+/*
+ * k_mx_prod.hip — which kernel a product with MXFP4 weights takes (gfx950).
+ */
+#include "ghip_device.h"
+#include "ghip_internal.h"
+
+static uint32_t g_mx_ncu;                        /* CUs: the routes' rounds */
+
+static const GhipMxTile *tiles_of(int mode, int xt, int *n) {
+    *n = 0;
+    return xt == GHIP_MXFP8 ? ghip_mx_fp8_tiles(mode, n) : xt == GHIP_MXFP4 ? ghip_mx_fp4_tiles(mode, n) : nullptr;
+}
+
+/* Offsets inside a tile of 256 rows are of 31 bits. */
+extern "C" int ghip_mx_gemm_fits(const GhipMxProd *p) {
+    return p->xt != GHIP_BF16 && p->xld < ((size_t)1 << 23) && p->K < (1u << 23);
+}
+
+static size_t tile_grid(const GhipMxTile *t, const GhipMxProd *p) {
+    const size_t n = (((size_t)p->M + t->bm - 1) / t->bm) * (((size_t)p->N + t->bn - 1) / t->bn);
+    return n > GHIP_MAX_THREADS / 512 ? 0 : n;
+}
+
+extern "C" int ghip_mx_gemm_tiles(int mode, int xt) {
+    int n;
+    tiles_of(mode, xt, &n);
+    return n;
+}
+
+extern "C" hipError_t ghip_launch_mx_gemm(int mode, int tile, const GhipMxProd *p, const GhipEp *ep, hipStream_t st) {
+    int n;
+    const GhipMxTile *t = tiles_of(mode, p->xt, &n);
+    if (p->M == 0 || p->N == 0 || p->K == 0 || p->K % 32 || (mode != GHIP_EP_LINEAR && mode != GHIP_EP_GATED)
+        || !ghip_mx_gemm_fits(p) || tile < 0 || tile >= n || !tile_grid(t + tile, p))
+        return hipErrorInvalidValue;
+    t += tile;
+    t->launch(p, ep, (p->M + t->bm - 1) / t->bm, (p->N + t->bn - 1) / t->bn, st);
+    return hipGetLastError();
+}
+
+extern "C" hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp *ep, hipStream_t st) {
+    if (p->M > 64 && ghip_mx_gemm_fits(p)) return ghip_launch_mx_gemm(mode, p->M > 512 ? 0 : 3, p, ep, st);
+    return ghip_launch_mx_rows(mode, 0, p, ep, st);
+}
+
+extern "C" hipError_t ghip_mx_init(uint32_t n_cu) {
+    for (int i = 0; i < 4; i++) {
+        int n;
+        const GhipMxTile *t = tiles_of(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i < 2 ? GHIP_MXFP8 : GHIP_MXFP4, &n);
+        for (int k = 0; k < n; k++) {
+            const hipError_t e = hipFuncSetAttribute(t[k].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)t[k].lds);
+            if (e != hipSuccess) return e;
+        }
+    }
+    const hipError_t e = ghip_mx_rows_init();
+    if (e != hipSuccess) return e;
+    g_mx_ncu = n_cu;
+    return hipSuccess;
+}

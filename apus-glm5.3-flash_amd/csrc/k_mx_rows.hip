@@ -158,8 +158,8 @@ static const MrForm mr_gated[3] = {mr_form<GHIP_BF16, 2, 2, 2, GHIP_EP_GATED>(),
 #define MR_MAX_TILES ((size_t)65535)
 #define MR_MAX_BLOCKS (GHIP_MAX_THREADS / (MR_WAVES * 64))
 
-extern "C" hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp *ep, hipStream_t st) {
-    if (p->M == 0 || p->N == 0 || p->K == 0 || p->K % 32 || (mode != GHIP_EP_LINEAR && mode != GHIP_EP_GATED))
+extern "C" hipError_t ghip_launch_mx_rows(int mode, int form, const GhipMxProd *p, const GhipEp *ep, hipStream_t st) {
+    if (p->M == 0 || p->N == 0 || p->K == 0 || p->K % 32 || (mode != GHIP_EP_LINEAR && mode != GHIP_EP_GATED) || form)
         return hipErrorInvalidValue;
     const MrForm *c = (mode == GHIP_EP_GATED ? mr_gated : mr_linear) + p->xt;
     const size_t blocks = ((size_t)p->N + c->cols - 1) / c->cols, tiles = ((size_t)p->M + c->mr - 1) / c->mr;
@@ -174,8 +174,7 @@ extern "C" hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp
     return hipSuccess;
 }
 
-extern "C" hipError_t ghip_mx_init(uint32_t n_cu) {
-    (void)n_cu;
+extern "C" hipError_t ghip_mx_rows_init(void) {
     for (int i = 0; i < 6; i++) {
         const MrForm *c = i < 3 ? mr_linear + i : mr_gated + i - 3;
         const hipError_t e = hipFuncSetAttribute(c->kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)c->lds);

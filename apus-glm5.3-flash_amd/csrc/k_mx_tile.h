@@ -1,0 +1,23 @@
+/*
+ * k_mx_tile.h — an entry of a tile table (GhipMxTile) over k_mx_gemm.
+ */
+#ifndef K_MX_TILE_H
+#define K_MX_TILE_H
+
+#include "k_mx_gemm.h"
+
+template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
+static void mg_run(const GhipMxProd *p, const GhipEp *ep, uint32_t mt, uint32_t nt, hipStream_t st) {
+    using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
+    hipLaunchKernelGGL((k_mx_gemm<MODE, XT, WM, WN, RB, CB, R>), dim3(mt * nt), dim3(64 * WM * WN), T::RING, st,
+                       *p, *ep, mt, nt);
+}
+
+template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
+static constexpr GhipMxTile mg_tile(float low, float full, float over) {
+    using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
+    return {T::BM, T::OUTN, T::RING <= FG_LDS_MAX / 2 ? 2u : 1u, T::RING, low, full, over,
+            (const void *)k_mx_gemm<MODE, XT, WM, WN, RB, CB, R>, mg_run<MODE, XT, WM, WN, RB, CB, R>};
+}
+
+#endif /* K_MX_TILE_H */

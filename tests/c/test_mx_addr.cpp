@@ -1,0 +1,126 @@
+/*
+ * test_mx_addr.cpp — every lane of every load of the tiles with MXFP4 weights
+ * (k_mx_addr.h), over ragged rows and k: each address lies inside its matrix or
+ * past the buffer's span, and each operand read finds the row and k block that the
+ * matrix instruction's lane stands for. Exit 0 = as expected.
+ */
+#include <cstdio>
+#include <cstring>
+#include <vector>
+
+#include "k_mx_addr.h"
+
+static int bad;
+#define EXPECT(c, ...)                                        \
+    do {                                                      \
+        if (!(c)) {                                           \
+            if (bad++ < 10) { printf(__VA_ARGS__); puts(""); } \
+        }                                                     \
+    } while (0)
+
+/* What a 16-byte piece of LDS holds: matrix (0 x, 1 W, 2 up), row of the matrix's tile,
+ * byte of the row; zeros; or nothing. */
+struct Piece { int mat, row, byte; };
+enum { NOTHING = -1, ZERO = -2 };
+
+template <uint32_t XB, bool DUAL, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
+static void tile(uint32_t rows, uint32_t cols, uint32_t K, uint32_t xld) {
+    constexpr uint32_t NW = WM * WN, BM = 16 * RB * WM, BN = 16 * CB * WN;
+    const uint32_t nst = (K + 127) / 128, all = (nst + 1) & ~1u, wb = K / 2, xrow = XB == 128 ? K : wb;
+    for (uint32_t j = 0; j < all; j++) {
+        if (j > 2 && j + 3 < all) continue;
+        std::vector<Piece> x(BM * XB / 16, Piece{NOTHING, 0, 0}), w(BN * 4, Piece{NOTHING, 0, 0});
+        const int64_t xleft = (int64_t)xrow - XB * j, wleft = (int64_t)wb - 64 * j;
+        for (uint32_t wv = 0; wv < NW; wv++)
+            for (uint32_t lane = 0; lane < 64; lane++) {
+                const uint32_t ar = mg_row<XB>(wv, lane), aq = mg_byte<XB>(lane, ar);
+                for (uint32_t i = 0; i < BM * XB / 1024 / NW; i++) {
+                    const uint32_t off = mg_cut(ar * xld + aq + i * mg_rows_apart<XB, NW>(false) * xld, aq, (int32_t)xleft);
+                    const uint32_t span = rows * xld, r = ar + i * mg_rows_apart<XB, NW>(false);
+                    Piece &to = x[((wv + NW * i) * 1024 + 16 * lane) / 16];
+                    EXPECT(to.mat == NOTHING, "x: piece written twice");
+                    if (off >= span) {
+                        to = {ZERO, 0, 0};
+                        EXPECT(off <= FG_OOB && (r >= rows || (int64_t)aq >= xleft), "x: row %u of %u byte %u of %lld dropped", r, rows, aq, (long long)xleft);
+                    } else {
+                        to = {0, (int)(off / xld), (int)(off % xld)};
+                        EXPECT(r < rows && off == r * xld + aq && (int64_t)aq + 16 <= xleft, "x: row %u of %u, byte %u of %lld at %u", r, rows, aq, (long long)xleft, off);
+                    }
+                }
+                const uint32_t br = mg_row<64>(DUAL ? wv >> 1 : wv, lane), bq = mg_byte<64>(lane, br);
+                for (uint32_t i = 0; i < BN * 64 / 1024 / NW; i++) {
+                    const uint32_t off = mg_cut(br * wb + bq + i * mg_rows_apart<64, NW>(DUAL) * wb, bq, (int32_t)wleft);
+                    const uint32_t span = cols * wb, r = br + i * mg_rows_apart<64, NW>(DUAL);
+                    Piece &to = w[((wv + NW * i) * 1024 + 16 * lane) / 16];
+                    EXPECT(to.mat == NOTHING, "W: piece written twice");
+                    if (off >= span) {
+                        to = {ZERO, 0, 0};
+                        EXPECT(off <= FG_OOB && (r >= cols || (int64_t)bq >= wleft), "W: row %u of %u dropped", r, cols);
+                    } else {
+                        to = {DUAL && (wv & 1) ? 2 : 1, (int)(off / wb), (int)(off % wb)};
+                        EXPECT(r < cols && off == r * wb + bq && (int64_t)bq + 16 <= wleft, "W: row %u of %u, byte %u", r, cols, bq);
+                    }
+                }
+            }
+        /* operand reads */
+        auto check = [&](const char *what, const Piece &p, int mat, uint32_t row, uint32_t live, uint32_t byte, int64_t left) {
+            if (row >= live || (int64_t)byte >= left) EXPECT(p.mat == ZERO, "%s: row %u byte %u is not zero", what, row, byte);
+            else EXPECT(p.mat == mat && p.row == (int)row && p.byte == (int)byte, "%s: row %u byte %u holds %d, row %d, byte %d", what, row, byte, p.mat, p.row, p.byte);
+        };
+        for (uint32_t wr = 0; wr < WM; wr++)
+            for (uint32_t wc = 0; wc < WN; wc++)
+                for (uint32_t n = 0; n < 16; n++)
+                    for (uint32_t g = 0; g < 4; g++) {
+                        for (uint32_t r = 0; r < RB; r++) {
+                            const uint32_t row = 16 * (wr * RB + r) + n;
+                            for (uint32_t h = 0; h < (XB == 128 ? 2u : 1u); h++) {
+                                const uint32_t at = mg_at_x<XB>(wr * RB, n, g, h) + r * 16 * XB;
+                                EXPECT(at % 16 == 0 && at + 16 <= BM * XB, "x: read at %u", at);
+                                check("x", x[at / 16], 0, row, rows, XB == 128 ? 64 * h + 16 * g : 16 * g, xleft);
+                            }
+                            const uint32_t s = mg_at_sx(0, wr * RB, n, g) + 64 * r;
+                            EXPECT(s == 4 * row + g, "x's scale at %u", s);
+                        }
+                        for (uint32_t c = 0; c < CB; c++) {
+                            const uint32_t blk = wc * CB + c, row = 16 * (DUAL ? blk >> 1 : blk) + n;
+                            const uint32_t at = mg_at_w(0, wc * CB, n, g) + c * 1024;
+                            EXPECT(at % 16 == 0 && at + 16 <= BN * 64, "W: read at %u", at);
+                            check("W", w[at / 16], DUAL && (blk & 1) ? 2 : 1, row, cols, 16 * g, wleft);
+                            const uint32_t s = mg_at_sw(0, BM, wc * CB, n, g, DUAL) + mg_sw_step(c, BN, DUAL);
+                            bool second;
+                            const uint32_t sr = mg_scale_row(s / 4, BM, BN, DUAL, second);
+                            EXPECT(s / 4 >= BM && s / 4 < BM + BN && s % 4 == g && sr == row && second == (DUAL && (blk & 1)), "W's scale at %u", s);
+                        }
+                    }
+    }
+}
+
+template <uint32_t XB, bool DUAL, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
+static void shapes() {
+    constexpr uint32_t BM = 16 * RB * WM, OUT = 16 * CB * WN / (DUAL ? 2 : 1);
+    for (uint32_t K : {32u, 64u, 96u, 128u, 160u, 256u, 288u, 1120u, 4096u})
+        for (uint32_t rows : {1u, 15u, BM - 1, BM})
+            for (uint32_t cols : {1u, 17u, OUT - 1, OUT})
+                if (rows <= BM && cols <= OUT) tile<XB, DUAL, WM, WN, RB, CB>(rows, cols, K, XB == 128 ? K : K / 2);
+}
+template <uint32_t XB, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
+static void both() {
+    shapes<XB, false, WM, WN, RB, CB>();
+    shapes<XB, true, WM, WN, RB, CB>();
+}
+template <uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
+static void types() {
+    both<128, WM, WN, RB, CB>();
+    both<64, WM, WN, RB, CB>();
+}
+
+int main() {
+    types<2, 2, 8, 8>();
+    types<2, 2, 8, 4>();
+    types<2, 2, 4, 8>();
+    types<2, 2, 4, 4>();
+    types<2, 2, 2, 4>();
+    types<2, 2, 2, 2>();
+    printf(bad ? "FAIL\n" : "PASS\n");
+    return bad != 0;
+}
