@@ -22,8 +22,8 @@ C_SRCS = ["ghip_backend.c", "ghip_synth.c", "ghip_container.c"]
 HIP_SRCS = ["k_dequant.hip", "k_linear.hip", "k_gemm_bf16.hip", "k_rows.hip",
             "k_moe.hip", "k_moe_rows.hip", "k_moe_prefill.hip", "k_ffn.hip", "k_ffn_any.hip",
             "k_ffn_nt.hip", "k_ffn_nt8.hip", "k_ffn_bwd.hip", "k_ffn_grads.hip", "k_ffn_rows.hip",
-            "k_norm.hip", "k_mx.hip", "k_mx_rows.hip", "k_mx_fp8.hip", "k_mx_fp4.hip", "k_mx_prod.hip",
-            "k_synth.hip"]
+            "k_norm.hip", "k_mx.hip", "k_mx_rows.hip", "k_mx_bf16.hip", "k_mx_fp8.hip", "k_mx_fp4.hip",
+            "k_mx_prod.hip", "k_synth.hip"]
 
 INC = ["-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
 CFLAGS = ["-std=c11", "-O2", "-Wall", "-Wextra", "-fPIC", "-ffp-contract=off",

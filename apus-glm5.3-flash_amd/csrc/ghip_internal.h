@@ -438,6 +438,7 @@ typedef struct {
     const void *kern;
     void (*launch)(const GhipMxProd *, const GhipEp *, uint32_t, uint32_t, hipStream_t);
 } GhipMxTile;
+const GhipMxTile *ghip_mx_bf16_tiles(int mode, int *n);
 const GhipMxTile *ghip_mx_fp8_tiles(int mode, int *n);
 const GhipMxTile *ghip_mx_fp4_tiles(int mode, int *n);
 int ghip_mx_gemm_tiles(int mode, int xt);

@@ -29,10 +29,12 @@ __device__ __forceinline__ void mg_mfma(ghip_f32x4 &acc, const ghip_u32x4 &w, co
 
 template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
 struct MgTile {
-    static constexpr bool DUAL = ghip_ep_dual(MODE);
+    static constexpr bool DUAL = ghip_ep_dual(MODE), BF = XT == GHIP_BF16;
     static constexpr uint32_t NW = WM * WN, BM = 16u * RB * WM, BN = 16u * CB * WN, OUTN = DUAL ? BN / 2 : BN;
-    static constexpr uint32_t XB = XT == GHIP_MXFP8 ? 128u : 64u, AST = BM * XB, BST = BN * 64u;
-    static constexpr uint32_t NSL = (BM + BN + 64u * NW - 1u) / (64u * NW), SST = NSL * NW * 256u;
+    /* a step: k, bytes of a row of x and of W, words of scales */
+    static constexpr uint32_t KS = BF ? 64u : 128u, XB = XT == GHIP_MXFP4 ? 64u : 128u, WB = BF ? 32u : 64u;
+    static constexpr uint32_t SBM = BF ? 0u : BM, NSL = (SBM + BN + 64u * NW - 1u) / (64u * NW);
+    static constexpr uint32_t AST = BM * XB, BST = BN * WB, SST = NSL * NW * 256u;
     static constexpr uint32_t SLOT = AST + BST + SST, RING = R * SLOT;
     static constexpr uint32_t NAL = AST / 1024u / NW, NBL = BST / 1024u / NW, LPS = NAL + NBL + NSL;
     static_assert(AST % (1024u * NW) == 0 && BST % (1024u * NW) == 0, "whole loads");
@@ -44,8 +46,8 @@ template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
 __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipEp ep, uint32_t mt,
                                                              uint32_t nt) {
     using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
-    constexpr bool DUAL = T::DUAL;
-    constexpr uint32_t NW = T::NW, BM = T::BM, BN = T::BN, OUTN = T::OUTN, XB = T::XB;
+    constexpr bool DUAL = T::DUAL, BF = T::BF;
+    constexpr uint32_t NW = T::NW, BM = T::BM, BN = T::BN, OUTN = T::OUTN, XB = T::XB, WB = T::WB, KS = T::KS;
     constexpr uint32_t NAL = T::NAL, NBL = T::NBL, NSL = T::NSL, LPS = T::LPS, SLOT = T::SLOT;
     constexpr int NM = RB * CB;
     extern __shared__ __attribute__((aligned(1024))) uint8_t mg_lds[];
@@ -64,7 +66,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     const uint32_t sr = min(4u, mt - strip * 4u);
     const uint32_t row0 = (strip * 4u + in_strip % sr) * BM, col0 = in_strip / sr * OUTN;
     const uint32_t rows = min(p.M - row0, BM), cols = min(p.N - col0, OUTN);
-    const uint32_t nst = (p.K + 127u) >> 7, lds = 4u * nst, wb = p.K >> 1, xld = (uint32_t)p.xld;
+    const uint32_t nst = (p.K + KS - 1u) / KS, words = (p.K + 127u) >> 7, lds = 4u * words, wb = p.K >> 1, xld = (uint32_t)p.xld;
     const bool up = DUAL && (wv & 1u);
 
     /* loads: this lane's place in the first one; the others are a whole number of
@@ -73,16 +75,16 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     const uint8_t *pa = p.x + (size_t)row0 * p.xld, *pb = (up ? p.w2 : p.w) + (size_t)col0 * wb;
     const uint32_t aspan = rows * xld, bspan = cols * wb;
     const uint32_t ar = mg_row<XB>(wv, lane), aq = mg_byte<XB>(lane, ar), ao = ar * xld + aq;
-    const uint32_t br = mg_row<64>(DUAL ? wv >> 1 : wv, lane), bq = mg_byte<64>(lane, br), bo = br * wb + bq;
-    const uint32_t astep = mg_rows_apart<XB, NW>(false) * xld, bstep = mg_rows_apart<64, NW>(DUAL) * wb;
-    const uint32_t xrow = XT == GHIP_MXFP8 ? p.K : wb;   /* bytes of x's row */
+    const uint32_t br = mg_row<WB>(DUAL ? wv >> 1 : wv, lane), bq = mg_byte<WB>(lane, br), bo = br * wb + bq;
+    const uint32_t astep = mg_rows_apart<XB, NW>(false) * xld, bstep = mg_rows_apart<WB, NW>(DUAL) * wb;
+    const uint32_t xrow = BF ? 2u * p.K : XT == GHIP_MXFP8 ? p.K : wb;   /* bytes of x's row */
     const uint8_t *ps[NSL];
 #pragma unroll
     for (uint32_t i = 0; i < NSL; i++) {
         const uint32_t e = (wv + NW * i) * 64u + lane;
         bool second;
-        const uint32_t c = mg_scale_row(e, BM, BN, DUAL, second);
-        ps[i] = e < BM ? p.xs + (size_t)min(row0 + e, p.M - 1u) * lds
+        const uint32_t c = mg_scale_row(e, T::SBM, BN, DUAL, second);
+        ps[i] = e < T::SBM ? p.xs + (size_t)min(row0 + e, p.M - 1u) * lds
                        : (second ? p.ws2 : p.ws) + (size_t)min(col0 + c, p.N - 1u) * lds;
     }
     uint32_t jl = 0, sl = 0;                             /* the next step to load, its slot */
@@ -96,52 +98,66 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
             fg_dma16(pb, bspan, off, mg_lds + sl + T::AST + (wv + NW * (i - NAL)) * 1024u);
         } else {
             const uint32_t k = i - NAL - NBL;
-            mg_dma4(ps[k] + 4u * min(jl, nst - 1u), mg_lds + sl + T::AST + T::BST + (wv + NW * k) * 256u);
+            mg_dma4(ps[k] + 4u * min(BF ? jl >> 1 : jl, words - 1u), mg_lds + sl + T::AST + T::BST + (wv + NW * k) * 256u);
         }
     };
     auto next_load = [&]() {
         jl++;
         pa += XB;
-        pb += 64;
+        pb += WB;
         xleft -= (int32_t)XB;
-        wleft -= 64;
+        wleft -= (int32_t)WB;
         sl = sl == (R - 1u) * SLOT ? 0u : sl + SLOT;
     };
 
     /* Operands. W's are read one step ahead into the other set. x's row block r is read
      * again, for the next step, once its products are issued; the last one has two
      * sets, as its step ends with it */
-    using XReg = std::conditional_t<XT == GHIP_MXFP8, mg_i32x8, ghip_u32x4>;
+    using XReg = std::conditional_t<XT == GHIP_MXFP4, ghip_u32x4, mg_i32x8>;
+    using WReg = std::conditional_t<BF, mg_i32x8, ghip_u32x4>;
     XReg xa[RB], xl[2];
-    ghip_u32x4 wa[2][CB];
+    WReg wa[2][CB];
+    ghip_u32x2 codes[BF ? CB : 1];
     uint32_t sx[RB], sl_[2], sw[2][CB];
     constexpr uint32_t SC = T::AST + T::BST;
-    const uint32_t a0 = mg_at_x<XB>(wr * RB, n, g, 0), a1 = mg_at_x<XB>(wr * RB, n, g, 1);
-    const uint32_t b0 = mg_at_w(T::AST, wc * CB, n, g);
-    const uint32_t as = mg_at_sx(SC, wr * RB, n, g), bs = mg_at_sw(SC, BM, wc * CB, n, g, DUAL);
+    const uint32_t a0 = mg_at_x<XB>(wr * RB, n, g, 0, BF), a1 = mg_at_x<XB>(wr * RB, n, g, 1, BF);
+    const uint32_t b0 = mg_at_w<WB, CB>(T::AST, wc, n, g, DUAL);
+    const uint32_t as = mg_at_sx(SC, wr * RB, n) + g, bs = mg_at_sw(SC, T::SBM, wc * CB, n, DUAL) + (BF ? g >> 1 : g);
     auto read_x = [&](XReg &x, uint32_t &s, int r, const uint8_t *st) {
         const ghip_u32x4 lo = *(const ghip_u32x4 *)(st + a0 + r * (16u * XB));
-        if constexpr (XT == GHIP_MXFP8) {
+        if constexpr (XB == 128u) {
             const ghip_u32x4 hi = *(const ghip_u32x4 *)(st + a1 + r * (16u * XB));
             x = (mg_i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
         } else {
             x = lo;
         }
-        s = st[as + 64u * r];
+        if constexpr (!BF) s = st[as + 64u * r];
     };
     auto read_a = [&](auto set_c, auto r_c, const uint8_t *st) {
         constexpr int S = decltype(set_c)::value, r = decltype(r_c)::value;
         if constexpr (r == RB - 1) read_x(xl[S], sl_[S], r, st);
         else read_x(xa[r], sx[r], r, st);
     };
+    /* beside BF16: steps start in pairs, so that set S has bytes 2 S and 2 S + 1 of the word */
     auto read_b = [&](auto set_c, auto c_c, const uint8_t *st) {
         constexpr int S = decltype(set_c)::value, c = decltype(c_c)::value;
-        wa[S][c] = *(const ghip_u32x4 *)(st + b0 + c * 1024u);
-        sw[S][c] = st[bs + mg_sw_step(c, BN, DUAL)];
+        if constexpr (BF) codes[c] = *(const ghip_u32x2 *)(st + b0 + mg_w_step<WB>(c, DUAL));
+        else wa[S][c] = *(const ghip_u32x4 *)(st + b0 + mg_w_step<WB>(c, DUAL));
+        sw[S][c] = st[bs + mg_sw_step(c, BN, DUAL) + (BF ? 2 * S : 0)];
+    };
+    /* BF16: half h of W's block c of the next step; past: its k is past K, where the codes
+     * are zeros and the scale is any byte */
+    auto dequant = [&](auto set_c, auto c_c, auto h_c, bool past) {
+        if constexpr (BF) {
+            constexpr int S = decltype(set_c)::value, c = decltype(c_c)::value, h = decltype(h_c)::value;
+            const ghip_u32x4 d = mx_fp4_bf16(codes[c][h], past ? 1.0f : __uint_as_float(sw[S][c] << 23));
+#pragma unroll
+            for (int e = 0; e < 4; e++) wa[S][c][4 * h + e] = (int)d[e];
+        }
     };
     /* The step that K cuts: its blocks past K have any scale. A step past K (an odd
      * number of them) has zeros for codes, and the last one's scales */
-    const uint32_t rem = (p.K >> 5) & 3u;
+    const uint32_t nb = p.K >> 5, rem = nb & 3u;
     ghip_f32x4 acc[RB][CB];
 #pragma unroll
     for (int r = 0; r < RB; r++)
@@ -163,6 +179,11 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     __builtin_amdgcn_sched_barrier(0);
     fg_each<CB>([&](auto c) { read_b(S0{}, c, mg_lds); });
     fg_each<RB>([&](auto r) { read_a(S0{}, r, mg_lds); });
+    if constexpr (BF)
+        fg_each<2 * CB>([&](auto q) {
+            constexpr int Q = decltype(q)::value;
+            dequant(S0{}, std::integral_constant<int, Q / 2>{}, std::integral_constant<int, Q % 2>{}, g >= 2u * nb);
+        });
 
     uint32_t rs = 0;                                     /* slot of step j */
     auto step = [&](uint32_t j, auto set_c, auto main_c) {
@@ -176,7 +197,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
         __builtin_amdgcn_s_waitcnt(0xc07f);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!MAIN)
+        if constexpr (!MAIN && !BF)
             if (rem && j + 1u >= nst && g >= rem) {
                 fg_each<RB - 1>([&](auto r) { sx[decltype(r)::value] = 127u; });
                 sl_[S] = 127u;
@@ -187,24 +208,44 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
         const uint32_t ns = !more ? rs : rs == (R - 1u) * SLOT ? 0u : rs + SLOT;
         const uint8_t *st = mg_lds + ns;
         using NS = std::integral_constant<int, S ^ 1>;
+        const bool past = !MAIN && 2u * (j + 1u) + (g >> 1) >= nb;
         constexpr int NL = MAIN ? (int)LPS : 0, CU = CB + 1;
         fg_each<NM>([&](auto slot) {
             constexpr int I = decltype(slot)::value, Rr = I / CB, K = I % CB;
             constexpr int C = Rr & 1 ? CB - 1 - K : K;
-            if constexpr (Rr == RB - 1) mg_mfma(acc[Rr][C], wa[S][C], xl[S], sw[S][C], sl_[S]);
-            else mg_mfma(acc[Rr][C], wa[S][C], xa[Rr], sw[S][C], sx[Rr]);
-            /* W and x's last block over the first RB - 1 rows, x's others behind their own */
-            constexpr int B0 = fg_spread(CU, I, 0, NM - CB), B1 = fg_spread(CU, I + 1, 0, NM - CB);
+            auto mma = [&](const XReg &x, uint32_t s) {
+                if constexpr (BF) {
+                    const auto half = [](const mg_i32x8 &v, auto h) {
+                        constexpr int H = 4 * decltype(h)::value;
+                        return __builtin_bit_cast(ghip_bf16x8, __builtin_shufflevector(v, v, H, H + 1, H + 2, H + 3));
+                    };
+                    fg_mfma(acc[Rr][C], half(wa[S][C], S0{}), half(x, S0{}));
+                    fg_mfma(acc[Rr][C], half(wa[S][C], S1{}), half(x, S1{}));
+                } else {
+                    mg_mfma(acc[Rr][C], wa[S][C], x, sw[S][C], s);
+                }
+            };
+            if constexpr (Rr == RB - 1) mma(xl[S], sl_[S]);
+            else mma(xa[Rr], sx[Rr]);
+            /* W and x's last block over the first RB - 1 rows (codes for BF16 over the first
+             * third, dequantized behind), x's others behind their own */
+            constexpr int BE = BF ? NM / 3 : NM - CB, NQ = BF ? 2 * CB : 0;
+            constexpr int B0 = fg_spread(CU, I, 0, BE), B1 = fg_spread(CU, I + 1, 0, BE);
+            constexpr int Q0 = fg_spread(NQ, I, NM / 2, NM), Q1 = fg_spread(NQ, I + 1, NM / 2, NM);
             constexpr int L0 = fg_spread(NL, I, 0, NM), L1 = fg_spread(NL, I + 1, 0, NM);
             fg_each<B1 - B0>([&](auto k) {
                 constexpr int O = B0 + decltype(k)::value;
                 if constexpr (O < CB) read_b(NS{}, std::integral_constant<int, O>{}, st);
                 else read_a(NS{}, std::integral_constant<int, RB - 1>{}, st);
             });
+            fg_each<Q1 - Q0>([&](auto k) {
+                constexpr int Q = Q0 + decltype(k)::value;
+                dequant(NS{}, std::integral_constant<int, Q / 2>{}, std::integral_constant<int, Q % 2>{}, past);
+            });
             constexpr bool A = Rr > 0 && K == 0;
             if constexpr (A) read_a(NS{}, std::integral_constant<int, Rr - 1>{}, st);
             fg_each<L1 - L0>([&](auto k) { load(L0 + decltype(k)::value); });
-            if constexpr (A || B1 > B0 || L1 > L0) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (A || B1 > B0 || Q1 > Q0 || L1 > L0) __builtin_amdgcn_sched_barrier(0);
         });
         if constexpr (MAIN) next_load();
         __builtin_amdgcn_sched_barrier(0);

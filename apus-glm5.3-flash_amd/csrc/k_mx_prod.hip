@@ -7,13 +7,12 @@
 static uint32_t g_mx_ncu;                        /* CUs: the routes' rounds */
 
 static const GhipMxTile *tiles_of(int mode, int xt, int *n) {
-    *n = 0;
-    return xt == GHIP_MXFP8 ? ghip_mx_fp8_tiles(mode, n) : xt == GHIP_MXFP4 ? ghip_mx_fp4_tiles(mode, n) : nullptr;
+    return xt == GHIP_MXFP8 ? ghip_mx_fp8_tiles(mode, n) : xt == GHIP_MXFP4 ? ghip_mx_fp4_tiles(mode, n) : ghip_mx_bf16_tiles(mode, n);
 }
 
 /* Offsets inside a tile of 256 rows are of 31 bits. */
 extern "C" int ghip_mx_gemm_fits(const GhipMxProd *p) {
-    return p->xt != GHIP_BF16 && p->xld < ((size_t)1 << 23) && p->K < (1u << 23);
+    return p->xld < ((size_t)1 << 23) && p->K < (1u << 23);
 }
 
 static size_t tile_grid(const GhipMxTile *t, const GhipMxProd *p) {
@@ -44,9 +43,9 @@ extern "C" hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp
 }
 
 extern "C" hipError_t ghip_mx_init(uint32_t n_cu) {
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < 6; i++) {
         int n;
-        const GhipMxTile *t = tiles_of(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i < 2 ? GHIP_MXFP8 : GHIP_MXFP4, &n);
+        const GhipMxTile *t = tiles_of(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i >> 1, &n);
         for (int k = 0; k < n; k++) {
             const hipError_t e = hipFuncSetAttribute(t[k].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)t[k].lds);
             if (e != hipSuccess) return e;

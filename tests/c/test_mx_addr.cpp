@@ -23,14 +23,17 @@ static int bad;
 struct Piece { int mat, row, byte; };
 enum { NOTHING = -1, ZERO = -2 };
 
-template <uint32_t XB, bool DUAL, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
+enum { BF16, MXFP8, MXFP4 };
+
+template <int XT, bool DUAL, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
 static void tile(uint32_t rows, uint32_t cols, uint32_t K, uint32_t xld) {
     constexpr uint32_t NW = WM * WN, BM = 16 * RB * WM, BN = 16 * CB * WN;
-    const uint32_t nst = (K + 127) / 128, all = (nst + 1) & ~1u, wb = K / 2, xrow = XB == 128 ? K : wb;
+    constexpr uint32_t XB = XT == MXFP4 ? 64 : 128, WB = XT == BF16 ? 32 : 64, KS = XT == BF16 ? 64 : 128, SBM = XT == BF16 ? 0 : BM;
+    const uint32_t nst = (K + KS - 1) / KS, all = (nst + 1) & ~1u, wb = K / 2, xrow = XT == BF16 ? 2 * K : XT == MXFP8 ? K : wb;
     for (uint32_t j = 0; j < all; j++) {
         if (j > 2 && j + 3 < all) continue;
-        std::vector<Piece> x(BM * XB / 16, Piece{NOTHING, 0, 0}), w(BN * 4, Piece{NOTHING, 0, 0});
-        const int64_t xleft = (int64_t)xrow - XB * j, wleft = (int64_t)wb - 64 * j;
+        std::vector<Piece> x(BM * XB / 16, Piece{NOTHING, 0, 0}), w(BN * WB / 16, Piece{NOTHING, 0, 0});
+        const int64_t xleft = (int64_t)xrow - XB * j, wleft = (int64_t)wb - WB * j;
         for (uint32_t wv = 0; wv < NW; wv++)
             for (uint32_t lane = 0; lane < 64; lane++) {
                 const uint32_t ar = mg_row<XB>(wv, lane), aq = mg_byte<XB>(lane, ar);
@@ -47,10 +50,10 @@ static void tile(uint32_t rows, uint32_t cols, uint32_t K, uint32_t xld) {
                         EXPECT(r < rows && off == r * xld + aq && (int64_t)aq + 16 <= xleft, "x: row %u of %u, byte %u of %lld at %u", r, rows, aq, (long long)xleft, off);
                     }
                 }
-                const uint32_t br = mg_row<64>(DUAL ? wv >> 1 : wv, lane), bq = mg_byte<64>(lane, br);
-                for (uint32_t i = 0; i < BN * 64 / 1024 / NW; i++) {
-                    const uint32_t off = mg_cut(br * wb + bq + i * mg_rows_apart<64, NW>(DUAL) * wb, bq, (int32_t)wleft);
-                    const uint32_t span = cols * wb, r = br + i * mg_rows_apart<64, NW>(DUAL);
+                const uint32_t br = mg_row<WB>(DUAL ? wv >> 1 : wv, lane), bq = mg_byte<WB>(lane, br);
+                for (uint32_t i = 0; i < BN * WB / 1024 / NW; i++) {
+                    const uint32_t off = mg_cut(br * wb + bq + i * mg_rows_apart<WB, NW>(DUAL) * wb, bq, (int32_t)wleft);
+                    const uint32_t span = cols * wb, r = br + i * mg_rows_apart<WB, NW>(DUAL);
                     Piece &to = w[((wv + NW * i) * 1024 + 16 * lane) / 16];
                     EXPECT(to.mat == NOTHING, "W: piece written twice");
                     if (off >= span) {
@@ -74,44 +77,47 @@ static void tile(uint32_t rows, uint32_t cols, uint32_t K, uint32_t xld) {
                         for (uint32_t r = 0; r < RB; r++) {
                             const uint32_t row = 16 * (wr * RB + r) + n;
                             for (uint32_t h = 0; h < (XB == 128 ? 2u : 1u); h++) {
-                                const uint32_t at = mg_at_x<XB>(wr * RB, n, g, h) + r * 16 * XB;
+                                const uint32_t at = mg_at_x<XB>(wr * RB, n, g, h, XT == BF16) + r * 16 * XB;
                                 EXPECT(at % 16 == 0 && at + 16 <= BM * XB, "x: read at %u", at);
-                                check("x", x[at / 16], 0, row, rows, XB == 128 ? 64 * h + 16 * g : 16 * g, xleft);
+                                check("x", x[at / 16], 0, row, rows, XT == BF16 ? 32 * g + 16 * h : XT == MXFP8 ? 64 * h + 16 * g : 16 * g, xleft);
                             }
-                            const uint32_t s = mg_at_sx(0, wr * RB, n, g) + 64 * r;
-                            EXPECT(s == 4 * row + g, "x's scale at %u", s);
+                            const uint32_t s = mg_at_sx(0, wr * RB, n) + 64 * r;
+                            EXPECT(XT == BF16 || s == 4 * row, "x's scale at %u", s);
                         }
                         for (uint32_t c = 0; c < CB; c++) {
                             const uint32_t blk = wc * CB + c, row = 16 * (DUAL ? blk >> 1 : blk) + n;
-                            const uint32_t at = mg_at_w(0, wc * CB, n, g) + c * 1024;
-                            EXPECT(at % 16 == 0 && at + 16 <= BN * 64, "W: read at %u", at);
-                            check("W", w[at / 16], DUAL && (blk & 1) ? 2 : 1, row, cols, 16 * g, wleft);
-                            const uint32_t s = mg_at_sw(0, BM, wc * CB, n, g, DUAL) + mg_sw_step(c, BN, DUAL);
+                            const uint32_t at = mg_at_w<WB, CB>(0, wc, n, g, DUAL) + mg_w_step<WB>(c, DUAL);
+                            EXPECT(at % (WB / 4) == 0 && at + WB / 4 <= BN * WB, "W: read at %u", at);
+                            check("W", w[at / 16], DUAL && (blk & 1) ? 2 : 1, row, cols, WB == 64 ? 16 * g : 16 * (g >> 1), wleft);
+                            EXPECT(WB == 64 || at % 16 == 8 * (g & 1), "W: half %u", at % 16);
+                            const uint32_t s = mg_at_sw(0, SBM, wc * CB, n, DUAL) + mg_sw_step(c, BN, DUAL);
                             bool second;
-                            const uint32_t sr = mg_scale_row(s / 4, BM, BN, DUAL, second);
-                            EXPECT(s / 4 >= BM && s / 4 < BM + BN && s % 4 == g && sr == row && second == (DUAL && (blk & 1)), "W's scale at %u", s);
+                            const uint32_t sr = mg_scale_row(s / 4, SBM, BN, DUAL, second);
+                            EXPECT(s / 4 >= SBM && s / 4 < SBM + BN && s % 4 == 0 && sr == row && second == (DUAL && (blk & 1)), "W's scale at %u", s);
                         }
                     }
     }
 }
 
-template <uint32_t XB, bool DUAL, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
+template <int XT, bool DUAL, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
 static void shapes() {
     constexpr uint32_t BM = 16 * RB * WM, OUT = 16 * CB * WN / (DUAL ? 2 : 1);
     for (uint32_t K : {32u, 64u, 96u, 128u, 160u, 256u, 288u, 1120u, 4096u})
         for (uint32_t rows : {1u, 15u, BM - 1, BM})
             for (uint32_t cols : {1u, 17u, OUT - 1, OUT})
-                if (rows <= BM && cols <= OUT) tile<XB, DUAL, WM, WN, RB, CB>(rows, cols, K, XB == 128 ? K : K / 2);
+                for (uint32_t pad : {0u, 48u})
+                    if (rows <= BM && cols <= OUT && (XT == BF16 || !pad))
+                        tile<XT, DUAL, WM, WN, RB, CB>(rows, cols, K, XT == BF16 ? 2 * K + pad : XT == MXFP8 ? K : K / 2);
 }
-template <uint32_t XB, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
+template <int XT, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
 static void both() {
-    shapes<XB, false, WM, WN, RB, CB>();
-    shapes<XB, true, WM, WN, RB, CB>();
+    shapes<XT, false, WM, WN, RB, CB>();
+    shapes<XT, true, WM, WN, RB, CB>();
 }
 template <uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
 static void types() {
-    both<128, WM, WN, RB, CB>();
-    both<64, WM, WN, RB, CB>();
+    both<MXFP8, WM, WN, RB, CB>();
+    both<MXFP4, WM, WN, RB, CB>();
 }
 
 int main() {
@@ -121,6 +127,11 @@ int main() {
     types<2, 2, 4, 4>();
     types<2, 2, 2, 4>();
     types<2, 2, 2, 2>();
+    both<BF16, 1, 4, 16, 4>();
+    both<BF16, 1, 4, 12, 4>();
+    both<BF16, 1, 4, 8, 4>();
+    both<BF16, 1, 4, 8, 2>();
+    both<BF16, 1, 4, 4, 2>();
     printf(bad ? "FAIL\n" : "PASS\n");
     return bad != 0;
 }

@@ -260,20 +260,21 @@ def test_scales_of_every_size(ghip, M, N, xt):
     R.check(wide(y.get()), *X.linear(x.values, w.values, None, None, R.NONE, xt), "linear")
 
 
-@pytest.mark.parametrize("M,N,K", [(3, 520, 96), (40, 200, 1056), (300, 777, 160)])
+@pytest.mark.parametrize("M,N,K", [(3, 520, 96), (40, 200, 1056), (300, 777, 160), (300, 130, 32), (300, 130, 96)])
 def test_bytes_behind_the_last_scale_are_not_read(ghip, M, N, K):
     """The scale rows' words behind K's last block hold NaN scales."""
     rng = seed(48, M, N, K)
-    w, x = weights(rng, N, K), acts(rng, M, K)
-    a8 = Act(X.MXFP8, x)
-    y = [Mat.out(M, N) for _ in range(2)]
-    ok(ghip, linear(ghip, w, a8, None, None, y[0], R.NONE))
-    for m in (w, a8.mx):
-        s = m.scales.download(np.uint8, (m.values.shape[0], X.scale_ld(K)))
-        s[:, K // 32:] = 255
-        m.scales.upload(s)
-    ok(ghip, linear(ghip, w, a8, None, None, y[1], R.NONE))
-    assert np.array_equal(y[0].get(), y[1].get())
+    x = acts(rng, M, K)
+    for xt in XTYPES:
+        w, a = weights(rng, N, K), Act(xt, x)
+        y = [Mat.out(M, N) for _ in range(2)]
+        ok(ghip, linear(ghip, w, a, None, None, y[0], R.NONE))
+        for m in (w, a.mx) if xt else (w,):
+            s = m.scales.download(np.uint8, (m.values.shape[0], X.scale_ld(K)))
+            s[:, K // 32:] = 255
+            m.scales.upload(s)
+        ok(ghip, linear(ghip, w, a, None, None, y[1], R.NONE))
+        assert np.array_equal(y[0].get(), y[1].get())
 
 
 BWD = [(1, 40, 32), (5, 264, 96), (40, 392, 384), (300, 520, 1088), (500, 1030, 256), (130, 77, 64)]

@@ -27,11 +27,11 @@ def one(lib, kind, mode, form, xt, M, N, K, **more):
     R.check(wide(y.get()), *want, "form %d, %s" % (form, (M, N, K)))
 
 
-STEPS = [32, 128, 160, 256, 352, 384, 512, 608, 640, 768, 896, 1024, 1120, 1216]
+STEPS = [32, 64, 96, 128, 160, 256, 352, 384, 512, 608, 640, 768, 896, 1024, 1120, 1216]
 
 
 @pytest.mark.parametrize("mode", [F.LINEAR, F.GATED])
-@pytest.mark.parametrize("xt", [X.MXFP8, X.MXFP4])
+@pytest.mark.parametrize("xt", [X.BF16, X.MXFP8, X.MXFP4])
 def test_tiles_at_every_number_of_steps(ghip, mode, xt):
     for form in range(F.tiles(ghip, mode, xt)):
         for K in STEPS:
@@ -39,7 +39,7 @@ def test_tiles_at_every_number_of_steps(ghip, mode, xt):
 
 
 @pytest.mark.parametrize("mode", [F.LINEAR, F.GATED])
-@pytest.mark.parametrize("xt", [X.MXFP8, X.MXFP4])
+@pytest.mark.parametrize("xt", [X.BF16, X.MXFP8, X.MXFP4])
 def test_tiles_at_ragged_sizes(ghip, mode, xt):
     for form in range(F.tiles(ghip, mode, xt)):
         for M, N, K in [(1, 1, 96), (15, 17, 512), (257, 255, 288), (300, 520, 640), (513, 264, 160), (1030, 1031, 128)]:
