@@ -428,7 +428,12 @@ hipError_t ghip_mx_init(uint32_t n_cu);
 
 /* The weight-streaming kernel's forms (k_mx_rows.hip). */
 hipError_t ghip_launch_mx_rows(int mode, int form, const GhipMxProd *p, const GhipEp *ep, hipStream_t st);
-hipError_t ghip_mx_rows_init(void);
+int ghip_mx_rows_forms(int mode, int xt);
+int ghip_mx_rows_fits(int mode, int form, const GhipMxProd *p);
+/* The form (the tile, below) with the least estimated time, in microseconds in us; -1: none takes
+ * this shape. No device needed. */
+int ghip_mx_rows_pick(int mode, const GhipMxProd *p, float *us);
+hipError_t ghip_mx_rows_init(uint32_t n_cu);
 /* The tiles of a mode and type (k_mx_gemm.h): the launch's rows and output columns,
  * workgroups a CU holds, LDS, and microseconds of a step on a nearly empty and a full
  * chip and of a round besides. */
@@ -443,6 +448,7 @@ const GhipMxTile *ghip_mx_fp8_tiles(int mode, int *n);
 const GhipMxTile *ghip_mx_fp4_tiles(int mode, int *n);
 int ghip_mx_gemm_tiles(int mode, int xt);
 int ghip_mx_gemm_fits(const GhipMxProd *p);
+int ghip_mx_gemm_pick(int mode, const GhipMxProd *p, float *us);
 hipError_t ghip_launch_mx_gemm(int mode, int tile, const GhipMxProd *p, const GhipEp *ep, hipStream_t st);
 
 /* One expert slab record of a converted v2 container's apus.index.json

@@ -7,13 +7,13 @@
 template <int MODE>
 static const GhipMxTile *tiles(int *n) {
     static const GhipMxTile t[] = {
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 8, 8, 4>(1.0f, 1.0f, 1.0f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 8, 4, 6>(1.0f, 1.0f, 1.0f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 8, 5>(1.0f, 1.0f, 1.0f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 4, 3>(1.0f, 1.0f, 1.0f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 4, 8>(1.0f, 1.0f, 1.0f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 2, 4, 4>(1.0f, 1.0f, 1.0f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 2, 2, 5>(1.0f, 1.0f, 1.0f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 8, 8, 4>(0.64f, 1.36f, 6.1f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 8, 4, 6>(0.45f, 0.99f, 3.2f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 8, 5>(0.55f, 1.05f, 2.7f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 4, 3>(0.29f, 1.02f, 0.8f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 4, 8>(0.31f, 0.61f, 1.9f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 2, 4, 4>(0.27f, 0.84f, 0.0f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 2, 2, 5>(0.19f, 0.68f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;

@@ -4,7 +4,7 @@
 #include "ghip_device.h"
 #include "ghip_internal.h"
 
-static uint32_t g_mx_ncu;                        /* CUs: the routes' rounds */
+static uint32_t g_mx_ncu = 256;                  /* CUs: the routes' rounds */
 
 static const GhipMxTile *tiles_of(int mode, int xt, int *n) {
     return xt == GHIP_MXFP8 ? ghip_mx_fp8_tiles(mode, n) : xt == GHIP_MXFP4 ? ghip_mx_fp4_tiles(mode, n) : ghip_mx_bf16_tiles(mode, n);
@@ -37,9 +37,39 @@ extern "C" hipError_t ghip_launch_mx_gemm(int mode, int tile, const GhipMxProd *
     return hipGetLastError();
 }
 
+/* Estimated microseconds of a tile: 3 for the launch, and for each round of the chip
+ * its steps and what a round costs besides; steps of a round that does not fill the chip
+ * lie between the empty chip's time and the full one's. */
+static double tile_us(const GhipMxTile *t, const GhipMxProd *p) {
+    const double cap = (double)g_mx_ncu * t->occ, rounds = (double)tile_grid(t, p) / cap;
+    const double whole = (double)(size_t)rounds, part = rounds - whole;
+    const uint32_t k = p->xt == GHIP_BF16 ? 64 : 128;
+    const double steps = (double)(((p->K + k - 1) / k + 1) & ~1u);
+    return 3.0 + whole * (steps * t->full + t->over)
+         + (part > 0.0 ? steps * (t->low + (t->full - t->low) * part) + t->over : 0.0);
+}
+
+extern "C" int ghip_mx_gemm_pick(int mode, const GhipMxProd *p, float *us) {
+    int n, best = -1;
+    const GhipMxTile *t = tiles_of(mode, p->xt, &n);
+    for (int i = 0; ghip_mx_gemm_fits(p) && i < n; i++) {
+        if (!tile_grid(t + i, p)) continue;
+        const float e = (float)tile_us(t + i, p);
+        if (best < 0 || e < *us) {
+            best = i;
+            *us = e;
+        }
+    }
+    return best;
+}
+
+/* The form with the least estimated time: rows of weights streamed past a few rows of
+ * x, or tiles. */
 extern "C" hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp *ep, hipStream_t st) {
-    if (p->M > 64 && ghip_mx_gemm_fits(p)) return ghip_launch_mx_gemm(mode, p->M > 512 ? 0 : 3, p, ep, st);
-    return ghip_launch_mx_rows(mode, 0, p, ep, st);
+    float tile_t = 0.0f, rows_t = 0.0f;
+    const int tile = ghip_mx_gemm_pick(mode, p, &tile_t), form = ghip_mx_rows_pick(mode, p, &rows_t);
+    if (form >= 0 && (tile < 0 || rows_t <= tile_t)) return ghip_launch_mx_rows(mode, form, p, ep, st);
+    return ghip_launch_mx_gemm(mode, tile, p, ep, st);       /* -1: refused */
 }
 
 extern "C" hipError_t ghip_mx_init(uint32_t n_cu) {
@@ -51,7 +81,7 @@ extern "C" hipError_t ghip_mx_init(uint32_t n_cu) {
             if (e != hipSuccess) return e;
         }
     }
-    const hipError_t e = ghip_mx_rows_init();
+    const hipError_t e = ghip_mx_rows_init(n_cu);
     if (e != hipSuccess) return e;
     g_mx_ncu = n_cu;
     return hipSuccess;

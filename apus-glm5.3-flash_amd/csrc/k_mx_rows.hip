@@ -4,13 +4,16 @@
  * instruction.
  */
 #include <type_traits>
+#include <utility>
 
 #include "ghip_epilogue.h"
 #include "ghip_mx.h"
+#include "k_ffn_addr.h"
 
 typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
 
 #define MR_WAVES 8
+#define MR_OOB 0xFFFFFFF0u                       /* past every buffer */
 
 /* acc += W (MXFP4, 16 rows) . x^T (16 rows) over 128 k. Lane (n, g): W's row n, block
  * g; x's row n, bytes as its type has them (MXFP8: k 16 g + [0, 16) and 64 + 16 g +
@@ -28,157 +31,423 @@ __device__ __forceinline__ void mx_mfma(ghip_f32x4 &acc, const ghip_u32x4 &w, ui
     acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, XT == GHIP_MXFP8 ? 0 : 4, 0, sw, 0, sx);
 }
 
-/* A workgroup's 8 waves: 8 / KS groups of 16 NT weight rows, k over KS waves; 16 MT
- * rows of x. */
-template <int XT, int MT, int NT, int KS, int MODE>
-__global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, GhipEp ep, uint32_t blk0,
-                                                              uint32_t tile0) {
+/* f(0), f(1), ... f(N - 1), the argument a constant */
+template <typename F, int... I>
+__device__ __forceinline__ void mr_each_of(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void mr_each(F f) {
+    mr_each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+/* Words of four steps, lane group g's that of step g, as bytes: byte s of lane group
+ * g's result is block g of step s. Two exchanges between lane groups, a byte
+ * permutation behind each. */
+struct MrBytes {
+    uint32_t s16, s32;                                   /* this lane's selectors */
+};
+__device__ __forceinline__ MrBytes mr_bytes(uint32_t g) {
+    return {g & 1u ? 0x07030501u : 0x06020400u, g & 2u ? 0x07060302u : 0x05040100u};
+}
+__device__ __forceinline__ uint32_t mr_transpose(uint32_t v, const MrBytes &b) {
+    /* even and odd lane groups' words, then the lower and upper pair's */
+    const auto e = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    const uint32_t u = __builtin_amdgcn_perm(e[1], e[0], b.s16);
+    const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_amdgcn_perm(h[1], h[0], b.s32);
+}
+
+/* Bytes of x's row in a step, and where piece q of row r lies in LDS: the 16 rows that
+ * one lane group reads are in distinct banks. */
+template <int XT>
+constexpr uint32_t mr_xrow() { return XT == GHIP_BF16 ? 256u : XT == GHIP_MXFP8 ? 128u : 64u; }
+template <int XT>
+__device__ __forceinline__ uint32_t mr_spot(uint32_t r, uint32_t q) {
+    constexpr uint32_t XR = mr_xrow<XT>();
+    return r * XR + 16u * (XT == GHIP_BF16 ? q ^ (r & 15u) : XT == GHIP_MXFP8 ? q ^ fg_rot8(r) : q ^ fg_rot4(r));
+}
+
+/* Most steps of a wave's share. */
+template <uint32_t KS>
+__host__ __device__ constexpr uint32_t mr_share(uint32_t nst) {
+    return 2u * (((nst + 1u) / 2u + KS - 1u) / KS);
+}
+
+/* A workgroup's 8 waves: 8 / KS groups of 16 NT weight rows, k over KS waves; mr (up
+ * to 16) rows of x. It takes every gridDim.x-th block of weight rows: a wave copies its share
+ * of x to LDS once, and its stream of weights, 4 Q steps of 128 k ahead with one load
+ * of scales for four, runs on from one block into the next. */
+template <int XT, int NT, int KS, int MODE>
+__global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, GhipEp ep, uint32_t blocks,
+                                                              uint32_t row0, uint32_t mr) {
     constexpr bool DUAL = ghip_ep_dual(MODE), BF = XT == GHIP_BF16;
-    constexpr uint32_t GPP = MR_WAVES / KS, OG = DUAL ? NT / 2 : NT, MR = 16 * MT;
+    constexpr uint32_t GPP = MR_WAVES / KS, OG = DUAL ? NT / 2 : NT, XR = mr_xrow<XT>();
     constexpr int XI = BF ? 4 : XT == GHIP_MXFP8 ? 2 : 1;          /* 16-byte pieces of x a step */
+    constexpr uint32_t RED = MR_WAVES * 256u * NT;                 /* f32 sums of a block */
     static_assert(!DUAL || NT % 2 == 0, "gate and up groups alternate");
-    extern __shared__ __attribute__((aligned(16))) float red[];    /* [8 waves][MR][16 NT] */
+    extern __shared__ __attribute__((aligned(16))) float red[];    /* the sums, W's way to its operands, x */
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, g = lane >> 4;
     const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t part = wv % KS, slot = wv / KS;
     const uint32_t nst = (p.K + 127u) >> 7, nb = p.K >> 5, lds = 4u * nst;
-    const uint32_t c0 = part * nst / KS, c1 = (part + 1u) * nst / KS;
-    const uint32_t blk = blk0 + blockIdx.x, row0 = (blk * GPP + slot) * (16u * OG);
-    const uint32_t m0 = (tile0 + blockIdx.y) * MR, mrows = min(p.M - m0, MR);
-    ghip_f32x4 acc[MT][NT];
+    /* the wave's share, whole lines of W's rows: steps c0 .. c1 */
+    const uint32_t np = (nst + 1u) >> 1, c0 = 2u * (part * np / KS), c1 = min(2u * ((part + 1u) * np / KS), nst);
+    const uint32_t nc = c1 - c0, nq = (nc + 3u) >> 2;
+    const uint32_t m0 = row0 + blockIdx.y * mr, mrows = min(p.M - m0, mr);
+
+    /* x's rows over the wave's share: [step][row][XR], zeros past K. The first loads go
+     * ahead of the weights', the rest behind them */
+    uint8_t *const wl = (uint8_t *)(red + RED) + wv * (2048u * NT);
+    uint8_t *const xl = (uint8_t *)(red + RED) + MR_WAVES * (2048u * NT) + wv * (mrows * XR * mr_share<KS>(nst));
+    constexpr uint32_t PP = XR / 16u;                    /* pieces of a row in a step */
+    const uint32_t per = nc * PP, all = mrows * per, xbytes = p.K * (BF ? 4u : XT == GHIP_MXFP8 ? 2u : 1u) / 2u;
+    ghip_u32x4 xd[8];
+    uint32_t xat[8];
+    auto x_load = [&](uint32_t v0) {
 #pragma unroll
-    for (int a = 0; a < MT; a++)
-#pragma unroll
-        for (int b = 0; b < NT; b++) acc[a][b] = (ghip_f32x4){0.f, 0.f, 0.f, 0.f};
-    if (row0 < p.N) {
-        const uint8_t *w[NT], *ws[NT], *x[MT], *xs[MT];
-#pragma unroll
-        for (int b = 0; b < NT; b++) {
-            const size_t r = min(row0 + 16u * (DUAL ? b >> 1 : b) + n, p.N - 1u);
-            w[b] = (DUAL && (b & 1) ? p.w2 : p.w) + r * (p.K / 2u);
-            ws[b] = (DUAL && (b & 1) ? p.ws2 : p.ws) + r * lds;
+        for (int i = 0; i < 8; i++) {
+            const uint32_t v = v0 + 64u * i + lane, r = v / per, e = v - r * per, t = e / PP, q = e % PP;
+            const uint32_t byte = (c0 + t) * XR + 16u * q;
+            xd[i] = (ghip_u32x4){0u, 0u, 0u, 0u};
+            xat[i] = v < all ? t * (mrows * XR) + mr_spot<XT>(r, q) : ~0u;
+            if (v < all && byte < xbytes) xd[i] = *(const ghip_u32x4 *)(p.x + (size_t)(m0 + r) * p.xld + byte);
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto x_store = [&]() {
 #pragma unroll
-        for (int a = 0; a < MT; a++) {
-            const size_t r = m0 + min(16u * a + n, mrows - 1u);
-            x[a] = p.x + r * p.xld;
-            if (!BF) xs[a] = p.xs + r * lds;
-        }
-        for (uint32_t t = c0; t < c1; t++) {
-            const bool past = 4u * t + g >= nb;          /* the step that K cuts */
-            const uint32_t blkg = past ? 4u * t : 4u * t + g;
-            ghip_u32x4 wr[NT], xr[MT][XI];
-            uint32_t sw[NT], sx[MT];
-#pragma unroll
-            for (int b = 0; b < NT; b++) {
-                wr[b] = *(const ghip_u32x4 *)(w[b] + 16u * blkg);
-                sw[b] = past ? 127u : *(const uint32_t *)(ws[b] + 4u * t) >> (8u * g) & 255u;
-            }
-#pragma unroll
-            for (int a = 0; a < MT; a++) {
-                if constexpr (!BF) sx[a] = past ? 127u : *(const uint32_t *)(xs[a] + 4u * t) >> (8u * g) & 255u;
-#pragma unroll
-                for (int i = 0; i < XI; i++) {
-                    /* byte offset of the piece, and the block it lies in */
-                    const uint32_t q = BF ? 256u * t + 64u * g + 16u * i
-                                     : XT == GHIP_MXFP8 ? 128u * t + 64u * i + 16u * g : 64u * t + 16u * g;
-                    const uint32_t at = XT == GHIP_MXFP8 ? 4u * t + 2u * i + (g >> 1) : 4u * t + g;
-                    xr[a][i] = *(const ghip_u32x4 *)(x[a] + (at < nb ? q : 0u));
-                    if (at >= nb) xr[a][i] = (ghip_u32x4){0u, 0u, 0u, 0u};
-                }
-            }
-#pragma unroll
-            for (int b = 0; b < NT; b++) {
-                if constexpr (BF) {
-                    const float s = __uint_as_float(sw[b] << 23);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const ghip_bf16x8 wb = __builtin_bit_cast(ghip_bf16x8, mx_fp4_bf16(wr[b][i], s));
-#pragma unroll
-                        for (int a = 0; a < MT; a++)
-                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                wb, __builtin_bit_cast(ghip_bf16x8, xr[a][i]), acc[a][b], 0, 0, 0);
-                    }
-                } else {
-#pragma unroll
-                    for (int a = 0; a < MT; a++) mx_mfma<XT>(acc[a][b], wr[b], sw[b], xr[a], sx[a]);
-                }
-            }
-        }
-    }
-    /* the KS partial sums of each group, added in order; register i of a block: weight
-     * row 4 g + i, x's row n */
-#pragma unroll
-    for (int a = 0; a < MT; a++)
+        for (int i = 0; i < 8; i++)
+            if (xat[i] != ~0u) *(ghip_u32x4 *)(xl + xat[i]) = xd[i];
+    };
+    if (nc) x_load(0);
+
+    /* the weights' stream: block lblk, quad lq of the wave's share */
+    const uint32_t wb = p.K >> 1, wend = min(64u * c1, wb);
+    uint32_t lblk = blockIdx.x, lq = 0;
+    const uint32_t mine = min(n, mrows - 1u);
+    const uint8_t *const xs = BF ? nullptr : p.xs + (size_t)(m0 + mine) * lds;
+    ghip_u32x4 wr[4][NT];
+    uint32_t sw[NT], sx = 0u, bw[NT], bx = 0u;
+    /* The stream's next four steps: their scales, and half h of their codes (two steps).
+     * What lies past the wave's share, a row's end, the matrix or the stream is past the
+     * buffer: zeros, and no access (a second load from a line on its way costs a trip of
+     * its own) */
+    auto stream = [&](int b, const uint8_t *m, const uint8_t *m2, uint32_t ld) {
+        const uint32_t r0 = (lblk * GPP + slot) * (16u * OG) + 16u * (DUAL ? b >> 1 : b);
+        const uint32_t live = lblk < blocks && r0 < p.N ? min(p.N - r0, 16u) : 0u;
+        return __builtin_amdgcn_make_buffer_rsrc((void *)((DUAL && (b & 1) ? m2 : m) + (size_t)r0 * ld), 0, live * ld, 0x20000);
+    };
+    auto load_scales = [&]() {
+        const uint32_t t = c0 + 4u * lq + g;
 #pragma unroll
         for (int b = 0; b < NT; b++)
-            *(ghip_f32x4 *)(red + (wv * MR + 16u * a + n) * (16u * NT) + 16u * b + 4u * g) = acc[a][b];
-    __syncthreads();
-    ghip_with_act(ep.act, [&](auto act) {
-        for (uint32_t v = tid; v < GPP * MR * 16u * OG; v += MR_WAVES * 64u) {
-            const uint32_t sl = v / (MR * 16u * OG), e = v - sl * (MR * 16u * OG);
-            const uint32_t m = e / (16u * OG), c = e % (16u * OG), o = (blk * GPP + sl) * (16u * OG) + c;
-            if (m >= mrows || o >= p.N) continue;
-            const float *q = red + (sl * KS * MR + m) * (16u * NT) + (DUAL ? 32u * (c >> 4) + (c & 15u) : c);
-            float s0 = 0.0f, s1 = 0.0f;
+            sw[b] = __builtin_amdgcn_raw_buffer_load_b32(stream(b, p.ws, p.ws2, lds), t < nst ? n * lds + 4u * t : MR_OOB, 0, 0);
+        if constexpr (!BF) sx = *(const uint32_t *)(xs + 4u * min(t, nst - 1u));
+    };
+    auto load_codes = [&](auto h_c) {
+        constexpr int h = decltype(h_c)::value;
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                s0 += q[k * MR * 16u * NT];
-                if (DUAL) s1 += q[k * MR * 16u * NT + 16u];
+        for (int b = 0; b < NT; b++) {
+            const __amdgpu_buffer_rsrc_t m = stream(b, p.w, p.w2, wb);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t r = 8u * i + (lane >> 3), byte = 64u * (c0 + 4u * lq + 2u * h) + 16u * ((lane & 7u) ^ fg_rot8(r));
+                wr[2 * h + i][b] = __builtin_amdgcn_raw_buffer_load_b128(m, byte < wend ? r * wb + byte : MR_OOB, 0, 0);
             }
-            ghip_ep_store<MODE, decltype(act)::value>(ep, ep.out, m0 + m, o, s0, s1);
         }
-    });
+    };
+    auto advance = [&]() {
+        if (++lq == nq) {
+            lq = 0;
+            lblk += gridDim.x;
+        }
+    };
+    if (nc) {
+        load_scales();
+        mr_each<2>(load_codes);
+        advance();
+        __builtin_amdgcn_sched_barrier(0);
+        x_store();
+        for (uint32_t v0 = 512u; v0 < all; v0 += 512u) {
+            x_load(v0);
+            x_store();
+        }
+    }
+
+    /* the epilogue's inputs, on their way during the products: value v of a block's
+     * outputs is of thread v % 512 */
+    constexpr uint32_t NOUT = GPP * 256u * OG, NV = (NOUT + MR_WAVES * 64u - 1u) / (MR_WAVES * 64u);
+    uint16_t ein[NV], ebias[NV];
+    uint32_t blk = blockIdx.x, j = 0;
+    auto place = [&](uint32_t v, uint32_t &m, uint32_t &o) {
+        const uint32_t sl = v / (256u * OG), e = v - sl * (256u * OG);
+        m = e / (16u * OG);
+        o = (blk * GPP + sl) * (16u * OG) + e % (16u * OG);
+        return v < NOUT && m < mrows && o < p.N;
+    };
+    auto inputs = [&]() {
+#pragma unroll
+        for (uint32_t i = 0; i < NV; i++) {
+            uint32_t m, o;
+            const bool live = place(tid + i * (MR_WAVES * 64u), m, o);
+            ein[i] = live && ep.in ? ep.in[(size_t)(m0 + m) * ep.ldin + o] : (uint16_t)0;
+            ebias[i] = live && ep.bias ? ep.bias[o] : (uint16_t)0;
+        }
+    };
+    inputs();
+    ghip_f32x4 acc[NT];
+#pragma unroll
+    for (int b = 0; b < NT; b++) acc[b] = (ghip_f32x4){0.f, 0.f, 0.f, 0.f};
+    /* a block's end: the KS partial sums of each group, added in order (register i of a
+     * group: weight row 4 g + i, x's row n) */
+    auto finish = [&]() {
+        if (blk != blockIdx.x) {                         /* the block before has been read */
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            __builtin_amdgcn_s_barrier();
+        }
+#pragma unroll
+        for (int b = 0; b < NT; b++) {
+            *(ghip_f32x4 *)(red + (wv * 16u + n) * (16u * NT) + 16u * b + 4u * g) = acc[b];
+            acc[b] = (ghip_f32x4){0.f, 0.f, 0.f, 0.f};
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        __builtin_amdgcn_s_barrier();
+        ghip_with_act(ep.act, [&](auto act) {
+#pragma unroll
+            for (uint32_t i = 0; i < NV; i++) {
+                uint32_t m, o;
+                const uint32_t v = tid + i * (MR_WAVES * 64u);
+                if (!place(v, m, o)) continue;
+                const uint32_t sl = v / (256u * OG), c = v % (16u * OG);
+                /* dual: gate group, up group, ... of 16 columns */
+                const float *q = red + (sl * KS * 16u + m) * (16u * NT) + (DUAL ? 32u * (c >> 4) + (c & 15u) : c);
+                float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    s0 += q[k * 256u * NT];
+                    if (DUAL) s1 += q[k * 256u * NT + 16u];
+                }
+                ghip_ep_put<MODE, decltype(act)::value>(ep, ep.out, m0 + m, o, s0, s1, ghip_bf16_f32(ebias[i]),
+                                                        ghip_bf16_f32(ein[i]));
+            }
+        });
+        blk += gridDim.x;
+        if (blk < blocks) inputs();
+    };
+    if (nc == 0u) {                                      /* fewer steps than waves */
+        while (blk < blocks) finish();
+        return;
+    }
+    const MrBytes bytes = mr_bytes(g);
+    uint32_t xo[XI];
+#pragma unroll
+    for (int i = 0; i < XI; i++) xo[i] = mr_spot<XT>(mine, BF ? 4u * g + i : XT == GHIP_MXFP8 ? 4u * i + g : g);
+    const uint32_t w0 = fg_at0(n, g), w1 = fg_at0(n, 4u + g);
+    for (;;) {
+        const uint32_t t = c0 + 4u * j;
+#pragma unroll
+        for (int b = 0; b < NT; b++) bw[b] = mr_transpose(sw[b], bytes);
+        if constexpr (!BF) bx = mr_transpose(sx, bytes);
+        load_scales();
+        mr_each<2>([&](auto h_c) {
+            constexpr int h = decltype(h_c)::value;
+            /* two steps of W to LDS as they were loaded, the registers' next load, and back
+             * as operands; a wave's LDS accesses are in order */
+#pragma unroll
+            for (int b = 0; b < NT; b++) {
+                *(ghip_u32x4 *)(wl + 2048 * b + 16u * lane) = wr[2 * h][b];
+                *(ghip_u32x4 *)(wl + 2048 * b + 1024 + 16u * lane) = wr[2 * h + 1][b];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_codes(h_c);
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 2u * h >= c1) return;
+            ghip_u32x4 wo[2][NT];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int b = 0; b < NT; b++) wo[i][b] = *(const ghip_u32x4 *)(wl + 2048 * b + (i ? w1 : w0));
+            mr_each<2>([&](auto i_c) {
+                constexpr int i = decltype(i_c)::value, s = 2 * h + i;
+                if (i && t + s >= c1) return;
+                const bool past = 4u * (t + s) + g >= nb;    /* codes and x are zeros there */
+                const uint8_t *const xt = xl + (t + s - c0) * (mrows * XR);
+                ghip_u32x4 xr[XI];
+#pragma unroll
+                for (int k = 0; k < XI; k++) xr[k] = *(const ghip_u32x4 *)(xt + xo[k]);
+#pragma unroll
+                for (int b = 0; b < NT; b++) {
+                    const uint32_t sb = past ? 127u : bw[b] >> (8 * s) & 255u;
+                    if constexpr (BF) {
+                        const float f = __uint_as_float(sb << 23);
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                __builtin_bit_cast(ghip_bf16x8, mx_fp4_bf16(wo[i][b][k], f)),
+                                __builtin_bit_cast(ghip_bf16x8, xr[k]), acc[b], 0, 0, 0);
+                    } else {
+                        mx_mfma<XT>(acc[b], wo[i][b], sb, xr, past ? 127u : bx >> (8 * s) & 255u);
+                    }
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        advance();
+        if (++j == nq) {
+            j = 0;
+            finish();
+            if (blk >= blocks) break;
+        }
+    }
 }
 
+/* One launchable form: output columns, and microseconds of the launch, of four steps of
+ * a wave, of a block besides, and of a KB of a wave's share of x. */
 struct MrForm {
-    uint32_t mr, cols;
+    uint32_t cols, nt, ks, red;
+    float base, quad, over, copy;
     const void *kern;
-    uint32_t lds;
-    void (*launch)(dim3, uint32_t, hipStream_t, const GhipMxProd &, const GhipEp &, uint32_t, uint32_t);
+    void (*launch)(dim3, uint32_t, hipStream_t, const GhipMxProd &, const GhipEp &, uint32_t, uint32_t,
+                   uint32_t);
 };
-template <int XT, int MT, int NT, int KS, int MODE>
+template <int XT, int NT, int KS, int MODE>
 static void mr_run(dim3 grid, uint32_t lds, hipStream_t st, const GhipMxProd &p, const GhipEp &ep,
-                   uint32_t blk0, uint32_t tile0) {
-    hipLaunchKernelGGL((k_mx_rows<XT, MT, NT, KS, MODE>), grid, dim3(MR_WAVES * 64), lds, st, p, ep, blk0, tile0);
+                   uint32_t blocks, uint32_t row0, uint32_t mr) {
+    hipLaunchKernelGGL((k_mx_rows<XT, NT, KS, MODE>), grid, dim3(MR_WAVES * 64), lds, st, p, ep, blocks, row0, mr);
 }
-template <int XT, int MT, int NT, int KS, int MODE>
-static constexpr MrForm mr_form() {
-    return {16 * MT, (ghip_ep_dual(MODE) ? 8u : 16u) * NT * (MR_WAVES / KS),
-            (const void *)k_mx_rows<XT, MT, NT, KS, MODE>, MR_WAVES * 16u * MT * 16u * NT * 4u,
-            mr_run<XT, MT, NT, KS, MODE>};
+template <int XT, int NT, int KS, int MODE>
+static constexpr MrForm mr_form(float base, float quad, float over, float copy) {
+    return {(ghip_ep_dual(MODE) ? 8u : 16u) * NT * (MR_WAVES / KS), NT, KS, MR_WAVES * 256u * NT * 4u, base, quad, over, copy,
+            (const void *)k_mx_rows<XT, NT, KS, MODE>, mr_run<XT, NT, KS, MODE>};
 }
-static const MrForm mr_linear[3] = {mr_form<GHIP_BF16, 2, 2, 2, GHIP_EP_LINEAR>(),
-                                    mr_form<GHIP_MXFP8, 2, 2, 2, GHIP_EP_LINEAR>(),
-                                    mr_form<GHIP_MXFP4, 2, 2, 2, GHIP_EP_LINEAR>()};
-static const MrForm mr_gated[3] = {mr_form<GHIP_BF16, 2, 2, 2, GHIP_EP_GATED>(),
-                                   mr_form<GHIP_MXFP8, 2, 2, 2, GHIP_EP_GATED>(),
-                                   mr_form<GHIP_MXFP4, 2, 2, 2, GHIP_EP_GATED>()};
 
-#define MR_MAX_TILES ((size_t)65535)
-#define MR_MAX_BLOCKS (GHIP_MAX_THREADS / (MR_WAVES * 64))
+static const MrForm mr_linear_bf16[] = {
+    mr_form<GHIP_BF16, 1, 8, GHIP_EP_LINEAR>(2.1f, 0.92f, 0.32f, 0.18f),
+    mr_form<GHIP_BF16, 1, 4, GHIP_EP_LINEAR>(2.3f, 1.01f, 0.21f, 0.14f),
+    mr_form<GHIP_BF16, 2, 8, GHIP_EP_LINEAR>(1.5f, 1.75f, 0.59f, 0.22f),
+    mr_form<GHIP_BF16, 2, 4, GHIP_EP_LINEAR>(1.9f, 1.74f, 0.44f, 0.18f),
+};
+static const MrForm mr_linear_mxfp8[] = {
+    mr_form<GHIP_MXFP8, 1, 8, GHIP_EP_LINEAR>(2.4f, 0.67f, 0.36f, 0.16f),
+    mr_form<GHIP_MXFP8, 1, 4, GHIP_EP_LINEAR>(2.3f, 0.61f, 0.56f, 0.17f),
+    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_LINEAR>(1.7f, 1.14f, 0.83f, 0.23f),
+    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_LINEAR>(2.0f, 1.05f, 0.95f, 0.21f),
+};
+static const MrForm mr_linear_mxfp4[] = {
+    mr_form<GHIP_MXFP4, 1, 8, GHIP_EP_LINEAR>(2.6f, 0.39f, 0.50f, 0.22f),
+    mr_form<GHIP_MXFP4, 1, 4, GHIP_EP_LINEAR>(2.6f, 0.66f, 0.37f, 0.13f),
+    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_LINEAR>(1.8f, 0.53f, 1.29f, 0.34f),
+    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_LINEAR>(2.2f, 1.12f, 0.93f, 0.16f),
+};
+static const MrForm mr_gated_bf16[] = {
+    mr_form<GHIP_BF16, 2, 8, GHIP_EP_GATED>(1.7f, 1.70f, 0.43f, 0.20f),
+    mr_form<GHIP_BF16, 2, 4, GHIP_EP_GATED>(1.9f, 1.86f, 0.19f, 0.17f),
+};
+static const MrForm mr_gated_mxfp8[] = {
+    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_GATED>(1.8f, 1.53f, 0.55f, 0.18f),
+    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_GATED>(1.7f, 1.40f, 0.87f, 0.17f),
+};
+static const MrForm mr_gated_mxfp4[] = {
+    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_GATED>(1.4f, 0.83f, 1.21f, 0.39f),
+    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_GATED>(2.1f, 1.58f, 0.47f, 0.10f),
+};
+static const MrForm *mr_forms(int mode, int xt, int *n) {
+    const bool dual = mode == GHIP_EP_GATED;
+    *n = dual ? 2 : 4;
+    if (xt == GHIP_MXFP8) return dual ? mr_gated_mxfp8 : mr_linear_mxfp8;
+    if (xt == GHIP_MXFP4) return dual ? mr_gated_mxfp4 : mr_linear_mxfp4;
+    return dual ? mr_gated_bf16 : mr_linear_bf16;
+}
+
+#define MR_LDS_MAX (160u * 1024u)
+#define MR_MAX_TILES 65535u
+
+static uint32_t g_mr_ncu = 256;
+
+/* How a form takes this shape: the rows of a tile, as many as fit beside the sums and
+ * two steps of weights (up to 16, tiles of as many rows each), and its LDS; 0 rows: k
+ * is too long. */
+struct MrPlan {
+    uint32_t mr, tiles, lds, blocks, grid, turns;
+    float us;                            /* estimated */
+};
+static MrPlan plan(const MrForm *c, const GhipMxProd *p) {
+    const size_t nst = ((size_t)p->K + 127) / 128;
+    const size_t row = MR_WAVES * (p->xt == GHIP_BF16 ? 256 : p->xt == GHIP_MXFP8 ? 128 : 64) * 2 * (((nst + 1) / 2 + c->ks - 1) / c->ks);
+    const size_t rest = c->red + MR_WAVES * 2048 * c->nt;
+    size_t most = (MR_LDS_MAX - rest) / row;
+    if (most > 16) most = 16;
+    MrPlan r = {};
+    if (most == 0) return r;
+    r.tiles = (uint32_t)(((size_t)p->M + most - 1) / most);
+    r.mr = (uint32_t)(((size_t)p->M + r.tiles - 1) / r.tiles);
+    r.lds = (uint32_t)(rest + r.mr * row);
+    r.blocks = (uint32_t)(((size_t)p->N + c->cols - 1) / c->cols);
+    /* as many workgroups as there is room for, each with as many blocks of weights */
+    const size_t occ = r.lds <= MR_LDS_MAX / 2 ? 2 : 1, room = (g_mr_ncu * occ + r.tiles - 1) / r.tiles;
+    r.turns = (uint32_t)((r.blocks + room - 1) / room);
+    r.grid = (r.blocks + r.turns - 1) / r.turns;
+    /* the rounds of the chip, or the weights at 6.5 TB/s, and a tenth of the other */
+    const double quads = (double)((((nst + 1) / 2 + c->ks - 1) / c->ks + 1) / 2);
+    const double rounds = (double)(((size_t)r.grid * r.tiles + g_mr_ncu * occ - 1) / (g_mr_ncu * occ));
+    const double chain = c->base + rounds * (r.turns * (quads * c->quad + c->over) + (double)(r.mr * row) / MR_WAVES / 1024.0 * c->copy);
+    const double hbm = 2.6 + (double)p->N * p->K * (p->w2 ? 2 : 1) * 17.0 / 32.0 / 6.5e6;
+    r.us = (float)(chain > hbm ? chain + 0.1 * hbm : hbm + 0.1 * chain);
+    return r;
+}
+
+extern "C" int ghip_mx_rows_forms(int mode, int xt) {
+    int n;
+    mr_forms(mode, xt, &n);
+    return n;
+}
+
+extern "C" int ghip_mx_rows_fits(int mode, int form, const GhipMxProd *p) {
+    int n;
+    const MrForm *c = mr_forms(mode, p->xt, &n);
+    return form >= 0 && form < n && plan(c + form, p).mr != 0u;
+}
+
+extern "C" int ghip_mx_rows_pick(int mode, const GhipMxProd *p, float *us) {
+    int n, best = -1;
+    const MrForm *c = mr_forms(mode, p->xt, &n);
+    for (int i = 0; i < n; i++) {
+        const MrPlan r = plan(c + i, p);
+        if (r.mr != 0u && (best < 0 || r.us < *us)) {
+            best = i;
+            *us = r.us;
+        }
+    }
+    return best;
+}
 
 extern "C" hipError_t ghip_launch_mx_rows(int mode, int form, const GhipMxProd *p, const GhipEp *ep, hipStream_t st) {
-    if (p->M == 0 || p->N == 0 || p->K == 0 || p->K % 32 || (mode != GHIP_EP_LINEAR && mode != GHIP_EP_GATED) || form)
+    int n;
+    const MrForm *c = mr_forms(mode, p->xt, &n);
+    if (p->M == 0 || p->N == 0 || p->K == 0 || p->K % 32 || (mode != GHIP_EP_LINEAR && mode != GHIP_EP_GATED)
+        || !ghip_mx_rows_fits(mode, form, p))
         return hipErrorInvalidValue;
-    const MrForm *c = (mode == GHIP_EP_GATED ? mr_gated : mr_linear) + p->xt;
-    const size_t blocks = ((size_t)p->N + c->cols - 1) / c->cols, tiles = ((size_t)p->M + c->mr - 1) / c->mr;
-    for (size_t t0 = 0; t0 < tiles; t0 += MR_MAX_TILES)
-        for (size_t b0 = 0; b0 < blocks; b0 += MR_MAX_BLOCKS) {
-            const size_t nt = tiles - t0 < MR_MAX_TILES ? tiles - t0 : MR_MAX_TILES;
-            const size_t nb = blocks - b0 < MR_MAX_BLOCKS ? blocks - b0 : MR_MAX_BLOCKS;
-            c->launch(dim3((uint32_t)nb, (uint32_t)nt), c->lds, st, *p, *ep, (uint32_t)b0, (uint32_t)t0);
-            const hipError_t e = hipGetLastError();
-            if (e != hipSuccess) return e;
-        }
+    c += form;
+    const MrPlan r = plan(c, p);
+    for (uint32_t t = 0; t < r.tiles; t += MR_MAX_TILES) {
+        const uint32_t nt = r.tiles - t < MR_MAX_TILES ? r.tiles - t : MR_MAX_TILES;
+        c->launch(dim3(r.grid, nt), r.lds, st, *p, *ep, r.blocks, t * r.mr, r.mr);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     return hipSuccess;
 }
 
-extern "C" hipError_t ghip_mx_rows_init(void) {
+extern "C" hipError_t ghip_mx_rows_init(uint32_t n_cu) {
     for (int i = 0; i < 6; i++) {
-        const MrForm *c = i < 3 ? mr_linear + i : mr_gated + i - 3;
-        const hipError_t e = hipFuncSetAttribute(c->kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)c->lds);
-        if (e != hipSuccess) return e;
+        int n;
+        const MrForm *c = mr_forms(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i >> 1, &n);
+        for (int k = 0; k < n; k++) {
+            const hipError_t e = hipFuncSetAttribute(c[k].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)MR_LDS_MAX);
+            if (e != hipSuccess) return e;
+        }
     }
+    g_mr_ncu = n_cu;
     return hipSuccess;
 }

@@ -21,6 +21,15 @@ def tiles(lib, mode, xt):
     return lib.ghip_mx_gemm_tiles(mode, xt)
 
 
+def rows(lib, mode, xt):
+    return lib.ghip_mx_rows_forms(mode, xt)
+
+
+def rows_fits(lib, mode, form, xt, M, N, K):
+    at = 1 << 20                                                    # never read
+    return lib.ghip_mx_rows_fits(mode, form, ctypes.byref(prod(xt, M, N, K, at, at, at, at, at, at)))
+
+
 def launch(lib, kind, mode, form, p, ep, st=None):
     """kind: gemm or rows; the hipError_t."""
     return getattr(lib, "ghip_launch_mx_" + kind)(mode, form, ctypes.byref(p), ctypes.byref(ep), st)

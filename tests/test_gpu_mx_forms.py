@@ -46,6 +46,17 @@ def test_tiles_at_ragged_sizes(ghip, mode, xt):
             one(ghip, "gemm", mode, form, xt, M, N, K, off=9)
 
 
+@pytest.mark.parametrize("mode", [F.LINEAR, F.GATED])
+@pytest.mark.parametrize("xt", [X.BF16, X.MXFP8, X.MXFP4])
+def test_row_forms(ghip, mode, xt):
+    """One to several tiles of rows; k of fewer steps than waves, than are in flight, and of many, whole and cut."""
+    for form in range(F.rows(ghip, mode, xt)):
+        for M, N, K in [(1, 1, 32), (1, 70, 96), (3, 300, 544), (16, 33, 1024), (17, 129, 2080), (40, 64, 4096), (65, 40, 8224), (5, 530, 6400),
+                        (20, 20, 20000), (3, 9000, 256), (16, 300, 4096)]:
+            if F.rows_fits(ghip, mode, form, xt, M, N, K):
+                one(ghip, "rows", mode, form, xt, M, N, K)
+
+
 def test_what_the_launchers_refuse(ghip):
     p, e = F.prod(X.MXFP8, 4, 4, 64, 1 << 20, 1 << 20, 1 << 20, 1 << 20), F.F.Ep()
     for kind, mode, form, change in [("gemm", F.LINEAR, 99, {}), ("gemm", F.LINEAR, -1, {}), ("gemm", 0, 0, {}), ("gemm", F.LINEAR, 0, {"K": 40}),
