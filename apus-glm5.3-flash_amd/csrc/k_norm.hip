@@ -190,7 +190,7 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_long(GhipNorm p, size_t row0) 
 
 /* dx's columns [col, col + 8); a = rstd, b = rstd^3 mean(gamma dy s). */
 __device__ __forceinline__ void nm_dx(const GhipNormGrad &p, size_t row, uint32_t col, const nm_u16x8 &s,
-                                      const nm_u16x8 &dy, const nm_u16x8 &g, float a, float b) {
+                                      const nm_u16x8 &dy, const nm_u16x8 &g, const nm_u16x8 &ds, float a, float b) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -198,11 +198,9 @@ __device__ __forceinline__ void nm_dx(const GhipNormGrad &p, size_t row, uint32_
         if (p.gamma) d *= ghip_bf16_f32(g[e]);
         v[e] = a * d - b * ghip_bf16_f32(s[e]);
     }
-    if (p.ds) {
-        const nm_u16x8 in = nm_load(p.ds + row * p.ldds, col, p.D);
+    if (p.ds)
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += ghip_bf16_f32(in[e]);
-    }
+        for (int e = 0; e < 8; e++) v[e] += ghip_bf16_f32(ds[e]);
     nm_store(p.dx + row * p.lddx, col, p.D, nm_pack(v));
 }
 
@@ -234,20 +232,34 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm_grad(GhipNormGrad
         const uint32_t col = 8u * (t + T * i);
         if (p.gamma && col < p.D) g[i] = nm_load(p.gamma, col, p.D);
     }
-    /* every group of a block makes as many rounds (the barriers of nm_sum) */
-    for (size_t first = (size_t)blockIdx.x * PER; first < p.M; first += groups) {
+    /* Every group of a block makes as many rounds (the barriers of nm_sum); rows past the
+     * last are read as it and come to nothing. The next row is on its way while this one
+     * is summed (but for the longest rows, which fill the registers) */
+    constexpr bool AHEAD = V <= 2;
+    constexpr int V1 = AHEAD ? V : 1;
+    nm_u16x8 s[V], dy[V], ds[V], s1[V1], dy1[V1], ds1[V1];
+    float given = 0.0f, given1 = 0.0f;
+    auto load = [&](size_t first, nm_u16x8 (&s)[V], nm_u16x8 (&dy)[V], nm_u16x8 (&ds)[V], float &given) {
         const size_t row = first + threadIdx.x / T, r = row < p.M ? row : p.M - 1;
-        nm_u16x8 s[V], dy[V];
-        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const uint32_t col = 8u * (t + T * i);
             if (col < p.D) {
                 s[i] = nm_load(p.s + r * p.lds, col, p.D);
                 dy[i] = nm_load(p.dy + r * p.lddy, col, p.D);
+                if (p.ds && p.dx) ds[i] = nm_load(p.ds + r * p.ldds, col, p.D);
             }
         }
-        const float given = p.rstd ? p.rstd[r] : 0.0f;
+        if (p.rstd) given = p.rstd[r];
+    };
+    size_t first = (size_t)blockIdx.x * PER;
+    load(first, s, dy, ds, given);
+    for (;;) {
+        const size_t row = first + threadIdx.x / T, next = first + groups;
+        const bool more = next < p.M;
+        if constexpr (AHEAD)
+            if (more) load(next, s1, dy1, ds1, given1);
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < V; i++)
             if (8u * (t + T * i) < p.D) nm_products(p, s[i], dy[i], g[i], sum);
@@ -259,11 +271,24 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm_grad(GhipNormGrad
             for (int i = 0; i < V; i++) {
                 const uint32_t col = 8u * (t + T * i);
                 if (col < p.D) {
-                    if (p.dx) nm_dx(p, row, col, s[i], dy[i], g[i], a, b);
+                    if (p.dx) nm_dx(p, row, col, s[i], dy[i], g[i], ds[i], a, b);
 #pragma unroll
                     for (int e = 0; e < 8; e++) acc[i][e] += ghip_bf16_f32(dy[i][e]) * (ghip_bf16_f32(s[i][e]) * a);
                 }
             }
+        }
+        if (!more) break;
+        first = next;
+        if constexpr (AHEAD) {
+            given = given1;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                s[i] = s1[i];
+                dy[i] = dy1[i];
+                ds[i] = ds1[i];
+            }
+        } else {
+            load(first, s, dy, ds, given);
         }
     }
     if (p.part) {
@@ -297,7 +322,8 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_grad_long(GhipNormGrad p, size
         return;
     }
     for (uint32_t col = 8u * threadIdx.x; col < p.D; col += 8192u)
-        nm_dx(p, row, col, nm_load(s, col, p.D), nm_load(dy, col, p.D), gamma(col), a, b);
+        nm_dx(p, row, col, nm_load(s, col, p.D), nm_load(dy, col, p.D), gamma(col),
+              p.ds ? nm_load(p.ds + row * p.ldds, col, p.D) : nm_u16x8{}, a, b);
 }
 
 __global__ __launch_bounds__(256) void k_rmsnorm_dgamma_long(GhipNormGrad p) {
