@@ -435,11 +435,11 @@ int ghip_mx_rows_fits(int mode, int form, const GhipMxProd *p);
 int ghip_mx_rows_pick(int mode, const GhipMxProd *p, float *us);
 hipError_t ghip_mx_rows_init(uint32_t n_cu);
 /* The tiles of a mode and type (k_mx_gemm.h): the launch's rows and output columns,
- * workgroups a CU holds, LDS, and microseconds of a step on a nearly empty and a full
- * chip and of a round besides. */
+ * workgroups a CU holds, LDS, and microseconds of a step on a nearly empty chip, with
+ * one workgroup a CU where it holds two, and on a full chip, and of a round besides. */
 typedef struct {
     uint32_t bm, bn, occ, lds;
-    float low, full, over;
+    float low, mid, full, over;
     const void *kern;
     void (*launch)(const GhipMxProd *, const GhipEp *, uint32_t, uint32_t, hipStream_t);
 } GhipMxTile;

@@ -7,13 +7,12 @@
 template <int MODE>
 static const GhipMxTile *tiles(int *n) {
     static const GhipMxTile t[] = {
-        mg_tile<MODE, GHIP_BF16, 1, 4, 12, 4, 4>(0.80f, 1.09f, 5.1f),
-        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 4, 6>(0.60f, 0.91f, 4.0f),
-        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 4, 3>(0.57f, 1.64f, 2.8f),
-        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 2, 6>(0.42f, 0.66f, 1.4f),
-        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 2, 3>(0.41f, 1.10f, 0.4f),
-        mg_tile<MODE, GHIP_BF16, 1, 4, 4, 2, 6>(0.34f, 0.87f, 0.0f),
-        mg_tile<MODE, GHIP_BF16, 1, 4, 2, 2, 8>(0.29f, 0.75f, 0.0f),
+        mg_tile<MODE, GHIP_BF16, 1, 4, 12, 4, 4>(0.81f, 0.00f, 1.08f, 5.1f),
+        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 4, 6>(0.60f, 0.00f, 0.90f, 4.1f),
+        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 4, 3>(0.59f, 0.89f, 1.93f, 3.0f),
+        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 2, 3>(0.43f, 0.64f, 1.18f, 0.4f),
+        mg_tile<MODE, GHIP_BF16, 1, 4, 4, 2, 6>(0.36f, 0.54f, 0.90f, 0.0f),
+        mg_tile<MODE, GHIP_BF16, 1, 4, 2, 2, 8>(0.32f, 0.44f, 0.78f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;

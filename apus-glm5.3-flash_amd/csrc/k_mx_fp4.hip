@@ -7,13 +7,11 @@
 template <int MODE>
 static const GhipMxTile *tiles(int *n) {
     static const GhipMxTile t[] = {
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 8, 8, 4>(0.64f, 1.36f, 6.1f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 8, 4, 6>(0.45f, 0.99f, 3.2f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 8, 5>(0.55f, 1.05f, 2.7f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 4, 3>(0.29f, 1.02f, 0.8f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 4, 8>(0.31f, 0.61f, 1.9f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 2, 4, 4>(0.27f, 0.84f, 0.0f),
-        mg_tile<MODE, GHIP_MXFP4, 2, 2, 2, 2, 5>(0.19f, 0.68f, 0.0f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 8, 8, 4>(0.64f, 0.00f, 1.35f, 6.1f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 8, 4, 6>(0.45f, 0.00f, 0.99f, 3.1f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 4, 4, 3>(0.30f, 0.57f, 1.09f, 0.8f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 2, 4, 4>(0.28f, 0.48f, 0.88f, 0.0f),
+        mg_tile<MODE, GHIP_MXFP4, 2, 2, 2, 2, 5>(0.21f, 0.36f, 0.71f, 0.0f),
     };
     *n = sizeof t / sizeof *t;
     return t;

@@ -274,6 +274,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     constexpr uint32_t PER = T::RING / NW;
     constexpr int G = PER >= 1024u * CB * RB ? RB : PER >= 512u * CB * RB ? RB / 2 : PER >= 256u * CB * RB ? RB / 4 : 1;
     static_assert(PER >= 1024u * CB * G && RB % G == 0, "epilogue staging");
+    static_assert(G * (DUAL ? CB : 2 * CB) % 4 == 0, "whole passes over the staged rows");
     constexpr uint32_t RBY = 64u * CB;
     constexpr uint32_t LPR = DUAL ? CB : 2u * CB;
     constexpr int IT = G * (int)LPR / 4, U = IT % 4 == 0 ? 4 : IT % 2 == 0 ? 2 : 1;

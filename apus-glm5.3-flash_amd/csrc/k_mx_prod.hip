@@ -1,6 +1,8 @@
 /*
  * k_mx_prod.hip — which kernel a product with MXFP4 weights takes (gfx950).
  */
+#include <math.h>
+
 #include "ghip_device.h"
 #include "ghip_internal.h"
 
@@ -38,15 +40,19 @@ extern "C" hipError_t ghip_launch_mx_gemm(int mode, int tile, const GhipMxProd *
 }
 
 /* Estimated microseconds of a tile: 3 for the launch, and for each round of the chip
- * its steps and what a round costs besides; steps of a round that does not fill the chip
- * lie between the empty chip's time and the full one's. */
+ * its steps and what a round costs besides. A round that does not fill the chip runs at
+ * a time between the empty chip's and the full one's; where a CU holds two workgroups,
+ * the few that share a CU set the round's time long before all do. */
 static double tile_us(const GhipMxTile *t, const GhipMxProd *p) {
     const double cap = (double)g_mx_ncu * t->occ, rounds = (double)tile_grid(t, p) / cap;
     const double whole = (double)(size_t)rounds, part = rounds - whole;
     const uint32_t k = p->xt == GHIP_BF16 ? 64 : 128;
     const double steps = (double)(((p->K + k - 1) / k + 1) & ~1u);
-    return 3.0 + whole * (steps * t->full + t->over)
-         + (part > 0.0 ? steps * (t->low + (t->full - t->low) * part) + t->over : 0.0);
+    double us = t->low + (t->full - t->low) * part;
+    if (t->occ == 2)
+        us = part <= 0.5 ? t->low + (t->mid - t->low) * 2.0 * part
+                         : t->mid + (t->full - t->mid) * sqrt(2.0 * part - 1.0);
+    return 3.0 + whole * (steps * t->full + t->over) + (part > 0.0 ? steps * us + t->over : 0.0);
 }
 
 extern "C" int ghip_mx_gemm_pick(int mode, const GhipMxProd *p, float *us) {

@@ -303,10 +303,11 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
 }
 
 /* One launchable form: output columns, and microseconds of the launch, of four steps of
- * a wave, of a block besides, and of a KB of a wave's share of x. */
+ * a wave, of a block besides, and of a KB of a wave's share of x; two: how much longer
+ * these are where CUs hold two workgroups. */
 struct MrForm {
     uint32_t cols, nt, ks, red;
-    float base, quad, over, copy;
+    float base, quad, over, copy, two;
     const void *kern;
     void (*launch)(dim3, uint32_t, hipStream_t, const GhipMxProd &, const GhipEp &, uint32_t, uint32_t,
                    uint32_t);
@@ -317,40 +318,40 @@ static void mr_run(dim3 grid, uint32_t lds, hipStream_t st, const GhipMxProd &p,
     hipLaunchKernelGGL((k_mx_rows<XT, NT, KS, MODE>), grid, dim3(MR_WAVES * 64), lds, st, p, ep, blocks, row0, mr);
 }
 template <int XT, int NT, int KS, int MODE>
-static constexpr MrForm mr_form(float base, float quad, float over, float copy) {
-    return {(ghip_ep_dual(MODE) ? 8u : 16u) * NT * (MR_WAVES / KS), NT, KS, MR_WAVES * 256u * NT * 4u, base, quad, over, copy,
+static constexpr MrForm mr_form(float base, float quad, float over, float copy, float two) {
+    return {(ghip_ep_dual(MODE) ? 8u : 16u) * NT * (MR_WAVES / KS), NT, KS, MR_WAVES * 256u * NT * 4u, base, quad, over, copy, two,
             (const void *)k_mx_rows<XT, NT, KS, MODE>, mr_run<XT, NT, KS, MODE>};
 }
 
 static const MrForm mr_linear_bf16[] = {
-    mr_form<GHIP_BF16, 1, 8, GHIP_EP_LINEAR>(2.1f, 0.92f, 0.32f, 0.18f),
-    mr_form<GHIP_BF16, 1, 4, GHIP_EP_LINEAR>(2.3f, 1.01f, 0.21f, 0.14f),
-    mr_form<GHIP_BF16, 2, 8, GHIP_EP_LINEAR>(1.5f, 1.75f, 0.59f, 0.22f),
-    mr_form<GHIP_BF16, 2, 4, GHIP_EP_LINEAR>(1.9f, 1.74f, 0.44f, 0.18f),
+    mr_form<GHIP_BF16, 1, 8, GHIP_EP_LINEAR>(2.0f, 0.92f, 0.31f, 0.19f, 0.95f),
+    mr_form<GHIP_BF16, 1, 4, GHIP_EP_LINEAR>(2.2f, 1.00f, 0.21f, 0.15f, 0.94f),
+    mr_form<GHIP_BF16, 2, 8, GHIP_EP_LINEAR>(1.3f, 1.75f, 0.58f, 0.23f, 0.87f),
+    mr_form<GHIP_BF16, 2, 4, GHIP_EP_LINEAR>(1.9f, 1.73f, 0.45f, 0.18f, 0.88f),
 };
 static const MrForm mr_linear_mxfp8[] = {
-    mr_form<GHIP_MXFP8, 1, 8, GHIP_EP_LINEAR>(2.4f, 0.67f, 0.36f, 0.16f),
-    mr_form<GHIP_MXFP8, 1, 4, GHIP_EP_LINEAR>(2.3f, 0.61f, 0.56f, 0.17f),
-    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_LINEAR>(1.7f, 1.14f, 0.83f, 0.23f),
-    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_LINEAR>(2.0f, 1.05f, 0.95f, 0.21f),
+    mr_form<GHIP_MXFP8, 1, 8, GHIP_EP_LINEAR>(2.5f, 0.65f, 0.36f, 0.16f, 1.00f),
+    mr_form<GHIP_MXFP8, 1, 4, GHIP_EP_LINEAR>(2.3f, 0.61f, 0.56f, 0.17f, 0.94f),
+    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_LINEAR>(1.7f, 1.16f, 0.81f, 0.22f, 0.94f),
+    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_LINEAR>(2.0f, 1.05f, 0.94f, 0.21f, 0.97f),
 };
 static const MrForm mr_linear_mxfp4[] = {
-    mr_form<GHIP_MXFP4, 1, 8, GHIP_EP_LINEAR>(2.6f, 0.39f, 0.50f, 0.22f),
-    mr_form<GHIP_MXFP4, 1, 4, GHIP_EP_LINEAR>(2.6f, 0.66f, 0.37f, 0.13f),
-    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_LINEAR>(1.8f, 0.53f, 1.29f, 0.34f),
-    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_LINEAR>(2.2f, 1.12f, 0.93f, 0.16f),
+    mr_form<GHIP_MXFP4, 1, 8, GHIP_EP_LINEAR>(2.5f, 0.39f, 0.52f, 0.23f, 1.38f),
+    mr_form<GHIP_MXFP4, 1, 4, GHIP_EP_LINEAR>(2.5f, 0.67f, 0.39f, 0.13f, 0.98f),
+    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_LINEAR>(1.8f, 0.54f, 1.25f, 0.35f, 1.51f),
+    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_LINEAR>(2.2f, 1.12f, 0.91f, 0.16f, 0.97f),
 };
 static const MrForm mr_gated_bf16[] = {
-    mr_form<GHIP_BF16, 2, 8, GHIP_EP_GATED>(1.7f, 1.70f, 0.43f, 0.20f),
-    mr_form<GHIP_BF16, 2, 4, GHIP_EP_GATED>(1.9f, 1.86f, 0.19f, 0.17f),
+    mr_form<GHIP_BF16, 2, 8, GHIP_EP_GATED>(1.6f, 1.71f, 0.40f, 0.21f, 0.96f),
+    mr_form<GHIP_BF16, 2, 4, GHIP_EP_GATED>(1.9f, 1.86f, 0.19f, 0.17f, 0.86f),
 };
 static const MrForm mr_gated_mxfp8[] = {
-    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_GATED>(1.8f, 1.53f, 0.55f, 0.18f),
-    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_GATED>(1.7f, 1.40f, 0.87f, 0.17f),
+    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_GATED>(1.8f, 1.51f, 0.55f, 0.18f, 0.91f),
+    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_GATED>(1.7f, 1.40f, 0.87f, 0.17f, 0.90f),
 };
 static const MrForm mr_gated_mxfp4[] = {
-    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_GATED>(1.4f, 0.83f, 1.21f, 0.39f),
-    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_GATED>(2.1f, 1.58f, 0.47f, 0.10f),
+    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_GATED>(1.6f, 0.86f, 1.22f, 0.35f, 1.36f),
+    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_GATED>(2.1f, 1.59f, 0.47f, 0.09f, 0.94f),
 };
 static const MrForm *mr_forms(int mode, int xt, int *n) {
     const bool dual = mode == GHIP_EP_GATED;
@@ -391,7 +392,8 @@ static MrPlan plan(const MrForm *c, const GhipMxProd *p) {
     /* the rounds of the chip, or the weights at 6.5 TB/s, and a tenth of the other */
     const double quads = (double)((((nst + 1) / 2 + c->ks - 1) / c->ks + 1) / 2);
     const double rounds = (double)(((size_t)r.grid * r.tiles + g_mr_ncu * occ - 1) / (g_mr_ncu * occ));
-    const double chain = c->base + rounds * (r.turns * (quads * c->quad + c->over) + (double)(r.mr * row) / MR_WAVES / 1024.0 * c->copy);
+    const double two = (size_t)r.grid * r.tiles > g_mr_ncu ? c->two : 1.0;
+    const double chain = c->base + two * rounds * (r.turns * (quads * c->quad + c->over) + (double)(r.mr * row) / MR_WAVES / 1024.0 * c->copy);
     const double hbm = 2.6 + (double)p->N * p->K * (p->w2 ? 2 : 1) * 17.0 / 32.0 / 6.5e6;
     r.us = (float)(chain > hbm ? chain + 0.1 * hbm : hbm + 0.1 * chain);
     return r;

@@ -14,9 +14,9 @@ static void mg_run(const GhipMxProd *p, const GhipEp *ep, uint32_t mt, uint32_t 
 }
 
 template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
-static constexpr GhipMxTile mg_tile(float low, float full, float over) {
+static constexpr GhipMxTile mg_tile(float low, float mid, float full, float over) {
     using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
-    return {T::BM, T::OUTN, T::RING <= FG_LDS_MAX / 2 ? 2u : 1u, T::RING, low, full, over,
+    return {T::BM, T::OUTN, T::RING <= FG_LDS_MAX / 2 ? 2u : 1u, T::RING, low, mid, full, over,
             (const void *)k_mx_gemm<MODE, XT, WM, WN, RB, CB, R>, mg_run<MODE, XT, WM, WN, RB, CB, R>};
 }
 
