@@ -37,12 +37,15 @@ FG_ADDR uint32_t mg_cut(uint32_t off, uint32_t byte, int32_t left) {
     return (int32_t)byte >= left ? FG_OOB : off;
 }
 
-/* Word e of a step's scales in LDS: rows of x, then of W (dual: the gate's, then the up
- * projection's). Returns W's row of the tile. */
-FG_ADDR uint32_t mg_scale_row(uint32_t e, uint32_t BM, uint32_t BN, bool dual, bool &second) {
-    const uint32_t c = e - BM;
-    second = dual && c >= BN / 2u;
-    return second ? c - BN / 2u : c;
+/* Byte offset of word `word` of the scales of a row; past every buffer behind the row's
+ * `words`. */
+FG_ADDR uint32_t mg_scale(uint32_t row, uint32_t word, uint32_t words) {
+    return word < words ? row * (4u * words) + 4u * word : FG_OOB;
+}
+/* Where a lane reads from the scales in LDS, 16 bytes a row: quads of 16-row blocks from
+ * block `first` on of the matrix that begins at unit `unit` of 64 rows. */
+FG_ADDR uint32_t mg_scale_at(uint32_t unit, uint32_t first, uint32_t blocks, uint32_t lane) {
+    return 1024u * unit + 16u * (16u * first + (blocks < 4u ? lane & (16u * blocks - 1u) : lane));
 }
 
 /* Operand reads, from the slot's start: x's half h of block r of 16 rows (MXFP8: k 16 g
@@ -64,15 +67,6 @@ FG_ADDR uint32_t mg_at_w(uint32_t ast, uint32_t wc, uint32_t n, uint32_t g, bool
 template <uint32_t WB>
 FG_ADDR constexpr uint32_t mg_w_step(uint32_t c, bool dual) {
     return WB == 64u ? c * 1024u : dual ? 512u * ((c & 1u) * 2u + ((c >> 1) & 1u) + (c >> 2) * 4u) : c * 512u;
-}
-/* Scales: byte `byte` of a row's word. */
-FG_ADDR uint32_t mg_at_sx(uint32_t base, uint32_t first, uint32_t n) { return base + 4u * (16u * first + n); }
-FG_ADDR uint32_t mg_at_sw(uint32_t base, uint32_t BM, uint32_t first, uint32_t n, bool dual) {
-    return base + 4u * (BM + (dual ? 8u : 16u) * first + n);
-}
-/* ... and of block c behind the first. */
-FG_ADDR constexpr uint32_t mg_sw_step(uint32_t c, uint32_t BN, bool dual) {
-    return dual ? 64u * (c >> 1) + (c & 1u) * 2u * BN : 64u * c;
 }
 
 #endif /* K_MX_ADDR_H */

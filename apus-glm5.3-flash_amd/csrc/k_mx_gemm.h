@@ -10,35 +10,66 @@
 
 typedef int mg_i32x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ void mg_dma4(const void *src, void *lds_wave) {
-    __builtin_amdgcn_global_load_lds((ghip_glb_t *)src, (ghip_lds_t *)lds_wave, 4, 0, 0);
-}
-
-/* acc += w (16 rows of MXFP4) . x^T over 128 k, in place; sw, sx: the blocks' scales
- * in the low byte. As fg_mfma the compiler knows no MFMA in it. */
+/* acc += w (16 rows of MXFP4) . x^T over 128 k, in place; byte Q of sw and sx: the
+ * blocks' scales. As fg_mfma the compiler knows no MFMA in it. */
+template <int Q>
 __device__ __forceinline__ void mg_mfma(ghip_f32x4 &acc, const ghip_u32x4 &w, const mg_i32x8 &x, uint32_t sw,
                                         uint32_t sx) {
-    asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4"
-        : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0] cbsz:4"
+        : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx), "n"(Q & 1), "n"(Q >> 1));
+#endif
 }
+template <int Q>
 __device__ __forceinline__ void mg_mfma(ghip_f32x4 &acc, const ghip_u32x4 &w, const ghip_u32x4 &x, uint32_t sw,
                                         uint32_t sx) {
-    asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
-        : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx));
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%5,%5,0] op_sel_hi:[%6,%6,0] cbsz:4 blgp:4"
+        : "+a"(acc) : "v"(w), "v"(x), "v"(sw), "v"(sx), "n"(Q & 1), "n"(Q >> 1));
+#endif
+}
+
+/* 4 words of 4 bytes in each of 64 lanes, lane (n, b) a row of scales of block b of 16
+ * rows: out[b] of lane (n, g) is byte g of the words of block b's row n. */
+__device__ __forceinline__ ghip_u32x4 mg_turn(const ghip_u32x4 &v) {
+    const uint32_t lo01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400u), hi01 = __builtin_amdgcn_perm(v[1], v[0], 0x07030602u);
+    const uint32_t lo23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400u), hi23 = __builtin_amdgcn_perm(v[3], v[2], 0x07030602u);
+    /* byte g of the words, then bytes against lane groups */
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_amdgcn_perm(lo23, lo01, 0x05040100u), __builtin_amdgcn_perm(lo23, lo01, 0x07060302u), false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(__builtin_amdgcn_perm(hi23, hi01, 0x05040100u), __builtin_amdgcn_perm(hi23, hi01, 0x07060302u), false, false);
+    const auto e = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false);
+    const auto o = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+    return (ghip_u32x4){e[0], o[0], e[1], o[1]};
+}
+
+/* Whether one of the n steps before one of quarter qu is of quarter 2, steps before the
+ * first among them: n up to 4, so at most one is. */
+constexpr int mg_third(int qu, int n) {
+    int c = 0;
+    for (int i = 1; i <= (n < 4 ? n : 4); i++) c += (qu + 8 - i) % 4 == 2;
+    return c;
+}
+template <int N>
+__device__ __forceinline__ void mg_wait() {
+    constexpr int M = N < 63 ? N : 63;
+    GHIP_VMCNT(M);
 }
 
 template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
 struct MgTile {
     static constexpr bool DUAL = ghip_ep_dual(MODE), BF = XT == GHIP_BF16;
     static constexpr uint32_t NW = WM * WN, BM = 16u * RB * WM, BN = 16u * CB * WN, OUTN = DUAL ? BN / 2 : BN;
-    /* a step: k, bytes of a row of x and of W, words of scales */
+    /* a step: k, bytes of a row of x and of W */
     static constexpr uint32_t KS = BF ? 64u : 128u, XB = XT == GHIP_MXFP4 ? 64u : 128u, WB = BF ? 32u : 64u;
-    static constexpr uint32_t SBM = BF ? 0u : BM, NSL = (SBM + BN + 64u * NW - 1u) / (64u * NW);
-    static constexpr uint32_t AST = BM * XB, BST = BN * WB, SST = NSL * NW * 256u;
-    static constexpr uint32_t SLOT = AST + BST + SST, RING = R * SLOT;
-    static constexpr uint32_t NAL = AST / 1024u / NW, NBL = BST / 1024u / NW, LPS = NAL + NBL + NSL;
+    static constexpr uint32_t AST = BM * XB, BST = BN * WB;
+    static constexpr uint32_t SLOT = AST + BST, RING = R * SLOT;
+    static constexpr uint32_t NAL = AST / 1024u / NW, NBL = BST / 1024u / NW, LPS = NAL + NBL;
+    /* scales of four words of k, 16 bytes a row: x's rows, W's, the second matrix's, each
+     * in units of 64 rows */
+    static constexpr uint32_t XU = BF ? 0u : (BM + 63u) / 64u, WU = (OUTN + 63u) / 64u, NU = XU + WU * (DUAL ? 2u : 1u);
+    static constexpr uint32_t NSL = (NU + NW - 1u) / NW, LDS = RING + NU * 1024u;
     static_assert(AST % (1024u * NW) == 0 && BST % (1024u * NW) == 0, "whole loads");
-    static_assert(RING <= FG_LDS_MAX && R >= 2 && (R - 2) * LPS <= 63, "ring, waits");
+    static_assert(LDS <= FG_LDS_MAX && R >= 2 && (R - 2) * LPS <= 63, "ring, waits");
     static_assert(!DUAL || CB % 2 == 0, "gate and up blocks alternate");
 };
 
@@ -48,7 +79,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
     constexpr bool DUAL = T::DUAL, BF = T::BF;
     constexpr uint32_t NW = T::NW, BM = T::BM, BN = T::BN, OUTN = T::OUTN, XB = T::XB, WB = T::WB, KS = T::KS;
-    constexpr uint32_t NAL = T::NAL, NBL = T::NBL, NSL = T::NSL, LPS = T::LPS, SLOT = T::SLOT;
+    constexpr uint32_t NAL = T::NAL, NBL = T::NBL, LPS = T::LPS, SLOT = T::SLOT;
     constexpr int NM = RB * CB;
     extern __shared__ __attribute__((aligned(1024))) uint8_t mg_lds[];
     const uint32_t tid = threadIdx.x, lane = tid & 63u;
@@ -78,27 +109,15 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     const uint32_t br = mg_row<WB>(DUAL ? wv >> 1 : wv, lane), bq = mg_byte<WB>(lane, br), bo = br * wb + bq;
     const uint32_t astep = mg_rows_apart<XB, NW>(false) * xld, bstep = mg_rows_apart<WB, NW>(DUAL) * wb;
     const uint32_t xrow = BF ? 2u * p.K : XT == GHIP_MXFP8 ? p.K : wb;   /* bytes of x's row */
-    const uint8_t *ps[NSL];
-#pragma unroll
-    for (uint32_t i = 0; i < NSL; i++) {
-        const uint32_t e = (wv + NW * i) * 64u + lane;
-        bool second;
-        const uint32_t c = mg_scale_row(e, T::SBM, BN, DUAL, second);
-        ps[i] = e < T::SBM ? p.xs + (size_t)min(row0 + e, p.M - 1u) * lds
-                       : (second ? p.ws2 : p.ws) + (size_t)min(col0 + c, p.N - 1u) * lds;
-    }
     uint32_t jl = 0, sl = 0;                             /* the next step to load, its slot */
     int32_t xleft = (int32_t)xrow, wleft = (int32_t)wb;
     auto load = [&](uint32_t i) {
         if (i < NAL) {
             const uint32_t off = mg_cut(ao + i * astep, aq, xleft);
             fg_dma16(pa, aspan, off, mg_lds + sl + (wv + NW * i) * 1024u);
-        } else if (i < NAL + NBL) {
+        } else {
             const uint32_t off = mg_cut(bo + (i - NAL) * bstep, bq, wleft);
             fg_dma16(pb, bspan, off, mg_lds + sl + T::AST + (wv + NW * (i - NAL)) * 1024u);
-        } else {
-            const uint32_t k = i - NAL - NBL;
-            mg_dma4(ps[k] + 4u * min(BF ? jl >> 1 : jl, words - 1u), mg_lds + sl + T::AST + T::BST + (wv + NW * k) * 256u);
         }
     };
     auto next_load = [&]() {
@@ -118,12 +137,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     XReg xa[RB], xl[2];
     WReg wa[2][CB];
     ghip_u32x2 codes[BF ? CB : 1];
-    uint32_t sx[RB], sl_[2], sw[2][CB];
-    constexpr uint32_t SC = T::AST + T::BST;
     const uint32_t a0 = mg_at_x<XB>(wr * RB, n, g, 0, BF), a1 = mg_at_x<XB>(wr * RB, n, g, 1, BF);
     const uint32_t b0 = mg_at_w<WB, CB>(T::AST, wc, n, g, DUAL);
-    const uint32_t as = mg_at_sx(SC, wr * RB, n) + g, bs = mg_at_sw(SC, T::SBM, wc * CB, n, DUAL) + (BF ? g >> 1 : g);
-    auto read_x = [&](XReg &x, uint32_t &s, int r, const uint8_t *st) {
+    auto read_x = [&](XReg &x, int r, const uint8_t *st) {
         const ghip_u32x4 lo = *(const ghip_u32x4 *)(st + a0 + r * (16u * XB));
         if constexpr (XB == 128u) {
             const ghip_u32x4 hi = *(const ghip_u32x4 *)(st + a1 + r * (16u * XB));
@@ -131,32 +147,97 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
         } else {
             x = lo;
         }
-        if constexpr (!BF) s = st[as + 64u * r];
     };
     auto read_a = [&](auto set_c, auto r_c, const uint8_t *st) {
         constexpr int S = decltype(set_c)::value, r = decltype(r_c)::value;
-        if constexpr (r == RB - 1) read_x(xl[S], sl_[S], r, st);
-        else read_x(xa[r], sx[r], r, st);
+        if constexpr (r == RB - 1) read_x(xl[S], r, st);
+        else read_x(xa[r], r, st);
     };
-    /* beside BF16: steps start in pairs, so that set S has bytes 2 S and 2 S + 1 of the word */
     auto read_b = [&](auto set_c, auto c_c, const uint8_t *st) {
         constexpr int S = decltype(set_c)::value, c = decltype(c_c)::value;
         if constexpr (BF) codes[c] = *(const ghip_u32x2 *)(st + b0 + mg_w_step<WB>(c, DUAL));
         else wa[S][c] = *(const ghip_u32x4 *)(st + b0 + mg_w_step<WB>(c, DUAL));
-        sw[S][c] = st[bs + mg_sw_step(c, BN, DUAL) + (BF ? 2 * S : 0)];
     };
-    /* BF16: half h of W's block c of the next step; past: its k is past K, where the codes
-     * are zeros and the scale is any byte */
-    auto dequant = [&](auto set_c, auto c_c, auto h_c, bool past) {
+
+    /* Scales. The workgroup's waves share out its rows, 64 a load: 16 bytes of a row, the
+     * scales of four steps (eight of 64 k), go through registers to LDS four steps behind
+     * their load. From there a wave reads its blocks', four at a time, and turns them
+     * (mg_turn) into words that the MFMA picks a step's byte from by number. Each of the
+     * simpler ways costs more than a small tile's step: 4 bytes a row every step, as the
+     * line is in flight already and the loads wait for it one after the other (64 x 64
+     * tiles, 4096 x 4096 x 4096: 193 us, 93 with no scales at all); every wave its own
+     * blocks', as the waves of a row of tiles ask for the same lines */
+    constexpr uint32_t NSL = T::NSL, XU = T::XU, WU = T::WU, NU = T::NU;
+    constexpr int XQ = BF ? 0 : (RB + 3) / 4, WQ = DUAL ? (CB / 2 + 3) / 4 : (CB + 3) / 4, NQD = XQ + WQ * (DUAL ? 2 : 1);
+    constexpr int GS = BF ? 8 : 4, WB16 = DUAL ? CB / 2 : CB;
+    uint8_t *const sc = mg_lds + T::RING;
+    ghip_u32x4 next[NSL], raw[NQD], cur[NQD];
+    uint32_t sw[BF ? 2 * CB : 1];
+    auto scale_load = [&](uint32_t word) {
+        fg_each<NSL>([&](auto i_c) {
+            constexpr uint32_t i = decltype(i_c)::value;
+            const uint32_t u = wv + NW * i, first = u < XU ? 0u : u < XU + WU ? XU : XU + WU;
+            const uint8_t *const s = u < XU ? p.xs : !DUAL || u < XU + WU ? p.ws : p.ws2;
+            const uint32_t base = u < XU ? row0 : col0, live = u < XU ? rows : u < NU ? cols : 0u;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)(s + (size_t)base * lds), 0, live * lds, 0x20000);
+            const uint32_t row = 64u * (u - first) + lane;
+            if (word + 4u <= words) {
+                next[i] = __builtin_amdgcn_raw_buffer_load_b128(r, mg_scale(row, word, words), 0, 0);
+            } else {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; e++) next[i][e] = __builtin_amdgcn_raw_buffer_load_b32(r, mg_scale(row, word + e, words), 0, 0);
+            }
+        });
+    };
+    auto scale_store = [&]() {
+        fg_each<NSL>([&](auto i_c) {
+            constexpr uint32_t i = decltype(i_c)::value;
+            const uint32_t u = wv + NW * i;
+            if (NU % NW == 0 || u < NU) *(ghip_u32x4 *)(sc + 1024u * u + 16u * lane) = next[i];
+        });
+    };
+    /* quad q of a wave's blocks: x's, W's, the second matrix's; of two or one, lanes
+     * behind these read the same rows again */
+    const uint32_t scx = mg_scale_at(0u, wr * RB, RB, lane), scw = mg_scale_at(XU, wc * WB16, WB16, lane);
+    auto scale_read = [&](auto q_c) {
+        constexpr int q = decltype(q_c)::value;
+        constexpr uint32_t at = q < XQ ? 1024u * q : q < XQ + WQ ? 1024u * (q - XQ) : 1024u * (q - XQ - WQ + WU);
+        raw[q] = *(const ghip_u32x4 *)(sc + (q < XQ ? scx : scw) + at);
+    };
+    auto scale_turn = [&](auto q_c) { raw[decltype(q_c)::value] = mg_turn(raw[decltype(q_c)::value]); };
+    /* BF16: a row's steps take half a word each; sw[c] has the even ones' scales (lane
+     * groups 0 and 1 block 0 of the word, 2 and 3 block 1), sw[CB + c] the odd ones' */
+    auto sx_of = [&](auto r_c) { constexpr int r = decltype(r_c)::value; return cur[r / 4][r % 4]; };
+    auto sw_of = [&](auto c_c) {
+        constexpr int c = decltype(c_c)::value, i = DUAL ? c >> 1 : c;
+        return cur[XQ + (DUAL && (c & 1) ? WQ : 0) + i / 4][i % 4];
+    };
+    auto scale_take = [&]() {
+        fg_each<NQD>([&](auto q) { cur[decltype(q)::value] = raw[decltype(q)::value]; });
+        if constexpr (BF)
+            fg_each<CB>([&](auto c) {
+                const uint32_t v = sw_of(c);
+                const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const auto q = __builtin_amdgcn_permlane16_swap(h[e], h[e], false, false);
+                    sw[e * CB + decltype(c)::value] = g & 2u ? q[1] : q[0];
+                }
+            });
+    };
+    /* BF16: half h of W's block c of step j, of set S; past: its k is past K, where the
+     * codes are zeros and the scale is any byte */
+    auto dequant = [&](auto set_c, auto c_c, auto h_c, uint32_t j, bool past) {
         if constexpr (BF) {
             constexpr int S = decltype(set_c)::value, c = decltype(c_c)::value, h = decltype(h_c)::value;
-            const ghip_u32x4 d = mx_fp4_bf16(codes[c][h], past ? 1.0f : __uint_as_float(sw[S][c] << 23));
+            const uint32_t b = sw[S * CB + c] >> (8u * ((j >> 1) & 3u)) & 255u;
+            const ghip_u32x4 d = mx_fp4_bf16(codes[c][h], past ? 1.0f : __uint_as_float(b << 23));
 #pragma unroll
             for (int e = 0; e < 4; e++) wa[S][c][4 * h + e] = (int)d[e];
         }
     };
     /* The step that K cuts: its blocks past K have any scale. A step past K (an odd
-     * number of them) has zeros for codes, and the last one's scales */
+     * number of them) has zeros for codes and scales */
     const uint32_t nb = p.K >> 5, rem = nb & 3u;
     ghip_f32x4 acc[RB][CB];
 #pragma unroll
@@ -167,6 +248,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     using S0 = std::integral_constant<int, 0>;
     using S1 = std::integral_constant<int, 1>;
     const uint32_t all = (nst + 1u) & ~1u;               /* steps, in pairs */
+    scale_load(0u);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (uint32_t j = 0; j < (uint32_t)R; j++)
         if (j < all) {
@@ -175,58 +258,75 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
             next_load();
         }
     ghip_wait_stages<LPS, R - 1>(min(all, (uint32_t)R) - 1u);
+    scale_store();
+    __builtin_amdgcn_sched_barrier(0);
+    scale_load(4u);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
+    fg_each<NQD>(scale_read);
+    fg_each<NQD>(scale_turn);
+    scale_take();
     fg_each<CB>([&](auto c) { read_b(S0{}, c, mg_lds); });
     fg_each<RB>([&](auto r) { read_a(S0{}, r, mg_lds); });
     if constexpr (BF)
         fg_each<2 * CB>([&](auto q) {
             constexpr int Q = decltype(q)::value;
-            dequant(S0{}, std::integral_constant<int, Q / 2>{}, std::integral_constant<int, Q % 2>{}, g >= 2u * nb);
+            dequant(S0{}, std::integral_constant<int, Q / 2>{}, std::integral_constant<int, Q % 2>{}, 0u, (g >> 1) >= nb);
         });
 
     uint32_t rs = 0;                                     /* slot of step j */
-    auto step = [&](uint32_t j, auto set_c, auto main_c) {
-        constexpr int S = decltype(set_c)::value;
+    auto step = [&](uint32_t j, auto quarter_c, auto main_c) {
+        constexpr int QU = decltype(quarter_c)::value, S = QU & 1;
         constexpr bool MAIN = decltype(main_c)::value;
-        const bool more = MAIN || j + 1u < all;
-        /* own loads of step j + 1 done, own reads of step j done; after the barrier that
-         * holds for every wave */
-        if (MAIN) GHIP_VMCNT((R - 2) * LPS);
+        const bool more = MAIN || j + 1u < all, loads = MAIN || j + R < all;
+        /* own loads of step j + 1 done, own reads of step j done; after the barrier that holds
+         * for every wave. Behind them are those of R - 2 steps, and scales where one of these
+         * loaded some (fewer are assumed where that is not known: a longer wait) */
+        if (MAIN) mg_wait<(R - 2) * LPS + (BF ? 0 : NSL * mg_third(QU, R - 2))>();
         else ghip_wait_stages<LPS, R - 2>(more ? all - 2u - j : 0u);
         __builtin_amdgcn_s_waitcnt(0xc07f);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!MAIN && !BF)
             if (rem && j + 1u >= nst && g >= rem) {
-                fg_each<RB - 1>([&](auto r) { sx[decltype(r)::value] = 127u; });
-                sl_[S] = 127u;
-                fg_each<CB>([&](auto c) { sw[S][decltype(c)::value] = 127u; });
+                fg_each<NQD>([&](auto q) { cur[decltype(q)::value] = (ghip_u32x4){0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu}; });
                 asm volatile("s_nop 3");                 /* VALU to MFMA */
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        /* the next scales: to LDS in a third step, from there in the fourth */
+        const bool scales = !BF || (j & 4u);
+        if constexpr (QU == 2)
+            if (scales) {
+                scale_store();
+                __builtin_amdgcn_sched_barrier(0);
+                scale_load(4u * (j / GS + 2u));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        if constexpr (QU == 3)
+            if (scales) {
+                fg_each<NQD>(scale_read);
                 __builtin_amdgcn_sched_barrier(0);
             }
         const uint32_t ns = !more ? rs : rs == (R - 1u) * SLOT ? 0u : rs + SLOT;
         const uint8_t *st = mg_lds + ns;
         using NS = std::integral_constant<int, S ^ 1>;
         const bool past = !MAIN && 2u * (j + 1u) + (g >> 1) >= nb;
-        constexpr int NL = MAIN ? (int)LPS : 0, CU = CB + 1;
+        constexpr int NL = (int)LPS, CU = CB + 1, TE = BF ? NM / 2 : NM;
         fg_each<NM>([&](auto slot) {
             constexpr int I = decltype(slot)::value, Rr = I / CB, K = I % CB;
             constexpr int C = Rr & 1 ? CB - 1 - K : K;
-            auto mma = [&](const XReg &x, uint32_t s) {
-                if constexpr (BF) {
-                    const auto half = [](const mg_i32x8 &v, auto h) {
-                        constexpr int H = 4 * decltype(h)::value;
-                        return __builtin_bit_cast(ghip_bf16x8, __builtin_shufflevector(v, v, H, H + 1, H + 2, H + 3));
-                    };
-                    fg_mfma(acc[Rr][C], half(wa[S][C], S0{}), half(x, S0{}));
-                    fg_mfma(acc[Rr][C], half(wa[S][C], S1{}), half(x, S1{}));
-                } else {
-                    mg_mfma(acc[Rr][C], wa[S][C], x, sw[S][C], s);
-                }
-            };
-            if constexpr (Rr == RB - 1) mma(xl[S], sl_[S]);
-            else mma(xa[Rr], sx[Rr]);
+            const XReg &x = Rr == RB - 1 ? xl[S] : xa[Rr];
+            if constexpr (BF) {
+                const auto half = [](const mg_i32x8 &v, auto h) {
+                    constexpr int H = 4 * decltype(h)::value;
+                    return __builtin_bit_cast(ghip_bf16x8, __builtin_shufflevector(v, v, H, H + 1, H + 2, H + 3));
+                };
+                fg_mfma(acc[Rr][C], half(wa[S][C], S0{}), half(x, S0{}));
+                fg_mfma(acc[Rr][C], half(wa[S][C], S1{}), half(x, S1{}));
+            } else {
+                mg_mfma<QU>(acc[Rr][C], wa[S][C], x, sw_of(std::integral_constant<int, C>{}), sx_of(std::integral_constant<int, Rr>{}));
+            }
             /* W and x's last block over the first RB - 1 rows (codes for BF16 over the first
              * third, dequantized behind), x's others behind their own */
             constexpr int BE = BF ? NM / 3 : NM - CB, NQ = BF ? 2 * CB : 0;
@@ -238,34 +338,33 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
                 if constexpr (O < CB) read_b(NS{}, std::integral_constant<int, O>{}, st);
                 else read_a(NS{}, std::integral_constant<int, RB - 1>{}, st);
             });
+            constexpr int T0 = QU == 3 ? fg_spread(NQD, I, TE / 4, TE) : 0, T1 = QU == 3 ? fg_spread(NQD, I + 1, TE / 4, TE) : 0;
+            if constexpr (T1 > T0)
+                if (scales) {
+                    fg_each<T1 - T0>([&](auto k) { scale_turn(std::integral_constant<int, T0 + decltype(k)::value>{}); });
+                    if constexpr (BF && T1 == NQD) scale_take();   /* all of this step's are used up */
+                }
             fg_each<Q1 - Q0>([&](auto k) {
                 constexpr int Q = Q0 + decltype(k)::value;
-                dequant(NS{}, std::integral_constant<int, Q / 2>{}, std::integral_constant<int, Q % 2>{}, past);
+                dequant(NS{}, std::integral_constant<int, Q / 2>{}, std::integral_constant<int, Q % 2>{}, j + 1u, past);
             });
             constexpr bool A = Rr > 0 && K == 0;
             if constexpr (A) read_a(NS{}, std::integral_constant<int, Rr - 1>{}, st);
-            fg_each<L1 - L0>([&](auto k) { load(L0 + decltype(k)::value); });
-            if constexpr (A || B1 > B0 || Q1 > Q0 || L1 > L0) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (L1 > L0)
+                if (loads) fg_each<L1 - L0>([&](auto k) { load(L0 + decltype(k)::value); });
+            if constexpr (A || B1 > B0 || Q1 > Q0 || L1 > L0 || T1 > T0) __builtin_amdgcn_sched_barrier(0);
         });
-        if constexpr (MAIN) next_load();
+        if constexpr (!BF && QU == 3) scale_take();
+        if (loads) next_load();
         __builtin_amdgcn_sched_barrier(0);
         rs = ns;
     };
     uint32_t j = 0;
-    for (; j + R + 1u < all; j += 2u) {
-        step(j, S0{}, std::true_type{});
-        step(j + 1u, S1{}, std::true_type{});
-    }
-    if constexpr (R & 1)                                 /* one more to load */
-        if (j + R < all) {
-            step(j, S0{}, std::true_type{});
-            step(j + 1u, S1{}, std::false_type{});
-            j += 2u;
-        }
-    for (; j < all; j += 2u) {
-        step(j, S0{}, std::false_type{});
-        step(j + 1u, S1{}, std::false_type{});
-    }
+    for (; j + 3u + R < all; j += 4u) fg_each<4>([&](auto q) { step(j + decltype(q)::value, q, std::true_type{}); });
+    for (; j < all; j += 4u)
+        fg_each<4>([&](auto q) {
+            if (j + decltype(q)::value < all) step(j + decltype(q)::value, q, std::false_type{});
+        });
     fg_settle(acc);
 
     /* the sums through LDS, 8 columns of a row a lane (as k_ffn_gemm.h) */

@@ -9,14 +9,14 @@
 template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
 static void mg_run(const GhipMxProd *p, const GhipEp *ep, uint32_t mt, uint32_t nt, hipStream_t st) {
     using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
-    hipLaunchKernelGGL((k_mx_gemm<MODE, XT, WM, WN, RB, CB, R>), dim3(mt * nt), dim3(64 * WM * WN), T::RING, st,
+    hipLaunchKernelGGL((k_mx_gemm<MODE, XT, WM, WN, RB, CB, R>), dim3(mt * nt), dim3(64 * WM * WN), T::LDS, st,
                        *p, *ep, mt, nt);
 }
 
 template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
 static constexpr GhipMxTile mg_tile(float low, float mid, float full, float over) {
     using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
-    return {T::BM, T::OUTN, T::RING <= FG_LDS_MAX / 2 ? 2u : 1u, T::RING, low, mid, full, over,
+    return {T::BM, T::OUTN, T::LDS <= FG_LDS_MAX / 2 ? 2u : 1u, T::LDS, low, mid, full, over,
             (const void *)k_mx_gemm<MODE, XT, WM, WN, RB, CB, R>, mg_run<MODE, XT, WM, WN, RB, CB, R>};
 }
 

@@ -28,8 +28,8 @@ enum { BF16, MXFP8, MXFP4 };
 template <int XT, bool DUAL, uint32_t WM, uint32_t WN, uint32_t RB, uint32_t CB>
 static void tile(uint32_t rows, uint32_t cols, uint32_t K, uint32_t xld) {
     constexpr uint32_t NW = WM * WN, BM = 16 * RB * WM, BN = 16 * CB * WN;
-    constexpr uint32_t XB = XT == MXFP4 ? 64 : 128, WB = XT == BF16 ? 32 : 64, KS = XT == BF16 ? 64 : 128, SBM = XT == BF16 ? 0 : BM;
-    const uint32_t nst = (K + KS - 1) / KS, all = (nst + 1) & ~1u, wb = K / 2, xrow = XT == BF16 ? 2 * K : XT == MXFP8 ? K : wb;
+    constexpr uint32_t XB = XT == MXFP4 ? 64 : 128, WB = XT == BF16 ? 32 : 64, KS = XT == BF16 ? 64 : 128;
+    const uint32_t words = (K + 127) / 128, nst = (K + KS - 1) / KS, all = (nst + 1) & ~1u, wb = K / 2, xrow = XT == BF16 ? 2 * K : XT == MXFP8 ? K : wb;
     for (uint32_t j = 0; j < all; j++) {
         if (j > 2 && j + 3 < all) continue;
         std::vector<Piece> x(BM * XB / 16, Piece{NOTHING, 0, 0}), w(BN * WB / 16, Piece{NOTHING, 0, 0});
@@ -65,6 +65,42 @@ static void tile(uint32_t rows, uint32_t cols, uint32_t K, uint32_t xld) {
                     }
                 }
             }
+        /* scales: every word of a row, none of another's, past the last row past the span;
+         * each unit of 64 rows once, and each block of a wave from its rows */
+        if (j == 0) {
+            constexpr uint32_t OUT = BN / (DUAL ? 2 : 1), XU = XT == BF16 ? 0 : (BM + 63) / 64, WU = (OUT + 63) / 64, NU = XU + WU * (DUAL ? 2 : 1);
+            std::vector<Piece> sc(64 * NU, Piece{NOTHING, 0, 0});
+            for (uint32_t u = 0; u < NU; u++)
+                for (uint32_t lane = 0; lane < 64; lane++) {
+                    const int mat = u < XU ? 0 : u < XU + WU ? 1 : 2;
+                    const uint32_t row = 64 * (mat == 0 ? u : mat == 1 ? u - XU : u - XU - WU) + lane, live = mat ? cols : rows, span = live * 4 * words;
+                    sc[64 * u + lane] = row < live ? Piece{mat, (int)row, 0} : Piece{ZERO, 0, 0};
+                    for (uint32_t word = 0; word < words + 4; word++) {
+                        const uint32_t off = mg_scale(row, word, words);
+                        if (word < words && row < live) EXPECT(off + 4 <= span && off == (row * words + word) * 4, "scale of row %u, word %u at %u", row, word, off);
+                        else EXPECT(off >= span, "scale of row %u, word %u at %u of %u", row, word, off, span);
+                        if (word + 4 <= words && row < live) EXPECT(off + 16 <= span, "scales of row %u, word %u at %u", row, word, off);
+                    }
+                }
+            constexpr uint32_t WBL = DUAL ? CB / 2 : CB;
+            for (uint32_t wv = 0; wv < NW; wv++)
+                for (int mat = XT == BF16; mat < (DUAL ? 3 : 2); mat++)
+                    for (uint32_t b = 0; b < (mat ? WBL : RB); b++)
+                        for (uint32_t n = 0; n < 16; n++) {
+                            const uint32_t wr = wv / WN, wc = wv % WN, first = mat ? wc * WBL : wr * RB, nb = mat ? WBL : RB, live = mat ? cols : rows;
+                            const uint32_t at = mg_scale_at(mat ? XU : 0, first, nb, 16 * (b & 3) + n) + 1024 * (b / 4) + (mat == 2 ? 1024 * WU : 0);
+                            const uint32_t row = 16 * (first + b) + n;
+                            EXPECT(at % 16 == 0 && at < 1024 * NU, "scales read at %u", at);
+                            const Piece &q = sc[at / 16];
+                            if (row < live) EXPECT(q.mat == mat && q.row == (int)row, "scales of matrix %d row %u: %d, %d", mat, row, q.mat, q.row);
+                            else EXPECT(q.mat == ZERO, "scales of matrix %d row %u are not zero", mat, row);
+                        }
+            for (uint32_t lane = 0; lane < 64; lane++)
+                for (uint32_t wv = 0; wv < NW; wv++) {
+                    EXPECT(mg_scale_at(0, wv / WN * RB, RB, lane) + 16 <= 1024 * NU || XT == BF16, "x's scales of lane %u", lane);
+                    EXPECT(mg_scale_at(XU, wv % WN * WBL, WBL, lane) + 1024 * ((WBL - 1) / 4) + 16 <= 1024 * (XU + WU), "W's scales of lane %u", lane);
+                }
+        }
         /* operand reads */
         auto check = [&](const char *what, const Piece &p, int mat, uint32_t row, uint32_t live, uint32_t byte, int64_t left) {
             if (row >= live || (int64_t)byte >= left) EXPECT(p.mat == ZERO, "%s: row %u byte %u is not zero", what, row, byte);
@@ -81,8 +117,6 @@ static void tile(uint32_t rows, uint32_t cols, uint32_t K, uint32_t xld) {
                                 EXPECT(at % 16 == 0 && at + 16 <= BM * XB, "x: read at %u", at);
                                 check("x", x[at / 16], 0, row, rows, XT == BF16 ? 32 * g + 16 * h : XT == MXFP8 ? 64 * h + 16 * g : 16 * g, xleft);
                             }
-                            const uint32_t s = mg_at_sx(0, wr * RB, n) + 64 * r;
-                            EXPECT(XT == BF16 || s == 4 * row, "x's scale at %u", s);
                         }
                         for (uint32_t c = 0; c < CB; c++) {
                             const uint32_t blk = wc * CB + c, row = 16 * (DUAL ? blk >> 1 : blk) + n;
@@ -90,10 +124,6 @@ static void tile(uint32_t rows, uint32_t cols, uint32_t K, uint32_t xld) {
                             EXPECT(at % (WB / 4) == 0 && at + WB / 4 <= BN * WB, "W: read at %u", at);
                             check("W", w[at / 16], DUAL && (blk & 1) ? 2 : 1, row, cols, WB == 64 ? 16 * g : 16 * (g >> 1), wleft);
                             EXPECT(WB == 64 || at % 16 == 8 * (g & 1), "W: half %u", at % 16);
-                            const uint32_t s = mg_at_sw(0, SBM, wc * CB, n, DUAL) + mg_sw_step(c, BN, DUAL);
-                            bool second;
-                            const uint32_t sr = mg_scale_row(s / 4, SBM, BN, DUAL, second);
-                            EXPECT(s / 4 >= SBM && s / 4 < SBM + BN && s % 4 == 0 && sr == row && second == (DUAL && (blk & 1)), "W's scale at %u", s);
                         }
                     }
     }
