@@ -7,13 +7,12 @@
 template <int MODE>
 static const GhipMxTile *tiles(int *n) {
     static const GhipMxTile t[] = {
-        mg_tile<MODE, GHIP_MXFP8, 2, 2, 8, 8, 3>(0.97f, 0.00f, 1.61f, 6.3f),
-        mg_tile<MODE, GHIP_MXFP8, 2, 2, 8, 4, 3>(0.60f, 0.00f, 1.14f, 2.6f),
-        mg_tile<MODE, GHIP_MXFP8, 2, 2, 4, 8, 3>(0.67f, 0.00f, 1.17f, 2.5f),
-        mg_tile<MODE, GHIP_MXFP8, 2, 2, 4, 4, 3>(0.42f, 0.70f, 1.25f, 0.7f),
-        mg_tile<MODE, GHIP_MXFP8, 2, 2, 2, 4, 4>(0.36f, 0.55f, 0.96f, 0.0f),
-        mg_tile<MODE, GHIP_MXFP8, 2, 2, 2, 2, 5>(0.31f, 0.41f, 0.78f, 0.0f),
-        mg_tile<MODE, GHIP_MXFP8, 1, 2, 2, 2, 8>(0.22f, 0.24f, 0.46f, 0.5f),
+        mg_tile<MODE, GHIP_MXFP8, 2, 2, 8, 8, 3>({1.00f, 0.00f, 1.46f, 7.0f}, {1.00f, 0.00f, 1.43f, 7.8f}),
+        mg_tile<MODE, GHIP_MXFP8, 2, 2, 8, 4, 3>({0.56f, 0.00f, 0.87f, 4.0f}, {0.58f, 0.00f, 0.85f, 4.2f}),
+        mg_tile<MODE, GHIP_MXFP8, 2, 2, 4, 4, 3>({0.32f, 0.53f, 1.00f, 2.0f}, {0.34f, 0.57f, 0.96f, 2.0f}),
+        mg_tile<MODE, GHIP_MXFP8, 2, 2, 2, 4, 4>({0.22f, 0.34f, 0.63f, 1.2f}, {0.23f, 0.38f, 0.62f, 1.5f}),
+        mg_tile<MODE, GHIP_MXFP8, 2, 2, 2, 2, 6>({0.18f, 0.22f, 0.42f, 1.4f}, {0.19f, 0.25f, 0.42f, 1.7f}),
+        mg_tile<MODE, GHIP_MXFP8, 1, 2, 2, 2, 8>({0.15f, 0.17f, 0.30f, 1.7f}, {0.17f, 0.22f, 0.32f, 2.2f}),
     };
     *n = sizeof t / sizeof *t;
     return t;

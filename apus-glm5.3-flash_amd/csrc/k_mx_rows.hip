@@ -324,34 +324,34 @@ static constexpr MrForm mr_form(float base, float quad, float over, float copy, 
 }
 
 static const MrForm mr_linear_bf16[] = {
-    mr_form<GHIP_BF16, 1, 8, GHIP_EP_LINEAR>(2.0f, 0.92f, 0.31f, 0.19f, 0.95f),
-    mr_form<GHIP_BF16, 1, 4, GHIP_EP_LINEAR>(2.2f, 1.00f, 0.21f, 0.15f, 0.94f),
-    mr_form<GHIP_BF16, 2, 8, GHIP_EP_LINEAR>(1.3f, 1.75f, 0.58f, 0.23f, 0.87f),
-    mr_form<GHIP_BF16, 2, 4, GHIP_EP_LINEAR>(1.9f, 1.73f, 0.45f, 0.18f, 0.88f),
+    mr_form<GHIP_BF16, 1, 8, GHIP_EP_LINEAR>(2.0f, 0.93f, 0.30f, 0.18f, 0.96f),
+    mr_form<GHIP_BF16, 1, 4, GHIP_EP_LINEAR>(2.2f, 1.01f, 0.20f, 0.15f, 0.94f),
+    mr_form<GHIP_BF16, 2, 8, GHIP_EP_LINEAR>(1.4f, 1.74f, 0.64f, 0.22f, 0.86f),
+    mr_form<GHIP_BF16, 2, 4, GHIP_EP_LINEAR>(1.9f, 1.74f, 0.42f, 0.17f, 0.89f),
 };
 static const MrForm mr_linear_mxfp8[] = {
-    mr_form<GHIP_MXFP8, 1, 8, GHIP_EP_LINEAR>(2.5f, 0.65f, 0.36f, 0.16f, 1.00f),
-    mr_form<GHIP_MXFP8, 1, 4, GHIP_EP_LINEAR>(2.3f, 0.61f, 0.56f, 0.17f, 0.94f),
-    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_LINEAR>(1.7f, 1.16f, 0.81f, 0.22f, 0.94f),
-    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_LINEAR>(2.0f, 1.05f, 0.94f, 0.21f, 0.97f),
+    mr_form<GHIP_MXFP8, 1, 8, GHIP_EP_LINEAR>(2.5f, 0.67f, 0.37f, 0.15f, 0.97f),
+    mr_form<GHIP_MXFP8, 1, 4, GHIP_EP_LINEAR>(2.3f, 0.60f, 0.58f, 0.16f, 0.95f),
+    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_LINEAR>(1.7f, 1.16f, 0.82f, 0.22f, 0.94f),
+    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_LINEAR>(2.0f, 1.05f, 0.95f, 0.21f, 0.97f),
 };
 static const MrForm mr_linear_mxfp4[] = {
-    mr_form<GHIP_MXFP4, 1, 8, GHIP_EP_LINEAR>(2.5f, 0.39f, 0.52f, 0.23f, 1.38f),
-    mr_form<GHIP_MXFP4, 1, 4, GHIP_EP_LINEAR>(2.5f, 0.67f, 0.39f, 0.13f, 0.98f),
-    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_LINEAR>(1.8f, 0.54f, 1.25f, 0.35f, 1.51f),
-    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_LINEAR>(2.2f, 1.12f, 0.91f, 0.16f, 0.97f),
+    mr_form<GHIP_MXFP4, 1, 8, GHIP_EP_LINEAR>(2.5f, 0.39f, 0.53f, 0.22f, 1.37f),
+    mr_form<GHIP_MXFP4, 1, 4, GHIP_EP_LINEAR>(2.5f, 0.67f, 0.39f, 0.13f, 0.97f),
+    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_LINEAR>(2.0f, 0.53f, 1.06f, 0.34f, 1.63f),
+    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_LINEAR>(2.2f, 1.12f, 0.94f, 0.16f, 0.96f),
 };
 static const MrForm mr_gated_bf16[] = {
-    mr_form<GHIP_BF16, 2, 8, GHIP_EP_GATED>(1.6f, 1.71f, 0.40f, 0.21f, 0.96f),
-    mr_form<GHIP_BF16, 2, 4, GHIP_EP_GATED>(1.9f, 1.86f, 0.19f, 0.17f, 0.86f),
+    mr_form<GHIP_BF16, 2, 8, GHIP_EP_GATED>(1.6f, 1.70f, 0.47f, 0.19f, 0.95f),
+    mr_form<GHIP_BF16, 2, 4, GHIP_EP_GATED>(1.9f, 1.86f, 0.20f, 0.16f, 0.87f),
 };
 static const MrForm mr_gated_mxfp8[] = {
-    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_GATED>(1.8f, 1.51f, 0.55f, 0.18f, 0.91f),
-    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_GATED>(1.7f, 1.40f, 0.87f, 0.17f, 0.90f),
+    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_GATED>(1.8f, 1.49f, 0.57f, 0.17f, 0.90f),
+    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_GATED>(1.7f, 1.39f, 0.94f, 0.17f, 0.87f),
 };
 static const MrForm mr_gated_mxfp4[] = {
-    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_GATED>(1.6f, 0.86f, 1.22f, 0.35f, 1.36f),
-    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_GATED>(2.1f, 1.59f, 0.47f, 0.09f, 0.94f),
+    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_GATED>(1.6f, 0.84f, 1.28f, 0.32f, 1.34f),
+    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_GATED>(2.1f, 1.56f, 0.48f, 0.10f, 0.95f),
 };
 static const MrForm *mr_forms(int mode, int xt, int *n) {
     const bool dual = mode == GHIP_EP_GATED;

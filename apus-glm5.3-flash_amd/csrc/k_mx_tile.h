@@ -13,10 +13,15 @@ static void mg_run(const GhipMxProd *p, const GhipEp *ep, uint32_t mt, uint32_t 
                        *p, *ep, mt, nt);
 }
 
+/* A mode's microseconds (GhipMxTile). */
+struct MgTimes {
+    float low, mid, full, over;
+};
 template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
-static constexpr GhipMxTile mg_tile(float low, float mid, float full, float over) {
+static constexpr GhipMxTile mg_tile(MgTimes linear, MgTimes gated) {
     using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
-    return {T::BM, T::OUTN, T::LDS <= FG_LDS_MAX / 2 ? 2u : 1u, T::LDS, low, mid, full, over,
+    const MgTimes us = MODE == GHIP_EP_GATED ? gated : linear;
+    return {T::BM, T::OUTN, T::LDS <= FG_LDS_MAX / 2 ? 2u : 1u, T::LDS, us.low, us.mid, us.full, us.over,
             (const void *)k_mx_gemm<MODE, XT, WM, WN, RB, CB, R>, mg_run<MODE, XT, WM, WN, RB, CB, R>};
 }
 
