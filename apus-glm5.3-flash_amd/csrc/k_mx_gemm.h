@@ -42,6 +42,15 @@ __device__ __forceinline__ ghip_u32x4 mg_turn(const ghip_u32x4 &v) {
     return (ghip_u32x4){e[0], o[0], e[1], o[1]};
 }
 
+/* v, in a register of its own from here on: a copy that the compiler makes of it later could
+ * be too near an MFMA, which it knows nothing of. */
+__device__ __forceinline__ uint32_t mg_keep(uint32_t v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(v));
+#endif
+    return v;
+}
+
 /* Whether one of the n steps before one of quarter qu is of quarter 2, steps before the
  * first among them: n up to 4, so at most one is. */
 constexpr int mg_third(int qu, int n) {
@@ -171,8 +180,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     constexpr int XQ = BF ? 0 : (RB + 3) / 4, WQ = DUAL ? (CB / 2 + 3) / 4 : (CB + 3) / 4, NQD = XQ + WQ * (DUAL ? 2 : 1);
     constexpr int GS = BF ? 8 : 4, WB16 = DUAL ? CB / 2 : CB;
     uint8_t *const sc = mg_lds + T::RING;
-    ghip_u32x4 next[NSL], raw[NQD], cur[NQD];
-    uint32_t sw[BF ? 2 * CB : 1];
+    ghip_u32x4 next[NSL], raw[NQD];
+    uint32_t sx[BF ? 1 : RB], sw[BF ? 2 * CB : CB];
     auto scale_load = [&](uint32_t word) {
         fg_each<NSL>([&](auto i_c) {
             constexpr uint32_t i = decltype(i_c)::value;
@@ -207,23 +216,26 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     auto scale_turn = [&](auto q_c) { raw[decltype(q_c)::value] = mg_turn(raw[decltype(q_c)::value]); };
     /* BF16: a row's steps take half a word each; sw[c] has the even ones' scales (lane
      * groups 0 and 1 block 0 of the word, 2 and 3 block 1), sw[CB + c] the odd ones' */
-    auto sx_of = [&](auto r_c) { constexpr int r = decltype(r_c)::value; return cur[r / 4][r % 4]; };
-    auto sw_of = [&](auto c_c) {
-        constexpr int c = decltype(c_c)::value, i = DUAL ? c >> 1 : c;
-        return cur[XQ + (DUAL && (c & 1) ? WQ : 0) + i / 4][i % 4];
-    };
     auto scale_take = [&]() {
-        fg_each<NQD>([&](auto q) { cur[decltype(q)::value] = raw[decltype(q)::value]; });
-        if constexpr (BF)
-            fg_each<CB>([&](auto c) {
-                const uint32_t v = sw_of(c);
+        if constexpr (!BF)
+            fg_each<RB>([&](auto r_c) {
+                constexpr int r = decltype(r_c)::value;
+                sx[r] = mg_keep(raw[r / 4][r % 4]);
+            });
+        fg_each<CB>([&](auto c_c) {
+            constexpr int c = decltype(c_c)::value, i = DUAL ? c >> 1 : c;
+            const uint32_t v = raw[XQ + (DUAL && (c & 1) ? WQ : 0) + i / 4][i % 4];
+            if constexpr (BF) {
                 const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const auto q = __builtin_amdgcn_permlane16_swap(h[e], h[e], false, false);
-                    sw[e * CB + decltype(c)::value] = g & 2u ? q[1] : q[0];
+                    sw[e * CB + c] = g & 2u ? q[1] : q[0];
                 }
-            });
+            } else {
+                sw[c] = mg_keep(v);
+            }
+        });
     };
     /* BF16: half h of W's block c of step j, of set S; past: its k is past K, where the
      * codes are zeros and the scale is any byte */
@@ -290,7 +302,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!MAIN && !BF)
             if (rem && j + 1u >= nst && g >= rem) {
-                fg_each<NQD>([&](auto q) { cur[decltype(q)::value] = (ghip_u32x4){0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu}; });
+                fg_each<RB>([&](auto r) { sx[decltype(r)::value] = 0x7f7f7f7fu; });
+                fg_each<CB>([&](auto c) { sw[decltype(c)::value] = 0x7f7f7f7fu; });
                 asm volatile("s_nop 3");                 /* VALU to MFMA */
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -325,7 +338,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
                 fg_mfma(acc[Rr][C], half(wa[S][C], S0{}), half(x, S0{}));
                 fg_mfma(acc[Rr][C], half(wa[S][C], S1{}), half(x, S1{}));
             } else {
-                mg_mfma<QU>(acc[Rr][C], wa[S][C], x, sw_of(std::integral_constant<int, C>{}), sx_of(std::integral_constant<int, Rr>{}));
+                mg_mfma<QU>(acc[Rr][C], wa[S][C], x, sw[C], sx[Rr]);
             }
             /* W and x's last block over the first RB - 1 rows (codes for BF16 over the first
              * third, dequantized behind), x's others behind their own */
