@@ -78,7 +78,7 @@ struct MgTile {
     static constexpr uint32_t XU = BF ? 0u : (BM + 63u) / 64u, WU = (OUTN + 63u) / 64u, NU = XU + WU * (DUAL ? 2u : 1u);
     static constexpr uint32_t NSL = (NU + NW - 1u) / NW, LDS = RING + NU * 1024u;
     static_assert(AST % (1024u * NW) == 0 && BST % (1024u * NW) == 0, "whole loads");
-    static_assert(LDS <= FG_LDS_MAX && R >= 2 && (R - 2) * LPS <= 63, "ring, waits");
+    static_assert(LDS <= FG_LDS_MAX && R >= 3 && (R - 2) * LPS <= 63, "ring, waits");
     static_assert(!DUAL || CB % 2 == 0, "gate and up blocks alternate");
 };
 

@@ -188,15 +188,16 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_long(GhipNorm p, size_t row0) 
 
 /* ---- gradient ------------------------------------------------------------ */
 
-/* dx's columns [col, col + 8); a = rstd, b = rstd^3 mean(gamma dy s). */
+/* dx's columns [col, col + 8); a = rstd, c = rstd mean(gamma dy s). s rstd and c are of the size
+ * of 1 and of dy whatever the row's is; rstd^3 leaves the f32 range for rows past 2^42. */
 __device__ __forceinline__ void nm_dx(const GhipNormGrad &p, size_t row, uint32_t col, const nm_u16x8 &s,
-                                      const nm_u16x8 &dy, const nm_u16x8 &g, const nm_u16x8 &ds, float a, float b) {
+                                      const nm_u16x8 &dy, const nm_u16x8 &g, const nm_u16x8 &ds, float a, float c) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         float d = ghip_bf16_f32(dy[e]);
         if (p.gamma) d *= ghip_bf16_f32(g[e]);
-        v[e] = a * d - b * ghip_bf16_f32(s[e]);
+        v[e] = a * (d - ghip_bf16_f32(s[e]) * a * c);
     }
     if (p.ds)
 #pragma unroll
@@ -265,13 +266,13 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm_grad(GhipNormGrad
             if (8u * (t + T * i) < p.D) nm_products(p, s[i], dy[i], g[i], sum);
         nm_sum<T, 2>(sum, lds);
         const float a = p.rstd ? given : nm_rstd(sum[1], p.D, p.eps);
-        const float b = a * a * a * (sum[0] / (float)p.D);
+        const float c = a * (sum[0] / (float)p.D);
         if (row < p.M) {
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const uint32_t col = 8u * (t + T * i);
                 if (col < p.D) {
-                    if (p.dx) nm_dx(p, row, col, s[i], dy[i], g[i], ds[i], a, b);
+                    if (p.dx) nm_dx(p, row, col, s[i], dy[i], g[i], ds[i], a, c);
 #pragma unroll
                     for (int e = 0; e < 8; e++) acc[i][e] += ghip_bf16_f32(dy[i][e]) * (ghip_bf16_f32(s[i][e]) * a);
                 }
@@ -316,14 +317,14 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_grad_long(GhipNormGrad p, size
         nm_products(p, nm_load(s, col, p.D), nm_load(dy, col, p.D), gamma(col), sum);
     nm_sum<1024, 2>(sum, lds);
     const float a = p.rstd ? p.rstd[row] : nm_rstd(sum[1], p.D, p.eps);
-    const float b = a * a * a * (sum[0] / (float)p.D);
+    const float c = a * (sum[0] / (float)p.D);
     if (!p.dx) {
         if (threadIdx.x == 0u) p.part[row] = a;
         return;
     }
     for (uint32_t col = 8u * threadIdx.x; col < p.D; col += 8192u)
         nm_dx(p, row, col, nm_load(s, col, p.D), nm_load(dy, col, p.D), gamma(col),
-              p.ds ? nm_load(p.ds + row * p.ldds, col, p.D) : nm_u16x8{}, a, b);
+              p.ds ? nm_load(p.ds + row * p.ldds, col, p.D) : nm_u16x8{}, a, c);
 }
 
 __global__ __launch_bounds__(256) void k_rmsnorm_dgamma_long(GhipNormGrad p) {

@@ -153,6 +153,20 @@ def test_gradient(ghip, M, D, given):
     check_grad(got, s, gain, dy, ds)
 
 
+@pytest.mark.parametrize("M,D", [(13, 96), (13, 2048), (13, 8000), (13, 17024)])
+@pytest.mark.parametrize("given", [False, True])
+def test_gradient_of_rows_of_any_size(ghip, M, D, given):
+    """Rows from 2^-55 to 2^53, whose rstd^3 is no f32."""
+    s, _, g, dy = inputs(M, D, 9)
+    s = bf(O.bf16_to_f32(s) * np.exp2(np.linspace(-55, 53, M)).astype(np.float32)[:, None])
+    rstd = G.dev((1 / np.sqrt((wide(s) ** 2).mean(1))).astype(np.float32)) if given else None
+    got = run_grad(ghip, Mat(s), Mat(g), rstd, Mat(dy), None, M, D, eps=0.0)
+    dx, dg = X.norm_backward(wide(s), wide(g)[0], wide(dy), None, 0.0)
+    for m in range(M):
+        R.check(wide(got["dx"])[m:m + 1], dx[0][m:m + 1], dx[1][m:m + 1], "dx %d" % m)
+    R.check(wide(got["dgamma"])[0], *dg, "dgamma")
+
+
 @pytest.mark.parametrize("M,D", [(40, 96), (600, 2048), (3, 5000), (2, 16500)])
 def test_gradients_left_out(ghip, M, D):
     s, ds, g, dy = inputs(M, D, 4)
