@@ -8,8 +8,7 @@ template <int MODE>
 static const GhipMxTile *tiles(int *n) {
     static const GhipMxTile t[] = {
         mg_tile<MODE, GHIP_BF16, 1, 4, 12, 4, 4>({0.85f, 0.00f, 1.03f, 6.2f}, {0.85f, 0.00f, 1.03f, 6.4f}),
-        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 4, 6>({0.64f, 0.00f, 0.80f, 5.6f}, {0.64f, 0.00f, 0.78f, 6.0f}),
-        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 4, 3>({0.64f, 0.80f, 1.84f, 4.0f}, {0.66f, 0.78f, 1.78f, 4.2f}),
+        mg_tile<MODE, GHIP_BF16, 1, 4, 8, 4, 3>({0.64f, 0.00f, 0.80f, 4.0f}, {0.65f, 0.00f, 0.79f, 4.2f}),
         mg_tile<MODE, GHIP_BF16, 1, 4, 8, 2, 3>({0.39f, 0.50f, 0.91f, 2.1f}, {0.40f, 0.52f, 0.89f, 2.2f}),
         mg_tile<MODE, GHIP_BF16, 1, 4, 4, 2, 6>({0.27f, 0.33f, 0.56f, 2.1f}, {0.28f, 0.34f, 0.55f, 2.2f}),
         mg_tile<MODE, GHIP_BF16, 1, 4, 2, 2, 8>({0.23f, 0.25f, 0.41f, 1.8f}, {0.23f, 0.27f, 0.40f, 2.1f}),

@@ -21,7 +21,8 @@ template <int MODE, int XT, int WM, int WN, int RB, int CB, int R>
 static constexpr GhipMxTile mg_tile(MgTimes linear, MgTimes gated) {
     using T = MgTile<MODE, XT, WM, WN, RB, CB, R>;
     const MgTimes us = MODE == GHIP_EP_GATED ? gated : linear;
-    return {T::BM, T::OUTN, T::LDS <= FG_LDS_MAX / 2 ? 2u : 1u, T::LDS, us.low, us.mid, us.full, us.over,
+    /* two fit a CU by LDS, and by registers where the sums take 64 or fewer */
+    return {T::BM, T::OUTN, T::LDS <= FG_LDS_MAX / 2 && RB * CB < 32 ? 2u : 1u, T::LDS, us.low, us.mid, us.full, us.over,
             (const void *)k_mx_gemm<MODE, XT, WM, WN, RB, CB, R>, mg_run<MODE, XT, WM, WN, RB, CB, R>};
 }
 

@@ -380,6 +380,19 @@ __global__ __launch_bounds__(256) void k_rmsnorm_dgamma(const float *__restrict_
 
 /* ---- which form ----------------------------------------------------------- */
 
+/* By the row's length: as few threads a row as hold it in one or two pieces each, for a
+ * wave needs no barrier, and more threads than pieces idle at it. Microseconds of 2^26
+ * values (a residual, y in BF16; the gradient with dgamma), the next forms beside:
+ *   D          norm                                      gradient
+ *   512        64x1 91, 64x2 92, 256x1 143               64x2 93, 64x1 94, 256x1 318
+ *   1024       64x2 98, 256x1 99, 512x1 149              64x2 93, 256x1 182, 512x1 206
+ *   2048       512x1 92, 256x1 94, 1024x1 130            256x1 101, 512x1 111, 256x4 121
+ *   (MXFP8     256x1 81, 512x1 94)
+ *   4096       512x1 91, 1024x1 94, 256x2 98             512x1 84, 256x4 91, 256x2 93
+ *   8192       1024x1 92, 512x2 98, 256x4 102            256x4 86, 1024x1 91, 512x2 110
+ *   16384      1024x2 100, 512x4 105, two passes 115     512x4 103, 1024x2 132
+ * A single row takes 3.3 us at 8192 by 1024x1, 4.8 by 256x4. */
+
 /* Launches of at most this many blocks (2^32 threads along x are refused). */
 #define NM_BLOCKS ((size_t)1 << 21)
 #define NM_GRAD_BLOCKS ((size_t)512)
@@ -402,9 +415,9 @@ extern "C" hipError_t ghip_launch_rmsnorm(const GhipNorm *p, hipStream_t st) {
     if (p->D <= 512) return norm_run<64, 1>(p, st);
     if (p->D <= 1024) return norm_run<64, 2>(p, st);
     if (p->D <= 2048) return norm_run<256, 1>(p, st);
-    if (p->D <= 4096) return norm_run<256, 2>(p, st);
-    if (p->D <= 8192) return norm_run<256, 4>(p, st);
-    if (p->D <= 16384) return norm_run<512, 4>(p, st);
+    if (p->D <= 4096) return norm_run<512, 1>(p, st);
+    if (p->D <= 8192) return norm_run<1024, 1>(p, st);
+    if (p->D <= 16384) return norm_run<1024, 2>(p, st);
     for (size_t r = 0; r < p->M; r += NM_BLOCKS) {
         hipLaunchKernelGGL(k_rmsnorm_long, dim3((uint32_t)(p->M - r < NM_BLOCKS ? p->M - r : NM_BLOCKS)),
                            dim3(1024), 0, st, *p, r);
@@ -442,8 +455,8 @@ static bool grad_form(size_t D, F f) {
     if (D <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
     else if (D <= 1024) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
     else if (D <= 2048) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
-    else if (D <= 4096) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-    else if (D <= 8192) f(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+    else if (D <= 4096) f(integral_constant<int, 512>{}, integral_constant<int, 1>{});
+    else if (D <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
     else if (D <= 16384) f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
     else return false;
     return true;
