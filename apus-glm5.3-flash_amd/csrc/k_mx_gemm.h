@@ -1,5 +1,27 @@
 /*
- * k_mx_gemm.h — the tiled product with MXFP4 weights (gfx950).
+ * k_mx_gemm.h — x W^T on tiles, W in MXFP4, x in MXFP8, MXFP4 or BF16 (gfx950).
+ *
+ *   y[m, n] = sum over blocks b of 32 k: 2^(sx + sw - 254) sum_k x[m, k] w[n, k]
+ *
+ * Microscaled x goes to v_mfma_scale_f32_16x16x128_f8f6f4 as it lies: the instruction
+ * multiplies the block's two scales in, so nothing is dequantized, and MXFP4 against
+ * MXFP4 has twice the rate of MXFP8 (dense peaks 10 and 5 PFLOP/s). BF16 x takes W's
+ * codes to BF16 at the operand, exactly, by the conversion that takes a scale: two
+ * codes an instruction, over the second half of the step before.
+ *
+ * Bound by the MFMAs at the chip's power limit for large products, by what a step costs
+ * with few workgroups. Four waves; a step of 128 k (BF16 64) comes straight to LDS, R
+ * steps in a ring; a wave waits for its own loads by count, so those of R - 2 steps stay
+ * in flight over the one barrier of a step. Between the MFMAs of a step, in places set
+ * by hand, stand the next step's operand reads and the loads of step j + R. The
+ * accumulators of the largest tile fill all 256 AGPRs and stay in place through an
+ * assembly MFMA; what the compiler then does not know is read from the built code by
+ * tests/test_mx_asm.py.
+ *
+ * Measured (us; TFLOP/s): MXFP4 8192 x 8192 x 8192 266 (4130), 4096^3 45.6 (3010);
+ * MXFP8 8192^3 362 (3035), 4096^3 57.8 (2380), gated 8192 x 12288 x 4096 593-606 (2720-2780);
+ * BF16 8192^3 791 (1390). The library's plain products of 8192^3 in the same types run at
+ * 2990, 1290 and 1390.
  */
 #ifndef K_MX_GEMM_H
 #define K_MX_GEMM_H
@@ -174,8 +196,9 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
      * (mg_turn) into words that the MFMA picks a step's byte from by number. Each of the
      * simpler ways costs more than a small tile's step: 4 bytes a row every step, as the
      * line is in flight already and the loads wait for it one after the other (64 x 64
-     * tiles, 4096 x 4096 x 4096: 193 us, 93 with no scales at all); every wave its own
-     * blocks', as the waves of a row of tiles ask for the same lines */
+     * tiles, 4096 x 4096 x 4096: 193 us, 93 with no scales at all, 112 so); every wave its
+     * own blocks', as the waves of a row of tiles ask for the same lines (256 x 256, 8192 x
+     * 8192 x 8192 in MXFP4: 302 us, 277 so) */
     constexpr uint32_t NSL = T::NSL, XU = T::XU, WU = T::WU, NU = T::NU;
     constexpr int XQ = BF ? 0 : (RB + 3) / 4, WQ = DUAL ? (CB / 2 + 3) / 4 : (CB + 3) / 4, NQD = XQ + WQ * (DUAL ? 2 : 1);
     constexpr int GS = BF ? 8 : 4, WB16 = DUAL ? CB / 2 : CB;
@@ -428,8 +451,8 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
             else load8(std::false_type{}, ep.bias, bias);
         }
     /* The residual, U rows ahead: the first ones come while the sums are laid out, the next
-     * while U are computed (4096 x 4096 tiles of 256 x 256 in one round: 118 us with each
-     * batch loaded when it was needed) */
+     * while U are computed (4096 x 4096 x 12288 in MXFP4, one round of 256 x 256 tiles: 112
+     * us, 118 with each batch loaded where it was needed) */
     ghip_u32x4 res[U];
     const bool ahead = BIAS && fast && ep.in;
     auto fetch = [&](int at) {

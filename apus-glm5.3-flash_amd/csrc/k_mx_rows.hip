@@ -1,7 +1,20 @@
 /*
- * k_mx_rows.hip — products of a few rows with MXFP4 weights (gfx950): every wave
- * loads its weights' codes straight into the operand registers of the matrix
- * instruction.
+ * k_mx_rows.hip — products of a few rows of x with MXFP4 weights (gfx950).
+ *
+ * Bound by HBM: the weights are read once, 17/32 bytes a value, in whole lines of 128
+ * bytes (256 k of a row). A wave copies its share of x's rows to LDS once and streams
+ * blocks of weight rows past them, four steps of 128 k in registers ahead of the four in
+ * use; a grid as large as the chip, or a whole fraction of the blocks, so that x is
+ * copied few times and the stream does not end with a block. The codes cross LDS on
+ * their way, as a line's 16 bytes are loaded by lanes beside each other and used by
+ * lanes a row apart; each line is asked for once, because a second load from a line that
+ * is in flight waits for it and then makes a trip of its own (operands loaded straight
+ * into their registers, 64 bytes of a line at a time: 1 x 4096 x 12288 67.6 us, 7.8 so).
+ * k is split over 8 or 4 waves, whose sums meet in LDS in a fixed order.
+ *
+ * Measured: 1 x 4096 x 12288 7.8 us (26.7 MB, 3.4 TB/s of an operand set that the chip's
+ * cache holds in part); 5 x 12288 x 4096 gated 11.8 (53.5 MB, 4.5 TB/s), from launch to
+ * end: an empty launch takes 2.5 to 3 of it.
  */
 #include <type_traits>
 #include <utility>
@@ -304,7 +317,17 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
 
 /* One launchable form: output columns, and microseconds of the launch, of four steps of
  * a wave, of a block besides, and of a KB of a wave's share of x; two: how much longer
- * these are where CUs hold two workgroups. */
+ * these are where CUs hold two workgroups. The times are least-squares fits to sweeps of
+ * 1 to 192 rows over N x K of 256 x 1024 to 12288 x 4096, 4096 x 12288, 8192 x 512 and 512 x
+ * 8192, every form timed (0.05 to 0.1 rms of the logarithm). Two groups
+ * share an operand of x but make fewer workgroups, 8 waves along k shorten a wave's chain
+ * and 4 halve the joins. BF16, NT x KS, us:
+ *                              1x8    1x4    2x8    2x4
+ *   linear 1 x 12288 x 4096    8.1    7.7    8.6    8.1
+ *   linear 1 x 4096 x 12288    6.9    9.3    8.9   13.5
+ *   linear 16 x 4096 x 12288  17.4   28.5   15.8   25.1
+ *   gated 4 x 12288 x 4096                  15.6   13.6
+ *   gated 1 x 256 x 1024                     4.2    4.8 */
 struct MrForm {
     uint32_t cols, nt, ks, red;
     float base, quad, over, copy, two;

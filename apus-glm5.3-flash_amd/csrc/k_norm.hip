@@ -12,6 +12,14 @@
  * fixed order. Sums, statistics and the values in between are f32. s is rounded
  * before the norm because it is what the stream holds and what the gradient is
  * given; y is rounded once, to bf16 or, with its block's scale, to MXFP8.
+ *
+ * The gradient's groups of threads walk the rows a grid apart, so that dgamma's sums
+ * stay in registers and 512 workgroups' worth of them goes to memory once; a second
+ * launch adds these in order. The next row is loaded while one is summed.
+ *
+ * Measured: 8192 x 4096 with a residual to s and MXFP8 43.5 us (236 MB, 5.4 TB/s); its
+ * gradient with ds 53.4 + 4.7 (268 MB and 17: 5.0 TB/s; 71.5 in all with no row loaded
+ * ahead); one row of 4096 3.0, a launch's time; 300 x 1536 gradient 4.2 + 3.1.
  */
 #include <type_traits>
 
