@@ -979,11 +979,12 @@ static int mx_forward(int mode, const uint8_t *w, const uint8_t *ws, const uint8
                       size_t O, size_t K, size_t ldx, size_t ldr, size_t ldy, int act, float limit,
                       hipStream_t st) {
     const int wide = x_type == GHIP_BF16;
+    const char *const ld = mode == GHIP_EP_GATED ? "ldh" : "ldy";
     if (check_sizes(M, O, K) || check_blocks("K", K) || check_aligned("codes", w, 16)
         || check_aligned("scales", ws, 4)
         || (mode == GHIP_EP_GATED && (check_aligned("up codes", w2, 16) || check_aligned("up scales", ws2, 4)))
         || check_aligned("x", x, 16) || check_ptr("the output", y) || check_act(act, limit)
-        || check_ld("ldx", &ldx, K) || check_ld("ldy", &ldy, O) || check_ld("ldr", &ldr, O))
+        || check_ld("ldx", &ldx, K) || check_ld(ld, &ldy, O) || check_ld("ldr", &ldr, O))
         return 1;
     if (x_type < GHIP_BF16 || x_type > GHIP_MXFP4) {
         ghip_seterr("unknown type %d of x", x_type);
@@ -992,6 +993,11 @@ static int mx_forward(int mode, const uint8_t *w, const uint8_t *ws, const uint8
     if (!wide && (check_aligned("x's scales", x_scales, 4))) return 1;
     if (wide ? ldx % 8 != 0 : ldx != K) {
         ghip_seterr(wide ? "ldx %zu is no multiple of 8" : "ldx %zu: microscaled rows are dense", ldx);
+        return 1;
+    }
+    /* the tiles' offsets are of 32 bits, the row forms hold x's rows in LDS */
+    if (K >> 22 || (wide && K > 1u << 15 && ldx >> 22)) {
+        ghip_seterr("K %zu, ldx %zu: too long", K, ldx);
         return 1;
     }
     DEVICE_SCOPE;

@@ -205,6 +205,31 @@ def test_rows_in_wider_buffers(ghip, M, N, K, xt, pad, off):
 
 
 @pytest.mark.parametrize("xt", XTYPES)
+def test_k_past_the_row_forms(ghip, xt):
+    """A row of x longer than LDS: few rows go to tiles."""
+    M, N, K = 3, 40, (1 << 17) + 96
+    rng = seed(50, xt)
+    w, x, y = weights(rng, N, K), Act(xt, acts(rng, M, K)), Mat.out(M, N)
+    ok(ghip, linear(ghip, w, x, None, None, y, R.NONE))
+    R.check(wide(y.get()), *X.linear(x.values, w.values, None, None, R.NONE, xt), "linear")
+
+
+@pytest.mark.parametrize("xt", XTYPES)
+@pytest.mark.parametrize("M,N,K", [(4, 512, 1024), (300, 520, 640), (1024, 1032, 256), (5000, 2056, 128)])
+def test_called_again(ghip, M, N, K, xt):
+    """The same bits from call to call, many workgroups a CU among them."""
+    rng = seed(51, M, N, K, xt)
+    w, x, res = weights(rng, N, K), Act(xt, acts(rng, M, K)), Mat(bf(rng.standard_normal((M, N))))
+    first = None
+    for _ in range(4):
+        y = Mat.out(M, N)
+        ok(ghip, linear(ghip, w, x, None, res, y, R.NONE))
+        got = y.get()
+        assert first is None or np.array_equal(first, got)
+        first = got
+
+
+@pytest.mark.parametrize("xt", XTYPES)
 @pytest.mark.parametrize("M,N,K", [(1, 4096, 1024), (9, 1040, 512), (333, 777, 192)])
 def test_residual_in_place(ghip, M, N, K, xt):
     rng = seed(45, M, N, K, xt)

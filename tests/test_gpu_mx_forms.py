@@ -48,6 +48,15 @@ def test_tiles_at_ragged_sizes(ghip, mode, xt):
 
 @pytest.mark.parametrize("mode", [F.LINEAR, F.GATED])
 @pytest.mark.parametrize("xt", [X.BF16, X.MXFP8, X.MXFP4])
+def test_tiles_over_many_steps(ghip, mode, xt):
+    """Rings and scales that come round many times, k cut in every quarter of four steps; several tiles."""
+    for form in range(F.tiles(ghip, mode, xt)):
+        for M, N, K in [(70, 136, 2208), (33, 72, 4096), (40, 40, 5152), (17, 24, 6304), (290, 520, 4000), (3, 8, 20544)]:
+            one(ghip, "gemm", mode, form, xt, M, N, K)
+
+
+@pytest.mark.parametrize("mode", [F.LINEAR, F.GATED])
+@pytest.mark.parametrize("xt", [X.BF16, X.MXFP8, X.MXFP4])
 def test_row_forms(ghip, mode, xt):
     """One to several tiles of rows; k of fewer steps than waves, than are in flight, and of many, whole and cut."""
     for form in range(F.rows(ghip, mode, xt)):

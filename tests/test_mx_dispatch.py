@@ -61,4 +61,11 @@ def test_what_each_kind_takes(lib, xt):
     assert pick(lib, F.LINEAR, xt, 1, 64, 1 << 24) == ("tiles", -1)
     assert picks(lib, F.LINEAR, xt, (1 << 31) - 1, (1 << 31) - 1, 32)[0][0] == -1
     assert pick(lib, F.LINEAR, xt, (1 << 31) - 1, (1 << 31) - 1, 32)[0] == "rows"
+    # what the entries let through has a kernel: any stride up to k of 2^15, less than 2^22 elements to 2^22
+    for mode in (F.LINEAR, F.GATED):
+        for M, K, ld in [(1, 1 << 15, 1 << 30), (4096, 1 << 15, 1 << 30), (1, (1 << 22) - 32, (1 << 22) - 32), (4096, (1 << 22) - 32, (1 << 22) - 8)]:
+            p = F.prod(xt, M, 64, K, AT, AT, AT, AT, AT, AT)
+            p.xld = 2 * ld if xt == 0 else K if xt == 1 else K // 2
+            us = ctypes.c_float()
+            assert max(f(mode, ctypes.byref(p), ctypes.byref(us)) for f in (lib.ghip_mx_gemm_pick, lib.ghip_mx_rows_pick)) >= 0
     assert all(us > 2.0 for _, us in picks(lib, F.LINEAR, xt, 1, 1, 32))
