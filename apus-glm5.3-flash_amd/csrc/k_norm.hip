@@ -15,11 +15,12 @@
  *
  * The gradient's groups of threads walk the rows a grid apart, so that dgamma's sums
  * stay in registers and 512 workgroups' worth of them goes to memory once; a second
- * launch adds these in order. The next row is loaded while one is summed.
+ * launch adds these in order. The next row is loaded while one is summed. Of a few rows
+ * whose rstd is given one launch makes both, dgamma from s and dy read again.
  *
  * Measured: 8192 x 4096 with a residual to s and MXFP8 43.5 us (236 MB, 5.4 TB/s); its
  * gradient with ds 53.4 + 4.7 (268 MB and 17: 5.0 TB/s; 71.5 in all with no row loaded
- * ahead); one row of 4096 3.0, a launch's time; 300 x 1536 gradient 4.2 + 3.1.
+ * ahead); one row of 4096 3.0, a launch's time; 300 x 1536 gradient 3.5.
  */
 #include <type_traits>
 
@@ -314,6 +315,70 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm_grad(GhipNormGrad
     }
 }
 
+/* A few rows whose rstd is given, in one launch: row_blocks workgroups take a row (or
+ * four) each for dx, the others 32 columns each for dgamma, which read s and dy again.
+ * dx may not be dy. */
+template <int T, int V>
+__global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm_grad_few(GhipNormGrad p, uint32_t row_blocks) {
+    constexpr uint32_t TH = T < 256 ? 256 : T, PER = TH / T, Q = TH / 4u;
+    __shared__ float lds[Q * 33u];
+    if (blockIdx.x < row_blocks) {
+        const uint32_t t = threadIdx.x % T;
+        const size_t row = (size_t)blockIdx.x * PER + threadIdx.x / T;
+        if (T == 64 && row >= p.M) return;
+        nm_u16x8 s[V], dy[V], g[V], ds[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const uint32_t col = 8u * (t + T * i);
+            if (col < p.D) {
+                s[i] = nm_load(p.s + row * p.lds, col, p.D);
+                dy[i] = nm_load(p.dy + row * p.lddy, col, p.D);
+                if (p.gamma) g[i] = nm_load(p.gamma, col, p.D);
+                if (p.ds) ds[i] = nm_load(p.ds + row * p.ldds, col, p.D);
+            }
+        }
+        const float a = p.rstd[row];
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (8u * (t + T * i) < p.D) nm_products(p, s[i], dy[i], g[i], sum);
+        nm_sum<T, 2>(sum, lds);
+        const float c = a * (sum[0] / (float)p.D);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const uint32_t col = 8u * (t + T * i);
+            if (col < p.D) nm_dx(p, row, col, s[i], dy[i], g[i], ds[i], a, c);
+        }
+        return;
+    }
+    const uint32_t q = threadIdx.x >> 2, c = 8u * (threadIdx.x & 3u), first = (blockIdx.x - row_blocks) * 32u;
+    float v[8] = {};
+    if (first + c < p.D)
+#pragma unroll 4
+        for (size_t row = q; row < p.M; row += Q) {
+            const nm_u16x8 s = nm_load(p.s + row * p.lds, first + c, p.D), dy = nm_load(p.dy + row * p.lddy, first + c, p.D);
+            const float a = p.rstd[row];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] += ghip_bf16_f32(dy[e]) * (ghip_bf16_f32(s[e]) * a);
+        }
+#pragma unroll
+    for (int e = 0; e < 8; e++) lds[q * 33u + c + e] = v[e];
+    __syncthreads();
+    const uint32_t n = threadIdx.x & 31u, h = threadIdx.x >> 5;
+    float s = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < 8; k++) s += lds[(8u * h + k) * 33u + n];
+    __syncthreads();
+    lds[h * 33u + n] = s;
+    __syncthreads();
+    if (threadIdx.x < 32u && first + n < p.D) {
+        s = 0.0f;
+#pragma unroll
+        for (uint32_t k = 0; k < TH / 32u; k++) s += lds[k * 33u + n];
+        p.dgamma[first + n] = (uint16_t)ghip_bf16_bits(s);
+    }
+}
+
 /* Rows of any length, dx or (dx NULL) rstd to part. */
 __global__ __launch_bounds__(1024) void k_rmsnorm_grad_long(GhipNormGrad p, size_t row0) {
     __shared__ float lds[32];
@@ -445,9 +510,28 @@ static size_t grad_blocks(size_t M) {
     return n < NM_GRAD_BLOCKS ? n : NM_GRAD_BLOCKS;
 }
 
+/* Whether one launch that reads s and dy twice is taken: its columns' walk over the rows
+ * grows with their number, its second reads with their size. us of M x D, one launch : two
+ * (all with ds):
+ *   M       1536          4096          8192          16384
+ *   1       3.4 :  5.9    3.2 :  5.8    4.0 :  7.5    4.4 :  8.4
+ *   300     3.5 :  7.0    3.8 :  9.4    6.5 : 16.1   16.2 : 24.4
+ *   512     3.8 :  7.9    4.5 : 12.3   11.0 : 19.3   25.7 : 33.3
+ *   1024    6.2 :  9.0   12.2 : 14.8   23.2 : 23.9   46.8 : 44.1
+ *   2048   16.0 : 11.7   26.8 : 18.3   44.1 : 33.7   88.8 : 71.2 */
+static bool grad_few(const GhipNormGrad *p) {
+    return p->dgamma && p->rstd && p->dx != p->dy && p->M <= 1024 && p->M * p->D <= (size_t)1 << 23;
+}
+
 template <int T, int V>
 static hipError_t grad_run(const GhipNormGrad *p, hipStream_t st) {
     const size_t blocks = grad_blocks<T>(p->M);
+    if (grad_few(p)) {
+        const uint32_t rows = p->dx ? (uint32_t)((p->M + grad_per<T>() - 1) / grad_per<T>()) : 0u;
+        hipLaunchKernelGGL((k_rmsnorm_grad_few<T, V>), dim3(rows + (p->D + 31u) / 32u), dim3(T < 256 ? 256 : T), 0, st,
+                           *p, rows);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL((k_rmsnorm_grad<T, V>), dim3((uint32_t)blocks), dim3(T < 256 ? 256 : T), 0, st, *p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p->dgamma) return e;

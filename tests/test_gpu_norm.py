@@ -197,6 +197,18 @@ def test_in_place(ghip, M, D):
         assert np.array_equal(got["dx"], grads["dx"]) and np.array_equal(got["dgamma"], grads["dgamma"])
 
 
+@pytest.mark.parametrize("M,D", [(1, 33), (5, 100), (300, 1536), (1024, 520), (1025, 520), (1024, 8192), (600, 9000), (1000, 9000), (130, 16384)])
+@pytest.mark.parametrize("place", ["dy", "ds", "own", "none"])
+def test_rstd_given(ghip, M, D, place):
+    """Few rows and more, dx in dy's buffer, in ds's, in its own and left out."""
+    s, ds, g, dy = inputs(M, D, 10)
+    rstd = G.dev((1 / np.sqrt((wide(s) ** 2).mean(1) + EPS)).astype(np.float32))
+    d, e = Mat(dy, 1), Mat(ds, 2)
+    want = ("dgamma",) if place == "none" else ("dx", "dgamma")
+    got = run_grad(ghip, Mat(s), Mat(g), rstd, d, e, M, D, want, dx={"dy": d, "ds": e}.get(place))
+    check_grad(got, s, g, dy, ds, want)
+
+
 @pytest.mark.parametrize("D", [96, 1024, 4096, 17024])
 def test_extreme_rows(ghip, D):
     """A row of zeros, of the least numbers, of large ones, one with an infinity, one with a NaN: each by the formula, none
