@@ -996,7 +996,7 @@ static int mx_forward(int mode, const uint8_t *w, const uint8_t *ws, const uint8
         return 1;
     }
     /* the tiles' offsets are of 32 bits, the row forms hold x's rows in LDS */
-    if (K >> 22 || (wide && K > 1u << 15 && ldx >> 22)) {
+    if (K >> 22 || (wide && (mode == GHIP_EP_LINEAR || K > 1u << 15) && ldx >> 22)) {
         ghip_seterr("K %zu, ldx %zu: too long", K, ldx);
         return 1;
     }

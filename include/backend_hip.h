@@ -483,8 +483,8 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
  *     MXFP8, everything else in f32.
  *   - Codes and BF16 x of the projections are 16-byte aligned, scales 4-byte, x's
  *     stride is whole 16 bytes (microscaled x is dense); all other matrices may have
- *     any alignment. K is below 2^22, and where it is past 2^15 the rows of BF16 x are
- *     less than 2^22 elements apart; more is refused.
+ *     any alignment. K is below 2^22, and the rows of BF16 x are less than 2^22
+ *     elements apart (gated: where K is past 2^15); more is refused.
  *   - No output may overlap an input or another output but as said. Deterministic
  *     run to run. Asynchronous on `stream` (a hipStream_t of the backend's device,
  *     NULL = its null stream), whichever device is current; no allocation, no

@@ -148,7 +148,7 @@ LIN = dict(w=P, ws=P, t=1, x=P, xs=P, bias=None, res=None, y=2 * P, M=4, O=24, K
     (dict(x=P + 2), ["x", "16-byte"]), (dict(xs=P + 2), ["scales", "4-byte"]), (dict(t=3), ["type 3"]), (dict(t=-1), ["type -1"]),
     (dict(K=40), ["40", "32"]), (dict(M=0), ["empty"]), (dict(ldx=128), ["ldx 128", "dense"]), (dict(t=0, ldx=68), ["ldx 68", "8"]),
     (dict(t=0, ldx=32), ["ldx"]), (dict(ldr=8), ["ldr"]), (dict(ldy=8), ["ldy"]), (dict(act=5), ["activation"]),
-    (dict(K=1 << 22), ["K 4194304", "long"]), (dict(t=0, K=1 << 22), ["long"]), (dict(t=0, K=32800, ldx=1 << 22), ["ldx 4194304", "long"])])
+    (dict(K=1 << 22), ["K 4194304", "long"]), (dict(t=0, K=1 << 22), ["long"]), (dict(t=0, ldx=1 << 22), ["ldx 4194304", "long"])])
 def test_linear_refuses(lib, change, words):
     refused(lib, lib.apus_ghip_mxfp4_linear_dev(*{**LIN, **change}.values(), None), *words)
 
@@ -159,7 +159,7 @@ GATED = dict(wg=P, gs=P, wu=P, us=P, t=2, x=P, xs=P, h=2 * P, M=4, I=24, K=64, l
 @pytest.mark.parametrize("change,words", [
     (dict(wg=None), ["codes", "NULL"]), (dict(wu=None), ["up codes", "NULL"]), (dict(us=None), ["up scales", "NULL"]),
     (dict(wu=P + 8), ["up codes", "16-byte"]), (dict(us=P + 2), ["up scales", "4-byte"]), (dict(limit=-1.0), ["limit"]),
-    (dict(limit=float("nan")), ["limit"]), (dict(ldh=8), ["ldh"]), (dict(K=31), ["31", "32"])])
+    (dict(limit=float("nan")), ["limit"]), (dict(ldh=8), ["ldh"]), (dict(t=0, K=32800, ldx=1 << 22), ["ldx 4194304", "long"]), (dict(K=31), ["31", "32"])])
 def test_gated_refuses(lib, change, words):
     refused(lib, lib.apus_ghip_mxfp4_gated_dev(*{**GATED, **change}.values(), None), *words)
 
