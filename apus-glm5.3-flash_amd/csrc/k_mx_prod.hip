@@ -5,12 +5,10 @@
  * timed every one of them at 16 (1) to 4096 rows, the three types of x, linear and gated,
  * eight N x K. Over it the pick is 1 to 2% behind the best one's time on average and 22%
  * at worst (gated MXFP4 32 x 4096 x 4096: 8.5 us, 6.9 best). Rows against tiles, us:
- *   linear MXFP8, 4096 x 4096     16 rows 5.2 : 9.6
- *   linear MXFP8, 12288 x 4096    16 rows 7.6 : 10.2,  32 9.8 : 10.6
+ *   gated MXFP8, 4096 x 4096      16 rows 6.7 : 10.9
+ *   gated MXFP8, 12288 x 4096     16 rows 13.0 : 17.0
  *   gated BF16, 12288 x 4096      16 rows 20.1 : 22.8
- *   linear MXFP8, 4096 x 12288    16 rows 9.5 : 19.8
- * The linear with BF16 x takes tiles for any number of rows (k_mx_rows.hip), and tiles
- * against each other in MXFP8: 300 x 1537 x 4096 32x64 10.0, 64x64 10.8, 128x128
+ * The linear takes tiles for any number of rows (k_mx_rows.hip). Tiles against each other in MXFP8: 300 x 1537 x 4096 32x64 10.0, 64x64 10.8, 128x128
  * 16.6, 256x256 46.3; 4096 x 4096 x 4096 175, 112, 69.6 (256x128), 57.8.
  */
 #include <math.h>

@@ -205,7 +205,7 @@ def test_rows_in_wider_buffers(ghip, M, N, K, xt, pad, off):
 
 
 @pytest.mark.parametrize("xt", XTYPES)
-def test_k_past_the_row_forms(ghip, xt):
+def test_long_k(ghip, xt):
     """A row of x longer than LDS: few rows go to tiles."""
     M, N, K = 3, 40, (1 << 17) + 96
     rng = seed(50, xt)

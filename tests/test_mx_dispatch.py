@@ -49,8 +49,8 @@ def test_every_kernel_is_the_pick_of_some_shape(lib, mode, xt):
 @pytest.mark.parametrize("xt", [0, 1, 2])
 def test_few_rows_stream_and_many_take_tiles(lib, mode, xt):
     for N, K in [(4096, 4096), (12288, 4096), (4096, 12288)]:
-        # the linear with BF16 x has no row forms
-        few = "tiles" if (mode, xt) == (F.LINEAR, 0) else "rows"
+        # the linear has no row forms
+        few = "tiles" if mode == F.LINEAR else "rows"
         assert all(pick(lib, mode, xt, M, N, K)[0] == few for M in (1, 4, 16))
         assert pick(lib, mode, xt, 4096, N, K)[0] == "tiles"
 
@@ -59,10 +59,10 @@ def test_few_rows_stream_and_many_take_tiles(lib, mode, xt):
 def test_what_each_kind_takes(lib, xt):
     """A k too long for a row of x in LDS goes to tiles, one too long for their offsets to rows or nowhere; outputs of more
     workgroups than a launch takes go to rows."""
-    assert picks(lib, F.LINEAR, xt, 1, 64, 1 << 21)[1][0] == -1 and pick(lib, F.LINEAR, xt, 1, 64, 1 << 21)[0] == "tiles"
-    assert pick(lib, F.LINEAR, xt, 1, 64, 1 << 24) == ("tiles", -1)
-    assert picks(lib, F.LINEAR, xt, (1 << 31) - 1, (1 << 31) - 1, 32)[0][0] == -1
-    assert pick(lib, F.LINEAR, xt, (1 << 31) - 1, (1 << 31) - 1, 32)[0] == ("rows" if xt else "tiles")
+    assert picks(lib, F.GATED, xt, 1, 64, 1 << 21)[1][0] == -1 and pick(lib, F.GATED, xt, 1, 64, 1 << 21)[0] == "tiles"
+    assert pick(lib, F.GATED, xt, 1, 64, 1 << 24) == ("tiles", -1)
+    assert picks(lib, F.GATED, xt, (1 << 31) - 1, (1 << 31) - 1, 32)[0][0] == -1
+    assert pick(lib, F.GATED, xt, (1 << 31) - 1, (1 << 31) - 1, 32)[0] == "rows"
     # what the entries let through has a kernel: any stride up to k of 2^15 (not the linear's with BF16 x), less than 2^22
     # elements to 2^22
     for mode in (F.LINEAR, F.GATED):
