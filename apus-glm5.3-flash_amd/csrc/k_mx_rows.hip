@@ -148,7 +148,8 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
      * its own) */
     auto stream = [&](int b, const uint8_t *m, const uint8_t *m2, uint32_t ld) {
         const uint32_t r0 = (lblk * GPP + slot) * (16u * OG) + 16u * (DUAL ? b >> 1 : b);
-        const uint32_t live = lblk < blocks && r0 < p.N ? min(p.N - r0, 16u) : 0u;
+        /* no subtraction that wraps, not even one whose result is thrown away (build.py's flags) */
+        const uint32_t live = lblk < blocks ? max(min(r0 + 16u, p.N), r0) - r0 : 0u;
         return __builtin_amdgcn_make_buffer_rsrc((void *)((DUAL && (b & 1) ? m2 : m) + (size_t)r0 * ld), 0, live * ld, 0x20000);
     };
     auto load_scales = [&]() {
