@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
     const uint32_t br = mg_row<WB>(DUAL ? wv >> 1 : wv, lane), bq = mg_byte<WB>(lane, br), bo = br * wb + bq;
     const uint32_t astep = mg_rows_apart<XB, NW>(false) * xld, bstep = mg_rows_apart<WB, NW>(DUAL) * wb;
     const uint32_t xrow = BF ? 2u * p.K : XT == GHIP_MXFP8 ? p.K : wb;   /* bytes of x's row */
-    uint32_t jl = 0, sl = 0;                             /* the next step to load, its slot */
+    uint32_t sl = 0;                                     /* slot of the next step to load */
     int32_t xleft = (int32_t)xrow, wleft = (int32_t)wb;
     auto load = [&](uint32_t i) {
         if (i < NAL) {
@@ -152,7 +152,6 @@ __global__ __launch_bounds__(64 * WM * WN, 1) void k_mx_gemm(GhipMxProd p, GhipE
         }
     };
     auto next_load = [&]() {
-        jl++;
         pa += XB;
         pb += WB;
         xleft -= (int32_t)XB;

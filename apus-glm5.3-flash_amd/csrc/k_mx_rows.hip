@@ -21,12 +21,9 @@
 
 #include "ghip_epilogue.h"
 #include "ghip_mx.h"
-#include "k_ffn_addr.h"
+#include "k_mx_rows_addr.h"
 
 typedef int mx_i32x8 __attribute__((ext_vector_type(8)));
-
-#define MR_WAVES 8
-#define MR_OOB 0xFFFFFFF0u                       /* past every buffer */
 
 /* acc += W (MXFP4, 16 rows) . x^T (16 rows) over 128 k. Lane (n, g): W's row n, block
  * g; x's row n, bytes as its type has them (MXFP8: k 16 g + [0, 16) and 64 + 16 g +
@@ -71,60 +68,44 @@ __device__ __forceinline__ uint32_t mr_transpose(uint32_t v, const MrBytes &b) {
     return __builtin_amdgcn_perm(h[1], h[0], b.s32);
 }
 
-/* Bytes of x's row in a step, and where piece q of row r lies in LDS: the 16 rows that
- * one lane group reads are in distinct banks. */
-template <int XT>
-constexpr uint32_t mr_xrow() { return XT == GHIP_BF16 ? 256u : XT == GHIP_MXFP8 ? 128u : 64u; }
-template <int XT>
-__device__ __forceinline__ uint32_t mr_spot(uint32_t r, uint32_t q) {
-    constexpr uint32_t XR = mr_xrow<XT>();
-    return r * XR + 16u * (XT == GHIP_BF16 ? q ^ (r & 15u) : XT == GHIP_MXFP8 ? q ^ fg_rot8(r) : q ^ fg_rot4(r));
-}
+/* Bytes of x's row in a step. */
+constexpr uint32_t mr_xrow(int xt) { return xt == GHIP_BF16 ? 256u : xt == GHIP_MXFP8 ? 128u : 64u; }
 
-/* Most steps of a wave's share. */
-template <uint32_t KS>
-__host__ __device__ constexpr uint32_t mr_share(uint32_t nst) {
-    return 2u * (((nst + 1u) / 2u + KS - 1u) / KS);
-}
-
-/* A workgroup's 8 waves: 8 / KS groups of 16 NT weight rows, k over KS waves; mr (up
+/* A workgroup's 8 waves: 8 / KS slots of 16 rows of both matrices, k over KS waves; mr (up
  * to 16) rows of x. It takes every gridDim.x-th block of weight rows: a wave copies its share
- * of x to LDS once, and its stream of weights, 4 Q steps of 128 k ahead with one load
+ * of x to LDS once, and its stream of weights, four steps of 128 k ahead with one load
  * of scales for four, runs on from one block into the next. */
-template <int XT, int NT, int KS, int MODE>
+template <int XT, int KS>
 __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, GhipEp ep, uint32_t blocks,
                                                               uint32_t row0, uint32_t mr) {
-    constexpr bool DUAL = ghip_ep_dual(MODE), BF = XT == GHIP_BF16;
-    constexpr uint32_t GPP = MR_WAVES / KS, OG = DUAL ? NT / 2 : NT, XR = mr_xrow<XT>();
+    constexpr bool BF = XT == GHIP_BF16;
+    constexpr uint32_t GPP = MR_WAVES / KS, XR = mr_xrow(XT);
     constexpr int XI = BF ? 4 : XT == GHIP_MXFP8 ? 2 : 1;          /* 16-byte pieces of x a step */
-    constexpr uint32_t RED = MR_WAVES * 256u * NT;                 /* f32 sums of a block */
-    static_assert(!DUAL || NT % 2 == 0, "gate and up groups alternate");
     extern __shared__ __attribute__((aligned(16))) float red[];    /* the sums, W's way to its operands, x */
     const uint32_t tid = threadIdx.x, lane = tid & 63u, n = lane & 15u, g = lane >> 4;
     const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t part = wv % KS, slot = wv / KS;
-    const uint32_t nst = (p.K + 127u) >> 7, nb = p.K >> 5, lds = 4u * nst;
-    /* the wave's share, whole lines of W's rows: steps c0 .. c1 */
-    const uint32_t np = (nst + 1u) >> 1, c0 = 2u * (part * np / KS), c1 = min(2u * ((part + 1u) * np / KS), nst);
-    const uint32_t nc = c1 - c0, nq = (nc + 3u) >> 2;
+    const uint32_t nst = mr_steps(p.K), nb = p.K >> 5, lds = 4u * nst;
+    const MrShare share = mr_share<KS>(part, nst);
+    const uint32_t c0 = share.from, c1 = share.to, nc = c1 - c0, nq = (nc + 3u) >> 2;
     const uint32_t m0 = row0 + blockIdx.y * mr, mrows = min(p.M - m0, mr);
 
     /* x's rows over the wave's share: [step][row][XR], zeros past K. The first loads go
      * ahead of the weights', the rest behind them */
-    uint8_t *const wl = (uint8_t *)(red + RED) + wv * (2048u * NT);
-    uint8_t *const xl = (uint8_t *)(red + RED) + MR_WAVES * (2048u * NT) + wv * (mrows * XR * mr_share<KS>(nst));
-    constexpr uint32_t PP = XR / 16u;                    /* pieces of a row in a step */
-    const uint32_t per = nc * PP, all = mrows * per, xbytes = p.K * (BF ? 4u : XT == GHIP_MXFP8 ? 2u : 1u) / 2u;
+    uint8_t *const wl = (uint8_t *)red + mr_lds_codes(wv);
+    uint8_t *const xl = (uint8_t *)red + mr_lds_x(wv, mrows, XR, mr_share_most(nst, KS));
+    const uint32_t all = mrows * nc * (XR / 16u), xbytes = p.K * (BF ? 4u : XT == GHIP_MXFP8 ? 2u : 1u) / 2u;
     ghip_u32x4 xd[8];
     uint32_t xat[8];
     auto x_load = [&](uint32_t v0) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const uint32_t v = v0 + 64u * i + lane, r = v / per, e = v - r * per, t = e / PP, q = e % PP;
-            const uint32_t byte = (c0 + t) * XR + 16u * q;
+            const uint32_t v = v0 + 64u * i + lane;
+            const MrPiece at = mr_piece<XR>(v, nc);
+            const uint32_t byte = (c0 + at.t) * XR + 16u * at.q;
             xd[i] = (ghip_u32x4){0u, 0u, 0u, 0u};
-            xat[i] = v < all ? t * (mrows * XR) + mr_spot<XT>(r, q) : ~0u;
-            if (v < all && byte < xbytes) xd[i] = *(const ghip_u32x4 *)(p.x + (size_t)(m0 + r) * p.xld + byte);
+            xat[i] = v < all ? at.t * (mrows * XR) + mr_spot<XR>(at.r, at.q) : ~0u;
+            if (v < all && byte < xbytes) xd[i] = *(const ghip_u32x4 *)(p.x + (size_t)(m0 + at.r) * p.xld + byte);
         }
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -140,35 +121,33 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
     uint32_t lblk = blockIdx.x, lq = 0;
     const uint32_t mine = min(n, mrows - 1u);
     const uint8_t *const xs = BF ? nullptr : p.xs + (size_t)(m0 + mine) * lds;
-    ghip_u32x4 wr[4][NT];
-    uint32_t sw[NT], sx = 0u, bw[NT], bx = 0u;
+    ghip_u32x4 wr[4][2];
+    uint32_t sw[2], sx = 0u, bw[2], bx = 0u;
     /* The stream's next four steps: their scales, and half h of their codes (two steps).
      * What lies past the wave's share, a row's end, the matrix or the stream is past the
      * buffer: zeros, and no access (a second load from a line on its way costs a trip of
      * its own) */
-    auto stream = [&](int b, const uint8_t *m, const uint8_t *m2, uint32_t ld) {
-        const uint32_t r0 = (lblk * GPP + slot) * (16u * OG) + 16u * (DUAL ? b >> 1 : b);
-        /* no subtraction that wraps, not even one whose result is thrown away (build.py's flags) */
-        const uint32_t live = lblk < blocks ? max(min(r0 + 16u, p.N), r0) - r0 : 0u;
-        return __builtin_amdgcn_make_buffer_rsrc((void *)((DUAL && (b & 1) ? m2 : m) + (size_t)r0 * ld), 0, live * ld, 0x20000);
+    auto stream = [&](const uint8_t *m, uint32_t ld) {
+        const uint32_t first = mr_first<KS>(lblk, slot);
+        /* a vector instruction counts: back to a scalar, or the load goes lane by lane */
+        const uint32_t live = __builtin_amdgcn_readfirstlane(mr_live(first, p.N));
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(m + (size_t)mr_base(first, p.N) * ld), 0, live * ld, 0x20000);
     };
     auto load_scales = [&]() {
         const uint32_t t = c0 + 4u * lq + g;
 #pragma unroll
-        for (int b = 0; b < NT; b++)
-            sw[b] = __builtin_amdgcn_raw_buffer_load_b32(stream(b, p.ws, p.ws2, lds), t < nst ? n * lds + 4u * t : MR_OOB, 0, 0);
+        for (int b = 0; b < 2; b++)
+            sw[b] = __builtin_amdgcn_raw_buffer_load_b32(stream(b ? p.ws2 : p.ws, lds), mr_scale(n, t, nst), 0, 0);
         if constexpr (!BF) sx = *(const uint32_t *)(xs + 4u * min(t, nst - 1u));
     };
     auto load_codes = [&](auto h_c) {
         constexpr int h = decltype(h_c)::value;
 #pragma unroll
-        for (int b = 0; b < NT; b++) {
-            const __amdgpu_buffer_rsrc_t m = stream(b, p.w, p.w2, wb);
+        for (int b = 0; b < 2; b++) {
+            const __amdgpu_buffer_rsrc_t m = stream(b ? p.w2 : p.w, wb);
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint32_t r = 8u * i + (lane >> 3), byte = 64u * (c0 + 4u * lq + 2u * h) + 16u * ((lane & 7u) ^ fg_rot8(r));
-                wr[2 * h + i][b] = __builtin_amdgcn_raw_buffer_load_b128(m, byte < wend ? r * wb + byte : MR_OOB, 0, 0);
-            }
+            for (int i = 0; i < 2; i++)
+                wr[2 * h + i][b] = __builtin_amdgcn_raw_buffer_load_b128(m, mr_code(i, lane, c0 + 4u * lq + 2u * h, wend, wb), 0, 0);
         }
     };
     auto advance = [&]() {
@@ -189,65 +168,39 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
         }
     }
 
-    /* the epilogue's inputs, on their way during the products: value v of a block's
-     * outputs is of thread v % 512 */
-    constexpr uint32_t NOUT = GPP * 256u * OG, NV = (NOUT + MR_WAVES * 64u - 1u) / (MR_WAVES * 64u);
-    uint16_t ein[NV], ebias[NV];
     uint32_t blk = blockIdx.x, j = 0;
-    auto place = [&](uint32_t v, uint32_t &m, uint32_t &o) {
-        const uint32_t sl = v / (256u * OG), e = v - sl * (256u * OG);
-        m = e / (16u * OG);
-        o = (blk * GPP + sl) * (16u * OG) + e % (16u * OG);
-        return v < NOUT && m < mrows && o < p.N;
-    };
-    auto inputs = [&]() {
+    ghip_f32x4 acc[2];
 #pragma unroll
-        for (uint32_t i = 0; i < NV; i++) {
-            uint32_t m, o;
-            const bool live = place(tid + i * (MR_WAVES * 64u), m, o);
-            ein[i] = live && ep.in ? ep.in[(size_t)(m0 + m) * ep.ldin + o] : (uint16_t)0;
-            ebias[i] = live && ep.bias ? ep.bias[o] : (uint16_t)0;
-        }
-    };
-    inputs();
-    ghip_f32x4 acc[NT];
-#pragma unroll
-    for (int b = 0; b < NT; b++) acc[b] = (ghip_f32x4){0.f, 0.f, 0.f, 0.f};
-    /* a block's end: the KS partial sums of each group, added in order (register i of a
-     * group: weight row 4 g + i, x's row n) */
+    for (int b = 0; b < 2; b++) acc[b] = (ghip_f32x4){0.f, 0.f, 0.f, 0.f};
+    /* a block's end: the KS partial sums of each slot, added in order (register i: weight
+     * row 4 g + i, x's row n); its outputs, one a thread */
     auto finish = [&]() {
         if (blk != blockIdx.x) {                         /* the block before has been read */
             __builtin_amdgcn_s_waitcnt(0xc07f);
             __builtin_amdgcn_s_barrier();
         }
 #pragma unroll
-        for (int b = 0; b < NT; b++) {
-            *(ghip_f32x4 *)(red + (wv * 16u + n) * (16u * NT) + 16u * b + 4u * g) = acc[b];
+        for (int b = 0; b < 2; b++) {
+            *(ghip_f32x4 *)(red + mr_sum_put(wv, n, b, g)) = acc[b];
             acc[b] = (ghip_f32x4){0.f, 0.f, 0.f, 0.f};
         }
         __builtin_amdgcn_s_waitcnt(0xc07f);
         __builtin_amdgcn_s_barrier();
-        ghip_with_act(ep.act, [&](auto act) {
+        const MrOut at = mr_out(tid);
+        const uint32_t o = mr_first<KS>(blk, at.slot) + at.c;
+        if (at.slot < GPP && at.m < mrows && o < p.N) {
+            const float *q = red + mr_sum_get<KS>(at.slot, at.m, at.c);
+            float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-            for (uint32_t i = 0; i < NV; i++) {
-                uint32_t m, o;
-                const uint32_t v = tid + i * (MR_WAVES * 64u);
-                if (!place(v, m, o)) continue;
-                const uint32_t sl = v / (256u * OG), c = v % (16u * OG);
-                /* dual: gate group, up group, ... of 16 columns */
-                const float *q = red + (sl * KS * 16u + m) * (16u * NT) + (DUAL ? 32u * (c >> 4) + (c & 15u) : c);
-                float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    s0 += q[k * 256u * NT];
-                    if (DUAL) s1 += q[k * 256u * NT + 16u];
-                }
-                ghip_ep_put<MODE, decltype(act)::value>(ep, ep.out, m0 + m, o, s0, s1, ghip_bf16_f32(ebias[i]),
-                                                        ghip_bf16_f32(ein[i]));
+            for (int k = 0; k < KS; k++) {
+                s0 += q[k * 512u];
+                s1 += q[k * 512u + 16u];
             }
-        });
+            ghip_with_act(ep.act, [&](auto act) {
+                ghip_ep_put<GHIP_EP_GATED, decltype(act)::value>(ep, ep.out, m0 + at.m, o, s0, s1, 0.0f, 0.0f);
+            });
+        }
         blk += gridDim.x;
-        if (blk < blocks) inputs();
     };
     if (nc == 0u) {                                      /* fewer steps than waves */
         while (blk < blocks) finish();
@@ -256,12 +209,12 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
     const MrBytes bytes = mr_bytes(g);
     uint32_t xo[XI];
 #pragma unroll
-    for (int i = 0; i < XI; i++) xo[i] = mr_spot<XT>(mine, BF ? 4u * g + i : XT == GHIP_MXFP8 ? 4u * i + g : g);
-    const uint32_t w0 = fg_at0(n, g), w1 = fg_at0(n, 4u + g);
+    for (int i = 0; i < XI; i++) xo[i] = mr_spot<XR>(mine, mr_operand<XR>(g, i));
+    const uint32_t w0 = mr_code_get(n, g, 0), w1 = mr_code_get(n, g, 1);
     for (;;) {
         const uint32_t t = c0 + 4u * j;
 #pragma unroll
-        for (int b = 0; b < NT; b++) bw[b] = mr_transpose(sw[b], bytes);
+        for (int b = 0; b < 2; b++) bw[b] = mr_transpose(sw[b], bytes);
         if constexpr (!BF) bx = mr_transpose(sx, bytes);
         load_scales();
         mr_each<2>([&](auto h_c) {
@@ -269,19 +222,18 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
             /* two steps of W to LDS as they were loaded, the registers' next load, and back
              * as operands; a wave's LDS accesses are in order */
 #pragma unroll
-            for (int b = 0; b < NT; b++) {
-                *(ghip_u32x4 *)(wl + 2048 * b + 16u * lane) = wr[2 * h][b];
-                *(ghip_u32x4 *)(wl + 2048 * b + 1024 + 16u * lane) = wr[2 * h + 1][b];
-            }
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) *(ghip_u32x4 *)(wl + 2048 * b + mr_code_put(i, lane)) = wr[2 * h + i][b];
             __builtin_amdgcn_sched_barrier(0);
             load_codes(h_c);
             __builtin_amdgcn_sched_barrier(0);
             if (t + 2u * h >= c1) return;
-            ghip_u32x4 wo[2][NT];
+            ghip_u32x4 wo[2][2];
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
-                for (int b = 0; b < NT; b++) wo[i][b] = *(const ghip_u32x4 *)(wl + 2048 * b + (i ? w1 : w0));
+                for (int b = 0; b < 2; b++) wo[i][b] = *(const ghip_u32x4 *)(wl + 2048 * b + (i ? w1 : w0));
             mr_each<2>([&](auto i_c) {
                 constexpr int i = decltype(i_c)::value, s = 2 * h + i;
                 if (i && t + s >= c1) return;
@@ -291,7 +243,7 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
 #pragma unroll
                 for (int k = 0; k < XI; k++) xr[k] = *(const ghip_u32x4 *)(xt + xo[k]);
 #pragma unroll
-                for (int b = 0; b < NT; b++) {
+                for (int b = 0; b < 2; b++) {
                     const uint32_t sb = past ? 127u : bw[b] >> (8 * s) & 255u;
                     if constexpr (BF) {
                         const float f = __uint_as_float(sb << 23);
@@ -316,89 +268,70 @@ __global__ __launch_bounds__(MR_WAVES * 64, 1) void k_mx_rows(GhipMxProd p, Ghip
     }
 }
 
-/* One launchable form: output columns, and microseconds of the launch, of four steps of
+/* One launchable form: k's waves, and microseconds of the launch, of four steps of
  * a wave, of a block besides, and of a KB of a wave's share of x; two: how much longer
  * these are where CUs hold two workgroups. The times are least-squares fits to sweeps of
  * 1 to 192 rows over N x K of 256 x 1024 to 12288 x 4096, 4096 x 12288, 8192 x 512 and 512 x
- * 8192, every form timed (0.05 to 0.1 rms of the logarithm). Two groups
- * share an operand of x but make fewer workgroups, 8 waves along k shorten a wave's chain
- * and 4 halve the joins. BF16, NT x KS,
- * us:                          2x8    2x4
- *   gated 4 x 12288 x 4096    15.6   13.6
- *   gated 1 x 256 x 1024       4.2    4.8 */
+ * 8192, every form timed (0.05 to 0.1 rms of the logarithm). 8 waves along k shorten a
+ * wave's chain and 4 halve the joins; BF16, us:
+ *                         8 waves   4
+ *   4 x 12288 x 4096         15.6   13.6
+ *   1 x 256 x 1024            4.2    4.8 */
 struct MrForm {
-    uint32_t cols, nt, ks, red;
+    uint32_t ks;
     float base, quad, over, copy, two;
     const void *kern;
     void (*launch)(dim3, uint32_t, hipStream_t, const GhipMxProd &, const GhipEp &, uint32_t, uint32_t,
                    uint32_t);
 };
-template <int XT, int NT, int KS, int MODE>
+template <int XT, int KS>
 static void mr_run(dim3 grid, uint32_t lds, hipStream_t st, const GhipMxProd &p, const GhipEp &ep,
                    uint32_t blocks, uint32_t row0, uint32_t mr) {
-    hipLaunchKernelGGL((k_mx_rows<XT, NT, KS, MODE>), grid, dim3(MR_WAVES * 64), lds, st, p, ep, blocks, row0, mr);
+    hipLaunchKernelGGL((k_mx_rows<XT, KS>), grid, dim3(MR_WAVES * 64), lds, st, p, ep, blocks, row0, mr);
 }
-template <int XT, int NT, int KS, int MODE>
+template <int XT, int KS>
 static constexpr MrForm mr_form(float base, float quad, float over, float copy, float two) {
-    return {(ghip_ep_dual(MODE) ? 8u : 16u) * NT * (MR_WAVES / KS), NT, KS, MR_WAVES * 256u * NT * 4u, base, quad, over, copy, two,
-            (const void *)k_mx_rows<XT, NT, KS, MODE>, mr_run<XT, NT, KS, MODE>};
+    return {KS, base, quad, over, copy, two, (const void *)k_mx_rows<XT, KS>, mr_run<XT, KS>};
 }
 
-static const MrForm mr_gated_bf16[] = {
-    mr_form<GHIP_BF16, 2, 8, GHIP_EP_GATED>(1.6f, 1.70f, 0.47f, 0.19f, 0.95f),
-    mr_form<GHIP_BF16, 2, 4, GHIP_EP_GATED>(1.9f, 1.86f, 0.20f, 0.16f, 0.87f),
+static const MrForm mr_bf16[] = {
+    mr_form<GHIP_BF16, 8>(1.6f, 1.70f, 0.47f, 0.19f, 0.95f),
+    mr_form<GHIP_BF16, 4>(1.9f, 1.86f, 0.20f, 0.16f, 0.87f),
 };
-static const MrForm mr_gated_mxfp8[] = {
-    mr_form<GHIP_MXFP8, 2, 8, GHIP_EP_GATED>(1.8f, 1.49f, 0.57f, 0.17f, 0.90f),
-    mr_form<GHIP_MXFP8, 2, 4, GHIP_EP_GATED>(1.7f, 1.39f, 0.94f, 0.17f, 0.87f),
+static const MrForm mr_mxfp8[] = {
+    mr_form<GHIP_MXFP8, 8>(1.8f, 1.49f, 0.57f, 0.17f, 0.90f),
+    mr_form<GHIP_MXFP8, 4>(1.7f, 1.39f, 0.94f, 0.17f, 0.87f),
 };
-static const MrForm mr_gated_mxfp4[] = {
-    mr_form<GHIP_MXFP4, 2, 8, GHIP_EP_GATED>(1.6f, 0.84f, 1.28f, 0.32f, 1.34f),
-    mr_form<GHIP_MXFP4, 2, 4, GHIP_EP_GATED>(2.1f, 1.56f, 0.48f, 0.10f, 0.95f),
+static const MrForm mr_mxfp4[] = {
+    mr_form<GHIP_MXFP4, 8>(1.6f, 0.84f, 1.28f, 0.32f, 1.34f),
+    mr_form<GHIP_MXFP4, 4>(2.1f, 1.56f, 0.48f, 0.10f, 0.95f),
 };
-/* The gated mode's only: the linear's forms are off, as two runs of their tests ended in a
- * memory fault whose cause has not been found. */
+/* The gated mode's only. */
 static const MrForm *mr_forms(int mode, int xt, int *n) {
     *n = mode == GHIP_EP_GATED ? 2 : 0;
-    return xt == GHIP_MXFP8 ? mr_gated_mxfp8 : xt == GHIP_MXFP4 ? mr_gated_mxfp4 : mr_gated_bf16;
+    if (mode != GHIP_EP_GATED) return nullptr;
+    return xt == GHIP_MXFP8 ? mr_mxfp8 : xt == GHIP_MXFP4 ? mr_mxfp4 : mr_bf16;
 }
 
-#define MR_LDS_MAX (160u * 1024u)
 #define MR_MAX_TILES 65535u
 
 static uint32_t g_mr_ncu = 256;
 
-/* How a form takes this shape: the rows of a tile, as many as fit beside the sums and
- * two steps of weights (up to 16, tiles of as many rows each), and its LDS; 0 rows: k
- * is too long. */
-struct MrPlan {
-    uint32_t mr, tiles, lds, blocks, grid, turns;
-    float us;                            /* estimated */
-};
-static MrPlan plan(const MrForm *c, const GhipMxProd *p) {
-    const size_t nst = ((size_t)p->K + 127) / 128;
-    const size_t row = MR_WAVES * (p->xt == GHIP_BF16 ? 256 : p->xt == GHIP_MXFP8 ? 128 : 64) * 2 * (((nst + 1) / 2 + c->ks - 1) / c->ks);
-    const size_t rest = c->red + MR_WAVES * 2048 * c->nt;
-    size_t most = (MR_LDS_MAX - rest) / row;
-    if (most > 16) most = 16;
-    MrPlan r = {};
-    if (most == 0) return r;
-    r.tiles = (uint32_t)(((size_t)p->M + most - 1) / most);
-    r.mr = (uint32_t)(((size_t)p->M + r.tiles - 1) / r.tiles);
-    r.lds = (uint32_t)(rest + r.mr * row);
-    r.blocks = (uint32_t)(((size_t)p->N + c->cols - 1) / c->cols);
-    /* as many workgroups as there is room for, each with as many blocks of weights */
-    const size_t occ = r.lds <= MR_LDS_MAX / 2 ? 2 : 1, room = (g_mr_ncu * occ + r.tiles - 1) / r.tiles;
-    r.turns = (uint32_t)((r.blocks + room - 1) / room);
-    r.grid = (r.blocks + r.turns - 1) / r.turns;
-    /* the rounds of the chip, or the weights at 6.5 TB/s, and a tenth of the other */
-    const double quads = (double)((((nst + 1) / 2 + c->ks - 1) / c->ks + 1) / 2);
-    const double rounds = (double)(((size_t)r.grid * r.tiles + g_mr_ncu * occ - 1) / (g_mr_ncu * occ));
+static MrCut cut(const MrForm *c, const GhipMxProd *p) {
+    return mr_cut(p->M, p->N, p->K, mr_xrow(p->xt), c->ks, g_mr_ncu);
+}
+
+/* Estimated microseconds: the rounds of the chip, or the weights at 6.5 TB/s, and a
+ * tenth of the other. */
+static float form_us(const MrForm *c, const GhipMxProd *p, const MrCut &r) {
+    const uint32_t most = mr_share_most(mr_steps(p->K), c->ks);
+    const double quads = (double)((most / 2 + 1) / 2), chip = (double)g_mr_ncu * r.occ;
+    const double rounds = (double)(size_t)(((double)r.grid * r.tiles + chip - 1.0) / chip);
     const double two = (size_t)r.grid * r.tiles > g_mr_ncu ? c->two : 1.0;
-    const double chain = c->base + two * rounds * (r.turns * (quads * c->quad + c->over) + (double)(r.mr * row) / MR_WAVES / 1024.0 * c->copy);
-    const double hbm = 2.6 + (double)p->N * p->K * (p->w2 ? 2 : 1) * 17.0 / 32.0 / 6.5e6;
-    r.us = (float)(chain > hbm ? chain + 0.1 * hbm : hbm + 0.1 * chain);
-    return r;
+    const double copy = (double)r.mr * mr_xrow(p->xt) * most / 1024.0;
+    const double chain = c->base + two * rounds * (r.turns * (quads * c->quad + c->over) + copy * c->copy);
+    const double hbm = 2.6 + 2.0 * p->N * p->K * 17.0 / 32.0 / 6.5e6;
+    return (float)(chain > hbm ? chain + 0.1 * hbm : hbm + 0.1 * chain);
 }
 
 extern "C" int ghip_mx_rows_forms(int mode, int xt) {
@@ -410,17 +343,19 @@ extern "C" int ghip_mx_rows_forms(int mode, int xt) {
 extern "C" int ghip_mx_rows_fits(int mode, int form, const GhipMxProd *p) {
     int n;
     const MrForm *c = mr_forms(mode, p->xt, &n);
-    return form >= 0 && form < n && plan(c + form, p).mr != 0u;
+    return form >= 0 && form < n && cut(c + form, p).mr != 0u;
 }
 
 extern "C" int ghip_mx_rows_pick(int mode, const GhipMxProd *p, float *us) {
     int n, best = -1;
     const MrForm *c = mr_forms(mode, p->xt, &n);
     for (int i = 0; i < n; i++) {
-        const MrPlan r = plan(c + i, p);
-        if (r.mr != 0u && (best < 0 || r.us < *us)) {
+        const MrCut r = cut(c + i, p);
+        if (r.mr == 0u) continue;
+        const float t = form_us(c + i, p, r);
+        if (best < 0 || t < *us) {
             best = i;
-            *us = r.us;
+            *us = t;
         }
     }
     return best;
@@ -429,11 +364,10 @@ extern "C" int ghip_mx_rows_pick(int mode, const GhipMxProd *p, float *us) {
 extern "C" hipError_t ghip_launch_mx_rows(int mode, int form, const GhipMxProd *p, const GhipEp *ep, hipStream_t st) {
     int n;
     const MrForm *c = mr_forms(mode, p->xt, &n);
-    if (p->M == 0 || p->N == 0 || p->K == 0 || p->K % 32 || (mode != GHIP_EP_LINEAR && mode != GHIP_EP_GATED)
-        || !ghip_mx_rows_fits(mode, form, p))
+    if (p->M == 0 || p->N == 0 || p->K == 0 || p->K % 32 || !ghip_mx_rows_fits(mode, form, p))
         return hipErrorInvalidValue;
     c += form;
-    const MrPlan r = plan(c, p);
+    const MrCut r = cut(c, p);
     for (uint32_t t = 0; t < r.tiles; t += MR_MAX_TILES) {
         const uint32_t nt = r.tiles - t < MR_MAX_TILES ? r.tiles - t : MR_MAX_TILES;
         c->launch(dim3(r.grid, nt), r.lds, st, *p, *ep, r.blocks, t * r.mr, r.mr);
@@ -444,9 +378,9 @@ extern "C" hipError_t ghip_launch_mx_rows(int mode, int form, const GhipMxProd *
 }
 
 extern "C" hipError_t ghip_mx_rows_init(uint32_t n_cu) {
-    for (int i = 0; i < 6; i++) {
+    for (int xt = GHIP_BF16; xt <= GHIP_MXFP4; xt++) {
         int n;
-        const MrForm *c = mr_forms(i & 1 ? GHIP_EP_GATED : GHIP_EP_LINEAR, i >> 1, &n);
+        const MrForm *c = mr_forms(GHIP_EP_GATED, xt, &n);
         for (int k = 0; k < n; k++) {
             const hipError_t e = hipFuncSetAttribute(c[k].kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)MR_LDS_MAX);
             if (e != hipSuccess) return e;
