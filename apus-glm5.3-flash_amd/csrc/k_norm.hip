@@ -106,13 +106,30 @@ __device__ __forceinline__ float nm_rstd(float sum, uint32_t D, float eps) {
     return 1.0f / sqrtf(sum / (float)D + eps);
 }
 
-/* y's columns [col, col + 8) */
+/* What a row with this rstd is multiplied by before its squares and products are added: 1,
+ * or, of rows below 2^-50 and past 2^50, the power of two that keeps these sums f32
+ * numbers. Exact, so the sums are the same where the row's own would have been. */
+__device__ __forceinline__ float nm_up(float rstd) {
+    const uint32_t low = 77u << 23, high = 177u << 23;   /* 2^-50, 2^50 */
+    if (__float_as_uint(rstd) - low <= high - low) return 1.0f;
+    return rstd > 1.0f ? 0x1p80f : rstd < 1.0f ? 0x1p-80f : 1.0f;
+}
+
+__device__ __forceinline__ void nm_squares(const nm_u16x8 &s, float up, float (&sum)[1]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float v = ghip_bf16_f32(s[e]) * up;
+        sum[0] += v * v;
+    }
+}
+
+/* y's columns [col, col + 8); rstd of the row times up */
 __device__ __forceinline__ void nm_out(const GhipNorm &p, size_t row, uint32_t col, const nm_u16x8 &s,
-                                       const nm_u16x8 &g, float rstd) {
+                                       const nm_u16x8 &g, float up, float rstd) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        v[e] = ghip_bf16_f32(s[e]) * rstd;
+        v[e] = ghip_bf16_f32(s[e]) * up * rstd;
         if (p.gamma) v[e] *= ghip_bf16_f32(g[e]);
     }
     if (p.y) nm_store(p.y + row * p.ldy, col, p.D, nm_pack(v));
@@ -152,19 +169,27 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm(GhipNorm p, size_
         if (col < p.D) {
             if (p.r) s[i] = nm_add(s[i], g[i]);
             if (p.gamma) g[i] = nm_load(p.gamma, col, p.D);
-#pragma unroll
-            for (int e = 0; e < 8; e++) sum[0] += ghip_bf16_f32(s[i][e]) * ghip_bf16_f32(s[i][e]);
+            nm_squares(s[i], 1.0f, sum);
         }
     }
     nm_sum<T, 1>(sum, lds);
-    const float rstd = nm_rstd(sum[0], p.D, p.eps);
-    if (p.rstd && t == 0u) p.rstd[row] = rstd;
+    float rstd = nm_rstd(sum[0], p.D, p.eps);
+    const float up = nm_up(rstd);
+    if (up != 1.0f) {                            /* the whole row's threads */
+        sum[0] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            if (8u * (t + T * i) < p.D) nm_squares(s[i], up, sum);
+        nm_sum<T, 1>(sum, lds);
+        rstd = nm_rstd(sum[0], p.D, p.eps * up * up);
+    }
+    if (p.rstd && t == 0u) p.rstd[row] = rstd * up;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const uint32_t col = 8u * (t + T * i);
         if (col < p.D) {
             if (p.sum) nm_store(p.sum + row * p.lds, col, p.D, s[i]);
-            nm_out(p, row, col, s[i], g[i], rstd);
+            nm_out(p, row, col, s[i], g[i], up, rstd);
         }
     }
 }
@@ -180,18 +205,21 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_long(GhipNorm p, size_t row0) 
         const nm_u16x8 d = nm_load(x, col, p.D);
         return q ? nm_add(d, nm_load(q, col, p.D)) : d;
     };
-    for (uint32_t col = 8u * threadIdx.x; col < p.D; col += 8192u) {
-        const nm_u16x8 d = value(col);
-#pragma unroll
-        for (int e = 0; e < 8; e++) sum[0] += ghip_bf16_f32(d[e]) * ghip_bf16_f32(d[e]);
-    }
+    for (uint32_t col = 8u * threadIdx.x; col < p.D; col += 8192u) nm_squares(value(col), 1.0f, sum);
     nm_sum<1024, 1>(sum, lds);
-    const float rstd = nm_rstd(sum[0], p.D, p.eps);
-    if (p.rstd && threadIdx.x == 0u) p.rstd[row] = rstd;
+    float rstd = nm_rstd(sum[0], p.D, p.eps);
+    const float up = nm_up(rstd);
+    if (up != 1.0f) {
+        sum[0] = 0.0f;
+        for (uint32_t col = 8u * threadIdx.x; col < p.D; col += 8192u) nm_squares(value(col), up, sum);
+        nm_sum<1024, 1>(sum, lds);
+        rstd = nm_rstd(sum[0], p.D, p.eps * up * up);
+    }
+    if (p.rstd && threadIdx.x == 0u) p.rstd[row] = rstd * up;
     for (uint32_t col = 8u * threadIdx.x; col < p.D; col += 8192u) {
         const nm_u16x8 d = value(col), g = p.gamma ? nm_load(p.gamma, col, p.D) : d;
         if (p.sum) nm_store(p.sum + row * p.lds, col, p.D, d);
-        nm_out(p, row, col, d, g, rstd);
+        nm_out(p, row, col, d, g, up, rstd);
     }
 }
 
@@ -214,13 +242,13 @@ __device__ __forceinline__ void nm_dx(const GhipNormGrad &p, size_t row, uint32_
     nm_store(p.dx + row * p.lddx, col, p.D, nm_pack(v));
 }
 
-/* Sums of gamma dy s and s^2 over these columns. */
+/* Sums of gamma dy s and s^2 over these columns, s times up. */
 __device__ __forceinline__ void nm_products(const GhipNormGrad &p, const nm_u16x8 &s, const nm_u16x8 &dy,
-                                            const nm_u16x8 &g, float (&sum)[2]) {
+                                            const nm_u16x8 &g, float up, float (&sum)[2]) {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         float d = ghip_bf16_f32(dy[e]);
-        const float v = ghip_bf16_f32(s[e]);
+        const float v = ghip_bf16_f32(s[e]) * up;
         if (p.gamma) d *= ghip_bf16_f32(g[e]);
         sum[0] += d * v;
         sum[1] += v * v;
@@ -272,10 +300,20 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm_grad(GhipNormGrad
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < V; i++)
-            if (8u * (t + T * i) < p.D) nm_products(p, s[i], dy[i], g[i], sum);
+            if (8u * (t + T * i) < p.D) nm_products(p, s[i], dy[i], g[i], 1.0f, sum);
         nm_sum<T, 2>(sum, lds);
-        const float a = p.rstd ? given : nm_rstd(sum[1], p.D, p.eps);
-        const float c = a * (sum[0] / (float)p.D);
+        float a = p.rstd ? given : nm_rstd(sum[1], p.D, p.eps);
+        float c = a * (sum[0] / (float)p.D);
+        const float up = nm_up(a);
+        if (up != 1.0f) {                        /* the whole row's threads */
+            sum[0] = sum[1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; i++)
+                if (8u * (t + T * i) < p.D) nm_products(p, s[i], dy[i], g[i], up, sum);
+            nm_sum<T, 2>(sum, lds);
+            if (!p.rstd) a = nm_rstd(sum[1], p.D, p.eps * up * up) * up;
+            c = a / up * (sum[0] / (float)p.D);
+        }
         if (row < p.M) {
 #pragma unroll
             for (int i = 0; i < V; i++) {
@@ -337,13 +375,13 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void k_rmsnorm_grad_few(GhipNorm
                 if (p.ds) ds[i] = nm_load(p.ds + row * p.ldds, col, p.D);
             }
         }
-        const float a = p.rstd[row];
+        const float a = p.rstd[row], up = nm_up(a);
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < V; i++)
-            if (8u * (t + T * i) < p.D) nm_products(p, s[i], dy[i], g[i], sum);
+            if (8u * (t + T * i) < p.D) nm_products(p, s[i], dy[i], g[i], up, sum);
         nm_sum<T, 2>(sum, lds);
-        const float c = a * (sum[0] / (float)p.D);
+        const float c = a / up * (sum[0] / (float)p.D);
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const uint32_t col = 8u * (t + T * i);
@@ -386,11 +424,17 @@ __global__ __launch_bounds__(1024) void k_rmsnorm_grad_long(GhipNormGrad p, size
     const uint16_t *s = p.s + row * p.lds, *dy = p.dy + row * p.lddy;
     float sum[2] = {0.0f, 0.0f};
     auto gamma = [&](uint32_t col) { return p.gamma ? nm_load(p.gamma, col, p.D) : nm_u16x8{}; };
-    for (uint32_t col = 8u * threadIdx.x; col < p.D; col += 8192u)
-        nm_products(p, nm_load(s, col, p.D), nm_load(dy, col, p.D), gamma(col), sum);
-    nm_sum<1024, 2>(sum, lds);
-    const float a = p.rstd ? p.rstd[row] : nm_rstd(sum[1], p.D, p.eps);
-    const float c = a * (sum[0] / (float)p.D);
+    float up = p.rstd ? nm_up(p.rstd[row]) : 1.0f;
+    auto add = [&]() {
+        sum[0] = sum[1] = 0.0f;
+        for (uint32_t col = 8u * threadIdx.x; col < p.D; col += 8192u)
+            nm_products(p, nm_load(s, col, p.D), nm_load(dy, col, p.D), gamma(col), up, sum);
+        nm_sum<1024, 2>(sum, lds);
+    };
+    add();
+    if (!p.rstd && (up = nm_up(nm_rstd(sum[1], p.D, p.eps))) != 1.0f) add();
+    const float a = p.rstd ? p.rstd[row] : nm_rstd(sum[1], p.D, p.eps * up * up) * up;
+    const float c = a / up * (sum[0] / (float)p.D);
     if (!p.dx) {
         if (threadIdx.x == 0u) p.part[row] = a;
         return;

@@ -473,8 +473,11 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
  * Common rules.
  *   - ldx, ldr, lds, ldy, ...: elements from one BF16 row to the next (0 = its
  *     width); the columns between rows are neither read into a result nor written.
- *   - Norm: sums, statistics and products are f32 (a row whose squares add up past
- *     the f32 range gives 0); s is rounded, then normed. residual, gamma (1), sum,
+ *   - Norm: sums, statistics and products are f32, of rows of any size: where the
+ *     squares leave the f32 range the row is scaled by a power of two first. rstd is
+ *     f32 too, so it is an infinity for rows below 2^-128 with an eps as small, whose
+ *     gradient is none then; a row of zeros with an eps of 0 is 0 / 0, NaN. s is
+ *     rounded, then normed. residual, gamma (1), sum,
  *     rstd [M] may be NULL; without residual s is x. sum or y may be x or residual
  *     itself (same ld): each element is read before it is written.
  *   - Projections: act, limit, bias, residual and rounding as the dense
