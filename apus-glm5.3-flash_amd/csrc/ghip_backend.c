@@ -1007,7 +1007,12 @@ static int mx_forward(int mode, const uint8_t *w, const uint8_t *ws, const uint8
                            .M = (uint32_t)M, .N = (uint32_t)O, .K = (uint32_t)K, .xt = x_type };
     const GhipEp ep = { .bias = bias, .in = residual, .out = y, .ldin = ldr, .ldout = ldy,
                         .act = act, .limit = limit > 0.0f ? limit : INFINITY };
-    HIPCHK(ghip_launch_mx(mode, &p, &ep, st));
+    const hipError_t e = ghip_launch_mx(mode, &p, &ep, st);
+    if (e == hipErrorNotSupported) {
+        ghip_seterr("%zu x %zu outputs: more tiles than a launch takes", M, O);
+        return 1;
+    }
+    HIPCHK(e);
     G.dispatches++;
     return 0;
 }

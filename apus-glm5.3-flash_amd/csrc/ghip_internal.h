@@ -422,6 +422,8 @@ typedef struct {
     uint32_t M, N, K;
     int xt;
 } GhipMxProd;
+/* hipErrorNotSupported: no kernel takes the shape (its outputs are more tiles than a launch
+ * takes), nothing was launched. */
 hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp *ep, hipStream_t st);
 /* Set-up, by ghip_ffn_init. */
 hipError_t ghip_mx_init(uint32_t n_cu);

@@ -8,8 +8,9 @@
  *   gated MXFP8, 4096 x 4096      16 rows 6.7 : 10.9
  *   gated MXFP8, 12288 x 4096     16 rows 13.0 : 17.0
  *   gated BF16, 12288 x 4096      16 rows 20.1 : 22.8
- * The linear takes tiles for any number of rows (k_mx_rows.hip). Tiles against each other in MXFP8: 300 x 1537 x 4096 32x64 10.0, 64x64 10.8, 128x128
- * 16.6, 256x256 46.3; 4096 x 4096 x 4096 175, 112, 69.6 (256x128), 57.8.
+ * The linear takes tiles for any number of rows (k_mx_rows.hip). Tiles against each other
+ * in MXFP8: 300 x 1537 x 4096 32x64 10.0, 64x64 10.8, 128x128 16.6, 256x256 46.3; 4096 x
+ * 4096 x 4096 175, 112, 69.6 (256x128), 57.8.
  */
 #include <math.h>
 
@@ -85,7 +86,8 @@ extern "C" hipError_t ghip_launch_mx(int mode, const GhipMxProd *p, const GhipEp
     float tile_t = 0.0f, rows_t = 0.0f;
     const int tile = ghip_mx_gemm_pick(mode, p, &tile_t), form = ghip_mx_rows_pick(mode, p, &rows_t);
     if (form >= 0 && (tile < 0 || rows_t <= tile_t)) return ghip_launch_mx_rows(mode, form, p, ep, st);
-    return ghip_launch_mx_gemm(mode, tile, p, ep, st);       /* -1: refused */
+    if (tile < 0) return hipErrorNotSupported;               /* ghip_internal.h */
+    return ghip_launch_mx_gemm(mode, tile, p, ep, st);
 }
 
 extern "C" hipError_t ghip_mx_init(uint32_t n_cu) {
