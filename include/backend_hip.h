@@ -468,7 +468,9 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
  * written as 0 and not read as scales. Quantizing takes the smallest power of two
  * (2^-127 at least) at which no value of the block is past 448 (6), and rounds to
  * nearest, ties to even; a block with a NaN or an infinity becomes NaN (scale 255,
- * codes 0).
+ * codes 0). This is not the scale of the OCP conversion, the block maximum's exponent
+ * less the type's, at which values past 448 (6) saturate: such codes differ, and are
+ * read all the same.
  *
  * Common rules.
  *   - ldx, ldr, lds, ldy, ...: elements from one BF16 row to the next (0 = its
@@ -477,12 +479,14 @@ int apus_ghip_bf16_gated_backward_dev(const uint16_t *wg, const uint16_t *wu, co
  *     squares leave the f32 range the row is scaled by a power of two first. rstd is
  *     f32 too, so it is an infinity for rows below 2^-128 with an eps as small, whose
  *     gradient is none then; a row of zeros with an eps of 0 is 0 / 0, NaN. s is
- *     rounded, then normed. residual, gamma (1), sum,
- *     rstd [M] may be NULL; without residual s is x. sum or y may be x or residual
- *     itself (same ld): each element is read before it is written.
+ *     rounded, then normed. residual, gamma (1), sum, rstd [M] may be NULL; without
+ *     residual s is x. sum or y may be x or residual itself (same ld): each element
+ *     is read before it is written.
  *   - Projections: act, limit, bias, residual and rounding as the dense
- *     feed-forward operators above; residual may be y. The matrix instruction adds
- *     the products of 32 k with 13 bits below the largest where one operand is
+ *     feed-forward operators above; residual may be y. BF16 x and the backward passes
+ *     take the weights as BF16: exactly, but for 2^128 and more (codes of 4 and 6 at
+ *     scale 253, of 2 and more at 254), which are infinities. The matrix instruction
+ *     adds the products of 32 k with 13 bits below the largest where one operand is
  *     MXFP8, everything else in f32.
  *   - Codes and BF16 x of the projections are 16-byte aligned, scales 4-byte, x's
  *     stride is whole 16 bytes (microscaled x is dense); all other matrices may have
