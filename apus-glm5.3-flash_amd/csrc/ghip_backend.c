@@ -1036,7 +1036,7 @@ int apus_ghip_mxfp4_gated_dev(const uint8_t *gate_codes, const uint8_t *gate_sca
 }
 
 /* The backward passes read the weights as BF16, which holds MXFP4 values exactly
- * (between 2^-126 and 2^127): n matrices of them stand in the workspace in front of
+ * (below 2^128): n matrices of them stand in the workspace in front of
  * that of the BF16 operator. */
 static size_t mx_wide(size_t O, size_t K) { return (O * K * 2 + 255) & ~(size_t)255; }
 

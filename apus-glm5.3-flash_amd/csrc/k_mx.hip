@@ -5,7 +5,7 @@
  * maximum takes two DPP steps; nothing goes through LDS. Four pieces a thread, all
  * loaded before the first is used.
  *
- * Measured: 12288 x 4096 to MXFP4 26.5 us and back 19.9 (127 MB each way: 4.8 and 6.4
+ * Measured: 12288 x 4096 to MXFP4 26.8 us and back 19.8 (127 MB each way: 4.8 and 6.4
  * TB/s), 1111 x 2048 to MXFP8 3.9 (a launch's time).
  */
 #include "ghip_mx.h"

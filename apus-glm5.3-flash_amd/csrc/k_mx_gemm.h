@@ -19,7 +19,7 @@
  * tests/test_mx_asm.py.
  *
  * Measured (us; TFLOP/s): MXFP4 8192 x 8192 x 8192 266 (4130), 4096^3 45.6 (3010);
- * MXFP8 8192^3 362 (3035), 4096^3 57.8 (2380), gated 8192 x 12288 x 4096 593-606 (2720-2780);
+ * MXFP8 8192^3 362 (3035), 4096^3 57.8 (2380), gated 8192 x 12288 x 4096 603-625 (2640-2740);
  * BF16 8192^3 791 (1390). The library's plain products of 8192^3 in the same types run at
  * 2990, 1290 and 1390.
  */

@@ -18,8 +18,8 @@
  * launch adds these in order. The next row is loaded while one is summed. Of a few rows
  * whose rstd is given one launch makes both, dgamma from s and dy read again.
  *
- * Measured: 8192 x 4096 with a residual to s and MXFP8 43.5 us (236 MB, 5.4 TB/s); its
- * gradient with ds 53.4 + 4.7 (268 MB and 17: 5.0 TB/s; 71.5 in all with no row loaded
+ * Measured: 8192 x 4096 with a residual to s and MXFP8 44.1 us (236 MB, 5.4 TB/s); its
+ * gradient with ds 53.0 + 4.9 (268 MB and 17: 5.0 TB/s; 71.5 in all with no row loaded
  * ahead); one row of 4096 3.0, a launch's time; 300 x 1536 gradient 3.5.
  */
 #include <type_traits>
