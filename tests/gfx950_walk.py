@@ -22,7 +22,7 @@ import numpy as np
 
 from test_ffn_asm import OBJDUMP
 
-VCC, EXEC = 106, 126                                                # register pairs
+VCC, EXEC, M0 = 106, 126, 124                                       # scalar registers; pairs, the first two
 FULL = (1 << 64) - 1
 LANES = np.arange(64)
 
@@ -65,12 +65,13 @@ def decode(s):
 
 
 def registers(t):
-    """("v" or "s", numbers) of an operand, or None."""
-    m = re.match(r"^[-|]*([vs])(?:(\d+)|\[(\d+):(\d+)\])\|?$", t)
+    """("v" or "s", numbers) of an operand, or None; accumulators are vector registers from 256 on."""
+    m = re.match(r"^[-|]*([vsa])(?:(\d+)|\[(\d+):(\d+)\])\|?$", t)
     if m:
-        a = int(m.group(2) or m.group(3))
-        return m.group(1), range(a, int(m.group(4) or a) + 1)
-    return {"vcc": ("s", range(VCC, VCC + 2)), "exec": ("s", range(EXEC, EXEC + 2))}.get(t)
+        a, b = int(m.group(2) or m.group(3)), int(m.group(4) or m.group(2) or 0)
+        up = 256 if m.group(1) == "a" else 0
+        return "v" if up else m.group(1), range(a + up, b + up + 1)
+    return {"vcc": ("s", range(VCC, VCC + 2)), "exec": ("s", range(EXEC, EXEC + 2)), "m0": ("s", range(M0, M0 + 1))}.get(t)
 
 
 def literal(t):
@@ -99,20 +100,22 @@ WORDS = {  # 32 bits in, 32 bits out
     "bfe_u32": lambda a, b, c: a >> (b & np.uint32(31)) & ((np.uint32(1) << (c & np.uint32(31))) - np.uint32(1)),
     "mad_u32_u24": lambda a, b, c: (a & np.uint32(0xFFFFFF)) * (b & np.uint32(0xFFFFFF)) + c,
     "med3_i32": lambda a, b, c: np.sort(np.stack([a, b, c]).view(np.int32), 0)[1].view(np.uint32)}
-FLOATS = {"add_f32", "sub_f32", "mul_f32", "fma_f32", "fmac_f32", "fmaak_f32", "fmamk_f32", "max_f32", "min_f32", "rcp_f32", "exp_f32", "perm_b32"}
+FLOATS = {"add_f32", "sub_f32", "fma_f32", "fmac_f32", "fmaak_f32", "fmamk_f32", "max_f32", "min_f32", "rcp_f32", "exp_f32", "perm_b32", "cvt_pk_bf16_f32"}
 BYTES = {"dwordx4": 16, "dwordx2": 8, "dword": 4, "ushort": 2, "short_d16_hi": 2, "short": 2}
 
 
 class Wave:
     """One wave of a workgroup; buffers: {name: (address, bytes, written)}; args: the kernel's argument bytes, its blocks' count
-    behind them; lds: bytes; stores: {address: number of stores}."""
+    behind them; lds: bytes; stores: {address: number of stores}; based: a buffer descriptor's base has to be in a buffer also where
+    none of its loads is."""
 
-    def __init__(self, code, args, buffers, lds, wave, block, rng, stores):
+    def __init__(self, code, args, buffers, lds, wave, block, rng, stores, based=True):
+        self.based = based
         (self.ins, self.jumps), self.args, self.buffers, self.lds, self.rng, self.stores = code, args, buffers, lds, rng, stores
         self.s = [0] * 128
         self.s[0], self.s[1], self.s[2], self.s[3] = 0x1000, 0x77, *block
         self.s[EXEC] = self.s[EXEC + 1] = 0xFFFFFFFF
-        self.v = rng.integers(0, 1 << 32, (256, 64), dtype=np.uint32)
+        self.v = rng.integers(0, 1 << 32, (512, 64), dtype=np.uint32)
         self.v[0] = 64 * wave + LANES
         self.scc, self.barriers = False, 0
         self.loads, self.others = [], []                            # in flight: registers of vmcnt's, (kind, registers) of lgkmcnt's
@@ -198,16 +201,17 @@ class Wave:
         elif op == "s_nop":
             pass
         else:
-            self.not_in_flight(ops + ["vcc"] * ("vcc" in op))
+            self.not_in_flight(op, ops + ["vcc"] * ("vcc" in op))
             if "branch" in op:
                 how = {"s_branch": True, "s_cbranch_scc0": not self.scc, "s_cbranch_scc1": self.scc, "s_cbranch_vccz": not self.pair(VCC),
                        "s_cbranch_vccnz": self.pair(VCC), "s_cbranch_execz": not self.pair(EXEC), "s_cbranch_execnz": self.pair(EXEC)}
                 return self.jumps[at] if how[op] else None
             self.scalar(op, ops) if op.startswith("s_") else self.vector(op, ops, more)
 
-    def not_in_flight(self, ops):
+    def not_in_flight(self, op, ops):
+        """A load may be aimed at registers that another one is on its way to: they come in order."""
         if self.loads or self.others:
-            mine = {(r[0], k) for r in map(registers, ops) if r for k in r[1]}
+            mine = {(r[0], k) for r in map(registers, ops[1:] if op.startswith(("buffer_load", "global_load")) else ops) if r for k in r[1]}
             for d in self.loads + [d for _, d in self.others]:
                 if d & mine:
                     raise Fault("a load into %s is in flight" % sorted(d & mine))
@@ -223,21 +227,26 @@ class Wave:
             return
         name, _, kind = op[2:].rpartition("_")
         wide = kind.endswith("64")
+        if name in ("bitcmp0", "bitcmp1"):
+            self.scc = self.scalar_of(t[0]) >> (self.scalar_of(t[1]) & 31) & 1 == int(name[-1])
+            return
         if name.startswith("cmp"):
             a, b = self.scalar_of(t[0], wide), self.scalar_of(t[1], wide)
+            if name.startswith("cmpk"):
+                b = b & 0xFFFF | (0xFFFF0000 if kind == "i32" and b & 0x8000 else 0)
             a, b = (signed(a), signed(b)) if kind == "i32" else (a, b)
             self.scc = COMPARE[name.rpartition("_")[2]](a, b)
             return
         d = registers(t[0])[1][0]
-        if name == "and_saveexec":
+        if name in ("and_saveexec", "andn2_saveexec"):
             old = self.pair(EXEC)
-            self.put_pair(EXEC, self.scalar_of(t[1], True) & old)
+            self.put_pair(EXEC, self.scalar_of(t[1], True) & (old if name == "and_saveexec" else ~old))
             self.put_pair(d, old)
             self.scc = self.pair(EXEC) != 0
             return
         a = self.scalar_of(t[1], wide)
         b = self.scalar_of(t[2], wide) if len(t) > 2 else 0
-        if name in ("movk", "addk"):
+        if name in ("movk", "addk", "mulk"):
             a = (a & 0xFFFF) - (0x10000 if a & 0x8000 else 0)
         carry = None
         if name in ("mov", "movk"):
@@ -253,7 +262,10 @@ class Wave:
             carry = x >> 32 != 0
         elif name == "addk":
             x, carry = self.s[d] + a, False
-        elif name == "sub":
+        elif name == "mulk":
+            x = self.s[d] * a
+        elif name in ("sub", "subb"):
+            b += int(self.scc) if name == "subb" else 0
             x, carry = a - b, b > a
         elif name in ("min", "max"):
             u, w = (signed(a), signed(b)) if kind == "i32" else (a, b)
@@ -273,43 +285,50 @@ class Wave:
     def vector(self, op, t, more):
         mask = self.pair(EXEC)
         self.live = live = np.array([mask >> i & 1 for i in range(64)], bool) if mask != FULL else np.ones(64, bool)
-        m = re.search(r"offset:(\d+)", more)
+        m = re.search(r"offset:(-?\d+)", more)
         offset = int(m.group(1)) if m else 0
         if op.startswith("global_"):
             _, kind, width = op.split("_", 2)
             if t[2] != "off":
                 raise Fault("unknown")
-            a = self.pairs(t[1] if kind == "load" else t[0])[live] + np.uint64(offset)
+            a = self.pairs(t[1] if kind == "load" else t[0])[live] + np.uint64(offset & FULL)
             self.access(a, BYTES[width], kind == "store")
             if kind == "load":
                 self.random(t[0])
             self.loads.append({("v", k) for k in registers(t[0])[1]} if kind == "load" else set())
             return
         if op.startswith("buffer_load_"):
-            if more.split() != ["offen"] or t[3].split()[0] != "0":
+            to_lds = "lds" in more.split()                          # lane after lane from m0 on
+            t = ["m0"] + t if to_lds else t
+            if more.split() != ["offen"] + ["lds"] * to_lds or t[3] != "0":
                 raise Fault("unknown")
             r = registers(t[2])[1][0]
             base, records = self.s[r] | (self.s[r + 1] & 0xFFFF) << 32, self.s[r + 2]
             if self.s[r + 1] >> 16 or self.s[r + 3] != 0x20000:
                 raise Fault("descriptor")
-            if not any(b <= base < b + n for b, n, _ in self.buffers.values()):
+            if self.based and not any(b <= base < b + n for b, n, _ in self.buffers.values()):
                 raise Fault("a descriptor's base, %x, is in no buffer" % base)
             o = self.words(t[1]).astype(np.int64)
             self.access(base + o[live & (o < records)], BYTES[op[12:]])
-            self.random(t[0])
-            self.loads.append({("v", k) for k in registers(t[0])[1]})
+            if to_lds:
+                self.in_lds(np.uint32(self.s[M0] + BYTES[op[12:]] * LANES), BYTES[op[12:]])
+                self.loads.append(set())
+            else:
+                self.random(t[0])
+                self.loads.append({("v", k) for k in registers(t[0])[1]})
             return
         if op.startswith("ds_"):
             if op == "ds_write_b128":
                 self.in_lds(self.words(t[0]) + np.uint32(offset), 16)
             elif op == "ds_read_b128":
                 self.in_lds(self.words(t[1]) + np.uint32(offset), 16)
-            elif op in ("ds_read2_b32", "ds_read2st64_b32"):
+            elif op.startswith("ds_read2"):
+                n = 8 if op.endswith("b64") else 4
                 for o in ("offset0", "offset1"):
                     o = re.search(o + r":(\d+)", more)
-                    self.in_lds(self.words(t[1]) + np.uint32(int(o.group(1)) * (256 if "st64" in op else 4) if o else 0), 4)
-            elif op == "ds_read_b32":
-                self.in_lds(self.words(t[1]) + np.uint32(offset), 4)
+                    self.in_lds(self.words(t[1]) + np.uint32(int(o.group(1)) * n * (64 if "st64" in op else 1) if o else 0), n)
+            elif op in ("ds_read_b32", "ds_read_b64"):
+                self.in_lds(self.words(t[1]) + np.uint32(offset), int(op[-2:]) // 8)
             else:
                 raise Fault("unknown")
             if op.startswith("ds_read"):
@@ -319,7 +338,7 @@ class Wave:
         name = re.sub(r"_e(32|64)$", "", op[2:])
         if name == "readfirstlane_b32":
             self.s[registers(t[0])[1][0]] = int(self.words(t[1])[int(np.nonzero(live)[0][0]) if live.any() else 0])
-        elif name.startswith(("mfma", "cvt_scalef32")) or name.endswith("_sdwa") or name in FLOATS and not (name == "mul_f32" and t[1] == "0x4f7ffffe"):
+        elif name.startswith(("mfma", "accvgpr", "cvt_scalef32")) or name.endswith("_sdwa") or name in FLOATS:
             self.random(t[0])
         elif name.startswith("permlane"):
             self.random(t[0])
@@ -337,6 +356,8 @@ class Wave:
             self.put_pairs(t[0], np.array([v & FULL for v in x], np.uint64))
         elif name == "lshl_add_u64":
             self.put_pairs(t[0], (self.pairs(t[1]) << np.uint64(self.scalar_of(t[2]))) + self.pairs(t[3]))
+        elif name == "lshlrev_b64":
+            self.put_pairs(t[0], self.pairs(t[2]) << np.uint64(self.scalar_of(t[1])))
         elif name == "mov_b64":
             self.put_pairs(t[0], self.pairs(t[1]))
         elif name == "mov_b32":
@@ -355,16 +376,20 @@ class Wave:
             a, b = ((self.words(k).astype(np.int64) & 0xFFFFFF ^ 0x800000) - 0x800000 for k in t[1:3])
             self.put(registers(t[0])[1][0], ((a * b + self.words(t[3])) & 0xFFFFFFFF).astype(np.uint32))
         elif name == "rcp_iflag_f32":
-            q = 1.0 / self.words(t[1]).view(np.float32).astype(np.float64)
-            f = q.astype(np.float32)
+            with np.errstate(all="ignore"):
+                q = 1.0 / self.words(t[1]).view(np.float32).astype(np.float64)
+                f = q.astype(np.float32)
             low = np.where(f <= q, f, np.nextafter(f, np.float32(0)))
             self.put(registers(t[0])[1][0], (low if self.rng.random() < 0.5 else np.nextafter(low, np.float32(np.inf))).astype(np.float32).view(np.uint32))
         elif name == "mul_f32":
-            self.put(registers(t[0])[1][0], (self.words(t[1]).view(np.float32) * self.words(t[2]).view(np.float32)).view(np.uint32))
-        elif name == "cvt_f32_u32":
-            self.put(registers(t[0])[1][0], self.words(t[1]).astype(np.float32).view(np.uint32))
+            with np.errstate(all="ignore"):
+                self.put(registers(t[0])[1][0], (self.words(t[1]).view(np.float32) * self.words(t[2]).view(np.float32)).view(np.uint32))
+        elif name in ("cvt_f32_u32", "cvt_f32_ubyte0"):
+            x = self.words(t[1]) & np.uint32(255 if name.endswith("0") else 0xFFFFFFFF)
+            self.put(registers(t[0])[1][0], x.astype(np.float32).view(np.uint32))
         elif name == "cvt_u32_f32":
-            self.put(registers(t[0])[1][0], np.clip(self.words(t[1]).view(np.float32).astype(np.float64), 0, 2.0 ** 32 - 1).astype(np.uint32))
+            f = np.nan_to_num(self.words(t[1]).view(np.float32).astype(np.float64))
+            self.put(registers(t[0])[1][0], np.clip(f, 0, 2.0 ** 32 - 1).astype(np.uint32))
         elif name in WORDS and not more:
             self.put(registers(t[0])[1][0], WORDS[name](*(self.words(k) for k in t[1:])))
         else:
